@@ -15,7 +15,7 @@ import torch
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG_DIR, "libdyllm_b200.so")
 
-P, I, F, Z = c_void_p, c_int, c_float, c_size_t
+P, I, F, Z, L = c_void_p, c_int, c_float, c_size_t, c_int64
 
 # name -> (restype, argtypes); mirrors include/dyllm_b200.h one to one.
 SIGNATURES: dict[str, tuple] = {
@@ -58,6 +58,11 @@ SIGNATURES: dict[str, tuple] = {
     "dyllm_row_confidence": (I, [P, I, I, c_int64, P, P, P]),
     "dyllm_confidence_unmask": (I, [P, P, P, I, c_int64, P, I, I, I, I, I, c_int64, P, P, P]),
     "dyllm_kv_cache_update": (I, [P, P, P, P, P, P, I, P, P, P, P, I, I, P, I, I, P, P, P, P]),
+    "dyllm_fp8_cache_write": (I, [P, L, I, I, P, P, L, P, P, P, P, I, I, P]),
+    "dyllm_fp8_cache_read": (I, [P, P, L, I, I, P, P, P, P, P, I, I, P]),
+    "dyllm_fp8_kv_cache_update": (I, [P, L, P, L, P, P, P, P, I, P, P, P, P, I, I, P, I, I, P, P, L, P, P, L, P, P]),
+    "dyllm_attention_salient_rows_fp8_workspace_bytes": (Z, [I, I, I, I]),
+    "dyllm_attention_salient_rows_fp8": (I, [P, L, I, P, P, L, P, P, L, P, P, P, P, P, P, I, I, I, I, I, P, P, I, F, F, P, P, P, Z, P]),
     "dyllm_tp_comm_create": (I, [I, I, Z, P]),
     "dyllm_tp_comm_region_bytes": (Z, [P]),
     "dyllm_tp_comm_region": (P, [P]),
@@ -90,6 +95,8 @@ KERNELS_PER_CALL = {
     "dyllm_tp_push_rows": 1, "dyllm_tp_reduce_rows": 1, "dyllm_tp_allreduce_rows": 2, "dyllm_tp_push_f32": 1,
     "dyllm_tp_reduce_f32": 1, "dyllm_tp_allreduce_f32": 2, "dyllm_tp_gather_rows": 2, "dyllm_tp_gather_push": 1,
     "dyllm_tp_gather_finish": 1, "dyllm_tp_scatter_push": 1,
+    "dyllm_fp8_cache_write": 1, "dyllm_fp8_cache_read": 1, "dyllm_fp8_kv_cache_update": 1,
+    "dyllm_attention_salient_rows_fp8": 1,
 }
 launch_count = 0
 
@@ -147,3 +154,23 @@ def require_cuda(t: torch.Tensor, name: str, dtype: torch.dtype | None = None, d
         raise RuntimeError(f"{name} must be {dim}-D, got {t.dim()}-D")
     if not t.is_contiguous():
         raise RuntimeError(f"{name} must be contiguous")
+
+
+def require_on(index: int, t: torch.Tensor, name: str, dtype: torch.dtype, dim: int) -> None:
+    """:func:`require_cuda` for the device with this index (one look at each property: calls of a few microseconds)."""
+    try:
+        if t.dtype is dtype and t.dim() == dim and t.get_device() == index and t.is_contiguous():
+            return
+    except AttributeError:
+        pass
+    require_cuda(t, name, dtype, dim)
+    raise RuntimeError(f"{name} must be on cuda:{index}, got {t.device}")
+
+
+def call_on(index: int, name: str, *args) -> None:
+    """:func:`call` with the current stream of device ``index`` as the last argument, and that device current."""
+    if torch._C._cuda_getDevice() == index:
+        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(index))

@@ -409,6 +409,67 @@ int dyllm_rope_neox(void* x, const int64_t* positions, const int64_t* pos_idx, c
                     const int32_t* num_rows_dev, int heads, int head_dim, int max_pos, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * 8-bit caches of keys and values
+ *
+ * Per row and key/value head a cache holds 128 codes in e4m3 ([cache_rows, heads * 128] bytes, 16-byte aligned) and one fp32
+ * scale ([cache_rows, heads]): scale = 2^e, e the least integer >= -60 with amax <= 448 * 2^e; a value is code * scale,
+ * which bf16 holds exactly.  A head of a row with a NaN or an infinity gets codes of zero and a NaN scale: it reads as NaN,
+ * and a key that a row does not see never reaches its result.  Sequences lie in both arrays as in the bf16 caches:
+ * seq_starts[seq_ids[b]] is the first row of batch entry b.  A row that lies outside [0, cache_rows), or whose sequence has
+ * a negative start, is not written and reads as zeros.  heads > 0, head_dim 128.  No counterpart in the reference, whose
+ * caches are bf16 (dyllm/engine/cache_manager.py:11-60).
+ * ---------------------------------------------------------------------------------------------- */
+
+/* Quantises the packed rows x [total_rows, heads, 128] (bf16, row pitch ldx elements: a multiple of 8, so that x may be one
+ * half of a fused K/V product) into the rows of their sequences: row i of batch entry b goes to
+ * seq_starts[seq_ids[b]] + i, or, with cu_seqlens_k, to the same place among the last cu_seqlens[b+1] - cu_seqlens[b] rows
+ * of its len_k(b) rows.  The 8-bit form of dyllm_cache_reset_full / dyllm_cache_reset_block. */
+int dyllm_fp8_cache_write(const void* x, int64_t ldx, int heads, int head_dim, void* codes, float* scales,
+                          int64_t cache_rows, const int64_t* seq_starts, const int32_t* cu_seqlens,
+                          const int32_t* cu_seqlens_k, const int64_t* seq_ids, int batch, int total_rows, void* stream);
+
+/* The way back: out [total_rows, heads, 128] (bf16, packed) = codes * scales of the same rows.  Rows of out at or past
+ * cu_seqlens[batch] stay as they are.  The 8-bit form of dyllm_cache_get_seqs / dyllm_cache_get_block. */
+int dyllm_fp8_cache_read(const void* codes, const float* scales, int64_t cache_rows, int heads, int head_dim, void* out,
+                         const int64_t* seq_starts, const int32_t* cu_seqlens, const int32_t* cu_seqlens_k,
+                         const int64_t* seq_ids, int batch, int total_rows, void* stream);
+
+/* dyllm_kv_cache_update on 8-bit caches, i < min(num_rows, *num_rows_dev):
+ *   K row row_k(i) = quantised rope_neox(k_new[i], positions[pos_idx ? pos_idx[i] : i])
+ *   dv[i] = bf16(new - old) of the values that V row row_v(i) holds after and before;  V row row_v(i) = quantised v_new[i]
+ * The difference is taken between what the cache holds, so a value whose codes do not change adds nothing to a context (the
+ * rounding of the codes does not pile up over the steps).  k_new, v_new: [num_rows, kv_heads, 128] bf16 with row pitches ldk,
+ * ldv (multiples of 8); dv packed; rows_k without repetitions. */
+int dyllm_fp8_kv_cache_update(const void* k_new, int64_t ldk, const void* v_new, int64_t ldv, const int64_t* rows_k,
+                              const int64_t* positions, const int64_t* pos_idx, const float* cos_sin, int max_pos,
+                              const int32_t* cu_seqlens_k, const int64_t* k_seq_starts, const int64_t* v_seq_starts,
+                              const int64_t* seq_ids, int batch, int num_rows, const int32_t* num_rows_dev, int kv_heads,
+                              int head_dim, void* k_codes, float* k_scales, int64_t k_rows, void* v_codes, float* v_scales,
+                              int64_t v_rows, void* dv, void* stream);
+
+/* Bytes of workspace dyllm_attention_salient_rows_fp8 needs. */
+size_t dyllm_attention_salient_rows_fp8_workspace_bytes(int num_salient, int batch, int num_heads, int num_kv_heads);
+
+/* Exact attention of the listed query rows over the 8-bit keys and values of their sequence, read in place:
+ *   out[i] = sum_j softmax_j(s_j) v_j,  s_j = scale * q[idx_salient_row[i]] . k_j,
+ *   softcap > 0: s_j = softcap * tanh(s_j / softcap);  then slopes ([num_heads], nullable): s_j -= slopes[h] * |pos - j|,
+ * pos the row's place in its sequence (the queries of a sequence are its last len_q rows).  key_ranges (int32 [total_q, 2],
+ * nullable) gives every query row the keys [begin, end) that it sees, as places in its sequence, cut to [0, len_k): documents,
+ * prefixes, windows.  A row that sees no key gives zeros.  q: [total_q, num_heads, 128] bf16, row pitch ldq (a multiple of
+ * 8); out: [num_salient, num_heads, 128] bf16, of which the rows up to cu_salientlens[batch] (the live count, read on the
+ * device) are written; a listed row outside [0, total_q) gives zeros.  max_rows_per_seq: upper bound of the listed rows of
+ * one sequence; it chooses the kernels (a wrong bound costs time, not rows).  workspace: 16-byte aligned, need not be
+ * cleared; calls that may overlap on the GPU need different ones. */
+int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, const void* k_codes, const float* k_scales,
+                                     int64_t k_rows, const void* v_codes, const float* v_scales, int64_t v_rows,
+                                     const int64_t* k_seq_starts, const int64_t* v_seq_starts, const int64_t* seq_ids,
+                                     void* out, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int batch,
+                                     int max_rows_per_seq, int num_heads, int num_kv_heads, int head_dim,
+                                     const int32_t* cu_salientlens, const int32_t* idx_salient_row, int num_salient,
+                                     float scale, float softcap, const float* slopes, const int32_t* key_ranges,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
  * Tensor-parallel SUM exchange of the small per-layer tensors over peer memory (NVLink)
  *
  * One communicator per rank (process) and GPU.  Every rank owns a region of

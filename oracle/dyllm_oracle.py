@@ -390,3 +390,91 @@ def make_batch_layout(batch, prompt, response, response_only, device="cpu"):
     lq = response if response_only else L
     ar = torch.arange(batch + 1, dtype=torch.int32)
     return (ar * lq).to(device), (ar * L).to(device), (ar * prompt).to(device)
+
+
+# --------------------------------------------------------------------------------------------------
+# 8-bit caches of keys and values (no counterpart in the reference): definitions in 64 bits
+# --------------------------------------------------------------------------------------------------
+# every non-negative e4m3 number: code c = 8 * exponent field + fraction, 448 the largest, 0x7f is NaN
+E4M3 = np.array([(f / 8) * 2.0 ** -6 if e == 0 else (1 + f / 8) * 2.0 ** (e - 7) for e in range(16) for f in range(8)][:127])
+
+
+def fp8_quantise(x: torch.Tensor):
+    """(code values, scales) in float64 of ``x [..., 128]``: scale 2^e, e the least integer >= -60 with amax <= 448 * 2^e; the
+    nearest e4m3 number to x / scale, ties to the even code.  A NaN or an infinity: codes 0, scale NaN."""
+    v = x.detach().to("cpu", torch.float64).numpy()
+    amax = np.abs(v).max(-1, keepdims=True)
+    bad = ~np.isfinite(amax)
+    grid = 448.0 * 2.0 ** np.arange(-60, 125)
+    e = np.searchsorted(grid, np.where(bad, 0.0, amax).reshape(-1)).reshape(amax.shape) - 60.0
+    scale = 2.0 ** e
+    y = np.where(bad, 0.0, v) / scale
+    mids = (E4M3[1:] + E4M3[:-1]) / 2                     # exact
+    low = np.searchsorted(mids, np.abs(y).reshape(-1), side="left").reshape(y.shape)     # |y| <= mids[low]
+    tie = (low < len(mids)) & (np.abs(y) == mids[np.minimum(low, len(mids) - 1)]) & (low % 2 == 1)
+    code = np.copysign(E4M3[low + tie], y)
+    return torch.from_numpy(code), torch.from_numpy(np.where(bad, np.nan, scale)).squeeze(-1)
+
+
+def _fp8_rows(seq_starts, cu, seq_ids, cu_k=None):
+    rows = []
+    for b in range(len(seq_ids)):
+        n = int(cu[b + 1] - cu[b])
+        first = int(seq_starts[seq_ids[b]]) + (int(cu_k[b + 1] - cu_k[b]) - n if cu_k is not None else 0)
+        rows.extend(range(first, first + n))
+    return torch.tensor(rows, dtype=torch.int64)
+
+
+def fp8_cache_write(codes, scales, x, seq_starts, cu, seq_ids, cu_k=None):
+    """In place on float64 ``codes [rows, heads, 128]``, ``scales [rows, heads]``."""
+    at = _fp8_rows(seq_starts, cu, seq_ids, cu_k)
+    codes[at], scales[at] = fp8_quantise(x[: len(at)])
+    return codes, scales
+
+
+def fp8_cache_read(codes, scales, seq_starts, cu, seq_ids, cu_k=None):
+    at = _fp8_rows(seq_starts, cu, seq_ids, cu_k)
+    return codes[at] * scales[at].unsqueeze(-1)
+
+
+def fp8_kv_cache_update(k_new, v_new, rows_k, positions, pos_idx, cos_sin, cu_k, k_starts, v_starts, seq_ids, kc, ks, vc, vs):
+    """In place on float64 caches; returns dV in float64.  The rotation alone is in fp32, product by product, as defined."""
+    b = torch.searchsorted(cu_k[1:].long(), rows_k, right=True)
+    off = rows_k - cu_k.long()[b]
+    krow, vrow = k_starts[seq_ids[b]] + off, v_starts[seq_ids[b]] + off
+    cs = cos_sin.float()[positions[pos_idx]].unsqueeze(1)
+    c, s = cs[..., :64], cs[..., 64:]
+    x, y = k_new[..., :64].float(), k_new[..., 64:].float()
+    kc[krow], ks[krow] = fp8_quantise(torch.cat([x * c - y * s, y * c + x * s], -1))
+    old = vc[vrow] * vs[vrow].unsqueeze(-1)
+    vc[vrow], vs[vrow] = fp8_quantise(v_new)
+    return vc[vrow] * vs[vrow].unsqueeze(-1) - old
+
+
+def attention_rows_fp8(q, k, v, cu_q, cu_k, cu_rows, rows, scale=None, softcap=0.0, slopes=None, ranges=None):
+    """(out, sum of weight * |v|, largest scale * |q| . |k| + |bias|) in float64 of the listed rows; ``k``, ``v``: packed values
+    ``[total_k, kv_heads, 128]``.  The last two bound what rounding can do."""
+    q, k, v = q.double(), k.double(), v.double()
+    H, Hkv = q.size(1), k.size(1)
+    scale = q.size(2) ** -0.5 if scale is None else scale
+    out, mag, big = torch.zeros(len(rows), H, q.size(2)).double(), torch.zeros(len(rows), H, q.size(2)).double(), torch.zeros(len(rows), H).double()
+    for b in range(len(cu_q) - 1):
+        length = int(cu_k[b + 1] - cu_k[b])
+        kb, vb = k[int(cu_k[b]):int(cu_k[b + 1])], v[int(cu_k[b]):int(cu_k[b + 1])]
+        for i in range(int(cu_rows[b]), int(cu_rows[b + 1])):
+            r = int(rows[i])
+            pos = length - (int(cu_q[b + 1]) - r)
+            lo, hi = (0, length) if ranges is None else (max(0, int(ranges[r, 0])), min(length, int(ranges[r, 1])))
+            if lo >= hi:
+                continue
+            away = (pos - torch.arange(lo, hi)).abs().double()
+            for h in range(H):
+                g = h // (H // Hkv)
+                t = scale * (kb[lo:hi, g] @ q[r, h])
+                if softcap:
+                    t = softcap * torch.tanh(t / softcap)
+                bias = float(slopes[h]) * away if slopes is not None else torch.zeros_like(away)
+                p = torch.softmax(t - bias, 0)
+                out[i, h], mag[i, h] = p @ vb[lo:hi, g], p @ vb[lo:hi, g].abs()
+                big[i, h] = (abs(scale) * (kb[lo:hi, g].abs() @ q[r, h].abs()) + bias.abs()).max()
+    return out, mag, big
