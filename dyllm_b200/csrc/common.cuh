@@ -373,6 +373,9 @@ __device__ __forceinline__ uint32_t sw128_offset(uint32_t row, uint32_t chunk) {
 // 128-byte swizzle requires box_cols * 2 == 128.
 int encode_tmap_2d_bf16(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch_elems,
                         uint32_t box_rows, uint32_t box_cols, bool swizzle128);
+// 2-D byte tensor [rows][cols]; box = [box_rows][128] with the 128-byte swizzle.
+int encode_tmap_2d_u8(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch_bytes,
+                      uint32_t box_rows, uint32_t box_cols);
 // 3-D bf16 tensor [d2][d1][d0] (d0 innermost) with byte strides for d1 and d2.
 int encode_tmap_3d_bf16(CUtensorMap* out, const void* base, uint64_t d0, uint64_t d1, uint64_t d2,
                         uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t box0, uint32_t box1,

@@ -131,6 +131,25 @@ int encode_tmap_2d_bf16(CUtensorMap* out, const void* base, uint64_t rows, uint6
   return DYLLM_OK;
 }
 
+int encode_tmap_2d_u8(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch_bytes,
+                      uint32_t box_rows, uint32_t box_cols) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn)
+    return set_error(DYLLM_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {pitch_bytes};
+  cuuint32_t box[2] = {box_cols, box_rows};
+  cuuint32_t elem_strides[2] = {1, 1};
+  CUresult res = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem_strides,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (res != CUDA_SUCCESS)
+    return set_error(DYLLM_ERR_CUDA, "cuTensorMapEncodeTiled(2d, bytes) failed with %d (base %p rows %llu cols %llu pitch %llu)",
+                     static_cast<int>(res), base, (unsigned long long)rows, (unsigned long long)cols,
+                     (unsigned long long)pitch_bytes);
+  return DYLLM_OK;
+}
+
 int encode_tmap_3d_bf16(CUtensorMap* out, const void* base, uint64_t d0, uint64_t d1, uint64_t d2,
                         uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t box0, uint32_t box1,
                         uint32_t box2, bool swizzle128) {
