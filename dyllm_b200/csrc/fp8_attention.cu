@@ -71,33 +71,38 @@ __device__ __forceinline__ float value_exponent(float scale) {
 }
 
 // ----------------------------------------------------------------------------------------------
-// Few rows per sequence: bound by the bytes of the cache.  mma.sync on codes widened to half precision in registers.
+// Few rows per sequence: bound by the bytes of the cache, which go from the TMA ring to the tensor cores as they are.
 //
-// The rows of a tile are the (listed row, query head) pairs of one sequence and key head, 16 or 32 of them, so that grouped
-// query heads share one pass over their keys.  A unit of work is 128 keys of a tile; all units of the launch, in the order
-// (sequence, key head, tile, keys), are dealt out to the CTAs in equal contiguous shares that every CTA works out for itself
-// from the device-side counts.  A tile whose units lie in several CTAs is joined by the CTA that finishes last, in the order
-// of its parts.
+// The rows of a tile are the (listed row, query head) pairs of one sequence and key head, RN = 16 or 32 of them, so that
+// grouped query heads share one pass over their keys.  A unit of work is 128 keys of a tile; all units of the launch, in the
+// order (sequence, key head, tile, keys), are dealt out to the CTAs in equal contiguous shares that every CTA works out for
+// itself from the device-side counts.  A tile whose units lie in several CTAs is joined by the CTA that finishes last, in the
+// order of its parts.
 //
-// One producer warp feeds a ring of units (TMA boxes of 32 rows x 128 bytes, the scales by cp.async); each of four consumer
-// warps takes 32 keys of a unit on its own (own running maximum and sum), and the four are joined when the tile ends.
+// The products are transposed, keys (then head dimensions) in the M = 128 of tcgen05.mma.kind::f8f6f4:
+//   S^T = K Q^T         A: K tile as loaded (K-major), B: the queries as e4m3 + e5m2, two products into one accumulator
+//   O^T = V^T P^T       A: V tile as loaded (MN-major), B: the weights, 32 columns of e4m3 and 32 of their remainders
+// A query in bf16 (8 significant bits) is e4m3 (4 bits) plus a remainder of at most 3 bits, which e5m2 holds exactly down to
+// 2^-25 of the row's largest element.  A weight in [0, 1] is taken as e4m3(256 w) + e4m3(16 * remainder) / 16: off by at most
+// 2^-8 of itself, or 2^-22.  The codes of the cache are never widened.
 //
-// Operand layouts (g = lane / 4, c = lane % 4), chosen so that every shared-memory access is 16 bytes wide and the widening
-// of four codes is one or two instructions per pair:
-//   S = Q K^T    contraction step s = 0..7, thread c holds dimensions 32c + 4s .. +3 (two pairs) of key 8j + g: the 32 bytes
-//                of a key that a thread needs are contiguous.
-//   O = P V      output block nb = 0..15, column g is dimension 16g + nb: the 16 bytes of a key that a thread needs are
-//                contiguous, and a byte permutation pairs two keys' codes.
+// Softmax per chunk of up to kChunk tiles: thread = key, first the scores of all tiles of the chunk (kept in tensor memory in
+// place of the products) and their maxima, then weights tile by tile; the sums are rescaled between chunks.  Eight softmax
+// warps, two per quarter of the keys, each with half of the rows; a TMA warp and an MMA warp.  Two CTAs per SM.
 // ----------------------------------------------------------------------------------------------
 constexpr int kUnitKeys = 128;
-constexpr uint32_t kKvBytes = kUnitKeys * kD;                                  // codes of K or V of a unit
-constexpr uint32_t kScaleBytes = 2 * kUnitKeys * sizeof(float);
-template <int RG>
+constexpr int kRing = 4;                                     // slots of one K or V tile
+constexpr uint32_t kTileBytes = kUnitKeys * kD;
+constexpr int kFewThreads = 320;
+constexpr uint32_t kTmemCols = 256;
+template <int RN>
 struct FewCfg {
-  static constexpr int kRing = 2 * RG;
-  static constexpr int kThreads = 32 + 128 * RG;
-  static constexpr uint32_t kMergeBytes = RG * 4 * 16 * kD * sizeof(float);
-  static constexpr uint32_t kSmem = kRing * (2 * kKvBytes + kScaleBytes) + kMergeBytes + 1024;
+  static constexpr int kHalf = RN / 2;                       // rows of a softmax warp
+  static constexpr int kChunk = RN == 16 ? 8 : 6;
+  static constexpr uint32_t kTmemO = kChunk * RN;            // columns of O^T behind those of S^T: RN of 256 w, RN of remainders
+  static constexpr uint32_t kQBytes = RN * kD;
+  static constexpr uint32_t kSmem = (kRing + 2) * kTileBytes + 2 * kQBytes + 1024;
+  static_assert(kTmemO + 2 * RN <= kTmemCols, "tensor memory of two CTAs per SM");
 };
 
 struct FewParams {
@@ -163,10 +168,11 @@ __device__ __forceinline__ SeqWork seq_work(const FewParams& p, int b) {
 template <int MROWS>
 struct Walk {
   SeqWork w;
-  int64_t total, at, end, seq_first;    // units: of the launch, next, end of the share, first of the sequence
+  int64_t total, left;                  // units: of the launch, of the share that are still to come
+  int64_t tile_first;                   // first unit of the tile in the launch
   int hk, tile, first, last;            // the part: units [first, last) of the tile
   int ctas;                             // CTAs that have a share
-  int64_t tile_first;                   // first unit of the tile in the launch
+  bool begun;
 
   __device__ __forceinline__ void start(const FewParams& p) {
     const int lane = threadIdx.x & 31;
@@ -180,12 +186,13 @@ struct Walk {
       sum += __shfl_xor_sync(0xffffffffu, sum, s);
     total = sum * p.a.Hkv;
     ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total));      // no share is empty
-    at = end = 0;
+    left = 0;
+    begun = false;
     if (static_cast<int>(blockIdx.x) >= ctas)
       return;
-    at = total * blockIdx.x / ctas;
-    end = total * (blockIdx.x + 1) / ctas;
-    seq_first = 0;
+    const int64_t at = share(blockIdx.x);
+    left = share(blockIdx.x + 1) - at;
+    int64_t before = 0;
     for (int base = 0;; base += 32) {
       const SeqWork x = seq_work<MROWS>(p, base + lane);
       const int64_t mine = static_cast<int64_t>(x.tiles) * x.units * p.a.Hkv;
@@ -196,469 +203,588 @@ struct Walk {
         if (lane >= s)
           scan += o;
       }
-      const unsigned hit = __ballot_sync(0xffffffffu, seq_first + scan > at);
+      const unsigned hit = __ballot_sync(0xffffffffu, before + scan > at);
       if (hit) {
         const int src = __ffs(hit) - 1;
-        seq_first += __shfl_sync(0xffffffffu, scan - mine, src);
+        before += __shfl_sync(0xffffffffu, scan - mine, src);
         w = seq_work<MROWS>(p, base + src);
-        return;
+        break;
       }
-      seq_first += __shfl_sync(0xffffffffu, scan, 31);
+      before += __shfl_sync(0xffffffffu, scan, 31);
     }
+    const int64_t t = (at - before) / w.units;
+    first = static_cast<int>(at - before - t * w.units);
+    tile_first = at - first;
+    hk = static_cast<int>(t / w.tiles);
+    tile = static_cast<int>(t - static_cast<int64_t>(hk) * w.tiles);
   }
   // The next part, false at the end of the share.
   __device__ __forceinline__ bool next(const FewParams& p) {
-    if (at >= end)
+    if (left == 0)
       return false;
-    int64_t in_seq = at - seq_first;
-    while (in_seq >= static_cast<int64_t>(w.tiles) * w.units * p.a.Hkv) {
-      seq_first += static_cast<int64_t>(w.tiles) * w.units * p.a.Hkv;
-      in_seq = at - seq_first;
-      w = seq_work<MROWS>(p, w.b + 1);
+    if (begun) {
+      first = 0;
+      tile_first += w.units;
+      if (++tile == w.tiles) {
+        tile = 0;
+        if (++hk == p.a.Hkv) {
+          hk = 0;
+          do
+            w = seq_work<MROWS>(p, w.b + 1);
+          while (w.tiles == 0);
+        }
+      }
     }
-    const int t = static_cast<int>(in_seq / w.units);
-    first = static_cast<int>(in_seq - static_cast<int64_t>(t) * w.units);
-    hk = t / w.tiles;
-    tile = t - hk * w.tiles;
-    tile_first = at - first;
-    last = static_cast<int>(min(static_cast<int64_t>(w.units), first + (end - at)));
-    at += last - first;
+    begun = true;
+    last = static_cast<int>(min(static_cast<int64_t>(w.units), first + left));
+    left -= last - first;
     return true;
   }
-  // CTA whose share holds unit u
+  // First unit of a CTA's share, and the CTA whose share holds unit u.
+  __device__ __forceinline__ int64_t share(int64_t cta) const { return total * cta / ctas; }
   __device__ __forceinline__ int cta_of(int64_t u) const { return static_cast<int>(((u + 1) * ctas - 1) / total); }
 };
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// One arrival for the warp, after what all of its lanes have done (an arrival per lane is a shared-memory atomic each).
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0)
+    mbar_arrive(bar);
 }
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-template <int RG>
-__device__ __forceinline__ void consumers_sync() {
-  asm volatile("bar.sync 1, %0;" ::"n"(128 * RG) : "memory");
-}
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-// Power of two near 1 / amax and its inverse: queries go into half precision next to their row's largest element.
-__device__ __forceinline__ float2 query_scales(uint32_t amax) {
-  if (amax >= 0x7f800000u)
-    return make_float2(__uint_as_float(0x7fc00000u), 1.f);
-  const uint32_t e = min(max(amax >> 23, 1u), 252u);
-  return make_float2(__uint_as_float((254u - e) << 23), __uint_as_float(e << 23));
-}
-
-// Sixteen values of output row t of a sequence's (listed row, head) pairs.
-__device__ __forceinline__ void store_row(const FewParams& p, const SeqWork& w, int hk, int t, int oc, const float4 (&acc)[4], float sum,
-                                          int group) {
-  if (t >= w.rows)
-    return;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int i = t / group, h = hk * group + t - i * group;
-  uint4* dst = reinterpret_cast<uint4*>(p.a.out + ((static_cast<int64_t>(w.row0) + i) * p.a.H + h) * kD) + oc / 2;
+// Maximum or sum of each of N = 8 or 16 values over the lanes of a warp: lane l gets that of value l / (32 / N).
+template <int N, bool MAX>
+__device__ __forceinline__ float reduce_lanes(const float (&v)[N]) {
+  const int lane = threadIdx.x & 31;
+  auto join = [](float x, float y) { return MAX ? fmaxf(x, y) : x + y; };
+  float x[N];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const float x[8] = {acc[2 * j].x * inv, acc[2 * j].y * inv, acc[2 * j].z * inv, acc[2 * j].w * inv,
-                        acc[2 * j + 1].x * inv, acc[2 * j + 1].y * inv, acc[2 * j + 1].z * inv, acc[2 * j + 1].w * inv};
-    dst[j] = float_to_bf16x8(x);
+  for (int i = 0; i < N; ++i)
+    x[i] = v[i];
+  int bit = 16;
+#pragma unroll
+  for (int n = N / 2; n >= 1; n >>= 1, bit >>= 1) {
+    const bool up = lane & bit;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i)
+      if (i < n) {
+        const float keep = up ? x[i + n] : x[i], give = up ? x[i] : x[i + n];
+        x[i] = join(keep, __shfl_xor_sync(0xffffffffu, give, bit));
+      }
+  }
+#pragma unroll
+  for (int b = 16 / N; b >= 1; b >>= 1)
+    x[0] = join(x[0], __shfl_xor_sync(0xffffffffu, x[0], b));
+  return x[0];
+}
+
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&r)[N]) {
+  if constexpr (N == 16)
+    tmem_ld_32x16(addr, r);
+  else
+    tmem_ld_32x8(addr, r);
+}
+template <int N>
+__device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&r)[N]) {
+  if constexpr (N == 16)
+    tmem_st_32x16(addr, r);
+  else
+    tmem_st_32x8(addr, r);
+}
+// N consecutive floats of shared memory, 16-byte aligned, the same for all lanes
+template <int N>
+__device__ __forceinline__ void lds_row(float (&x)[N], const float* src) {
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i) {
+    const float4 v = *reinterpret_cast<const float4*>(src + 4 * i);
+    x[4 * i] = v.x;
+    x[4 * i + 1] = v.y;
+    x[4 * i + 2] = v.z;
+    x[4 * i + 3] = v.w;
   }
 }
 
-// RG: groups of 16 rows in a tile, four consumer warps each (RG = 2: one CTA per SM, twice the ring).
-template <int RG, bool PLAIN>
-__global__ void __launch_bounds__(FewCfg<RG>::kThreads, 3 - RG)
+// Keys of a part: [begin, end), in tiles from begin on.
+template <int RN>
+__device__ __forceinline__ int2 part_keys(const Walk<RN>& walk) {
+  const int begin = walk.w.lo + walk.first * kUnitKeys;
+  return make_int2(begin, min(walk.w.hi, walk.w.lo + walk.last * kUnitKeys));
+}
+
+template <int RN, bool PLAIN>
+__global__ void __launch_bounds__(kFewThreads, 2)
 fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const FewParams p) {
   pdl_wait();      // programmatic dependent launch: nothing before this reads an earlier kernel's data
   pdl_trigger();
-  using Cfg = FewCfg<RG>;
-  constexpr int MROWS = 16 * RG, kRing = Cfg::kRing;
+  using Cfg = FewCfg<RN>;
+  constexpr int HR = Cfg::kHalf, kChunk = Cfg::kChunk;
+  const Fp8AttnParams& a = p.a;
+  Walk<RN> walk;
+  walk.start(p);
+  if (walk.left == 0)
+    return;
+
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* k_ring = smem;
-  uint8_t* v_ring = smem + kRing * kKvBytes;
-  float* merge = reinterpret_cast<float*>(smem + 2 * kRing * kKvBytes);
-  float* scales = reinterpret_cast<float*>(smem + 2 * kRing * kKvBytes + Cfg::kMergeBytes);      // [stage][K, V][128]
-  __shared__ uint64_t full[kRing], empty[kRing];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* p_smem = ring + kRing * kTileBytes;               // two slots of [128 keys][128 bytes]: weights, then remainders
+  uint8_t* q_smem = p_smem + 2 * kTileBytes;                 // [RN][128] e4m3, then e5m2
+  __shared__ uint64_t full[kRing], empty[kRing], s_full[kChunk], p_full[2], p_free[2], q_full, s_free, pv_done, o_free;
+  __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag, joins;
-  __shared__ float2 s_ml[4 * RG][16];      // (maximum, sum) of a warp's rows
+  __shared__ __align__(16) float s_rf[RN], s_slope[RN], s_max[4][RN], s_sum[4][RN];
+  __shared__ int s_pos[RN];
+  __shared__ int64_t s_out[RN];
+  __shared__ int2 s_range[RN];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int i = 0; i < kRing; ++i) {
-      mbar_init(&full[i], 33);         // 32 lanes' scale copies and the bytes of the boxes
-      mbar_init(&empty[i], 4 * RG);
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
     }
+    for (int i = 0; i < kChunk; ++i)
+      mbar_init(&s_full[i], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&p_full[i], 8);
+      mbar_init(&p_free[i], 1);
+    }
+    mbar_init(&q_full, 8);
+    mbar_init(&s_free, 8);
+    mbar_init(&pv_done, 1);
+    mbar_init(&o_free, 8);
     fence_mbar_init();
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
   }
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
   __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_s = tmem_slot, tmem_o = tmem_slot + Cfg::kTmemO;
 
-  const Fp8AttnParams& a = p.a;
-  Walk<MROWS> walk;
-  walk.start(p);
-  if (walk.at >= walk.end)
-    return;
-
-  if (warp == 4 * RG) {
-    // ---------------------------------------------------------------- producer
-    if (lane == 0) {
-      tma_prefetch_desc(&tmap_k);
-      tma_prefetch_desc(&tmap_v);
-    }
+  if (warp == 0) {
+    // ---------------------------------------------------------------- producer: K tiles of a chunk, then its V tiles
     int n = 0;
-    bool ok = true;
-    while (ok && walk.next(p)) {
+    while (walk.next(p)) {
       const SeqWork& w = walk.w;
       if (w.hi <= w.lo)
         continue;
-      for (int u = walk.first; ok && u < walk.last; ++u, ++n) {
-        const int stage = n % kRing;
-        if (n >= kRing && !mbar_wait(&empty[stage], (n / kRing - 1) & 1, &abort_flag, p.status_word, 401)) {
-          ok = false;
-          break;
-        }
-        const int key = w.lo + u * kUnitKeys;
-        const int live = min(kUnitKeys, w.hi - key);
-        uint8_t* ks = k_ring + stage * kKvBytes;
-        uint8_t* vs = v_ring + stage * kKvBytes;
-        if (lane == 0) {
-          const int boxes = (live + 31) / 32;
-          mbar_arrive_expect_tx(&full[stage], boxes * 2 * 32 * kD);
-          for (int i = 0; i < boxes; ++i) {
-            tma_load_2d(ks + i * 32 * kD, &tmap_k, &full[stage], walk.hk * kD, static_cast<int>(w.k0) + key + 32 * i);
-            tma_load_2d(vs + i * 32 * kD, &tmap_v, &full[stage], walk.hk * kD, static_cast<int>(w.v0) + key + 32 * i);
+      const int2 keys = part_keys(walk);
+      const int tiles = (keys.y - keys.x + kUnitKeys - 1) / kUnitKeys;
+      for (int c0 = 0; c0 < tiles; c0 += kChunk) {
+        const int nt = min(kChunk, tiles - c0);
+        for (int i = 0; i < 2 * nt; ++i, ++n) {
+          const int slot = n % kRing;
+          if (n >= kRing)
+            mbar_wait(&empty[slot], (n / kRing - 1) & 1, &abort_flag, p.status_word, 401);
+          if (lane == 0) {
+            const CUtensorMap* map = i < nt ? &tmap_k : &tmap_v;
+            const int key = keys.x + (c0 + (i < nt ? i : i - nt)) * kUnitKeys;
+            const int row = static_cast<int>(i < nt ? w.k0 : w.v0) + key;
+            const int boxes = min(4, (keys.y - key + 31) / 32);      // no box of keys that do not belong to the part
+            mbar_arrive_expect_tx(&full[slot], boxes * 32 * kD);
+            for (int j = 0; j < boxes; ++j)
+              tma_load_2d(ring + slot * kTileBytes + j * 32 * kD, map, &full[slot], walk.hk * kD, row + 32 * j);
           }
+          __syncwarp();
         }
-        float* sc = scales + stage * 2 * kUnitKeys;
-        const float* ksrc = a.k_scales + (w.k0 + key) * a.Hkv + walk.hk;
-        const float* vsrc = a.v_scales + (w.v0 + key) * a.Hkv + walk.hk;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int j = lane + 32 * i;
-          if (j < live) {
-            cp_async4(sc + j, ksrc + static_cast<int64_t>(j) * a.Hkv);
-            cp_async4(sc + kUnitKeys + j, vsrc + static_cast<int64_t>(j) * a.Hkv);
-          }
-        }
-        cp_async_arrive(&full[stage]);
       }
     }
-    // a CTA may not end with copies on their way, also when a wait of its consumers has given up
+    // a CTA may not end with copies on their way, also when a wait of another warp has given up
     for (int i = max(0, n - kRing); i < n; ++i)
       mbar_wait(&full[i % kRing], (i / kRing) & 1, &abort_flag, p.status_word, 402);
-    return;
-  }
-
-  // ------------------------------------------------------------------ consumers
-  const int g = lane >> 2, c = lane & 3;
-  const int group = a.H / a.Hkv;
-  const int rg = warp >> 2, slice = warp & 3;       // row group and 32 keys of a unit
-  int n = 0;
-  while (walk.next(p)) {
-    const SeqWork w = walk.w;
-    const int hk = walk.hk;
-    // queries as A fragments
-    uint32_t qf[8][4];
-    float rf[2], slope[2];
-    int pos[2], lo[2], hi[2];
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer
+    constexpr uint32_t idesc_hi = umma_idesc_f8(128, RN, 0, 0, 0, 0), idesc_lo = umma_idesc_f8(128, RN, 0, 1, 0, 0);
+    constexpr uint32_t idesc_pv = umma_idesc_f8(128, 2 * RN, 0, 0, 1, 1);
+    const uint32_t q_addr = smem_u32(q_smem);
+    int n = 0, n_p = 0, n_chunk = 0, n_part = 0;
+    while (walk.next(p)) {
+      const SeqWork& w = walk.w;
+      if (w.hi <= w.lo)
+        continue;
+      const int2 keys = part_keys(walk);
+      const int tiles = (keys.y - keys.x + kUnitKeys - 1) / kUnitKeys;
+      mbar_wait(&q_full, n_part & 1, &abort_flag, p.status_word, 403);
+      for (int c0 = 0; c0 < tiles; c0 += kChunk, ++n_chunk) {
+        const int nt = min(kChunk, tiles - c0);
+        if (n_chunk > 0)
+          mbar_wait(&s_free, (n_chunk - 1) & 1, &abort_flag, p.status_word, 404);
+        for (int i = 0; i < nt; ++i, ++n) {
+          const int slot = n % kRing;
+          mbar_wait(&full[slot], (n / kRing) & 1, &abort_flag, p.status_word, 405);
+          tc_fence_after_sync();
+          if (lane == 0) {
+            const uint64_t a_desc = umma_smem_desc_sw128(smem_u32(ring + slot * kTileBytes), 16, 1024);
+            const uint64_t hi_desc = umma_smem_desc_sw128(q_addr, 16, 1024);
+            const uint64_t lo_desc = umma_smem_desc_sw128(q_addr + Cfg::kQBytes, 16, 1024);
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int t = walk.tile * MROWS + rg * 16 + r * 8 + g;      // row of the sequence's (listed row, head) pairs
-        const int i = t / group, h = hk * group + t - i * group;
-        int row = -1;
-        if (t < w.rows) {
-          row = __ldg(a.idx + w.row0 + i);
-          if (row >= a.total_q)
-            row = -1;
-        }
-        uint4 x[4] = {};
-        if (row >= 0) {
-          const uint4* src = reinterpret_cast<const uint4*>(a.q + row * a.ldq + h * kD) + c * 4;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            x[j] = __ldg(src + j);
-        }
-        lo[r] = 0;
-        hi[r] = row >= 0 ? w.hi : 0;
-        pos[r] = 0;
-        slope[r] = 0.f;
-        if (!PLAIN && row >= 0) {
-          pos[r] = __ldg(a.cu_k + w.b + 1) - __ldg(a.cu_k + w.b) - (__ldg(a.cu_q + w.b + 1) - row);
-          if (a.slopes)
-            slope[r] = __ldg(a.slopes + h) * kLog2e;
-          if (a.ranges) {
-            const int2 v = __ldg(a.ranges + row);
-            lo[r] = v.x;
-            hi[r] = min(v.y, w.hi);
+            for (int kk = 0; kk < 4; ++kk) {      // 32 head dimensions = 32 bytes a step
+              umma_ss_f8(tmem_s + i * RN, a_desc + 2 * kk, hi_desc + 2 * kk, idesc_hi, kk != 0 ? 1u : 0u);
+              umma_ss_f8(tmem_s + i * RN, a_desc + 2 * kk, lo_desc + 2 * kk, idesc_lo, 1u);
+            }
+            umma_commit(&empty[slot]);
+            umma_commit(&s_full[i]);
           }
+          __syncwarp();
         }
-        float y[32];
+        for (int i = 0; i < nt; ++i, ++n, ++n_p) {
+          const int slot = n % kRing, buf = n_p & 1;
+          mbar_wait(&full[slot], (n / kRing) & 1, &abort_flag, p.status_word, 406);
+          mbar_wait(&p_full[buf], (n_p >> 1) & 1, &abort_flag, p.status_word, 407);
+          if (c0 == 0 && i == 0 && n_part > 0)
+            mbar_wait(&o_free, (n_part - 1) & 1, &abort_flag, p.status_word, 408);
+          tc_fence_after_sync();
+          if (lane == 0) {
+            const uint32_t v_addr = smem_u32(ring + slot * kTileBytes), p_addr = smem_u32(p_smem + buf * kTileBytes);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)        // 32 keys = 32 rows of 128 bytes a step
+              umma_ss_f8(tmem_o, umma_smem_desc_sw128(v_addr + kk * 4096, kTileBytes, 1024),
+                         umma_smem_desc_sw128(p_addr + kk * 4096, kTileBytes, 1024), idesc_pv, (c0 | i | kk) != 0 ? 1u : 0u);
+            umma_commit(&empty[slot]);
+            umma_commit(&p_free[buf]);
+            if (i == nt - 1)
+              umma_commit(&pv_done);
+          }
+          __syncwarp();
+        }
+      }
+      ++n_part;
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax over the keys, epilogue
+    const int half = (warp - 2) >> 2;              // rows HR * half ..
+    const int quarter = warp & 3;                  // tensor-memory lanes: keys (head dimensions) 32 * quarter ..
+    const int tid = threadIdx.x - 64;
+    const int kl = quarter * 32 + lane;            // key of a tile, or head dimension
+    const uint32_t t_lane = static_cast<uint32_t>(quarter * 32) << 16;
+    const int group = a.H / a.Hkv;
+    const int r0 = half * HR;
+    uint32_t s_phase = 0;                          // bit i: phase of s_full[i]
+    int n = 0, n_p = 0, n_chunk = 0;
+    while (walk.next(p)) {
+      const SeqWork w = walk.w;
+      const int hk = walk.hk;
+      if (w.hi <= w.lo) {                          // no keys: zeros
+        for (int r = r0; r < r0 + HR && walk.tile * RN + r < w.rows; ++r) {
+          const int t = walk.tile * RN + r, i = t / group;
+          a.out[((static_cast<int64_t>(w.row0) + i) * a.H + hk * group + t - i * group) * kD + kl] = __float2bfloat16_rn(0.f);
+        }
+        continue;
+      }
+      // queries to shared memory; eight threads a row
+      if (tid < RN * 8) {
+        const int r = tid >> 3, part = tid & 7;
+        const int t = walk.tile * RN + r, i = t / group, h = hk * group + t - i * group;
+        int row = t < w.rows ? __ldg(a.idx + w.row0 + i) : -1;
+        if (row >= a.total_q)
+          row = -1;
+        uint4 x0 = make_uint4(0u, 0u, 0u, 0u), x1 = x0;
+        if (row >= 0) {
+          const uint4* src = reinterpret_cast<const uint4*>(a.q + row * a.ldq + h * kD) + part * 2;
+          x0 = __ldg(src);
+          x1 = __ldg(src + 1);
+        }
+        float y[16];
+        bf16x8_to_float(x0, y);
+        bf16x8_to_float(x1, y + 8);
         uint32_t m = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          bf16x8_to_float(x[j], y + 8 * j);
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
+        for (int j = 0; j < 16; ++j)
           m = max(m, __float_as_uint(y[j]) & 0x7fffffffu);
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const float2 qs = query_scales(m);
-        rf[r] = qs.y * a.scale * (PLAIN ? kLog2e : 1.f);
+        const uint32_t scale = fp8_scale_bits(fp8_amax8(m));
+        const float inv = fp8_inverse(scale);
+        uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int st = 0; st < 8; ++st) {
-          qf[st][r] = pack_half2(y[4 * st] * qs.x, y[4 * st + 1] * qs.x);
-          qf[st][2 + r] = pack_half2(y[4 * st + 2] * qs.x, y[4 * st + 3] * qs.x);
+        for (int j = 0; j < 4; ++j) {
+          float z[4], e[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            z[k] = scale >= 0x7f800000u ? 0.f : y[4 * j + k] * inv;
+          hi[j] = fp8_pack2(z[0], z[1]) | fp8_pack2(z[2], z[3]) << 16;
+          const float2 u = fp8_to_float2(hi[j] & 0xffffu), v = fp8_to_float2(hi[j] >> 16);
+          e[0] = z[0] - u.x, e[1] = z[1] - u.y, e[2] = z[2] - v.x, e[3] = z[3] - v.y;
+          lo[j] = fp8_pack2_e5m2(e[0], e[1]) | fp8_pack2_e5m2(e[2], e[3]) << 16;
         }
-      }
-    float o[16][4], mx[2], l[2];
-#pragma unroll
-      for (int nb = 0; nb < 16; ++nb)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          o[nb][j] = 0.f;
-      mx[0] = mx[1] = -INFINITY;
-      l[0] = l[1] = 0.f;
-
-    if (w.hi > w.lo) {
-      for (int u = walk.first; u < walk.last; ++u, ++n) {
-        const int stage = n % kRing;
-        if (!mbar_wait(&full[stage], (n / kRing) & 1, &abort_flag, p.status_word, 403))
-          break;
-        const int key = w.lo + u * kUnitKeys + slice * 32;
-        const int live = w.hi - key;                 // keys of this warp's 32 that exist
-        if (live > 0) {
-          const uint8_t* kt = k_ring + stage * kKvBytes + slice * 32 * kD;
-          const uint8_t* vt = v_ring + stage * kKvBytes + slice * 32 * kD;
-          const float* sc = scales + stage * 2 * kUnitKeys + slice * 32;
-          float s[4][4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int r = 8 * j + g;
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const uint4 x = *reinterpret_cast<const uint4*>(kt + r * kD + (((2 * c + half) ^ (r & 7)) << 4));
-              const uint32_t wd[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint32_t b0 = fp8_to_half2(wd[i] & 0xffffu), b1 = fp8_to_half2(wd[i] >> 16);
-                  const uint32_t* q4 = qf[half * 4 + i];
-                  mma_f16(s[j], q4[0], q4[1], q4[2], q4[3], b0, b1);
-              }
+        uint8_t* dst = q_smem + r * kD + ((part ^ (r & 7)) << 4);
+        *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(dst + Cfg::kQBytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        if (part == 0) {
+          s_rf[r] = __uint_as_float(scale);        // NaN: a query that is not finite
+          // output row, negative: none; the lowest bit: whether the row exists in q
+          s_out[r] = t < w.rows ? ((static_cast<int64_t>(w.row0) + i) * a.H + h) * 2 + (row >= 0) : -1;
+          if (!PLAIN) {
+            s_pos[r] = __ldg(a.cu_k + w.b + 1) - __ldg(a.cu_k + w.b) - (__ldg(a.cu_q + w.b + 1) - row);
+            s_slope[r] = a.slopes && row >= 0 ? __ldg(a.slopes + h) * kLog2e : 0.f;
+            int2 v = make_int2(0, row >= 0 ? w.hi : 0);
+            if (a.ranges && row >= 0) {
+              v = __ldg(a.ranges + row);
+              v.y = min(v.y, w.hi);
             }
-          }
-          // scores, their maxima, weights
-          uint32_t pf[4][2];
-            float inv[4][2];
-            float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float2 ks = *reinterpret_cast<const float2*>(sc + 8 * j + 2 * c);
-              const float2 vs = *reinterpret_cast<const float2*>(sc + kUnitKeys + 8 * j + 2 * c);
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const float kscale = e ? ks.y : ks.x;
-                const float ex = value_exponent(e ? vs.y : vs.x);
-                inv[j][e] = __uint_as_float(static_cast<uint32_t>(127 - static_cast<int>(ex)) << 23);
-                const int at = key + 8 * j + 2 * c + e;
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                  float t;
-                  if (PLAIN) {
-                    t = s[j][2 * r + e] * (kscale * rf[r]) + ex;
-                    t = at < hi[r] ? t : -INFINITY;
-                  } else {
-                    t = score_log2(s[j][2 * r + e] * (kscale * rf[r]), a.cap) - slope[r] * static_cast<float>(abs(pos[r] - at)) + ex;
-                    t = at >= lo[r] && at < hi[r] ? t : -INFINITY;
-                  }
-                  s[j][2 * r + e] = t;
-                  top[r] = fmaxf(top[r], t);
-                }
-              }
-            }
-            float base[2], old[2];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-              top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-              top[r] = fmaxf(top[r], mx[r]);
-              base[r] = top[r] == -INFINITY ? 0.f : top[r];
-              old[r] = exp2f(mx[r] - base[r]);
-            }
-            if (__any_sync(0xffffffffu, top[0] > mx[0] || top[1] > mx[1])) {
-#pragma unroll
-              for (int nb = 0; nb < 16; ++nb) {
-                o[nb][0] *= old[0];
-                o[nb][1] *= old[0];
-                o[nb][2] *= old[1];
-                o[nb][3] *= old[1];
-              }
-              l[0] *= old[0];
-              l[1] *= old[1];
-              mx[0] = top[0];
-              mx[1] = top[1];
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                float p0 = exp2f(s[j][2 * r] - base[r]), p1 = exp2f(s[j][2 * r + 1] - base[r]);
-                const int at = key + 8 * j + 2 * c;
-                // the value scale of a key that does not exist is whatever the ring held: its weight is zero all the same
-                l[r] += (at < w.hi ? p0 * inv[j][0] : 0.f) + (at + 1 < w.hi ? p1 * inv[j][1] : 0.f);
-                pf[j][r] = pack_half2(p0, p1);
-              }
-          // O += P V
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            uint4 v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int r = 16 * t + 2 * c + (i & 1) + (i >> 1) * 8;
-              v[i] = *reinterpret_cast<const uint4*>(vt + r * kD + ((g ^ (r & 7)) << 4));
-              if (live < 32 && r >= live)
-                v[i] = make_uint4(0u, 0u, 0u, 0u);      // rows behind the last key may hold any byte
-            }
-            const uint32_t* v0 = &v[0].x;
-            const uint32_t* v1 = &v[1].x;
-            const uint32_t* v2 = &v[2].x;
-            const uint32_t* v3 = &v[3].x;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t a01 = __byte_perm(v0[i], v1[i], 0x5140), a23 = __byte_perm(v0[i], v1[i], 0x7362);
-              const uint32_t b01 = __byte_perm(v2[i], v3[i], 0x5140), b23 = __byte_perm(v2[i], v3[i], 0x7362);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t x0 = e < 2 ? a01 : a23, x1 = e < 2 ? b01 : b23;
-                const uint32_t h0 = fp8_to_half2(e & 1 ? x0 >> 16 : x0 & 0xffffu);
-                const uint32_t h1 = fp8_to_half2(e & 1 ? x1 >> 16 : x1 & 0xffffu);
-                  mma_f16(o[4 * i + e], pf[2 * t][0], pf[2 * t][1], pf[2 * t + 1][0], pf[2 * t + 1][1], h0, h1);
-              }
-            }
+            s_range[r] = v;
           }
         }
-        __syncwarp();
-        if (lane == 0)
-          mbar_arrive(&empty[stage]);
+        fence_proxy_async_smem();
       }
-    }
+      warp_arrive(&q_full);
+      softmax_sync();
 
-    // ---------------------------------------------------------------- join the four warps of a row group
+      const int2 keys = part_keys(walk);
+      const int tiles = (keys.y - keys.x + kUnitKeys - 1) / kUnitKeys;
+      const float* k_scale = a.k_scales + w.k0 * a.Hkv + hk;
+      const float* v_scale = a.v_scales + w.v0 * a.Hkv + hk;
+      float top[HR], l[HR];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      if (c == 0)
-        s_ml[warp][r * 8 + g] = make_float2(mx[r], l[r]);
-    }
-    consumers_sync<RG>();
+      for (int r = 0; r < HR; ++r) {
+        top[r] = -INFINITY;
+        l[r] = 0.f;
+      }
+      for (int c0 = 0; c0 < tiles; c0 += kChunk, ++n_chunk) {
+        const int nt = min(kChunk, tiles - c0);
+        const int key0 = keys.x + c0 * kUnitKeys + kl;
+        // scores of all tiles of the chunk, their maxima
+        float mx[HR];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = r * 8 + g;
-      float top = s_ml[4 * rg][row].x;
+        for (int r = 0; r < HR; ++r)
+          mx[r] = -INFINITY;
+        {
+          float rf[HR];
+          lds_row(rf, s_rf + r0);
+          float ks_next = 0.f, vs_next = 1.f;
+          if (key0 < keys.y) {
+            ks_next = __ldg(k_scale + static_cast<int64_t>(key0) * a.Hkv);
+            vs_next = __ldg(v_scale + static_cast<int64_t>(key0) * a.Hkv);
+          }
+          for (int i = 0; i < nt; ++i) {
+            const int at = key0 + i * kUnitKeys;
+            const bool there = at < keys.y;
+            const float kk = ks_next * a.scale * (PLAIN ? kLog2e : 1.f), ex = value_exponent(vs_next);
+            if (at + kUnitKeys < keys.y) {
+              ks_next = __ldg(k_scale + static_cast<int64_t>(at + kUnitKeys) * a.Hkv);
+              vs_next = __ldg(v_scale + static_cast<int64_t>(at + kUnitKeys) * a.Hkv);
+            }
+            mbar_wait(&s_full[i], (s_phase >> i) & 1, &abort_flag, p.status_word, 409);
+            tc_fence_after_sync();
+            uint32_t s[HR];
+            tmem_ld(tmem_s + t_lane + i * RN + r0, s);
+            tmem_ld_wait();
 #pragma unroll
-      for (int i = 1; i < 4; ++i)
-        top = fmaxf(top, s_ml[4 * rg + i][row].x);
-      const float mul = exp2f(mx[r] - (top == -INFINITY ? 0.f : top));
-      float* dst = merge + (warp * 16 + row) * kD;
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int chunk = 8 * c + 4 * e + i;
-          *reinterpret_cast<float4*>(dst + ((chunk ^ (c + 4 * (g & 1))) << 2)) =
-              make_float4(o[4 * i][2 * r + e] * mul, o[4 * i + 1][2 * r + e] * mul, o[4 * i + 2][2 * r + e] * mul,
-                          o[4 * i + 3][2 * r + e] * mul);
+            for (int r = 0; r < HR; ++r) {
+              float t = __uint_as_float(s[r]) * (kk * rf[r]);
+              if (PLAIN) {
+                t += ex;
+                t = there ? t : -INFINITY;
+              } else {
+                const int2 range = s_range[r0 + r];
+                t = score_log2(t, a.cap) - s_slope[r0 + r] * static_cast<float>(abs(s_pos[r0 + r] - at)) + ex;
+                t = there && at >= range.x && at < range.y ? t : -INFINITY;
+              }
+              s[r] = __float_as_uint(t);
+              mx[r] = fmaxf(mx[r], t);
+            }
+            tmem_st(tmem_s + t_lane + i * RN + r0, s);
+          }
+          s_phase ^= (1u << nt) - 1;
         }
-    }
-    consumers_sync<RG>();
-    // a thread's share of the result: a row of the tile, four chunks of four values
-    const int orow = threadIdx.x >> 3, oc = (threadIdx.x & 7) * 4;
-    const float2* ml = &s_ml[4 * (orow >> 4)][orow & 15];
-    float top = ml[0].x;
+        tmem_st_wait();
+        {
+          const float v = reduce_lanes<HR, true>(mx);
+          if (lane % (32 / HR) == 0)
+            s_max[quarter][r0 + lane / (32 / HR)] = v;
+        }
+        softmax_sync();
+        bool grown = false;
+        float old[HR];
 #pragma unroll
-    for (int i = 1; i < 4; ++i)
-      top = fmaxf(top, ml[16 * i].x);
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-    float4 acc[4] = {};
+        for (int q4 = 0; q4 < 4; ++q4) {
+          float x[HR];
+          lds_row(x, s_max[q4] + r0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      sum += ml[16 * i].y * exp2f(ml[16 * i].x - base);
-      const float* src = merge + ((4 * (orow >> 4) + i) * 16 + (orow & 15)) * kD;
+          for (int r = 0; r < HR; ++r)
+            mx[r] = q4 == 0 ? fmaxf(x[r], top[r]) : fmaxf(mx[r], x[r]);
+        }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int chunk = oc + j;
-        const float4 x = *reinterpret_cast<const float4*>(src + ((chunk ^ ((chunk >> 3) + 4 * (orow & 1))) << 2));
-        acc[j].x += x.x;
-        acc[j].y += x.y;
-        acc[j].z += x.z;
-        acc[j].w += x.w;
+        for (int r = 0; r < HR; ++r) {
+          grown = grown || mx[r] > top[r];
+          old[r] = exp2f(top[r] - (mx[r] == -INFINITY ? 0.f : mx[r]));
+          top[r] = mx[r];
+          l[r] *= old[r];
+        }
+        if (c0 > 0)      // every phase is waited for, also where nothing is rescaled
+          mbar_wait(&pv_done, (n_chunk - 1) & 1, &abort_flag, p.status_word, 410);
+        if (c0 > 0 && grown) {      // the same rows in all four quarters
+          tc_fence_after_sync();
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint32_t o[HR];
+            tmem_ld(tmem_o + t_lane + j * RN + r0, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int r = 0; r < HR; ++r)
+              o[r] = __float_as_uint(__uint_as_float(o[r]) * old[r]);
+            tmem_st(tmem_o + t_lane + j * RN + r0, o);
+          }
+          tmem_st_wait();
+        }
+        // weights
+        for (int i = 0; i < nt; ++i, ++n_p) {
+          const int at = key0 + i * kUnitKeys, buf = n_p & 1;
+          uint32_t s[HR];
+          tmem_ld(tmem_s + t_lane + i * RN + r0, s);
+          float inv = 0.f;
+          if (at < keys.y) {
+            const float ex = value_exponent(__ldg(v_scale + static_cast<int64_t>(at) * a.Hkv));
+            inv = ex == ex ? exp2f(-ex) : 1.f;      // the weight of a NaN is a NaN where the key is seen, else zero
+          }
+          tmem_ld_wait();
+          if (n_p >= 2)
+            mbar_wait(&p_free[buf], ((n_p >> 1) - 1) & 1, &abort_flag, p.status_word, 411);
+          uint32_t hi[HR / 4], lo[HR / 4];
+#pragma unroll
+          for (int j = 0; j < HR / 4; ++j) {
+            float w4[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int r = 4 * j + k;
+              w4[k] = exp2f(__uint_as_float(s[r]) + (8.f - (top[r] == -INFINITY ? 0.f : top[r])));
+              l[r] += at < keys.y ? w4[k] * inv : 0.f;
+            }
+            hi[j] = fp8_pack2(w4[0], w4[1]) | fp8_pack2(w4[2], w4[3]) << 16;
+            const float2 u = fp8_to_float2(hi[j] & 0xffffu), v = fp8_to_float2(hi[j] >> 16);
+            lo[j] = fp8_pack2(16.f * w4[0] - 16.f * u.x, 16.f * w4[1] - 16.f * u.y) |
+                    fp8_pack2(16.f * w4[2] - 16.f * v.x, 16.f * w4[3] - 16.f * v.y) << 16;
+          }
+          // row kl of the slot: RN weights, then RN remainders, in 16-byte chunks that the swizzle permutes
+          uint8_t* dst = p_smem + buf * kTileBytes + kl * kD;
+          if constexpr (HR == 16) {
+            *reinterpret_cast<uint4*>(dst + ((half ^ (kl & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(dst + (((2 + half) ^ (kl & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          } else {
+            *reinterpret_cast<uint2*>(dst + ((0 ^ (kl & 7)) << 4) + 8 * half) = make_uint2(hi[0], hi[1]);
+            *reinterpret_cast<uint2*>(dst + ((1 ^ (kl & 7)) << 4) + 8 * half) = make_uint2(lo[0], lo[1]);
+          }
+          if (keys.y - (key0 - kl) - i * kUnitKeys < kUnitKeys && half == 0) {
+            // rows behind the last key may hold any byte, a NaN times a weight of zero among them
+            const int use = n + nt + i;
+            mbar_wait(&full[use % kRing], (use / kRing) & 1, &abort_flag, p.status_word, 412);
+            if (at >= keys.y) {
+              uint4* v = reinterpret_cast<uint4*>(ring + (use % kRing) * kTileBytes + kl * kD);
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                v[j] = make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
+          tc_fence_before_sync();
+          fence_proxy_async_smem();
+          warp_arrive(&p_full[buf]);
+        }
+        warp_arrive(&s_free);
+        n += 2 * nt;
       }
-    }
-    const int owner = walk.cta_of(walk.tile_first);
-    const int parts = walk.last - walk.first == w.units ? 1 : walk.cta_of(walk.tile_first + w.units - 1) - owner + 1;
-    if (parts == 1) {
-      store_row(p, w, hk, walk.tile * MROWS + orow, oc, acc, sum, group);
-      consumers_sync<RG>();      // merge and s_ml are free again
-      continue;
-    }
-    // ---------------------------------------------------------------- join the parts of a tile that several CTAs hold
-    constexpr int kPart = MROWS * kD + 2 * MROWS;
-    {
-      float* part = p.parts + (2 * static_cast<int64_t>(blockIdx.x) + (walk.first == 0 ? 1 : 0)) * kPart;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<float4*>(part + orow * kD + (oc + j) * 4) = acc[j];
-      if (oc == 0) {
-        part[MROWS * kD + orow] = top;
-        part[MROWS * kD + MROWS + orow] = sum;
+
+      // ---------------------------------------------------------------- thread = head dimension kl of HR rows
+      {
+        const float v = reduce_lanes<HR, false>(l);
+        if (lane % (32 / HR) == 0)
+          s_sum[quarter][r0 + lane / (32 / HR)] = v;
       }
-    }
-    __threadfence();
-    consumers_sync<RG>();
-    if (threadIdx.x == 0) {
-      open_join(p.tickets + owner, p.launch_id);
-      joins = last_to_join(p.tickets + owner, parts) ? 1 : 0;
-    }
-    consumers_sync<RG>();
-    if (!joins)
-      continue;
-    __threadfence();
-    top = -INFINITY;
-    for (int i = 0; i < parts; ++i)
-      top = fmaxf(top, __ldcg(p.parts + (2 * static_cast<int64_t>(owner + i) + (i == 0)) * kPart + MROWS * kD + orow));
-    const float last_base = top == -INFINITY ? 0.f : top;
-    sum = 0.f;
+      softmax_sync();
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-    for (int i = 0; i < parts; ++i) {
-      const float* src = p.parts + (2 * static_cast<int64_t>(owner + i) + (i == 0)) * kPart;
-      const float mul = exp2f(__ldcg(src + MROWS * kD + orow) - last_base);
-      sum += __ldcg(src + MROWS * kD + MROWS + orow) * mul;
+      for (int q4 = 0; q4 < 4; ++q4) {
+        float x[HR];
+        lds_row(x, s_sum[q4] + r0);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(src + orow * kD) + oc + j);
-        acc[j].x += x.x * mul;
-        acc[j].y += x.y * mul;
-        acc[j].z += x.z * mul;
-        acc[j].w += x.w * mul;
+        for (int r = 0; r < HR; ++r)
+          l[r] = q4 == 0 ? x[r] : l[r] + x[r];
       }
+      mbar_wait(&pv_done, (n_chunk - 1) & 1, &abort_flag, p.status_word, 413);
+      tc_fence_after_sync();
+      float o[HR];
+      {
+        uint32_t u[HR], v[HR];
+        tmem_ld(tmem_o + t_lane + r0, u);
+        tmem_ld(tmem_o + t_lane + RN + r0, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int r = 0; r < HR; ++r)
+          o[r] = __uint_as_float(u[r]) + __uint_as_float(v[r]) * 0.0625f;
+      }
+      tc_fence_before_sync();
+      warp_arrive(&o_free);
+
+      bool store = walk.last - walk.first == w.units;
+      if (!store) {
+        const int owner = walk.first == 0 ? blockIdx.x : walk.cta_of(walk.tile_first);
+        const int parts = walk.cta_of(walk.tile_first + w.units - 1) - owner + 1;
+        // join the parts of a tile that several CTAs hold
+        constexpr int kPart = RN * kD + 2 * RN;
+        float* part = p.parts + (2 * static_cast<int64_t>(blockIdx.x) + (walk.first == 0 ? 1 : 0)) * kPart;
+#pragma unroll
+        for (int r = 0; r < HR; ++r)
+          part[(r0 + r) * kD + kl] = o[r];
+        if (kl == 0) {
+#pragma unroll
+          for (int r = 0; r < HR; ++r) {
+            part[RN * kD + r0 + r] = top[r];
+            part[RN * kD + RN + r0 + r] = l[r];
+          }
+        }
+        __threadfence();
+        softmax_sync();
+        if (tid == 0) {
+          open_join(p.tickets + owner, p.launch_id);
+          joins = last_to_join(p.tickets + owner, parts) ? 1 : 0;
+        }
+        softmax_sync();
+        store = joins;
+        if (store) {
+          __threadfence();
+          const float* first = p.parts + (2 * static_cast<int64_t>(owner) + 1) * kPart;
+          const float* rest = p.parts + 2 * static_cast<int64_t>(owner) * kPart;
+#pragma unroll
+          for (int r = 0; r < HR; ++r) {
+            top[r] = -INFINITY;
+            o[r] = l[r] = 0.f;
+          }
+          for (int i = 0; i < parts; ++i) {
+            const float* src = i == 0 ? first : rest + 2 * static_cast<int64_t>(i) * kPart;
+#pragma unroll
+            for (int r = 0; r < HR; ++r)
+              top[r] = fmaxf(top[r], __ldcg(src + RN * kD + r0 + r));
+          }
+          for (int i = 0; i < parts; ++i) {
+            const float* src = i == 0 ? first : rest + 2 * static_cast<int64_t>(i) * kPart;
+#pragma unroll
+            for (int r = 0; r < HR; ++r) {
+              const float mul = exp2f(__ldcg(src + RN * kD + r0 + r) - (top[r] == -INFINITY ? 0.f : top[r]));
+              l[r] += __ldcg(src + RN * kD + RN + r0 + r) * mul;
+              o[r] += __ldcg(src + (r0 + r) * kD + kl) * mul;
+            }
+          }
+        }
+      }
+      if (store) {
+#pragma unroll
+        for (int r = 0; r < HR; ++r) {
+          const int64_t at = s_out[r0 + r];
+          if (at >= 0)
+            a.out[(at >> 1) * kD + kl] = __float2bfloat16_rn(l[r] == 0.f || !(at & 1) ? 0.f : o[r] * __fdividef(1.f, l[r]));
+        }
+      }
+      softmax_sync();      // what describes the rows is free again
     }
-    store_row(p, w, hk, walk.tile * MROWS + orow, oc, acc, sum, group);
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_slot, kTmemCols);
   }
 }
 
@@ -695,20 +821,20 @@ size_t few_workspace(int batch, int ctas) {
   return few_parts_offset(batch, ctas) + 2ull * ctas * (32 * kD + 2 * 32) * sizeof(float);
 }
 
-template <int RG, bool PLAIN>
+template <int RN, bool PLAIN>
 int launch_few(const CUtensorMap& tk, const CUtensorMap& tv, const FewParams& p, int ctas, cudaStream_t s) {
   static bool set[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   dev = (dev < 0 || dev >= 64) ? 0 : dev;
   if (!set[dev]) {
-    if (cudaFuncSetAttribute(fp8_few_rows_kernel<RG, PLAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(FewCfg<RG>::kSmem)) != cudaSuccess)
+    if (cudaFuncSetAttribute(fp8_few_rows_kernel<RN, PLAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(FewCfg<RN>::kSmem)) != cudaSuccess)
       return set_error(DYLLM_ERR_CUDA, "attention_salient_rows_fp8: cudaFuncSetAttribute failed: %s",
                        cudaGetErrorString(cudaGetLastError()));
     set[dev] = true;
   }
-  DYLLM_LAUNCH((fp8_few_rows_kernel<RG, PLAIN>), RG == 1 ? ctas : ctas / 2, FewCfg<RG>::kThreads, FewCfg<RG>::kSmem, s, tk, tv, p);
+  DYLLM_LAUNCH((fp8_few_rows_kernel<RN, PLAIN>), ctas, kFewThreads, FewCfg<RN>::kSmem, s, tk, tv, p);
   return check_launch("attention_salient_rows_fp8");
 }
 
@@ -812,9 +938,9 @@ int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, co
   const bool plain = softcap == 0.f && !slopes && !key_ranges;
   const bool one = static_cast<int64_t>(max_rows_per_seq) * (num_heads / num_kv_heads) <= 16;
   if (one)
-    rc = plain ? launch_few<1, true>(tk, tv, f, ctas, st) : launch_few<1, false>(tk, tv, f, ctas, st);
+    rc = plain ? launch_few<16, true>(tk, tv, f, ctas, st) : launch_few<16, false>(tk, tv, f, ctas, st);
   else
-    rc = plain ? launch_few<2, true>(tk, tv, f, ctas, st) : launch_few<2, false>(tk, tv, f, ctas, st);
+    rc = plain ? launch_few<32, true>(tk, tv, f, ctas, st) : launch_few<32, false>(tk, tv, f, ctas, st);
   return rc;
 }
 

@@ -23,6 +23,12 @@ __device__ __forceinline__ uint32_t fp8_pack2(float lo, float hi) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(hi), "f"(lo));
   return d;
 }
+// The same in e5m2.
+__device__ __forceinline__ uint32_t fp8_pack2_e5m2(float lo, float hi) {
+  uint16_t d;
+  asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(d) : "f"(hi), "f"(lo));
+  return d;
+}
 // The two codes in the low 16 bits as two half-precision numbers (exact).
 __device__ __forceinline__ uint32_t fp8_to_half2(uint32_t codes) {
   uint32_t d;

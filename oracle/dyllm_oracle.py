@@ -452,12 +452,13 @@ def fp8_kv_cache_update(k_new, v_new, rows_k, positions, pos_idx, cos_sin, cu_k,
 
 
 def attention_rows_fp8(q, k, v, cu_q, cu_k, cu_rows, rows, scale=None, softcap=0.0, slopes=None, ranges=None):
-    """(out, sum of weight * |v|, largest scale * |q| . |k| + |bias|) in float64 of the listed rows; ``k``, ``v``: packed values
-    ``[total_k, kv_heads, 128]``.  The last two bound what rounding can do."""
+    """(out, sum of weight * |v|, largest scale * |q| . |k| + |bias|, keys * largest weight * max |v|) in float64 of the listed
+    rows; ``k``, ``v``: packed values ``[total_k, kv_heads, 128]``.  The last three bound what rounding can do."""
     q, k, v = q.double(), k.double(), v.double()
     H, Hkv = q.size(1), k.size(1)
     scale = q.size(2) ** -0.5 if scale is None else scale
-    out, mag, big = torch.zeros(len(rows), H, q.size(2)).double(), torch.zeros(len(rows), H, q.size(2)).double(), torch.zeros(len(rows), H).double()
+    out, mag = (torch.zeros(len(rows), H, q.size(2)).double() for _ in range(2))
+    big, floor = (torch.zeros(len(rows), H).double() for _ in range(2))
     for b in range(len(cu_q) - 1):
         length = int(cu_k[b + 1] - cu_k[b])
         kb, vb = k[int(cu_k[b]):int(cu_k[b + 1])], v[int(cu_k[b]):int(cu_k[b + 1])]
@@ -477,4 +478,5 @@ def attention_rows_fp8(q, k, v, cu_q, cu_k, cu_rows, rows, scale=None, softcap=0
                 p = torch.softmax(t - bias, 0)
                 out[i, h], mag[i, h] = p @ vb[lo:hi, g], p @ vb[lo:hi, g].abs()
                 big[i, h] = (abs(scale) * (kb[lo:hi, g].abs() @ q[r, h].abs()) + bias.abs()).max()
-    return out, mag, big
+                floor[i, h] = (hi - lo) * (p * vb[lo:hi, g].abs().amax(-1)).max()
+    return out, mag, big, floor

@@ -234,17 +234,24 @@ def _attend(b, heads, hkv, counts, mask=None, cap=0.0, slopes=False, scale=None,
     assert torch.equal(torch.nan_to_num(again, nan=-5.0), torch.nan_to_num(out, nan=-5.0))      # run to run the same bits
     k = orc.fp8_cache_read(kc, ks, b.k_starts, b.cu_k, b.ids)
     v = orc.fp8_cache_read(vc, vs, b.v_starts, b.cu_k, b.ids)
-    want, mag, big = orc.attention_rows_fp8(q, k, v, b.cu_q, b.cu_k, cu, rows, scale, cap, slope, ranges)
-    return out[:n].cpu().double(), want, mag, big, cap
+    want, mag, big, floor = orc.attention_rows_fp8(q, k, v, b.cu_q, b.cu_k, cu, rows, scale, cap, slope, ranges)
+    return out[:n].cpu().double(), want, mag, big, floor, cap
 
 
-def _check(got, want, mag, big, cap):
-    """Half a step of bf16 for the result; a weight is held in half precision (2^-11) against a sum of unrounded weights; the
-    score is a sum of 128 products in fp32 (2^-24 a term, 2^-17 in all), of queries in half precision next to their largest
-    (2^-25 of it for an element that is small), times a scale, capped and biased (a few 2^-24 of the cap and the bias): 2^-16 of
-    what it is made of, which moves weights and sum by as much, relatively; exponential and quotient: 2^-20."""
+def _check(got, want, mag, big, floor, cap):
+    """Half a step of bf16 for the result (2^-8).
+
+    A weight w <= 1 (its largest in the row is 1, the values' scales included) is e4m3(256 w) + e4m3(16 r) / 16 with the
+    remainder r: |r| <= 2^-4 * 256 w (half a step of e4m3), rounded by 2^-4 of itself, or by 2^-10 / 16 where 16 r is below the
+    normal numbers: off by at most 2^-8 w or 2^-22.  The first moves the result by 2^-8 of sum(weight * |v|); the second by 2^-22
+    of the largest weight for each key, times its codes, which are at most twice the largest of the heaviest key.  Or weights
+    in half precision: 2^-11 w or 2^-25.
+
+    The score is a sum of 128 products in fp32 (2^-24 a term, 2^-17 in all) of queries that are exact above 2^-18 of their row's
+    largest and off by 2^-26 of it below, times a scale, capped and biased (a few 2^-24 of the cap and the bias): 2^-16 of what
+    it is made of, which moves weights and sum by as much, relatively.  Exponential and quotient: 2^-20."""
     delta = 2.0 ** -16 * (big + cap).unsqueeze(-1)
-    tol = 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -20 + 2 * delta) * mag + 1e-30
+    tol = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -20 + 2 * delta) * mag + 2.0 ** -21 * floor.unsqueeze(-1) + 1e-30
     assert torch.equal(torch.isnan(got), torch.isnan(want))
     bad = (got - want).abs() > tol
     assert not bool(bad.any()), (int(bad.sum()), float(((got - want).abs() / tol).nan_to_num().max()))
@@ -297,12 +304,12 @@ def test_nan_of_unseen_keys_stays_unseen(cuda_device, counts):
         kc[k0 + 150], ks[k0 + 150] = 0.0, math.nan
         vc[v0 + 170], vs[v0 + 170] = 0.0, math.nan
 
-    got, want, mag, big, cap = _attend(Batch([200], [200], seed=2), 2, 2, counts, "window", edit=edit)
+    got, want, mag, big, floor, cap = _attend(Batch([200], [200], seed=2), 2, 2, counts, "window", edit=edit)
     bad = torch.isnan(got).any(-1).any(-1)
     assert bool(bad.any()) == bool(torch.isnan(want).any()) and not bool(bad.all())
     fine = ~torch.isnan(want)
     assert torch.equal(torch.isnan(got), ~fine)
-    _check(got.masked_fill(~fine, 0), want.masked_fill(~fine, 0), mag.nan_to_num(), big.nan_to_num(), cap)
+    _check(got.masked_fill(~fine, 0), want.masked_fill(~fine, 0), mag.nan_to_num(), big.nan_to_num(), floor.nan_to_num(), cap)
 
 
 @pytest.mark.parametrize("counts", [[4], [100]])
