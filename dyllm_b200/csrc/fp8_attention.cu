@@ -55,12 +55,9 @@ __device__ __forceinline__ KeyRange keys_of(const Fp8AttnParams& p, int b) {
   return r;
 }
 
-// s * log2(e) of one score, capped.
-__device__ __forceinline__ float score_log2(float s, float cap) {
-  if (cap > 0.f)      // tanh(x) = 1 - 2 / (1 + e^2x), absolute error a few 2^-24 (the hardware tanh has 2^-11)
-    s = cap - 2.f * cap * __fdividef(1.f, 1.f + exp2f(__fdividef(2.f * kLog2e * s, cap)));
-  return s * kLog2e;
-}
+// cap * tanh(s / cap) from z = 2 log2(e) s / cap: tanh(x) = 1 - 2 / (1 + e^2x), absolute error a few 2^-24 (the hardware tanh
+// has 2^-11).
+__device__ __forceinline__ float capped(float z, float cap) { return cap - 2.f * cap * __fdividef(1.f, 1.f + exp2f(z)); }
 
 // Exponent of a value's scale (a power of two by definition).
 __device__ __forceinline__ float value_exponent(float scale) {
@@ -91,19 +88,14 @@ __device__ __forceinline__ float value_exponent(float scale) {
 // warps, two per quarter of the keys, each with half of the rows; a TMA warp and an MMA warp.  Two CTAs per SM.
 // ----------------------------------------------------------------------------------------------
 constexpr int kUnitKeys = 128;
-constexpr int kRing = 4;                                     // slots of one K or V tile
-constexpr uint32_t kTileBytes = kUnitKeys * kD;
-constexpr int kFewThreads = 320;
-constexpr uint32_t kTmemCols = 256;
-template <int RN>
-struct FewCfg {
-  static constexpr int kHalf = RN / 2;                       // rows of a softmax warp
-  static constexpr int kChunk = RN == 16 ? 8 : 6;
-  static constexpr uint32_t kTmemO = kChunk * RN;            // columns of O^T behind those of S^T: RN of 256 w, RN of remainders
-  static constexpr uint32_t kQBytes = RN * kD;
-  static constexpr uint32_t kSmem = (kRing + 2) * kTileBytes + 2 * kQBytes + 1024;
-  static_assert(kTmemO + 2 * RN <= kTmemCols, "tensor memory of two CTAs per SM");
-};
+constexpr int kRows = 32, kGroup = 8;                        // rows of a tile, of a softmax warp
+constexpr int kChunk = 4;                                    // tiles whose scores are in registers at a time
+constexpr int kRing = 8;                                     // slots of one K or V tile
+constexpr int kParts = 4;                                    // slots of part descriptions
+constexpr uint32_t kTileBytes = kUnitKeys * kD, kQBytes = kRows * kD;
+constexpr int kSoftmaxWarps = 16, kFewThreads = 32 * (kSoftmaxWarps + 3);
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kFewSmem = (kRing + kChunk / 2) * kTileBytes + 4 * kQBytes + 2 * kChunk * 2 * kUnitKeys * sizeof(float) + 1024;
 
 struct FewParams {
   Fp8AttnParams a;
@@ -137,7 +129,7 @@ __device__ __forceinline__ bool last_to_join(unsigned long long* word, int parts
 struct SeqWork {
   int b, row0, rows, tiles, units;      // rows: (listed row, head of the group) pairs
   int lo, hi;                           // keys
-  int64_t k0, v0;
+  int k0, v0;                           // first rows in the caches
 };
 template <int MROWS>
 __device__ __forceinline__ SeqWork seq_work(const FewParams& p, int b) {
@@ -145,56 +137,80 @@ __device__ __forceinline__ SeqWork seq_work(const FewParams& p, int b) {
   w.b = b;
   if (b >= p.a.batch)
     return w;
-  w.row0 = min(__ldg(p.a.cu_sal + b), p.a.num_salient);
-  const int n = min(__ldg(p.a.cu_sal + b + 1), p.a.num_salient) - w.row0;
+  // all loads that do not depend on one another first: a CTA starts with this chain
+  const int s0 = __ldg(p.a.cu_sal + b), s1 = __ldg(p.a.cu_sal + b + 1);
+  const int2 span = p.spans ? __ldg(p.spans + b) : make_int2(0, 0);
+  const KeyRange kr = keys_of(p.a, b);
+  w.row0 = min(s0, p.a.num_salient);
+  const int n = min(s1, p.a.num_salient) - w.row0;
   if (n <= 0)
     return w;
   w.rows = n * (p.a.H / p.a.Hkv);
-  const KeyRange kr = keys_of(p.a, b);
-  w.k0 = kr.k0;
-  w.v0 = kr.v0;
+  w.k0 = static_cast<int>(kr.k0);
+  w.v0 = static_cast<int>(kr.v0);
   w.hi = kr.len;
   if (p.spans) {
-    const int2 s = __ldg(p.spans + b);
-    w.lo = s.x;
-    w.hi = s.y;
+    w.lo = span.x;
+    w.hi = span.y;
   }
   w.tiles = (w.rows + MROWS - 1) / MROWS;
   w.units = max(1, (w.hi - w.lo + kUnitKeys - 1) / kUnitKeys);
   return w;
 }
 
+// a / b of non-negative numbers; the 64-bit routine only where it is needed.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0)
+    return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+
 // Walks over the parts of tiles that a CTA's share of the units consists of.  Uniform over a warp.
+//
+// Shares are cut at total * i / ctas, but no part of a tile is shorter than kMinPart units: a cut nearer to an end of its
+// tile moves there.  (Joining the parts of a tile costs a CTA about 7 us, a unit 1 to 2.)
+constexpr int kMinPart = 4;
 template <int MROWS>
 struct Walk {
   SeqWork w;
-  int64_t total, left;                  // units: of the launch, of the share that are still to come
+  int64_t total, end;                   // units: of the launch, end of the share before its cut is moved
   int64_t tile_first;                   // first unit of the tile in the launch
   int hk, tile, first, last;            // the part: units [first, last) of the tile
-  int ctas;                             // CTAs that have a share
+  int ctas;                             // shares
   bool begun;
 
+  static __device__ __forceinline__ int moved(int cut, int units) {
+    if (cut >= kMinPart && units - cut >= kMinPart)
+      return cut;
+    return 2 * cut < units ? 0 : units;
+  }
   __device__ __forceinline__ void start(const FewParams& p) {
     const int lane = threadIdx.x & 31;
-    int64_t sum = 0;
+    int64_t sum = 0, tiles = 0;
+    SeqWork x;
     for (int base = 0; base < p.a.batch; base += 32) {
-      const SeqWork x = seq_work<MROWS>(p, base + lane);
+      x = seq_work<MROWS>(p, base + lane);
       sum += static_cast<int64_t>(x.tiles) * x.units;
+      tiles += x.tiles;
     }
 #pragma unroll
-    for (int s = 16; s; s >>= 1)
+    for (int s = 16; s; s >>= 1) {
       sum += __shfl_xor_sync(0xffffffffu, sum, s);
+      tiles += __shfl_xor_sync(0xffffffffu, tiles, s);
+    }
     total = sum * p.a.Hkv;
-    ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total));      // no share is empty
-    left = 0;
+    ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), max(tiles * p.a.Hkv, total / kMinPart)));
+    end = tile_first = 0;
+    first = 0;
     begun = false;
     if (static_cast<int>(blockIdx.x) >= ctas)
       return;
     const int64_t at = share(blockIdx.x);
-    left = share(blockIdx.x + 1) - at;
+    end = share(blockIdx.x + 1);
     int64_t before = 0;
     for (int base = 0;; base += 32) {
-      const SeqWork x = seq_work<MROWS>(p, base + lane);
+      if (p.a.batch > 32)
+        x = seq_work<MROWS>(p, base + lane);
       const int64_t mine = static_cast<int64_t>(x.tiles) * x.units * p.a.Hkv;
       int64_t scan = mine;
 #pragma unroll
@@ -212,19 +228,22 @@ struct Walk {
       }
       before += __shfl_sync(0xffffffffu, scan, 31);
     }
-    const int64_t t = (at - before) / w.units;
-    first = static_cast<int>(at - before - t * w.units);
-    tile_first = at - first;
-    hk = static_cast<int>(t / w.tiles);
+    const int64_t t = quotient(at - before, w.units);
+    const int cut = static_cast<int>(at - before - t * w.units);
+    tile_first = at - cut;
+    hk = static_cast<int>(quotient(t, w.tiles));
     tile = static_cast<int>(t - static_cast<int64_t>(hk) * w.tiles);
+    first = moved(cut, w.units);
   }
   // The next part, false at the end of the share.
   __device__ __forceinline__ bool next(const FewParams& p) {
-    if (left == 0)
+    if (tile_first >= end)
       return false;
-    if (begun) {
+    if (begun || first == w.units) {
       first = 0;
       tile_first += w.units;
+      if (tile_first >= end)
+        return false;
       if (++tile == w.tiles) {
         tile = 0;
         if (++hk == p.a.Hkv) {
@@ -236,13 +255,18 @@ struct Walk {
       }
     }
     begun = true;
-    last = static_cast<int>(min(static_cast<int64_t>(w.units), first + left));
-    left -= last - first;
-    return true;
+    last = tile_first + w.units <= end ? w.units : moved(static_cast<int>(end - tile_first), w.units);
+    return last > first;
   }
-  // First unit of a CTA's share, and the CTA whose share holds unit u.
-  __device__ __forceinline__ int64_t share(int64_t cta) const { return total * cta / ctas; }
-  __device__ __forceinline__ int cta_of(int64_t u) const { return static_cast<int>(((u + 1) * ctas - 1) / total); }
+  // First unit of a share before its cut is moved; CTA that holds the first part of the tile; number of its parts.
+  __device__ __forceinline__ int64_t share(int64_t cta) const { return quotient(total * cta, ctas); }
+  __device__ __forceinline__ int first_cut() const {
+    return static_cast<int>(quotient((tile_first + kMinPart) * ctas + total - 1, total));
+  }
+  __device__ __forceinline__ int owner() const { return first_cut() - 1; }
+  __device__ __forceinline__ int parts() const {
+    return static_cast<int>(quotient((tile_first + w.units - kMinPart + 1) * ctas + total - 1, total)) - first_cut() + 1;
+  }
 };
 
 // One arrival for the warp, after what all of its lanes have done (an arrival per lane is a shared-memory atomic each).
@@ -251,13 +275,24 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
   if ((threadIdx.x & 31) == 0)
     mbar_arrive(bar);
 }
-__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
 
-// Maximum or sum of each of N = 8 or 16 values over the lanes of a warp: lane l gets that of value l / (32 / N).
-template <int N, bool MAX>
+__device__ __forceinline__ void group_sync(int group) { asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory"); }
+__device__ __forceinline__ float warp_max(float x) {
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// Sum of each of N = 8 or 16 values over the lanes of a warp: lane l gets that of value l / (32 / N).
+template <int N>
 __device__ __forceinline__ float reduce_lanes(const float (&v)[N]) {
   const int lane = threadIdx.x & 31;
-  auto join = [](float x, float y) { return MAX ? fmaxf(x, y) : x + y; };
   float x[N];
 #pragma unroll
   for (int i = 0; i < N; ++i)
@@ -270,29 +305,15 @@ __device__ __forceinline__ float reduce_lanes(const float (&v)[N]) {
     for (int i = 0; i < N / 2; ++i)
       if (i < n) {
         const float keep = up ? x[i + n] : x[i], give = up ? x[i] : x[i + n];
-        x[i] = join(keep, __shfl_xor_sync(0xffffffffu, give, bit));
+        x[i] = keep + __shfl_xor_sync(0xffffffffu, give, bit);
       }
   }
 #pragma unroll
   for (int b = 16 / N; b >= 1; b >>= 1)
-    x[0] = join(x[0], __shfl_xor_sync(0xffffffffu, x[0], b));
+    x[0] += __shfl_xor_sync(0xffffffffu, x[0], b);
   return x[0];
 }
 
-template <int N>
-__device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&r)[N]) {
-  if constexpr (N == 16)
-    tmem_ld_32x16(addr, r);
-  else
-    tmem_ld_32x8(addr, r);
-}
-template <int N>
-__device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&r)[N]) {
-  if constexpr (N == 16)
-    tmem_st_32x16(addr, r);
-  else
-    tmem_st_32x8(addr, r);
-}
 // N consecutive floats of shared memory, 16-byte aligned, the same for all lanes
 template <int N>
 __device__ __forceinline__ void lds_row(float (&x)[N], const float* src) {
@@ -306,37 +327,239 @@ __device__ __forceinline__ void lds_row(float (&x)[N], const float* src) {
   }
 }
 
-// Keys of a part: [begin, end), in tiles from begin on.
-template <int RN>
-__device__ __forceinline__ int2 part_keys(const Walk<RN>& walk) {
-  const int begin = walk.w.lo + walk.first * kUnitKeys;
-  return make_int2(begin, min(walk.w.hi, walk.w.lo + walk.last * kUnitKeys));
+// One step of a product of 8-bit tiles with rows of 128 bytes (128-byte swizzle, groups of 8 rows 1024 bytes apart) at these
+// shared-memory addresses.  Only the low words of the descriptors vary: an issue costs few instructions.
+__device__ __forceinline__ void umma_tile(uint32_t d_tmem, uint32_t a_addr, uint32_t b_addr, uint32_t idesc, uint32_t accumulate) {
+  constexpr uint32_t high = (1024u >> 4) | (1u << 14) | (2u << 29);      // stride, version, swizzle
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      ".reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %5};\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, p;\n\t"
+      "}\n" ::"r"(d_tmem),
+      "r"((a_addr >> 4) | (1u << 16)), "r"((b_addr >> 4) | (1u << 16)), "r"(idesc), "r"(accumulate), "n"(high)
+      : "memory");
 }
 
-template <int RN, bool PLAIN>
-__global__ void __launch_bounds__(kFewThreads, 2)
+// A value that all lanes share, in a register of the uniform datapath: what depends on it alone (loop counters, descriptors)
+// stays there, and an MMA issues every 33 cycles (its A operand's shared-memory read) instead of every 90.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __reduce_max_sync(0xffffffffu, x); }
+
+constexpr float kNothing = -1.0e30f;      // maximum of no scores (finite: it takes part in differences)
+
+// Four weights (times 256) as codes and the codes of 16 times what they leave.  By way of half precision (2^-11).
+__device__ __forceinline__ void split_weights(const float (&w)[4], uint32_t& hi, uint32_t& lo) {
+  uint32_t h[2], l[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const __half2 x = __floats2half2_rn(w[2 * i], w[2 * i + 1]);
+    h[i] = fp8_pack_half2(*reinterpret_cast<const uint32_t*>(&x));
+    const uint32_t back = fp8_to_half2(h[i]);
+    const __half2 rest = __hmul2(__hsub2(x, *reinterpret_cast<const __half2*>(&back)), __float2half2_rn(16.f));
+    l[i] = fp8_pack_half2(*reinterpret_cast<const uint32_t*>(&rest));
+  }
+  hi = h[0] | h[1] << 16;
+  lo = l[0] | l[1] << 16;
+}
+
+// A part of a tile as the scheduler hands it to the other warps.
+struct PartInfo {
+  int begin, end;              // keys; end < 0: the share is done
+  int owner, parts, slot;      // several CTAs hold the tile (parts > 1): the first of them, how many, this CTA's slot
+  int b, hk, row0, rows, t0;   // sequence, key head, the sequence's first listed row, its (row, head) pairs, the tile's first
+  int k0, v0, len;             // the sequence's first rows in the caches, its keys
+};
+
+// What a tile's rows are to the softmax warps.
+struct RowInfo {
+  int out;                     // output row, -1: none
+  float fix;                   // 1; 0: the row does not exist in q; NaN: the query is not finite
+  float slope;                 // times log2(e)
+  int pos, lo, hi;             // the row's place in its sequence, the keys that it sees
+};
+
+// Joins the parts of a tile that several CTAs hold: every CTA leaves its part in the workspace, the last one to do so adds them
+// up in their order (true: for the caller to store).  Rows r0 .. r0 + 7, head dimension kl of a thread.
+__device__ __forceinline__ bool join_parts(const FewParams& p, const PartInfo& part, float (&top)[kGroup], float (&l)[kGroup],
+                                           float (&o)[kGroup], int r0, int kl, int tid, int* joins) {
+  constexpr int kPart = kRows * kD + 2 * kRows;
+  float* mine = p.parts + static_cast<int64_t>(part.slot) * kPart;
+#pragma unroll
+  for (int r = 0; r < kGroup; ++r)
+    mine[(r0 + r) * kD + kl] = o[r];
+  if (kl == 0) {
+#pragma unroll
+    for (int r = 0; r < kGroup; ++r) {
+      mine[kRows * kD + r0 + r] = top[r];
+      mine[kRows * kD + kRows + r0 + r] = l[r];
+    }
+  }
+  const int owner = part.owner, parts = part.parts;
+  __threadfence();
+  softmax_sync();
+  if (tid == 0) {
+    open_join(p.tickets + owner, p.launch_id);
+    *joins = last_to_join(p.tickets + owner, parts) ? 1 : 0;
+  }
+  softmax_sync();
+  if (!*joins)
+    return false;
+  __threadfence();
+  const float* first = p.parts + (2 * static_cast<int64_t>(owner) + 1) * kPart;
+  const float* rest = p.parts + 2 * static_cast<int64_t>(owner) * kPart;
+#pragma unroll
+  for (int r = 0; r < kGroup; ++r) {
+    top[r] = kNothing;
+    o[r] = l[r] = 0.f;
+  }
+  for (int i = 0; i < parts; ++i) {
+    const float* src = i == 0 ? first : rest + 2 * static_cast<int64_t>(i) * kPart;
+#pragma unroll
+    for (int r = 0; r < kGroup; ++r)
+      top[r] = fmaxf(top[r], __ldcg(src + kRows * kD + r0 + r));
+  }
+#pragma unroll 2
+  for (int i = 0; i < parts; ++i) {
+    const float* src = i == 0 ? first : rest + 2 * static_cast<int64_t>(i) * kPart;
+#pragma unroll
+    for (int r = 0; r < kGroup; ++r) {
+      const float mul = exp2f(__ldcg(src + kRows * kD + r0 + r) - top[r]);
+      l[r] += __ldcg(src + kRows * kD + kRows + r0 + r) * mul;
+      o[r] += __ldcg(src + (r0 + r) * kD + kl) * mul;
+    }
+  }
+  return true;
+}
+
+// The query rows of a tile on their way to shared memory: eight threads a row (the first 256 softmax threads), 16 elements each.
+struct QueryLoad {
+  uint4 x0, x1;
+  int row, head, t;
+  __device__ __forceinline__ void index(const Fp8AttnParams& a, const PartInfo& w, int tid) {
+    const int group = a.H / a.Hkv;
+    row = -1;
+    t = w.t0 + (tid >> 3);
+    const int i = t / group;
+    head = w.hk * group + t - i * group;
+    if (t < w.rows) {
+      row = __ldg(a.idx + w.row0 + i);
+      row = row >= a.total_q ? -1 : row;
+    }
+  }
+  __device__ __forceinline__ void data(const Fp8AttnParams& a, int tid) {
+    x0 = x1 = make_uint4(0u, 0u, 0u, 0u);
+    if (row >= 0) {
+      const uint4* src = reinterpret_cast<const uint4*>(a.q + row * a.ldq + head * kD) + (tid & 7) * 2;
+      x0 = __ldg(src);
+      x1 = __ldg(src + 1);
+    }
+  }
+  // Codes next to the tile's largest element (an error of 2^-26 of it moves every score of the tile by as little), e4m3 and
+  // the e5m2 rest.
+  template <bool PLAIN>
+  __device__ __forceinline__ void store(const Fp8AttnParams& a, const PartInfo& w, int tid, uint8_t* q_smem, uint32_t* amax, RowInfo* info) {
+    float y[16];
+    bf16x8_to_float(x0, y);
+    bf16x8_to_float(x1, y + 8);
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      m = max(m, __float_as_uint(y[j]) & 0x7fffffffu);
+    m = fp8_amax8(m);
+    const bool finite = m < 0x7f800000u;
+    {
+      const uint32_t top = __reduce_max_sync(0xffffffffu, finite ? m : 0u);
+      if ((tid & 31) == 0)
+        atomicMax(amax, top);
+    }
+    asm volatile("bar.sync 6, 256;" ::: "memory");
+    const int r = tid >> 3, part = tid & 7;
+    const float inv = fp8_inverse(fp8_scale_bits(*amax));
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float z[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        z[e] = finite ? y[4 * j + e] * inv : 0.f;
+      hi[j] = fp8_pack2(z[0], z[1]) | fp8_pack2(z[2], z[3]) << 16;
+      const float2 u = fp8_to_float2(hi[j] & 0xffffu), v = fp8_to_float2(hi[j] >> 16);
+      lo[j] = fp8_pack2_e5m2(z[0] - u.x, z[1] - u.y) | fp8_pack2_e5m2(z[2] - v.x, z[3] - v.y) << 16;
+    }
+    uint8_t* dst = q_smem + r * kD + ((part ^ (r & 7)) << 4);
+    *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4*>(dst + kRows * kD) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    if (part == 0) {
+      RowInfo v = {};
+      v.out = t < w.rows ? (w.row0 + t / (a.H / a.Hkv)) * a.H + head : -1;
+      v.fix = row < 0 ? 0.f : finite ? 1.f : __uint_as_float(0x7fc00000u);
+      if (!PLAIN && row >= 0) {
+        v.pos = __ldg(a.cu_k + w.b + 1) - __ldg(a.cu_k + w.b) - (__ldg(a.cu_q + w.b + 1) - row);
+        v.slope = a.slopes ? __ldg(a.slopes + head) * kLog2e : 0.f;
+        v.hi = w.len;
+        if (a.ranges) {
+          const int2 range = __ldg(a.ranges + row);
+          v.lo = range.x;
+          v.hi = min(range.y, w.len);
+        }
+      }
+      info[r] = v;
+    }
+    fence_proxy_async_smem();
+  }
+};
+
+// The chunks of a CTA's share one after the other, as the producer and the MMA warp walk over them.  Uniform over a warp.
+struct Chunks {
+  int n, c0, tiles;            // part, first tile of the chunk, tiles of the part
+  int begin, end, hk, k0, v0;
+  __device__ __forceinline__ int count() const { return min(kChunk, tiles - c0); }
+  __device__ __forceinline__ bool open(uint64_t* full, uint64_t* done, const PartInfo* parts, int* abort_flag, int* status) {
+    const int slot = n % kParts;
+    if (!mbar_wait(&full[slot], (n / kParts) & 1, abort_flag, status, 420))
+      return false;
+    const PartInfo& w = parts[slot];
+    begin = uniform(w.begin);
+    end = static_cast<int>(uniform(w.end + 1)) - 1;
+    hk = uniform(w.hk);
+    k0 = uniform(w.k0);
+    v0 = uniform(w.v0);
+    warp_arrive(&done[slot]);
+    c0 = 0;
+    tiles = (end - begin + kUnitKeys - 1) / kUnitKeys;
+    return end >= 0;
+  }
+  __device__ __forceinline__ bool next(uint64_t* full, uint64_t* done, const PartInfo* parts, int* abort_flag, int* status) {
+    c0 += kChunk;
+    if (c0 < tiles)
+      return true;
+    ++n;
+    return open(full, done, parts, abort_flag, status);
+  }
+};
+
+template <bool PLAIN>
+__global__ void __launch_bounds__(kFewThreads, 1)
 fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const FewParams p) {
   pdl_wait();      // programmatic dependent launch: nothing before this reads an earlier kernel's data
   pdl_trigger();
-  using Cfg = FewCfg<RN>;
-  constexpr int HR = Cfg::kHalf, kChunk = Cfg::kChunk;
   const Fp8AttnParams& a = p.a;
-  Walk<RN> walk;
-  walk.start(p);
-  if (walk.left == 0)
-    return;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* p_smem = ring + kRing * kTileBytes;               // two slots of [128 keys][128 bytes]: weights, then remainders
-  uint8_t* q_smem = p_smem + 2 * kTileBytes;                 // [RN][128] e4m3, then e5m2
-  __shared__ uint64_t full[kRing], empty[kRing], s_full[kChunk], p_full[2], p_free[2], q_full, s_free, pv_done, o_free;
-  __shared__ uint32_t tmem_slot;
+  // weights of a chunk: tile i in block i / 2; row = key, 64 bytes at 64 * (i % 2): kRows weights, then kRows remainders
+  uint8_t* p_smem = ring + kRing * kTileBytes;
+  uint8_t* q_smem = p_smem + kChunk / 2 * kTileBytes;        // two slots of [kRows][128] e4m3, then e5m2
+  float* sc_smem = reinterpret_cast<float*>(q_smem + 4 * kQBytes);      // two slots of [kChunk][K, V][128] scales
+  __shared__ uint64_t full[kRing], empty[kRing], part_full[kParts], part_done[kParts], q_full[2], s_full[2], s_free[2], p_full, pv_done;
+  __shared__ PartInfo s_part[kParts];
+  __shared__ uint32_t tmem_slot, s_amax[kParts];
   __shared__ int abort_flag, joins;
-  __shared__ __align__(16) float s_rf[RN], s_slope[RN], s_max[4][RN], s_sum[4][RN];
-  __shared__ int s_pos[RN];
-  __shared__ int64_t s_out[RN];
-  __shared__ int2 s_range[RN];
+  __shared__ RowInfo s_row[2][kRows];
+  __shared__ __align__(16) float s_max[4][kRows], s_sum[4][kRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -344,16 +567,17 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < kChunk; ++i)
-      mbar_init(&s_full[i], 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&p_full[i], 8);
-      mbar_init(&p_free[i], 1);
+    for (int i = 0; i < kParts; ++i) {
+      mbar_init(&part_full[i], 1);
+      mbar_init(&part_done[i], kSoftmaxWarps + 2);
     }
-    mbar_init(&q_full, 8);
-    mbar_init(&s_free, 8);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 8);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_free[i], kSoftmaxWarps);
+    }
+    mbar_init(&p_full, kSoftmaxWarps);
     mbar_init(&pv_done, 1);
-    mbar_init(&o_free, 8);
     fence_mbar_init();
     tma_prefetch_desc(&tmap_k);
     tma_prefetch_desc(&tmap_v);
@@ -365,418 +589,437 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem_s = tmem_slot, tmem_o = tmem_slot + Cfg::kTmemO;
+  const uint32_t tmem = tmem_slot;      // S^T of two chunks, then O^T: kRows columns of 256 w, kRows of remainders
 
-  if (warp == 0) {
-    // ---------------------------------------------------------------- producer: K tiles of a chunk, then its V tiles
-    int n = 0;
-    while (walk.next(p)) {
+  if (warp == kSoftmaxWarps + 2) {
+    // ---------------------------------------------------------------- scheduler: the parts of this CTA's share
+    Walk<kRows> walk;
+    walk.start(p);
+    const int group = a.H / a.Hkv;
+    for (int n = 0;;) {
+      const bool more = walk.next(p);
       const SeqWork& w = walk.w;
-      if (w.hi <= w.lo)
-        continue;
-      const int2 keys = part_keys(walk);
-      const int tiles = (keys.y - keys.x + kUnitKeys - 1) / kUnitKeys;
-      for (int c0 = 0; c0 < tiles; c0 += kChunk) {
-        const int nt = min(kChunk, tiles - c0);
-        for (int i = 0; i < 2 * nt; ++i, ++n) {
-          const int slot = n % kRing;
-          if (n >= kRing)
-            mbar_wait(&empty[slot], (n / kRing - 1) & 1, &abort_flag, p.status_word, 401);
-          if (lane == 0) {
-            const CUtensorMap* map = i < nt ? &tmap_k : &tmap_v;
-            const int key = keys.x + (c0 + (i < nt ? i : i - nt)) * kUnitKeys;
-            const int row = static_cast<int>(i < nt ? w.k0 : w.v0) + key;
-            const int boxes = min(4, (keys.y - key + 31) / 32);      // no box of keys that do not belong to the part
-            mbar_arrive_expect_tx(&full[slot], boxes * 32 * kD);
-            for (int j = 0; j < boxes; ++j)
-              tma_load_2d(ring + slot * kTileBytes + j * 32 * kD, map, &full[slot], walk.hk * kD, row + 32 * j);
-          }
-          __syncwarp();
+      if (more && w.hi <= w.lo) {      // no keys: zeros
+        for (int r = 0; r < kRows && walk.tile * kRows + r < w.rows; ++r) {
+          const int t = walk.tile * kRows + r, i = t / group;
+          __nv_bfloat16* dst = a.out + ((static_cast<int64_t>(w.row0) + i) * a.H + walk.hk * group + t - i * group) * kD;
+          *reinterpret_cast<uint2*>(dst + lane * 4) = make_uint2(0u, 0u);
         }
+        continue;
       }
+      const int slot = n % kParts;
+      if (n >= kParts && !mbar_wait(&part_done[slot], (n / kParts - 1) & 1, &abort_flag, p.status_word, 400))
+        break;
+      if (lane == 0) {
+        PartInfo v = {};
+        v.end = -1;
+        if (more) {
+          const int begin = w.lo + walk.first * kUnitKeys;
+          v = {begin, min(w.hi, w.lo + walk.last * kUnitKeys), 0, 1, 0, w.b, walk.hk, w.row0, w.rows, walk.tile * kRows, w.k0, w.v0, w.hi};
+          if (walk.last - walk.first < w.units) {
+            v.owner = walk.owner();
+            v.parts = walk.parts();
+            v.slot = 2 * static_cast<int>(blockIdx.x) + (walk.first == 0 ? 1 : 0);
+          }
+        }
+        s_part[slot] = v;
+        s_amax[slot] = 0;
+      }
+      warp_arrive(&part_full[slot]);
+      ++n;
+      if (!more)
+        break;
+    }
+  } else if (warp == 0) {
+    // ---------------------------------------------------------------- producer: the K tiles of a chunk before the V tiles of the last
+    int n = 0;
+    auto load = [&](const CUtensorMap* map, const Chunks& c, int row0) {
+      for (int i = 0; i < c.count(); ++i, ++n) {
+        const int slot = n % kRing, key = c.begin + (c.c0 + i) * kUnitKeys;
+        if (n >= kRing)
+          mbar_wait(&empty[slot], (n / kRing - 1) & 1, &abort_flag, p.status_word, 401);
+        if (elect_one()) {
+          const int boxes = min(4, (c.end - key + 31) / 32);      // no box of keys that do not belong to the part
+          mbar_arrive_expect_tx(&full[slot], boxes * 32 * kD);
+          for (int j = 0; j < boxes; ++j)
+            tma_load_2d(ring + slot * kTileBytes + j * 32 * kD, map, &full[slot], c.hk * kD, row0 + key + 32 * j);
+        }
+        __syncwarp();
+      }
+    };
+    Chunks ahead = {};
+    bool more = ahead.open(part_full, part_done, s_part, &abort_flag, p.status_word);
+    if (more)
+      load(&tmap_k, ahead, ahead.k0);
+    while (more) {
+      const Chunks now = ahead;
+      more = ahead.next(part_full, part_done, s_part, &abort_flag, p.status_word);
+      if (more)
+        load(&tmap_k, ahead, ahead.k0);
+      load(&tmap_v, now, now.v0);
     }
     // a CTA may not end with copies on their way, also when a wait of another warp has given up
     for (int i = max(0, n - kRing); i < n; ++i)
       mbar_wait(&full[i % kRing], (i / kRing) & 1, &abort_flag, p.status_word, 402);
   } else if (warp == 1) {
-    // ---------------------------------------------------------------- MMA issuer
-    constexpr uint32_t idesc_hi = umma_idesc_f8(128, RN, 0, 0, 0, 0), idesc_lo = umma_idesc_f8(128, RN, 0, 1, 0, 0);
-    constexpr uint32_t idesc_pv = umma_idesc_f8(128, 2 * RN, 0, 0, 1, 1);
-    const uint32_t q_addr = smem_u32(q_smem);
-    int n = 0, n_p = 0, n_chunk = 0, n_part = 0;
-    while (walk.next(p)) {
-      const SeqWork& w = walk.w;
-      if (w.hi <= w.lo)
-        continue;
-      const int2 keys = part_keys(walk);
-      const int tiles = (keys.y - keys.x + kUnitKeys - 1) / kUnitKeys;
-      mbar_wait(&q_full, n_part & 1, &abort_flag, p.status_word, 403);
-      for (int c0 = 0; c0 < tiles; c0 += kChunk, ++n_chunk) {
-        const int nt = min(kChunk, tiles - c0);
-        if (n_chunk > 0)
-          mbar_wait(&s_free, (n_chunk - 1) & 1, &abort_flag, p.status_word, 404);
-        for (int i = 0; i < nt; ++i, ++n) {
-          const int slot = n % kRing;
-          mbar_wait(&full[slot], (n / kRing) & 1, &abort_flag, p.status_word, 405);
-          tc_fence_after_sync();
-          if (lane == 0) {
-            const uint64_t a_desc = umma_smem_desc_sw128(smem_u32(ring + slot * kTileBytes), 16, 1024);
-            const uint64_t hi_desc = umma_smem_desc_sw128(q_addr, 16, 1024);
-            const uint64_t lo_desc = umma_smem_desc_sw128(q_addr + Cfg::kQBytes, 16, 1024);
+    // ---------------------------------------------------------------- MMA issuer: the scores of a chunk before the sums of the last
+    constexpr uint32_t idesc_hi = umma_idesc_f8(128, kRows, 0, 0, 0, 0), idesc_lo = umma_idesc_f8(128, kRows, 0, 1, 0, 0);
+    constexpr uint32_t idesc_pv = umma_idesc_f8(128, 2 * kRows, 0, 0, 1, 1);
+    const uint32_t ring_addr = smem_u32(ring), p_addr = smem_u32(p_smem), t_s = uniform(tmem), t_o = t_s + 2 * kChunk * kRows;
+    int n = 0, n_s = 0, n_p = 0;
+    auto scores = [&](const Chunks& c) {
+      const int buf = n_s & 1;
+      if (c.c0 == 0)
+        mbar_wait(&q_full[c.n & 1], (c.n >> 1) & 1, &abort_flag, p.status_word, 403);
+      if (n_s >= 2)
+        mbar_wait(&s_free[buf], ((n_s >> 1) - 1) & 1, &abort_flag, p.status_word, 404);
+      const uint32_t q_addr = smem_u32(q_smem) + (c.n & 1) * 2 * kQBytes;
+      const int nt = c.count();
+      for (int i = 0; i < nt; ++i, ++n) {
+        const int slot = n % kRing;
+        mbar_wait(&full[slot], (n / kRing) & 1, &abort_flag, p.status_word, 405);
+        tc_fence_after_sync();
+        if (elect_one()) {
+          const uint32_t k_addr = ring_addr + slot * kTileBytes, d = t_s + (buf * kChunk + i) * kRows;
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {      // 32 head dimensions = 32 bytes a step
-              umma_ss_f8(tmem_s + i * RN, a_desc + 2 * kk, hi_desc + 2 * kk, idesc_hi, kk != 0 ? 1u : 0u);
-              umma_ss_f8(tmem_s + i * RN, a_desc + 2 * kk, lo_desc + 2 * kk, idesc_lo, 1u);
-            }
-            umma_commit(&empty[slot]);
-            umma_commit(&s_full[i]);
+          for (int kk = 0; kk < 4; ++kk) {      // 32 head dimensions = 32 bytes a step
+            umma_tile(d, k_addr + 32 * kk, q_addr + 32 * kk, idesc_hi, kk != 0 ? 1u : 0u);
+            umma_tile(d, k_addr + 32 * kk, q_addr + kQBytes + 32 * kk, idesc_lo, 1u);
           }
-          __syncwarp();
+          umma_commit(&empty[slot]);
+          if (i == nt - 1)
+            umma_commit(&s_full[buf]);
         }
-        for (int i = 0; i < nt; ++i, ++n, ++n_p) {
-          const int slot = n % kRing, buf = n_p & 1;
-          mbar_wait(&full[slot], (n / kRing) & 1, &abort_flag, p.status_word, 406);
-          mbar_wait(&p_full[buf], (n_p >> 1) & 1, &abort_flag, p.status_word, 407);
-          if (c0 == 0 && i == 0 && n_part > 0)
-            mbar_wait(&o_free, (n_part - 1) & 1, &abort_flag, p.status_word, 408);
-          tc_fence_after_sync();
-          if (lane == 0) {
-            const uint32_t v_addr = smem_u32(ring + slot * kTileBytes), p_addr = smem_u32(p_smem + buf * kTileBytes);
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)        // 32 keys = 32 rows of 128 bytes a step
-              umma_ss_f8(tmem_o, umma_smem_desc_sw128(v_addr + kk * 4096, kTileBytes, 1024),
-                         umma_smem_desc_sw128(p_addr + kk * 4096, kTileBytes, 1024), idesc_pv, (c0 | i | kk) != 0 ? 1u : 0u);
-            umma_commit(&empty[slot]);
-            umma_commit(&p_free[buf]);
-            if (i == nt - 1)
-              umma_commit(&pv_done);
-          }
-          __syncwarp();
-        }
+        __syncwarp();
       }
-      ++n_part;
+      ++n_s;
+    };
+    Chunks ahead = {};
+    bool more = ahead.open(part_full, part_done, s_part, &abort_flag, p.status_word);
+    if (more)
+      scores(ahead);
+    while (more) {
+      const Chunks now = ahead;
+      more = ahead.next(part_full, part_done, s_part, &abort_flag, p.status_word);
+      if (more)
+        scores(ahead);
+      const int nt = now.count();
+      mbar_wait(&p_full, n_p & 1, &abort_flag, p.status_word, 407);
+      ++n_p;
+      for (int i = 0; i < nt; ++i, ++n) {
+        const int slot = n % kRing;
+        mbar_wait(&full[slot], (n / kRing) & 1, &abort_flag, p.status_word, 406);
+        tc_fence_after_sync();
+        if (elect_one()) {
+          const uint32_t v_addr = ring_addr + slot * kTileBytes, w_addr = p_addr + (i >> 1) * kTileBytes + (i & 1) * 64;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)        // 32 keys = 32 rows of 128 bytes a step
+            umma_tile(t_o, v_addr + kk * 4096, w_addr + kk * 4096, idesc_pv, (now.c0 | i | kk) != 0 ? 1u : 0u);
+          umma_commit(&empty[slot]);
+          if (i == nt - 1)
+            umma_commit(&pv_done);
+        }
+        __syncwarp();
+      }
     }
   } else {
     // ---------------------------------------------------------------- softmax over the keys, epilogue
-    const int half = (warp - 2) >> 2;              // rows HR * half ..
+    const int rg = (warp - 2) >> 2;                // rows kGroup * rg ..
     const int quarter = warp & 3;                  // tensor-memory lanes: keys (head dimensions) 32 * quarter ..
     const int tid = threadIdx.x - 64;
     const int kl = quarter * 32 + lane;            // key of a tile, or head dimension
-    const uint32_t t_lane = static_cast<uint32_t>(quarter * 32) << 16;
-    const int group = a.H / a.Hkv;
-    const int r0 = half * HR;
-    uint32_t s_phase = 0;                          // bit i: phase of s_full[i]
-    int n = 0, n_p = 0, n_chunk = 0;
-    while (walk.next(p)) {
-      const SeqWork w = walk.w;
-      const int hk = walk.hk;
-      if (w.hi <= w.lo) {                          // no keys: zeros
-        for (int r = r0; r < r0 + HR && walk.tile * RN + r < w.rows; ++r) {
-          const int t = walk.tile * RN + r, i = t / group;
-          a.out[((static_cast<int64_t>(w.row0) + i) * a.H + hk * group + t - i * group) * kD + kl] = __float2bfloat16_rn(0.f);
-        }
-        continue;
-      }
-      // queries to shared memory; eight threads a row
-      if (tid < RN * 8) {
-        const int r = tid >> 3, part = tid & 7;
-        const int t = walk.tile * RN + r, i = t / group, h = hk * group + t - i * group;
-        int row = t < w.rows ? __ldg(a.idx + w.row0 + i) : -1;
-        if (row >= a.total_q)
-          row = -1;
-        uint4 x0 = make_uint4(0u, 0u, 0u, 0u), x1 = x0;
-        if (row >= 0) {
-          const uint4* src = reinterpret_cast<const uint4*>(a.q + row * a.ldq + h * kD) + part * 2;
-          x0 = __ldg(src);
-          x1 = __ldg(src + 1);
-        }
-        float y[16];
-        bf16x8_to_float(x0, y);
-        bf16x8_to_float(x1, y + 8);
-        uint32_t m = 0;
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          m = max(m, __float_as_uint(y[j]) & 0x7fffffffu);
-        const uint32_t scale = fp8_scale_bits(fp8_amax8(m));
-        const float inv = fp8_inverse(scale);
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float z[4], e[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            z[k] = scale >= 0x7f800000u ? 0.f : y[4 * j + k] * inv;
-          hi[j] = fp8_pack2(z[0], z[1]) | fp8_pack2(z[2], z[3]) << 16;
-          const float2 u = fp8_to_float2(hi[j] & 0xffffu), v = fp8_to_float2(hi[j] >> 16);
-          e[0] = z[0] - u.x, e[1] = z[1] - u.y, e[2] = z[2] - v.x, e[3] = z[3] - v.y;
-          lo[j] = fp8_pack2_e5m2(e[0], e[1]) | fp8_pack2_e5m2(e[2], e[3]) << 16;
-        }
-        uint8_t* dst = q_smem + r * kD + ((part ^ (r & 7)) << 4);
-        *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(dst + Cfg::kQBytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        if (part == 0) {
-          s_rf[r] = __uint_as_float(scale);        // NaN: a query that is not finite
-          // output row, negative: none; the lowest bit: whether the row exists in q
-          s_out[r] = t < w.rows ? ((static_cast<int64_t>(w.row0) + i) * a.H + h) * 2 + (row >= 0) : -1;
-          if (!PLAIN) {
-            s_pos[r] = __ldg(a.cu_k + w.b + 1) - __ldg(a.cu_k + w.b) - (__ldg(a.cu_q + w.b + 1) - row);
-            s_slope[r] = a.slopes && row >= 0 ? __ldg(a.slopes + h) * kLog2e : 0.f;
-            int2 v = make_int2(0, row >= 0 ? w.hi : 0);
-            if (a.ranges && row >= 0) {
-              v = __ldg(a.ranges + row);
-              v.y = min(v.y, w.hi);
-            }
-            s_range[r] = v;
-          }
-        }
-        fence_proxy_async_smem();
-      }
-      warp_arrive(&q_full);
-      softmax_sync();
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t t_o = t_lane + 2 * kChunk * kRows;
+    const int r0 = rg * kGroup;
+    const bool stages = warp < 10;                 // takes part in staging the queries
+    const float key_mul = a.scale * (PLAIN ? kLog2e : 1.f);
+    uint8_t* p_dst = p_smem + kl * kD + (rg & 1) * 8;
 
-      const int2 keys = part_keys(walk);
-      const int tiles = (keys.y - keys.x + kUnitKeys - 1) / kUnitKeys;
-      const float* k_scale = a.k_scales + w.k0 * a.Hkv + hk;
-      const float* v_scale = a.v_scales + w.v0 * a.Hkv + hk;
-      float top[HR], l[HR];
+    // Scales of the keys of a chunk, copied ahead of their use: K's by the first half of the threads, V's by the second.  The
+    // heads of a key lie side by side: CTAs that work on them at the same time start at different tiles.
+    auto request_scales = [&](const PartInfo& w, int key, int slot) {
+      const bool of_v = tid >= 256;
+      const float* src = (of_v ? a.v_scales + static_cast<int64_t>(w.v0) * a.Hkv : a.k_scales + static_cast<int64_t>(w.k0) * a.Hkv) + w.hk;
+      float* dst = sc_smem + slot * kChunk * 2 * kUnitKeys + (of_v ? kUnitKeys : 0) + (tid & 127);
 #pragma unroll
-      for (int r = 0; r < HR; ++r) {
-        top[r] = -INFINITY;
+      for (int j = 0; j < 2; ++j) {
+        const int i = (2 * j + ((tid >> 7) & 1) + w.hk) & (kChunk - 1), at = key + i * kUnitKeys + (tid & 127);
+        if (at < w.end)
+          cp_async4(dst + i * 2 * kUnitKeys, src + static_cast<int64_t>(at) * a.Hkv);
+      }
+      cp_async_commit();
+    };
+    auto wait_part = [&](int n) {
+      return mbar_wait(&part_full[n % kParts], (n / kParts) & 1, &abort_flag, p.status_word, 415) && s_part[n % kParts].end >= 0;
+    };
+    auto stage = [&](int n, QueryLoad& ql) {
+      if (stages) {
+        ql.template store<PLAIN>(a, s_part[n % kParts], tid, q_smem + (n & 1) * 2 * kQBytes, &s_amax[n % kParts], s_row[n & 1]);
+        warp_arrive(&q_full[n & 1]);
+      }
+    };
+
+    QueryLoad ql;
+    int n_chunk = 0, ring_at = 0;
+    bool more = wait_part(0), after = false;       // whether the part at hand and the one after it exist
+    if (more) {
+      request_scales(s_part[0], s_part[0].begin, 0);
+      if (stages) {
+        ql.index(a, s_part[0], tid);
+        ql.data(a, tid);
+      }
+      stage(0, ql);
+      after = wait_part(1);
+      if (after && stages) {
+        ql.index(a, s_part[1], tid);
+        ql.data(a, tid);
+      }
+      cp_async_wait_all();
+      softmax_sync();
+      ring_at = min(kChunk, (s_part[0].end - s_part[0].begin + kUnitKeys - 1) / kUnitKeys);
+    }
+    for (int n = 0; more; ++n) {
+      const PartInfo& part = s_part[n % kParts];
+      const RowInfo* rows = &s_row[n & 1][r0];
+      const int end = part.end, tiles = (end - part.begin + kUnitKeys - 1) / kUnitKeys;
+      const bool alive = rows[0].out >= 0;         // rows are filled from the first on
+      bool then = false;                           // whether the part after the next exists
+      float top[kGroup], l[kGroup];
+#pragma unroll
+      for (int r = 0; r < kGroup; ++r) {
+        top[r] = kNothing;
         l[r] = 0.f;
       }
       for (int c0 = 0; c0 < tiles; c0 += kChunk, ++n_chunk) {
-        const int nt = min(kChunk, tiles - c0);
-        const int key0 = keys.x + c0 * kUnitKeys + kl;
-        // scores of all tiles of the chunk, their maxima
-        float mx[HR];
-#pragma unroll
-        for (int r = 0; r < HR; ++r)
-          mx[r] = -INFINITY;
+        const int nt = min(kChunk, tiles - c0), buf = n_chunk & 1;
+        const bool last = c0 + kChunk >= tiles;
+        const int key0 = part.begin + c0 * kUnitKeys + kl;
+        float kk[kChunk], ex[kChunk];
         {
-          float rf[HR];
-          lds_row(rf, s_rf + r0);
-          float ks_next = 0.f, vs_next = 1.f;
-          if (key0 < keys.y) {
-            ks_next = __ldg(k_scale + static_cast<int64_t>(key0) * a.Hkv);
-            vs_next = __ldg(v_scale + static_cast<int64_t>(key0) * a.Hkv);
-          }
-          for (int i = 0; i < nt; ++i) {
-            const int at = key0 + i * kUnitKeys;
-            const bool there = at < keys.y;
-            const float kk = ks_next * a.scale * (PLAIN ? kLog2e : 1.f), ex = value_exponent(vs_next);
-            if (at + kUnitKeys < keys.y) {
-              ks_next = __ldg(k_scale + static_cast<int64_t>(at + kUnitKeys) * a.Hkv);
-              vs_next = __ldg(v_scale + static_cast<int64_t>(at + kUnitKeys) * a.Hkv);
-            }
-            mbar_wait(&s_full[i], (s_phase >> i) & 1, &abort_flag, p.status_word, 409);
-            tc_fence_after_sync();
-            uint32_t s[HR];
-            tmem_ld(tmem_s + t_lane + i * RN + r0, s);
-            tmem_ld_wait();
+          const float* sc = sc_smem + buf * kChunk * 2 * kUnitKeys + kl;
+          const float mul = key_mul * __uint_as_float(fp8_scale_bits(s_amax[n % kParts]));
 #pragma unroll
-            for (int r = 0; r < HR; ++r) {
-              float t = __uint_as_float(s[r]) * (kk * rf[r]);
-              if (PLAIN) {
-                t += ex;
-                t = there ? t : -INFINITY;
-              } else {
-                const int2 range = s_range[r0 + r];
-                t = score_log2(t, a.cap) - s_slope[r0 + r] * static_cast<float>(abs(s_pos[r0 + r] - at)) + ex;
-                t = there && at >= range.x && at < range.y ? t : -INFINITY;
+          for (int i = 0; i < kChunk; ++i) {
+            kk[i] = sc[i * 2 * kUnitKeys] * mul;
+            ex[i] = value_exponent(sc[(i * 2 + 1) * kUnitKeys]);
+          }
+        }
+        // products of the chunk; tensor memory is free for the next one
+        mbar_wait(&s_full[buf], (n_chunk >> 1) & 1, &abort_flag, p.status_word, 409);
+        tc_fence_after_sync();
+        uint32_t s[kChunk][kGroup];
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i)
+          if (i < nt)
+            tmem_ld_32x8(t_lane + (buf * kChunk + i) * kRows + r0, s[i]);
+        tmem_ld_wait();
+        tc_fence_before_sync();
+        warp_arrive(&s_free[buf]);
+        // what the next chunk needs
+        int next_tiles = 0;
+        if (!last) {
+          request_scales(part, part.begin + (c0 + kChunk) * kUnitKeys, buf ^ 1);
+          next_tiles = min(kChunk, tiles - c0 - kChunk);
+        } else if (after) {
+          stage(n + 1, ql);
+          const PartInfo& w = s_part[(n + 1) % kParts];
+          request_scales(w, w.begin, buf ^ 1);
+          next_tiles = min(kChunk, (w.end - w.begin + kUnitKeys - 1) / kUnitKeys);
+          then = wait_part(n + 2);
+          if (then && stages)
+            ql.index(a, s_part[(n + 2) % kParts], tid);
+        }
+        const int v_at = ring_at + next_tiles;      // the chunk's V tiles in the order of the ring
+        ring_at = v_at + nt;
+
+        float mx[kGroup];
+#pragma unroll
+        for (int r = 0; r < kGroup; ++r)
+          mx[r] = top[r];
+        if (alive) {
+          // scores (times log2 e, plus the exponents of the values' scales) and their maxima
+          if (PLAIN) {
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i)
+              if (key0 + i * kUnitKeys < end) {
+#pragma unroll
+                for (int r = 0; r < kGroup; ++r) {
+                  const float t = fmaf(__uint_as_float(s[i][r]), kk[i], ex[i]);
+                  s[i][r] = __float_as_uint(t);
+                  mx[r] = fmaxf(mx[r], t);
+                }
               }
-              s[r] = __float_as_uint(t);
-              mx[r] = fmaxf(mx[r], t);
-            }
-            tmem_st(tmem_s + t_lane + i * RN + r0, s);
-          }
-          s_phase ^= (1u << nt) - 1;
-        }
-        tmem_st_wait();
-        {
-          const float v = reduce_lanes<HR, true>(mx);
-          if (lane % (32 / HR) == 0)
-            s_max[quarter][r0 + lane / (32 / HR)] = v;
-        }
-        softmax_sync();
-        bool grown = false;
-        float old[HR];
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          float x[HR];
-          lds_row(x, s_max[q4] + r0);
-#pragma unroll
-          for (int r = 0; r < HR; ++r)
-            mx[r] = q4 == 0 ? fmaxf(x[r], top[r]) : fmaxf(mx[r], x[r]);
-        }
-#pragma unroll
-        for (int r = 0; r < HR; ++r) {
-          grown = grown || mx[r] > top[r];
-          old[r] = exp2f(top[r] - (mx[r] == -INFINITY ? 0.f : mx[r]));
-          top[r] = mx[r];
-          l[r] *= old[r];
-        }
-        if (c0 > 0)      // every phase is waited for, also where nothing is rescaled
-          mbar_wait(&pv_done, (n_chunk - 1) & 1, &abort_flag, p.status_word, 410);
-        if (c0 > 0 && grown) {      // the same rows in all four quarters
-          tc_fence_after_sync();
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            uint32_t o[HR];
-            tmem_ld(tmem_o + t_lane + j * RN + r0, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int r = 0; r < HR; ++r)
-              o[r] = __float_as_uint(__uint_as_float(o[r]) * old[r]);
-            tmem_st(tmem_o + t_lane + j * RN + r0, o);
-          }
-          tmem_st_wait();
-        }
-        // weights
-        for (int i = 0; i < nt; ++i, ++n_p) {
-          const int at = key0 + i * kUnitKeys, buf = n_p & 1;
-          uint32_t s[HR];
-          tmem_ld(tmem_s + t_lane + i * RN + r0, s);
-          float inv = 0.f;
-          if (at < keys.y) {
-            const float ex = value_exponent(__ldg(v_scale + static_cast<int64_t>(at) * a.Hkv));
-            inv = ex == ex ? exp2f(-ex) : 1.f;      // the weight of a NaN is a NaN where the key is seen, else zero
-          }
-          tmem_ld_wait();
-          if (n_p >= 2)
-            mbar_wait(&p_free[buf], ((n_p >> 1) - 1) & 1, &abort_flag, p.status_word, 411);
-          uint32_t hi[HR / 4], lo[HR / 4];
-#pragma unroll
-          for (int j = 0; j < HR / 4; ++j) {
-            float w4[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int r = 4 * j + k;
-              w4[k] = exp2f(__uint_as_float(s[r]) + (8.f - (top[r] == -INFINITY ? 0.f : top[r])));
-              l[r] += at < keys.y ? w4[k] * inv : 0.f;
-            }
-            hi[j] = fp8_pack2(w4[0], w4[1]) | fp8_pack2(w4[2], w4[3]) << 16;
-            const float2 u = fp8_to_float2(hi[j] & 0xffffu), v = fp8_to_float2(hi[j] >> 16);
-            lo[j] = fp8_pack2(16.f * w4[0] - 16.f * u.x, 16.f * w4[1] - 16.f * u.y) |
-                    fp8_pack2(16.f * w4[2] - 16.f * v.x, 16.f * w4[3] - 16.f * v.y) << 16;
-          }
-          // row kl of the slot: RN weights, then RN remainders, in 16-byte chunks that the swizzle permutes
-          uint8_t* dst = p_smem + buf * kTileBytes + kl * kD;
-          if constexpr (HR == 16) {
-            *reinterpret_cast<uint4*>(dst + ((half ^ (kl & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<uint4*>(dst + (((2 + half) ^ (kl & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
           } else {
-            *reinterpret_cast<uint2*>(dst + ((0 ^ (kl & 7)) << 4) + 8 * half) = make_uint2(hi[0], hi[1]);
-            *reinterpret_cast<uint2*>(dst + ((1 ^ (kl & 7)) << 4) + 8 * half) = make_uint2(lo[0], lo[1]);
-          }
-          if (keys.y - (key0 - kl) - i * kUnitKeys < kUnitKeys && half == 0) {
-            // rows behind the last key may hold any byte, a NaN times a weight of zero among them
-            const int use = n + nt + i;
-            mbar_wait(&full[use % kRing], (use / kRing) & 1, &abort_flag, p.status_word, 412);
-            if (at >= keys.y) {
-              uint4* v = reinterpret_cast<uint4*>(ring + (use % kRing) * kTileBytes + kl * kD);
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
-                v[j] = make_uint4(0u, 0u, 0u, 0u);
+            for (int i = 0; i < kChunk; ++i)
+#pragma unroll
+              for (int r = 0; r < kGroup; ++r)
+                s[i][r] = __float_as_uint(__uint_as_float(s[i][r]) * kk[i]);
+            if (a.cap > 0.f) {
+              const float to = 2.f * kLog2e / a.cap;
+#pragma unroll
+              for (int i = 0; i < kChunk; ++i)
+#pragma unroll
+                for (int r = 0; r < kGroup; ++r)
+                  s[i][r] = __float_as_uint(capped(__uint_as_float(s[i][r]) * to, a.cap));
+            }
+#pragma unroll
+            for (int r = 0; r < kGroup; ++r) {
+              const float slope = rows[r].slope;
+              const int pos = rows[r].pos, lo = rows[r].lo, hi = min(rows[r].hi, end);
+#pragma unroll
+              for (int i = 0; i < kChunk; ++i) {
+                const int at = key0 + i * kUnitKeys;
+                float t = fmaf(__uint_as_float(s[i][r]), kLog2e, ex[i]) - slope * static_cast<float>(abs(pos - at));
+                t = at >= lo && at < hi ? t : -INFINITY;
+                s[i][r] = __float_as_uint(t);
+                mx[r] = fmaxf(mx[r], t);
+              }
             }
           }
-          tc_fence_before_sync();
-          fence_proxy_async_smem();
-          warp_arrive(&p_full[buf]);
+#pragma unroll
+          for (int r = 0; r < kGroup; ++r)
+            mx[r] = warp_max(mx[r]);
+          if (lane == 0) {
+#pragma unroll
+            for (int r = 0; r < kGroup; r += 4)
+              *reinterpret_cast<float4*>(&s_max[quarter][r0 + r]) = make_float4(mx[r], mx[r + 1], mx[r + 2], mx[r + 3]);
+          }
+          group_sync(rg);
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            float x[kGroup];
+            lds_row(x, s_max[q4] + r0);
+#pragma unroll
+            for (int r = 0; r < kGroup; ++r)
+              mx[r] = fmaxf(mx[r], x[r]);
+          }
         }
-        warp_arrive(&s_free);
-        n += 2 * nt;
+        // the weights of the last chunk have been taken; the sums are rescaled where a maximum has grown
+        if (n_chunk > 0)
+          mbar_wait(&pv_done, (n_chunk - 1) & 1, &abort_flag, p.status_word, 410);
+        if (alive) {
+          bool grown = false;
+#pragma unroll
+          for (int r = 0; r < kGroup; ++r)
+            grown = grown || mx[r] > top[r];
+          if (c0 > 0 && grown) {      // the same rows in all four quarters
+            float old[kGroup];
+#pragma unroll
+            for (int r = 0; r < kGroup; ++r) {
+              old[r] = exp2f(top[r] - mx[r]);
+              l[r] *= old[r];
+            }
+            tc_fence_after_sync();
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              uint32_t o[kGroup];
+              tmem_ld_32x8(t_o + j * kRows + r0, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int r = 0; r < kGroup; ++r)
+                o[r] = __float_as_uint(__uint_as_float(o[r]) * old[r]);
+              tmem_st_32x8(t_o + j * kRows + r0, o);
+            }
+            tmem_st_wait();
+          }
+#pragma unroll
+          for (int r = 0; r < kGroup; ++r) {
+            top[r] = mx[r];
+            mx[r] = 8.f - mx[r];      // weights are taken times 256
+          }
+#pragma unroll
+          for (int i = 0; i < kChunk; ++i)
+            if (i < nt) {
+              uint32_t hi[2] = {0u, 0u}, lo[2] = {0u, 0u};
+              if (key0 + i * kUnitKeys < end) {
+                // the weight of a NaN is a NaN where its key is seen, else zero
+                const float inv = ex[i] == ex[i] ? exp2f(-ex[i]) : 1.f;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                  float w4[4];
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    w4[e] = exp2f(__uint_as_float(s[i][4 * j + e]) + mx[4 * j + e]);
+                    l[4 * j + e] = fmaf(w4[e], inv, l[4 * j + e]);
+                  }
+                  split_weights(w4, hi[j], lo[j]);
+                }
+              }
+              uint8_t* dst = p_dst + (i >> 1) * kTileBytes;
+              *reinterpret_cast<uint2*>(dst + (((4 * (i & 1) + (rg >> 1)) ^ (kl & 7)) << 4)) = make_uint2(hi[0], hi[1]);
+              *reinterpret_cast<uint2*>(dst + (((4 * (i & 1) + 2 + (rg >> 1)) ^ (kl & 7)) << 4)) = make_uint2(lo[0], lo[1]);
+            }
+        }
+        if (last && end - (key0 - kl) < nt * kUnitKeys && rg == 0) {
+          // rows behind the last key may hold any byte, a NaN times a weight of zero among them
+          const int use = v_at + nt - 1;
+          mbar_wait(&full[use % kRing], (use / kRing) & 1, &abort_flag, p.status_word, 412);
+          if (key0 + (nt - 1) * kUnitKeys >= end) {
+            uint4* v = reinterpret_cast<uint4*>(ring + (use % kRing) * kTileBytes + kl * kD);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              v[j] = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+        tc_fence_before_sync();
+        fence_proxy_async_smem();
+        warp_arrive(&p_full);
+        if (!last) {
+          cp_async_wait_all();
+          softmax_sync();      // everybody's scales of the next chunk are there
+        }
       }
 
-      // ---------------------------------------------------------------- thread = head dimension kl of HR rows
+      // ---------------------------------------------------------------- thread = head dimension kl of kGroup rows
+      if (then && stages)
+        ql.data(a, tid);
       {
-        const float v = reduce_lanes<HR, false>(l);
-        if (lane % (32 / HR) == 0)
-          s_sum[quarter][r0 + lane / (32 / HR)] = v;
+        const float v = reduce_lanes<kGroup>(l);
+        if (lane % (32 / kGroup) == 0)
+          s_sum[quarter][r0 + lane / (32 / kGroup)] = v;
       }
-      softmax_sync();
+      int dst[kGroup];
+      float fix[kGroup];
+#pragma unroll
+      for (int r = 0; r < kGroup; ++r) {
+        dst[r] = rows[r].out;
+        fix[r] = rows[r].fix;
+      }
+      const PartInfo joined = part;
+      cp_async_wait_all();
+      softmax_sync();          // the sums and the next part's scales and rows are there; this part's descriptions are not read again
+      warp_arrive(&part_done[n % kParts]);
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {
-        float x[HR];
+        float x[kGroup];
         lds_row(x, s_sum[q4] + r0);
 #pragma unroll
-        for (int r = 0; r < HR; ++r)
+        for (int r = 0; r < kGroup; ++r)
           l[r] = q4 == 0 ? x[r] : l[r] + x[r];
       }
       mbar_wait(&pv_done, (n_chunk - 1) & 1, &abort_flag, p.status_word, 413);
       tc_fence_after_sync();
-      float o[HR];
+      float o[kGroup];
       {
-        uint32_t u[HR], v[HR];
-        tmem_ld(tmem_o + t_lane + r0, u);
-        tmem_ld(tmem_o + t_lane + RN + r0, v);
+        uint32_t u[kGroup], v[kGroup];
+        tmem_ld_32x8(t_o + r0, u);
+        tmem_ld_32x8(t_o + kRows + r0, v);
         tmem_ld_wait();
 #pragma unroll
-        for (int r = 0; r < HR; ++r)
-          o[r] = __uint_as_float(u[r]) + __uint_as_float(v[r]) * 0.0625f;
+        for (int r = 0; r < kGroup; ++r)
+          o[r] = fmaf(__uint_as_float(v[r]), 0.0625f, __uint_as_float(u[r]));
       }
       tc_fence_before_sync();
-      warp_arrive(&o_free);
-
-      bool store = walk.last - walk.first == w.units;
-      if (!store) {
-        const int owner = walk.first == 0 ? blockIdx.x : walk.cta_of(walk.tile_first);
-        const int parts = walk.cta_of(walk.tile_first + w.units - 1) - owner + 1;
-        // join the parts of a tile that several CTAs hold
-        constexpr int kPart = RN * kD + 2 * RN;
-        float* part = p.parts + (2 * static_cast<int64_t>(blockIdx.x) + (walk.first == 0 ? 1 : 0)) * kPart;
+      if (joined.parts == 1 || join_parts(p, joined, top, l, o, r0, kl, tid, &joins)) {
 #pragma unroll
-        for (int r = 0; r < HR; ++r)
-          part[(r0 + r) * kD + kl] = o[r];
-        if (kl == 0) {
-#pragma unroll
-          for (int r = 0; r < HR; ++r) {
-            part[RN * kD + r0 + r] = top[r];
-            part[RN * kD + RN + r0 + r] = l[r];
-          }
-        }
-        __threadfence();
-        softmax_sync();
-        if (tid == 0) {
-          open_join(p.tickets + owner, p.launch_id);
-          joins = last_to_join(p.tickets + owner, parts) ? 1 : 0;
-        }
-        softmax_sync();
-        store = joins;
-        if (store) {
-          __threadfence();
-          const float* first = p.parts + (2 * static_cast<int64_t>(owner) + 1) * kPart;
-          const float* rest = p.parts + 2 * static_cast<int64_t>(owner) * kPart;
-#pragma unroll
-          for (int r = 0; r < HR; ++r) {
-            top[r] = -INFINITY;
-            o[r] = l[r] = 0.f;
-          }
-          for (int i = 0; i < parts; ++i) {
-            const float* src = i == 0 ? first : rest + 2 * static_cast<int64_t>(i) * kPart;
-#pragma unroll
-            for (int r = 0; r < HR; ++r)
-              top[r] = fmaxf(top[r], __ldcg(src + RN * kD + r0 + r));
-          }
-          for (int i = 0; i < parts; ++i) {
-            const float* src = i == 0 ? first : rest + 2 * static_cast<int64_t>(i) * kPart;
-#pragma unroll
-            for (int r = 0; r < HR; ++r) {
-              const float mul = exp2f(__ldcg(src + RN * kD + r0 + r) - (top[r] == -INFINITY ? 0.f : top[r]));
-              l[r] += __ldcg(src + RN * kD + RN + r0 + r) * mul;
-              o[r] += __ldcg(src + (r0 + r) * kD + kl) * mul;
-            }
-          }
-        }
+        for (int r = 0; r < kGroup; ++r)
+          if (dst[r] >= 0)
+            a.out[static_cast<int64_t>(dst[r]) * kD + kl] =
+                __float2bfloat16_rn(l[r] == 0.f || fix[r] == 0.f ? 0.f : o[r] * __fdividef(fix[r], l[r]));
       }
-      if (store) {
-#pragma unroll
-        for (int r = 0; r < HR; ++r) {
-          const int64_t at = s_out[r0 + r];
-          if (at >= 0)
-            a.out[(at >> 1) * kD + kl] = __float2bfloat16_rn(l[r] == 0.f || !(at & 1) ? 0.f : o[r] * __fdividef(1.f, l[r]));
-        }
-      }
-      softmax_sync();      // what describes the rows is free again
+      more = after;
+      after = then;
     }
   }
 
@@ -784,7 +1027,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
   __syncthreads();
   if (warp == 1) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem_slot, kTmemCols);
+    tmem_dealloc(tmem, kTmemCols);
   }
 }
 
@@ -818,23 +1061,23 @@ size_t few_parts_offset(int batch, int ctas) {
   return (ctas * sizeof(unsigned long long) + batch * sizeof(int2) + 255) / 256 * 256;
 }
 size_t few_workspace(int batch, int ctas) {
-  return few_parts_offset(batch, ctas) + 2ull * ctas * (32 * kD + 2 * 32) * sizeof(float);
+  return few_parts_offset(batch, ctas) + 2ull * ctas * (kRows * kD + 2 * kRows) * sizeof(float);
 }
 
-template <int RN, bool PLAIN>
+template <bool PLAIN>
 int launch_few(const CUtensorMap& tk, const CUtensorMap& tv, const FewParams& p, int ctas, cudaStream_t s) {
   static bool set[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   dev = (dev < 0 || dev >= 64) ? 0 : dev;
   if (!set[dev]) {
-    if (cudaFuncSetAttribute(fp8_few_rows_kernel<RN, PLAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(FewCfg<RN>::kSmem)) != cudaSuccess)
+    if (cudaFuncSetAttribute(fp8_few_rows_kernel<PLAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(kFewSmem)) != cudaSuccess)
       return set_error(DYLLM_ERR_CUDA, "attention_salient_rows_fp8: cudaFuncSetAttribute failed: %s",
                        cudaGetErrorString(cudaGetLastError()));
     set[dev] = true;
   }
-  DYLLM_LAUNCH((fp8_few_rows_kernel<RN, PLAIN>), ctas, kFewThreads, FewCfg<RN>::kSmem, s, tk, tv, p);
+  DYLLM_LAUNCH(fp8_few_rows_kernel<PLAIN>, ctas, kFewThreads, kFewSmem, s, tk, tv, p);
   return check_launch("attention_salient_rows_fp8");
 }
 
@@ -848,7 +1091,7 @@ extern "C" {
 size_t dyllm_attention_salient_rows_fp8_workspace_bytes(int num_salient, int batch, int num_heads, int num_kv_heads) {
   if (num_salient <= 0 || batch <= 0 || num_heads <= 0 || num_kv_heads <= 0)
     return 0;
-  return few_workspace(batch, 2 * sm_count());
+  return few_workspace(batch, sm_count());
 }
 
 int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, const void* k_codes, const float* k_scales,
@@ -878,6 +1121,8 @@ int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, co
                   "attention_salient_rows_fp8: q, codes and out must be 16-byte aligned");
   DYLLM_REQUIRE(k_rows < (1ll << 31) && v_rows < (1ll << 31), DYLLM_ERR_UNSUPPORTED,
                 "attention_salient_rows_fp8: caches of 2^31 rows or more");
+  DYLLM_REQUIRE(static_cast<int64_t>(num_salient) * num_heads < (1ll << 31), DYLLM_ERR_UNSUPPORTED,
+                "attention_salient_rows_fp8: 2^31 output rows or more");
   DYLLM_REQUIRE(ldq % 8 == 0 && ldq >= static_cast<int64_t>(num_heads) * kD, DYLLM_ERR_INVALID_ARGUMENT,
                 "attention_salient_rows_fp8: the row pitch of q (%lld) must be a multiple of 8 and at least heads * 128",
                 static_cast<long long>(ldq));
@@ -910,7 +1155,7 @@ int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, co
   p.slopes = slopes;
   p.ranges = reinterpret_cast<const int2*>(key_ranges);
   FewParams f = {};
-  const int ctas = 2 * sm_count();
+  const int ctas = sm_count();
   DYLLM_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, DYLLM_ERR_INVALID_ARGUMENT,
                 "attention_salient_rows_fp8: the workspace must be 16-byte aligned");
   DYLLM_REQUIRE(workspace && workspace_bytes >= few_workspace(batch, ctas), DYLLM_ERR_WORKSPACE,
@@ -936,12 +1181,7 @@ int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, co
   if (rc != DYLLM_OK)
     return rc;
   const bool plain = softcap == 0.f && !slopes && !key_ranges;
-  const bool one = static_cast<int64_t>(max_rows_per_seq) * (num_heads / num_kv_heads) <= 16;
-  if (one)
-    rc = plain ? launch_few<16, true>(tk, tv, f, ctas, st) : launch_few<16, false>(tk, tv, f, ctas, st);
-  else
-    rc = plain ? launch_few<32, true>(tk, tv, f, ctas, st) : launch_few<32, false>(tk, tv, f, ctas, st);
-  return rc;
+  return plain ? launch_few<true>(tk, tv, f, ctas, st) : launch_few<false>(tk, tv, f, ctas, st);
 }
 
 }  // extern "C"
