@@ -99,7 +99,7 @@ constexpr uint32_t kFewSmem = (kRing + kChunk / 2) * kTileBytes + 4 * kQBytes + 
 
 struct FewParams {
   Fp8AttnParams a;
-  const int2* spans;           // per sequence: keys that any of its listed rows sees (null: all)
+  const int2* spans;           // per tile of rows: keys that any of them sees (null: all)
   unsigned long long* tickets; // one per CTA
   float* parts;                // two per CTA: [rows][128] sums, [rows] maxima, [rows] sums of weights
   unsigned long long launch_id;
@@ -127,36 +127,38 @@ __device__ __forceinline__ bool last_to_join(unsigned long long* word, int parts
 
 // A sequence as the work list sees it.
 struct SeqWork {
-  int b, row0, rows, tiles, units;      // rows: (listed row, head of the group) pairs
-  int lo, hi;                           // keys
+  int b, row0, rows, tiles;             // rows: (listed row, head of the group) pairs
+  int len;                              // keys
   int k0, v0;                           // first rows in the caches
 };
 template <int MROWS>
-__device__ __forceinline__ SeqWork seq_work(const FewParams& p, int b) {
+__device__ __forceinline__ SeqWork seq_work(const Fp8AttnParams& a, int b) {
   SeqWork w = {};
   w.b = b;
-  if (b >= p.a.batch)
+  if (b >= a.batch)
     return w;
   // all loads that do not depend on one another first: a CTA starts with this chain
-  const int s0 = __ldg(p.a.cu_sal + b), s1 = __ldg(p.a.cu_sal + b + 1);
-  const int2 span = p.spans ? __ldg(p.spans + b) : make_int2(0, 0);
-  const KeyRange kr = keys_of(p.a, b);
-  w.row0 = min(s0, p.a.num_salient);
-  const int n = min(s1, p.a.num_salient) - w.row0;
+  const int s0 = __ldg(a.cu_sal + b), s1 = __ldg(a.cu_sal + b + 1);
+  const KeyRange kr = keys_of(a, b);
+  w.row0 = min(s0, a.num_salient);
+  const int n = min(s1, a.num_salient) - w.row0;
   if (n <= 0)
     return w;
-  w.rows = n * (p.a.H / p.a.Hkv);
+  w.rows = n * (a.H / a.Hkv);
   w.k0 = static_cast<int>(kr.k0);
   w.v0 = static_cast<int>(kr.v0);
-  w.hi = kr.len;
-  if (p.spans) {
-    w.lo = span.x;
-    w.hi = span.y;
-  }
+  w.len = kr.len;
   w.tiles = (w.rows + MROWS - 1) / MROWS;
-  w.units = max(1, (w.hi - w.lo + kUnitKeys - 1) / kUnitKeys);
   return w;
 }
+
+// A part of a tile as the scheduler hands it to the other warps.
+struct PartInfo {
+  int begin, end;              // keys; end < 0: the share is done
+  int owner, parts, slot;      // several CTAs hold the tile (parts > 1): the first of them, how many, this CTA's slot
+  int b, hk, row0, rows, t0;   // sequence, key head, the sequence's first listed row, its (row, head) pairs, the tile's first
+  int k0, v0, len;             // the sequence's first rows in the caches, its keys
+};
 
 // a / b of non-negative numbers; the 64-bit routine only where it is needed.
 __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
@@ -164,8 +166,10 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
     return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
   return a / b;
 }
+__device__ __forceinline__ int units_of(int2 span) { return max(1, (span.y - span.x + kUnitKeys - 1) / kUnitKeys); }
 
-// Walks over the parts of tiles that a CTA's share of the units consists of.  Uniform over a warp.
+// Walks over the parts of tiles that a CTA's share of the units consists of, in the order (sequence, tile, key head, keys).
+// Uniform over a warp.
 //
 // Shares are cut at total * i / ctas, but no part of a tile is shorter than kMinPart units: a cut nearer to an end of its
 // tile moves there.  (Joining the parts of a tile costs a CTA about 7 us, a unit 1 to 2.)
@@ -175,7 +179,9 @@ struct Walk {
   SeqWork w;
   int64_t total, end;                   // units: of the launch, end of the share before its cut is moved
   int64_t tile_first;                   // first unit of the tile in the launch
-  int hk, tile, first, last;            // the part: units [first, last) of the tile
+  int tile_base;                        // number of the sequence's first tile
+  int2 span;                            // keys that rows of the tile see
+  int hk, tile, units, first, last;     // the part: units [first, last) of the tile's
   int ctas;                             // shares
   bool begun;
 
@@ -184,22 +190,48 @@ struct Walk {
       return cut;
     return 2 * cut < units ? 0 : units;
   }
+  static __device__ __forceinline__ int scan(int x, int lane) {      // sum of the lanes up to this one
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, x, s);
+      if (lane >= s)
+        x += o;
+    }
+    return x;
+  }
+  // Units of a sequence's tiles, for one key head.
+  static __device__ __forceinline__ int64_t seq_units(const FewParams& p, const SeqWork& x, int base) {
+    if (!p.spans)
+      return static_cast<int64_t>(x.tiles) * units_of(make_int2(0, x.len));
+    int64_t sum = 0;
+    for (int t = 0; t < x.tiles; ++t)
+      sum += units_of(__ldg(p.spans + base + t));
+    return sum;
+  }
+  __device__ __forceinline__ void open(const FewParams& p) {
+    span = p.spans ? __ldg(p.spans + tile_base + tile) : make_int2(0, w.len);
+    units = units_of(span);
+  }
   __device__ __forceinline__ void start(const FewParams& p) {
     const int lane = threadIdx.x & 31;
-    int64_t sum = 0, tiles = 0;
+    int64_t sum = 0;
+    int all_tiles = 0;
     SeqWork x;
+    int x_base = 0;
+    int64_t mine = 0;
     for (int base = 0; base < p.a.batch; base += 32) {
-      x = seq_work<MROWS>(p, base + lane);
-      sum += static_cast<int64_t>(x.tiles) * x.units;
-      tiles += x.tiles;
+      x = seq_work<MROWS>(p.a, base + lane);
+      const int upto = scan(x.tiles, lane);
+      x_base = all_tiles + upto - x.tiles;
+      all_tiles += __shfl_sync(0xffffffffu, upto, 31);
+      mine = seq_units(p, x, x_base);
+      sum += mine;
     }
 #pragma unroll
-    for (int s = 16; s; s >>= 1) {
+    for (int s = 16; s; s >>= 1)
       sum += __shfl_xor_sync(0xffffffffu, sum, s);
-      tiles += __shfl_xor_sync(0xffffffffu, tiles, s);
-    }
     total = sum * p.a.Hkv;
-    ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), max(tiles * p.a.Hkv, total / kMinPart)));
+    ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), max(static_cast<int64_t>(all_tiles) * p.a.Hkv, total / kMinPart)));
     end = tile_first = 0;
     first = 0;
     begun = false;
@@ -208,54 +240,75 @@ struct Walk {
     const int64_t at = share(blockIdx.x);
     end = share(blockIdx.x + 1);
     int64_t before = 0;
+    all_tiles = 0;
     for (int base = 0;; base += 32) {
-      if (p.a.batch > 32)
-        x = seq_work<MROWS>(p, base + lane);
-      const int64_t mine = static_cast<int64_t>(x.tiles) * x.units * p.a.Hkv;
-      int64_t scan = mine;
+      if (p.a.batch > 32) {
+        x = seq_work<MROWS>(p.a, base + lane);
+        const int upto = scan(x.tiles, lane);
+        x_base = all_tiles + upto - x.tiles;
+        all_tiles += __shfl_sync(0xffffffffu, upto, 31);
+        mine = seq_units(p, x, x_base);
+      }
+      const int64_t here = mine * p.a.Hkv;
+      int64_t upto = here;
 #pragma unroll
       for (int s = 1; s < 32; s <<= 1) {
-        const int64_t o = __shfl_up_sync(0xffffffffu, scan, s);
+        const int64_t o = __shfl_up_sync(0xffffffffu, upto, s);
         if (lane >= s)
-          scan += o;
+          upto += o;
       }
-      const unsigned hit = __ballot_sync(0xffffffffu, before + scan > at);
+      const unsigned hit = __ballot_sync(0xffffffffu, before + upto > at);
       if (hit) {
         const int src = __ffs(hit) - 1;
-        before += __shfl_sync(0xffffffffu, scan - mine, src);
-        w = seq_work<MROWS>(p, base + src);
+        before += __shfl_sync(0xffffffffu, upto - here, src);
+        tile_base = __shfl_sync(0xffffffffu, x_base, src);
+        w = seq_work<MROWS>(p.a, base + src);
         break;
       }
-      before += __shfl_sync(0xffffffffu, scan, 31);
+      before += __shfl_sync(0xffffffffu, upto, 31);
     }
-    const int64_t t = quotient(at - before, w.units);
-    const int cut = static_cast<int>(at - before - t * w.units);
-    tile_first = at - cut;
-    hk = static_cast<int>(quotient(t, w.tiles));
-    tile = static_cast<int>(t - static_cast<int64_t>(hk) * w.tiles);
-    first = moved(cut, w.units);
+    tile = 0;
+    if (!p.spans) {
+      const int64_t t = quotient(at - before, static_cast<int64_t>(units_of(make_int2(0, w.len))) * p.a.Hkv);
+      tile = static_cast<int>(t);
+      open(p);
+      tile_first = before + t * units * p.a.Hkv;
+    } else {
+      tile_first = before;
+      for (;; ++tile) {
+        open(p);
+        if (tile_first + static_cast<int64_t>(units) * p.a.Hkv > at)
+          break;
+        tile_first += static_cast<int64_t>(units) * p.a.Hkv;
+      }
+    }
+    hk = static_cast<int>(quotient(at - tile_first, units));
+    tile_first += static_cast<int64_t>(hk) * units;
+    first = moved(static_cast<int>(at - tile_first), units);
   }
   // The next part, false at the end of the share.
   __device__ __forceinline__ bool next(const FewParams& p) {
     if (tile_first >= end)
       return false;
-    if (begun || first == w.units) {
+    if (begun || first == units) {
       first = 0;
-      tile_first += w.units;
+      tile_first += units;
       if (tile_first >= end)
         return false;
-      if (++tile == w.tiles) {
-        tile = 0;
-        if (++hk == p.a.Hkv) {
-          hk = 0;
-          do
-            w = seq_work<MROWS>(p, w.b + 1);
-          while (w.tiles == 0);
+      if (++hk == p.a.Hkv) {
+        hk = 0;
+        if (++tile == w.tiles) {
+          tile = 0;
+          do {
+            tile_base += w.tiles;
+            w = seq_work<MROWS>(p.a, w.b + 1);
+          } while (w.tiles == 0);
         }
+        open(p);
       }
     }
     begun = true;
-    last = tile_first + w.units <= end ? w.units : moved(static_cast<int>(end - tile_first), w.units);
+    last = tile_first + units <= end ? units : moved(static_cast<int>(end - tile_first), units);
     return last > first;
   }
   // First unit of a share before its cut is moved; CTA that holds the first part of the tile; number of its parts.
@@ -265,7 +318,18 @@ struct Walk {
   }
   __device__ __forceinline__ int owner() const { return first_cut() - 1; }
   __device__ __forceinline__ int parts() const {
-    return static_cast<int>(quotient((tile_first + w.units - kMinPart + 1) * ctas + total - 1, total)) - first_cut() + 1;
+    return static_cast<int>(quotient((tile_first + units - kMinPart + 1) * ctas + total - 1, total)) - first_cut() + 1;
+  }
+  // What the other warps need to know of the part.
+  __device__ __forceinline__ PartInfo info() const {
+    const int begin = span.x + first * kUnitKeys;
+    PartInfo v = {begin, min(span.y, span.x + last * kUnitKeys), 0, 1, 0, w.b, hk, w.row0, w.rows, tile * MROWS, w.k0, w.v0, w.len};
+    if (last - first < units) {
+      v.owner = owner();
+      v.parts = parts();
+      v.slot = 2 * static_cast<int>(blockIdx.x) + (first == 0 ? 1 : 0);
+    }
+    return v;
   }
 };
 
@@ -348,6 +412,38 @@ __device__ __forceinline__ void umma_tile(uint32_t d_tmem, uint32_t a_addr, uint
 // stays there, and an MMA issues every 33 cycles (its A operand's shared-memory read) instead of every 90.
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __reduce_max_sync(0xffffffffu, x); }
 
+__device__ __forceinline__ void loaders_sync() { asm volatile("bar.sync 7, 128;" ::: "memory"); }
+
+// Zeros for the rows t0 .. t0 + count - 1 of a sequence's (listed row, head) pairs; one warp.
+__device__ __forceinline__ void zero_rows(const Fp8AttnParams& a, const SeqWork& w, int hk, int t0, int count) {
+  const int group = a.H / a.Hkv;
+  for (int t = t0; t < min(t0 + count, w.rows); ++t) {
+    const int i = t / group;
+    __nv_bfloat16* dst = a.out + ((static_cast<int64_t>(w.row0) + i) * a.H + hk * group + t - i * group) * kD;
+    *reinterpret_cast<uint2*>(dst + (threadIdx.x & 31) * 4) = make_uint2(0u, 0u);
+  }
+}
+
+// Sixteen elements of a query times `inv` as codes: e4m3, and the rest in e5m2.
+__device__ __forceinline__ void split_query(const uint4& x0, const uint4& x1, float inv, uint4& hi, uint4& lo) {
+  float y[16];
+  bf16x8_to_float(x0, y);
+  bf16x8_to_float(x1, y + 8);
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float z[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      z[e] = y[4 * j + e] * inv;
+    h[j] = fp8_pack2(z[0], z[1]) | fp8_pack2(z[2], z[3]) << 16;
+    const float2 u = fp8_to_float2(h[j] & 0xffffu), v = fp8_to_float2(h[j] >> 16);
+    l[j] = fp8_pack2_e5m2(z[0] - u.x, z[1] - u.y) | fp8_pack2_e5m2(z[2] - v.x, z[3] - v.y) << 16;
+  }
+  hi = make_uint4(h[0], h[1], h[2], h[3]);
+  lo = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
 constexpr float kNothing = -1.0e30f;      // maximum of no scores (finite: it takes part in differences)
 
 // Four weights (times 256) as codes and the codes of 16 times what they leave.  By way of half precision (2^-11).
@@ -364,14 +460,6 @@ __device__ __forceinline__ void split_weights(const float (&w)[4], uint32_t& hi,
   hi = h[0] | h[1] << 16;
   lo = l[0] | l[1] << 16;
 }
-
-// A part of a tile as the scheduler hands it to the other warps.
-struct PartInfo {
-  int begin, end;              // keys; end < 0: the share is done
-  int owner, parts, slot;      // several CTAs hold the tile (parts > 1): the first of them, how many, this CTA's slot
-  int b, hk, row0, rows, t0;   // sequence, key head, the sequence's first listed row, its (row, head) pairs, the tile's first
-  int k0, v0, len;             // the sequence's first rows in the caches, its keys
-};
 
 // What a tile's rows are to the softmax warps.
 struct RowInfo {
@@ -478,20 +566,13 @@ struct QueryLoad {
     asm volatile("bar.sync 6, 256;" ::: "memory");
     const int r = tid >> 3, part = tid & 7;
     const float inv = fp8_inverse(fp8_scale_bits(*amax));
-    uint32_t hi[4], lo[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float z[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        z[e] = finite ? y[4 * j + e] * inv : 0.f;
-      hi[j] = fp8_pack2(z[0], z[1]) | fp8_pack2(z[2], z[3]) << 16;
-      const float2 u = fp8_to_float2(hi[j] & 0xffffu), v = fp8_to_float2(hi[j] >> 16);
-      lo[j] = fp8_pack2_e5m2(z[0] - u.x, z[1] - u.y) | fp8_pack2_e5m2(z[2] - v.x, z[3] - v.y) << 16;
-    }
+    uint4 hi, lo;
+    if (!finite)
+      x0 = x1 = make_uint4(0u, 0u, 0u, 0u);
+    split_query(x0, x1, inv, hi, lo);
     uint8_t* dst = q_smem + r * kD + ((part ^ (r & 7)) << 4);
-    *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    *reinterpret_cast<uint4*>(dst + kRows * kD) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    *reinterpret_cast<uint4*>(dst) = hi;
+    *reinterpret_cast<uint4*>(dst + kRows * kD) = lo;
     if (part == 0) {
       RowInfo v = {};
       v.out = t < w.rows ? (w.row0 + t / (a.H / a.Hkv)) * a.H + head : -1;
@@ -595,16 +676,10 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
     // ---------------------------------------------------------------- scheduler: the parts of this CTA's share
     Walk<kRows> walk;
     walk.start(p);
-    const int group = a.H / a.Hkv;
     for (int n = 0;;) {
       const bool more = walk.next(p);
-      const SeqWork& w = walk.w;
-      if (more && w.hi <= w.lo) {      // no keys: zeros
-        for (int r = 0; r < kRows && walk.tile * kRows + r < w.rows; ++r) {
-          const int t = walk.tile * kRows + r, i = t / group;
-          __nv_bfloat16* dst = a.out + ((static_cast<int64_t>(w.row0) + i) * a.H + walk.hk * group + t - i * group) * kD;
-          *reinterpret_cast<uint2*>(dst + lane * 4) = make_uint2(0u, 0u);
-        }
+      if (more && walk.span.y <= walk.span.x) {      // no keys: zeros
+        zero_rows(a, walk.w, walk.hk, walk.tile * kRows, kRows);
         continue;
       }
       const int slot = n % kParts;
@@ -613,15 +688,8 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
       if (lane == 0) {
         PartInfo v = {};
         v.end = -1;
-        if (more) {
-          const int begin = w.lo + walk.first * kUnitKeys;
-          v = {begin, min(w.hi, w.lo + walk.last * kUnitKeys), 0, 1, 0, w.b, walk.hk, w.row0, w.rows, walk.tile * kRows, w.k0, w.v0, w.hi};
-          if (walk.last - walk.first < w.units) {
-            v.owner = walk.owner();
-            v.parts = walk.parts();
-            v.slot = 2 * static_cast<int>(blockIdx.x) + (walk.first == 0 ? 1 : 0);
-          }
-        }
+        if (more)
+          v = walk.info();
         s_part[slot] = v;
         s_amax[slot] = 0;
       }
@@ -1031,21 +1099,654 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
   }
 }
 
-// Keys that any listed row of a sequence sees; one warp per sequence.
+// ----------------------------------------------------------------------------------------------
+// Many rows per sequence: bound by the exponentials and the instructions around them (a tile of 128 rows x 128 keys takes the
+// tensor cores 950 cycles, its exponentials 1024).
+//
+// Tiles of 128 (listed row, query head) pairs, rows in the M = 128 of the products:
+//   S = Q K^T    A: the queries as e4m3 + e5m2 (two products into one accumulator), B: the K tile as loaded (K-major)
+//   O = P V      A: the weights as e4m3 + e5m2, B: the V tile as loaded (MN-major)
+// Two teams of four softmax warps take the key tiles in turn, thread = row, each with scores, sums and a maximum of its own, and
+// meet when the part ends.  A weight is 64 * 2^(t - reference); the reference follows the maximum in steps, so that the sums are
+// rescaled only where a score lies more than 2.8 (log2) above it.  A weight is off by 2^-7 of itself or by 2^-23 of the largest.
+// Four loader warps stage the queries of the next part and the scales of the next tiles.
+// ----------------------------------------------------------------------------------------------
+constexpr int kManyRows = 128;
+constexpr int kManyRing = 4;                                 // slots of one K or V tile
+constexpr int kScaleSlots = 8;                               // tiles whose scales are staged ahead
+constexpr int kTeamWarps = 4, kManyThreads = 32 * (3 + 2 * kTeamWarps + 4);
+constexpr uint32_t kManyQBytes = kManyRows * kD;             // e4m3 or e5m2 part of the queries of a tile
+constexpr uint32_t kManySmem = (kManyRing + 4) * kTileBytes + 4 * kManyQBytes + kScaleSlots * 3 * kUnitKeys * sizeof(float) + 1024;
+constexpr float kWeightLog2 = 6.f;                           // the reference's weight: 2^6
+constexpr float kHeadroom = 2.8f;                            // 2^(6 + 2.8) < 448
+
+__device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 ra, rb, rc, rd;\n mov.b64 ra, {%2, %3};\n mov.b64 rb, {%4, %5};\n mov.b64 rc, {%6, %7};\n"
+      " fma.rn.f32x2 rd, ra, rb, rc;\n mov.b64 {%0, %1}, rd;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 ra, rb, rd;\n mov.b64 ra, {%2, %3};\n mov.b64 rb, {%4, %5};\n"
+      " add.rn.f32x2 rd, ra, rb;\n mov.b64 {%0, %1}, rd;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ void teams_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// Four weights as codes, and what they leave in e5m2.  By way of half precision (2^-11).
+__device__ __forceinline__ void split_weights_e5m2(float2 a, float2 b, uint32_t& hi, uint32_t& lo) {
+  const __half2 x = __floats2half2_rn(a.x, a.y), y = __floats2half2_rn(b.x, b.y);
+  const uint32_t h0 = fp8_pack_half2(*reinterpret_cast<const uint32_t*>(&x)), h1 = fp8_pack_half2(*reinterpret_cast<const uint32_t*>(&y));
+  const uint32_t u = fp8_to_half2(h0), v = fp8_to_half2(h1);
+  const __half2 r = __hsub2(x, *reinterpret_cast<const __half2*>(&u)), s = __hsub2(y, *reinterpret_cast<const __half2*>(&v));
+  hi = __byte_perm(h0, h1, 0x5410);
+  lo = __byte_perm(fp8_pack_half2_e5m2(*reinterpret_cast<const uint32_t*>(&r)), fp8_pack_half2_e5m2(*reinterpret_cast<const uint32_t*>(&s)), 0x5410);
+}
+
+// Joins the parts of a tile, as join_parts: a thread has its row and 64 head dimensions from c0 on.
+__device__ __forceinline__ bool join_many(const FewParams& p, int slot, int owner, int parts, int row, int c0, float& top, float& l,
+                                          float (&o)[64], int tid, int* joins) {
+  constexpr int kPart = kManyRows * kD + 2 * kManyRows;
+  float* mine = p.parts + static_cast<int64_t>(slot) * kPart;
+#pragma unroll
+  for (int j = 0; j < 64; j += 4)
+    *reinterpret_cast<float4*>(mine + row * kD + c0 + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+  if (c0 == 0) {
+    mine[kManyRows * kD + row] = top;
+    mine[kManyRows * kD + kManyRows + row] = l;
+  }
+  __threadfence();
+  teams_sync();
+  if (tid == 0) {
+    open_join(p.tickets + owner, p.launch_id);
+    *joins = last_to_join(p.tickets + owner, parts) ? 1 : 0;
+  }
+  teams_sync();
+  if (!*joins)
+    return false;
+  __threadfence();
+  const float* one = p.parts + (2 * static_cast<int64_t>(owner) + 1) * kPart;
+  const float* rest = p.parts + 2 * static_cast<int64_t>(owner) * kPart;
+  top = kNothing;
+  l = 0.f;
+#pragma unroll
+  for (int j = 0; j < 64; ++j)
+    o[j] = 0.f;
+  for (int i = 0; i < parts; ++i)
+    top = fmaxf(top, __ldcg((i == 0 ? one : rest + 2 * static_cast<int64_t>(i) * kPart) + kManyRows * kD + row));
+  for (int i = 0; i < parts; ++i) {
+    const float* src = i == 0 ? one : rest + 2 * static_cast<int64_t>(i) * kPart;
+    const float mul = exp2f(__ldcg(src + kManyRows * kD + row) - top);
+    l += __ldcg(src + kManyRows * kD + kManyRows + row) * mul;
+#pragma unroll
+    for (int j = 0; j < 64; j += 4) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(src + row * kD + c0 + j));
+      o[j] = fmaf(x.x, mul, o[j]);
+      o[j + 1] = fmaf(x.y, mul, o[j + 1]);
+      o[j + 2] = fmaf(x.z, mul, o[j + 2]);
+      o[j + 3] = fmaf(x.w, mul, o[j + 3]);
+    }
+  }
+  return true;
+}
+
+template <bool PLAIN>
+__global__ void __launch_bounds__(kManyThreads, 1)
+fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const FewParams p) {
+  pdl_wait();      // programmatic dependent launch: nothing before this reads an earlier kernel's data
+  pdl_trigger();
+  const Fp8AttnParams& a = p.a;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* p_smem = ring + kManyRing * kTileBytes;           // per team [128 rows][128 keys]: e4m3, then e5m2
+  uint8_t* q_smem = p_smem + 4 * kTileBytes;                 // two slots of [128 rows][128] e4m3, then e5m2
+  float* sc_smem = reinterpret_cast<float*>(q_smem + 4 * kManyQBytes);      // per tile: K scale * factors, V exponent, 1 / V scale
+  __shared__ uint64_t full[kManyRing], empty[kManyRing], part_full[kParts], part_done[kParts], q_full[2], q_free[2], s_full[2], s_free[2],
+      sc_full[kScaleSlots], sc_free[kScaleSlots], p_full[2], pv_done[2], o_free;
+  __shared__ PartInfo s_part[kParts];
+  __shared__ uint32_t tmem_slot, s_amax[2];
+  __shared__ int abort_flag, joins;
+  __shared__ RowInfo s_row[2][kManyRows];
+  __shared__ float2 s_ml[2][2][kManyRows];   // of parts in turn, per team: reference and sum of weights
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < kManyRing; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < kParts; ++i) {
+      mbar_init(&part_full[i], 1);
+      mbar_init(&part_done[i], 2 * kTeamWarps + 2 + 4);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 4);
+      mbar_init(&q_free[i], 2 * kTeamWarps);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_free[i], kTeamWarps);
+      mbar_init(&p_full[i], kTeamWarps);
+      mbar_init(&pv_done[i], 1);
+    }
+    for (int i = 0; i < kScaleSlots; ++i) {
+      mbar_init(&sc_full[i], 4);
+      mbar_init(&sc_free[i], kTeamWarps);
+    }
+    mbar_init(&o_free, 2 * kTeamWarps);
+    fence_mbar_init();
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;      // a team's S: columns 0 and 128, its O: 256 and 384
+  const int group = a.H / a.Hkv;
+
+  if (warp == 2) {
+    // ---------------------------------------------------------------- scheduler
+    Walk<kManyRows> walk;
+    walk.start(p);
+    for (int n = 0;;) {
+      const bool more = walk.next(p);
+      if (more && walk.span.y <= walk.span.x) {      // no keys: zeros
+        zero_rows(a, walk.w, walk.hk, walk.tile * kManyRows, kManyRows);
+        continue;
+      }
+      const int slot = n % kParts;
+      if (n >= kParts && !mbar_wait(&part_done[slot], (n / kParts - 1) & 1, &abort_flag, p.status_word, 500))
+        break;
+      if (lane == 0) {
+        PartInfo v = {};
+        v.end = -1;
+        if (more)
+          v = walk.info();
+        s_part[slot] = v;
+      }
+      warp_arrive(&part_full[slot]);
+      ++n;
+      if (!more)
+        break;
+    }
+  } else if (warp == 0) {
+    // ---------------------------------------------------------------- producer: K of a tile before V of the last
+    int n = 0;
+    auto load = [&](const CUtensorMap* map, int row, int left, int x) {
+      const int slot = n % kManyRing;
+      if (n >= kManyRing)
+        mbar_wait(&empty[slot], (n / kManyRing - 1) & 1, &abort_flag, p.status_word, 501);
+      if (elect_one()) {
+        const int boxes = min(4, (left + 31) / 32);      // no box of keys that do not belong to the part
+        mbar_arrive_expect_tx(&full[slot], boxes * 32 * kD);
+        for (int j = 0; j < boxes; ++j)
+          tma_load_2d(ring + slot * kTileBytes + j * 32 * kD, map, &full[slot], x, row + 32 * j);
+      }
+      __syncwarp();
+      ++n;
+    };
+    Chunks c = {};
+    int v_row = 0, v_left = 0, v_x = 0;
+    bool owed = false;
+    for (bool more = c.open(part_full, part_done, s_part, &abort_flag, p.status_word); more;) {
+      for (int i = 0; i < c.tiles; ++i) {
+        const int key = c.begin + i * kUnitKeys;
+        load(&tmap_k, c.k0 + key, c.end - key, c.hk * kD);
+        if (owed)
+          load(&tmap_v, v_row, v_left, v_x);
+        owed = true;
+        v_row = c.v0 + key;
+        v_left = c.end - key;
+        v_x = c.hk * kD;
+      }
+      ++c.n;
+      more = c.open(part_full, part_done, s_part, &abort_flag, p.status_word);
+    }
+    if (owed)
+      load(&tmap_v, v_row, v_left, v_x);
+    // a CTA may not end with copies on their way, also when a wait of another warp has given up
+    for (int i = max(0, n - kManyRing); i < n; ++i)
+      mbar_wait(&full[i % kManyRing], (i / kManyRing) & 1, &abort_flag, p.status_word, 502);
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer: scores of a tile before the sums of the last
+    constexpr uint32_t idesc_hi = umma_idesc_f8(128, 128, 1 * 0, 0, 0, 0), idesc_lo = umma_idesc_f8(128, 128, 1, 0, 0, 0);
+    constexpr uint32_t idesc_pv = umma_idesc_f8(128, 128, 0, 0, 0, 1), idesc_pv_lo = umma_idesc_f8(128, 128, 1, 0, 0, 1);
+    const uint32_t ring_addr = smem_u32(ring), p_addr = smem_u32(p_smem), t_s = uniform(tmem), t_o = t_s + 256;
+    int n = 0, n_s = 0, n_p = 0;
+    auto sums = [&](int part, int tile) {      // P V of the tile before, the tile-th of its part
+      const int team = n_p & 1;
+      const int slot = n % kManyRing;
+      mbar_wait(&full[slot], (n / kManyRing) & 1, &abort_flag, p.status_word, 506);
+      if (tile == 0 && part > 0)
+        mbar_wait(&o_free, (part - 1) & 1, &abort_flag, p.status_word, 508);
+      mbar_wait(&p_full[team], (n_p >> 1) & 1, &abort_flag, p.status_word, 507);
+      tc_fence_after_sync();
+      if (elect_one()) {
+        const uint32_t v_addr = ring_addr + slot * kTileBytes;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {      // 32 keys: 32 bytes of the weights' rows, 32 rows of V
+          const uint32_t w_addr = p_addr + team * 2 * kTileBytes + 32 * kk;
+          umma_tile(t_o + team * 128, w_addr, v_addr + kk * 4096, idesc_pv, tile < 2 && kk == 0 ? 0u : 1u);
+          umma_tile(t_o + team * 128, w_addr + kTileBytes, v_addr + kk * 4096, idesc_pv_lo, 1u);
+        }
+        umma_commit(&empty[slot]);
+        umma_commit(&pv_done[team]);
+      }
+      __syncwarp();
+      ++n;
+      ++n_p;
+    };
+    Chunks c = {};
+    int owed_part = -1, owed_tile = 0;
+    for (bool more = c.open(part_full, part_done, s_part, &abort_flag, p.status_word); more;) {
+      mbar_wait(&q_full[c.n & 1], (c.n >> 1) & 1, &abort_flag, p.status_word, 503);
+      const uint32_t q_addr = smem_u32(q_smem) + (c.n & 1) * 2 * kManyQBytes;
+      for (int i = 0; i < c.tiles; ++i) {
+        const int buf = n_s & 1, slot = n % kManyRing;
+        if (n_s >= 2)
+          mbar_wait(&s_free[buf], ((n_s >> 1) - 1) & 1, &abort_flag, p.status_word, 504);
+        mbar_wait(&full[slot], (n / kManyRing) & 1, &abort_flag, p.status_word, 505);
+        tc_fence_after_sync();
+        if (elect_one()) {
+          const uint32_t k_addr = ring_addr + slot * kTileBytes;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {      // 32 head dimensions = 32 bytes a step
+            umma_tile(t_s + buf * 128, q_addr + 32 * kk, k_addr + 32 * kk, idesc_hi, kk != 0 ? 1u : 0u);
+            umma_tile(t_s + buf * 128, q_addr + kManyQBytes + 32 * kk, k_addr + 32 * kk, idesc_lo, 1u);
+          }
+          umma_commit(&empty[slot]);
+          umma_commit(&s_full[buf]);
+        }
+        __syncwarp();
+        ++n;
+        ++n_s;
+        if (owed_part >= 0)
+          sums(owed_part, owed_tile);
+        owed_part = c.n;
+        owed_tile = i;
+      }
+      ++c.n;
+      more = c.open(part_full, part_done, s_part, &abort_flag, p.status_word);
+    }
+    if (owed_part >= 0)
+      sums(owed_part, owed_tile);
+  } else if (warp >= 3 + 2 * kTeamWarps) {
+    // ---------------------------------------------------------------- loaders: queries of a part, scales of its tiles
+    const int tid = threadIdx.x - 32 * (3 + 2 * kTeamWarps);
+    int n_sc = 0;
+    for (int n = 0;; ++n) {
+      const int slot = n % kParts, qb = n & 1;
+      if (!mbar_wait(&part_full[slot], (n / kParts) & 1, &abort_flag, p.status_word, 510))
+        break;
+      const PartInfo w = s_part[slot];
+      loaders_sync();
+      warp_arrive(&part_done[slot]);
+      if (w.end < 0)
+        break;
+      if (n >= 2)
+        mbar_wait(&q_free[qb], ((n >> 1) - 1) & 1, &abort_flag, p.status_word, 511);
+      // queries: eight threads a row, 16 rows at a time, twice: the largest element, then the codes
+      if (tid == 0)
+        s_amax[qb] = 0;
+      int row[8], head[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int t = w.t0 + 16 * k + (tid >> 3), i = t / group;
+        head[k] = w.hk * group + t - i * group;
+        row[k] = t < w.rows ? __ldg(a.idx + w.row0 + i) : -1;
+        row[k] = row[k] >= a.total_q ? -1 : row[k];
+      }
+      loaders_sync();
+      uint32_t finite = 0;
+      {
+        uint32_t top = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          uint4 x0 = make_uint4(0u, 0u, 0u, 0u), x1 = x0;
+          if (row[k] >= 0) {
+            const uint4* src = reinterpret_cast<const uint4*>(a.q + row[k] * a.ldq + head[k] * kD) + (tid & 7) * 2;
+            x0 = __ldg(src);
+            x1 = __ldg(src + 1);
+          }
+          float y[16];
+          bf16x8_to_float(x0, y);
+          bf16x8_to_float(x1, y + 8);
+          uint32_t m = 0;
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            m = max(m, __float_as_uint(y[j]) & 0x7fffffffu);
+          m = fp8_amax8(m);
+          if (m < 0x7f800000u) {
+            finite |= 1u << k;
+            top = max(top, m);
+          }
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (lane == 0)
+          atomicMax(&s_amax[qb], top);
+      }
+      loaders_sync();
+      const uint32_t scale = fp8_scale_bits(s_amax[qb]);
+      const float inv = fp8_inverse(scale);
+      uint8_t* q_dst = q_smem + qb * 2 * kManyQBytes;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int r = 16 * k + (tid >> 3), part = tid & 7;
+        uint4 x0 = make_uint4(0u, 0u, 0u, 0u), x1 = x0;
+        if (row[k] >= 0 && (finite >> k & 1)) {
+          const uint4* src = reinterpret_cast<const uint4*>(a.q + row[k] * a.ldq + head[k] * kD) + part * 2;
+          x0 = __ldg(src);
+          x1 = __ldg(src + 1);
+        }
+        uint4 hi, lo;
+        split_query(x0, x1, inv, hi, lo);
+        uint8_t* dst = q_dst + r * kD + ((part ^ (r & 7)) << 4);
+        *reinterpret_cast<uint4*>(dst) = hi;
+        *reinterpret_cast<uint4*>(dst + kManyQBytes) = lo;
+        if (part == 0) {
+          RowInfo v = {};
+          const int t = w.t0 + r;
+          v.out = t < w.rows ? (w.row0 + t / group) * a.H + head[k] : -1;
+          v.fix = row[k] < 0 ? 0.f : finite >> k & 1 ? 1.f : __uint_as_float(0x7fc00000u);
+          v.hi = row[k] < 0 ? 0 : w.len;
+          if (!PLAIN && row[k] >= 0) {
+            v.pos = __ldg(a.cu_k + w.b + 1) - __ldg(a.cu_k + w.b) - (__ldg(a.cu_q + w.b + 1) - row[k]);
+            v.slope = a.slopes ? __ldg(a.slopes + head[k]) * kLog2e : 0.f;
+            if (a.ranges) {
+              const int2 range = __ldg(a.ranges + row[k]);
+              v.lo = range.x;
+              v.hi = min(range.y, w.len);
+            }
+          }
+          s_row[qb][r] = v;
+        }
+      }
+      fence_proxy_async_smem();
+      warp_arrive(&q_full[qb]);
+      // scales: thread = key, four tiles' loads at a time
+      // scores come out times log2(e), or as twice the argument of the tanh that caps them
+      const float mul = a.scale * __uint_as_float(scale) * kLog2e * (a.cap > 0.f ? 2.f / a.cap : 1.f);
+      const float* ks = a.k_scales + static_cast<int64_t>(w.k0) * a.Hkv + w.hk;
+      const float* vs = a.v_scales + static_cast<int64_t>(w.v0) * a.Hkv + w.hk;
+      for (int key = w.begin + tid; key - tid < w.end; key += 4 * kUnitKeys) {
+        float x[4], y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int at = key + i * kUnitKeys;
+          x[i] = y[i] = 1.f;
+          if (at < w.end) {
+            x[i] = __ldg(ks + static_cast<int64_t>(at) * a.Hkv);
+            y[i] = __ldg(vs + static_cast<int64_t>(at) * a.Hkv);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (key - tid + i * kUnitKeys < w.end) {
+            const int sl = n_sc % kScaleSlots;
+            if (n_sc >= kScaleSlots)
+              mbar_wait(&sc_free[sl], (n_sc / kScaleSlots - 1) & 1, &abort_flag, p.status_word, 512);
+            const float ex = value_exponent(y[i]);
+            float* dst = sc_smem + sl * 3 * kUnitKeys + tid;
+            dst[0] = x[i] * mul;
+            dst[kUnitKeys] = ex;
+            dst[2 * kUnitKeys] = ex == ex ? exp2f(-ex) : 1.f;      // the weight of a NaN is a NaN where its key is seen, else zero
+            warp_arrive(&sc_full[sl]);
+            ++n_sc;
+          }
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax: thread = row
+    const int quarter = warp & 3, team = (warp - 3) >> 2;
+    const int tid = threadIdx.x - 96;
+    const int row = quarter * 32 + lane;
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16), t_s = t_lane + team * 128, t_o = t_lane + 256;
+    uint8_t* p_dst = p_smem + team * 2 * kTileBytes + row * kD;
+    int n_tile = 0;                   // tiles so far, of both teams
+    bool more = mbar_wait(&part_full[0], 0, &abort_flag, p.status_word, 515) && s_part[0].end >= 0;
+    for (int n = 0; more; ++n) {
+      const PartInfo& part = s_part[n % kParts];
+      const int qb = n & 1, begin = part.begin, end = part.end, tiles = (end - begin + kUnitKeys - 1) / kUnitKeys;
+      const bool alive = part.t0 + quarter * 32 < part.rows;
+      const int joined_slot = part.slot, joined_owner = part.owner, joined_parts = part.parts;
+      mbar_wait(&q_full[qb], (n >> 1) & 1, &abort_flag, p.status_word, 516);
+      const RowInfo me = s_row[qb][row];
+      warp_arrive(&part_done[n % kParts]);
+      more = mbar_wait(&part_full[(n + 1) % kParts], ((n + 1) / kParts) & 1, &abort_flag, p.status_word, 517) && s_part[(n + 1) % kParts].end >= 0;
+      float ref = kNothing, l = 0.f;
+      const int i0 = (n_tile ^ team) & 1;
+      for (int i = i0; i < tiles; i += 2) {
+        const int g = n_tile + i, sl = g % kScaleSlots, key0 = begin + i * kUnitKeys;
+        const float* sc = sc_smem + sl * 3 * kUnitKeys;
+        mbar_wait(&sc_full[sl], (g / kScaleSlots) & 1, &abort_flag, p.status_word, 518);
+        mbar_wait(&s_full[team], (g >> 1) & 1, &abort_flag, p.status_word, 519);
+        tc_fence_after_sync();
+        bool grown = false;
+        float old = 1.f;
+        if (alive) {
+          // scores (times log2 e, plus the exponents of the values' scales), in place of the products, and their maximum
+          float mx = kNothing;
+          const int lo = me.lo - key0, hi = min(me.hi, end) - key0;
+          const bool cut = __any_sync(0xffffffffu, me.out >= 0 && (lo > 0 || hi < kUnitKeys));
+          const float away = static_cast<float>(me.pos - key0);
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t s[32];
+            tmem_ld_32x32(t_s + c * 32, s);
+            tmem_ld_wait();
+            float2* t = reinterpret_cast<float2*>(s);
+            if (PLAIN || a.cap == 0.f) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const float4 kk = *reinterpret_cast<const float4*>(sc + c * 32 + 4 * j);
+                const float4 ex = *reinterpret_cast<const float4*>(sc + kUnitKeys + c * 32 + 4 * j);
+                t[2 * j] = ffma2(t[2 * j], make_float2(kk.x, kk.y), make_float2(ex.x, ex.y));
+                t[2 * j + 1] = ffma2(t[2 * j + 1], make_float2(kk.z, kk.w), make_float2(ex.z, ex.w));
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const float4 kk = *reinterpret_cast<const float4*>(sc + c * 32 + 4 * j);
+                const float4 ex = *reinterpret_cast<const float4*>(sc + kUnitKeys + c * 32 + 4 * j);
+                t[2 * j].x = fmaf(capped(t[2 * j].x * kk.x, a.cap), kLog2e, ex.x);
+                t[2 * j].y = fmaf(capped(t[2 * j].y * kk.y, a.cap), kLog2e, ex.y);
+                t[2 * j + 1].x = fmaf(capped(t[2 * j + 1].x * kk.z, a.cap), kLog2e, ex.z);
+                t[2 * j + 1].y = fmaf(capped(t[2 * j + 1].y * kk.w, a.cap), kLog2e, ex.w);
+              }
+            }
+            if (!PLAIN && a.slopes) {
+              const float d = away - static_cast<float>(c * 32);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                t[j].x = fmaf(-me.slope, fabsf(d - static_cast<float>(2 * j)), t[j].x);
+                t[j].y = fmaf(-me.slope, fabsf(d - static_cast<float>(2 * j + 1)), t[j].y);
+              }
+            }
+            if (cut) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                s[j] = c * 32 + j >= lo && c * 32 + j < hi ? s[j] : 0xff800000u;
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              mx = fmax3(mx, t[j].x, t[j].y);
+            tmem_st_32x32(t_s + c * 32, s);
+          }
+          tmem_st_wait();
+          grown = mx > ref + kHeadroom;
+          if (grown) {
+            old = exp2f(ref - mx);
+            ref = mx;
+          }
+        }
+        // the team's last weights have been taken
+        if (g >= 2)
+          mbar_wait(&pv_done[team], ((g >> 1) - 1) & 1, &abort_flag, p.status_word, 520);
+        if (alive) {
+          if (i >= 2 && __any_sync(0xffffffffu, grown)) {
+            tc_fence_after_sync();
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t o[32];
+              tmem_ld_32x32(t_o + team * 128 + c * 32, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                o[j] = __float_as_uint(__uint_as_float(o[j]) * old);
+              tmem_st_32x32(t_o + team * 128 + c * 32, o);
+            }
+            tmem_st_wait();
+          }
+          const float2 shift = make_float2(kWeightLog2 - ref, kWeightLog2 - ref);
+          float2 sum = make_float2(l * old, 0.f);
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t s[32];
+            tmem_ld_32x32(t_s + c * 32, s);
+            tmem_ld_wait();
+            float2* t = reinterpret_cast<float2*>(s);
+            uint32_t hi4[8], lo4[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float4 inv = *reinterpret_cast<const float4*>(sc + 2 * kUnitKeys + c * 32 + 4 * j);
+              float2 x = fadd2(t[2 * j], shift), y = fadd2(t[2 * j + 1], shift);
+              x = make_float2(exp2f(x.x), exp2f(x.y));
+              y = make_float2(exp2f(y.x), exp2f(y.y));
+              sum = ffma2(x, make_float2(inv.x, inv.y), sum);
+              sum = ffma2(y, make_float2(inv.z, inv.w), sum);
+              split_weights_e5m2(x, y, hi4[j], lo4[j]);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int chunk = ((c * 2 + h) ^ (row & 7)) << 4;
+              *reinterpret_cast<uint4*>(p_dst + chunk) = make_uint4(hi4[4 * h], hi4[4 * h + 1], hi4[4 * h + 2], hi4[4 * h + 3]);
+              *reinterpret_cast<uint4*>(p_dst + kTileBytes + chunk) = make_uint4(lo4[4 * h], lo4[4 * h + 1], lo4[4 * h + 2], lo4[4 * h + 3]);
+            }
+          }
+          l = sum.x + sum.y;
+        }
+        if (key0 + kUnitKeys > end) {
+          // rows of V behind the last key may hold any byte, a NaN times a weight of zero among them
+          const int use = 2 * g + 1 + (more ? 1 : 0);      // the order of the ring: K(0), K(1), V(0), K(2), V(1), ...
+          mbar_wait(&full[use % kManyRing], (use / kManyRing) & 1, &abort_flag, p.status_word, 521);
+          if (key0 + row >= end) {
+            uint4* v = reinterpret_cast<uint4*>(ring + (use % kManyRing) * kTileBytes + row * kD);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              v[j] = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+        tc_fence_before_sync();
+        fence_proxy_async_smem();
+        warp_arrive(&p_full[team]);
+        warp_arrive(&s_free[team]);
+        warp_arrive(&sc_free[sl]);
+      }
+      warp_arrive(&q_free[qb]);      // all scores of the part have been taken
+      // ---------------------------------------------------------------- the teams meet: a thread takes 64 head dimensions of its row
+      s_ml[n & 1][team][row] = make_float2(ref, l);
+      teams_sync();
+      const float2 a0 = s_ml[n & 1][0][row], a1 = s_ml[n & 1][1][row];
+      n_tile += tiles;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int done = (n_tile + 1 - t) >> 1;      // products of team t so far
+        if (done > 0)
+          mbar_wait(&pv_done[t], (done - 1) & 1, &abort_flag, p.status_word, 522);
+      }
+      tc_fence_after_sync();
+      float top = fmaxf(a0.x, a1.x);
+      const float f0 = exp2f(a0.x - top), f1 = exp2f(a1.x - top);
+      l = a0.y * f0 + a1.y * f1;
+      float o[64];
+      if (alive) {
+        // a part of one tile has left nothing in the other team's columns
+        const bool both = tiles > 1;
+        const int sole = (n_tile - 1) & 1;
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          uint32_t u[16], v[16];
+          tmem_ld_32x16(t_o + (both ? 0 : sole * 128) + team * 64 + h * 16, u);
+          tmem_ld_32x16(t_o + 128 + team * 64 + h * 16, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            o[h * 16 + j] = both ? fmaf(__uint_as_float(u[j]), f0, __uint_as_float(v[j]) * f1) : __uint_as_float(u[j]);
+        }
+        if (!both) {
+          top = sole ? a1.x : a0.x;
+          l = sole ? a1.y : a0.y;
+        }
+      }
+      tc_fence_before_sync();
+      warp_arrive(&o_free);
+      if ((joined_parts == 1 || join_many(p, joined_slot, joined_owner, joined_parts, row, team * 64, top, l, o, tid, &joins)) && alive &&
+          me.out >= 0) {
+        const bool none = l == 0.f || me.fix == 0.f;
+        const float mul = __fdividef(me.fix, l);
+        uint4* dst = reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(me.out) * kD + team * 64);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            x[e] = none ? 0.f : o[8 * j + e] * mul;
+          dst[j] = float_to_bf16x8(x);
+        }
+      }
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// Keys that any row of a tile sees; one warp per tile, numbered as Walk does.
+template <int MROWS>
 __global__ void __launch_bounds__(128) fp8_spans_kernel(const Fp8AttnParams p, int2* __restrict__ spans) {
   pdl_wait();      // programmatic dependent launch: nothing before this reads an earlier kernel's data
   pdl_trigger();
-  const int b = blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (b >= p.batch)
-    return;
-  const int len = keys_of(p, b).len;
-  int lo = len, hi = 0;
-  for (int i = min(__ldg(p.cu_sal + b), p.num_salient) + (threadIdx.x & 31); i < min(__ldg(p.cu_sal + b + 1), p.num_salient); i += 32) {
-    const int r = __ldg(p.idx + i);
+  const int lane = threadIdx.x & 31, group = p.H / p.Hkv;
+  int number = blockIdx.x * 4 + (threadIdx.x >> 5);
+  SeqWork w = {};
+  for (int base = 0;; base += 32) {      // the tile's sequence
+    if (base >= p.batch)
+      return;
+    const SeqWork x = seq_work<MROWS>(p, base + lane);
+    const int upto = Walk<MROWS>::scan(x.tiles, lane);
+    const unsigned hit = __ballot_sync(0xffffffffu, upto > number);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      number -= __shfl_sync(0xffffffffu, upto - x.tiles, src);
+      w = seq_work<MROWS>(p, base + src);
+      break;
+    }
+    number -= __shfl_sync(0xffffffffu, upto, 31);
+  }
+  int lo = w.len, hi = 0;
+  const int t0 = number * MROWS, t1 = min(t0 + MROWS, w.rows);
+  for (int i = t0 / group + lane; i <= (t1 - 1) / group; i += 32) {
+    const int r = __ldg(p.idx + w.row0 + i);
     if (r < 0 || r >= p.total_q)
       continue;
     const int2 v = __ldg(p.ranges + r);
-    const int x = max(v.x, 0), y = min(v.y, len);
+    const int x = max(v.x, 0), y = min(v.y, w.len);
     if (x < y) {
       lo = min(lo, x);
       hi = max(hi, y);
@@ -1053,32 +1754,40 @@ __global__ void __launch_bounds__(128) fp8_spans_kernel(const Fp8AttnParams p, i
   }
   lo = __reduce_min_sync(0xffffffffu, lo);
   hi = __reduce_max_sync(0xffffffffu, hi);
-  if ((threadIdx.x & 31) == 0)
-    spans[b] = lo < hi ? make_int2(lo, hi) : make_int2(0, 0);
+  const int before = blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (lane == 0)
+    spans[before] = lo < hi ? make_int2(lo, hi) : make_int2(0, 0);
 }
 
-size_t few_parts_offset(int batch, int ctas) {
-  return (ctas * sizeof(unsigned long long) + batch * sizeof(int2) + 255) / 256 * 256;
-}
-size_t few_workspace(int batch, int ctas) {
-  return few_parts_offset(batch, ctas) + 2ull * ctas * (kRows * kD + 2 * kRows) * sizeof(float);
+// Workspace: tickets, keys per tile (only with ranges), parts of tiles; for the kernel that needs most.
+int64_t most_tiles(int num_salient, int batch, int group) { return static_cast<int64_t>(num_salient) * group / kRows + batch; }
+size_t parts_offset(int64_t tiles, int ctas) { return (ctas * sizeof(unsigned long long) + tiles * sizeof(int2) + 255) / 256 * 256; }
+size_t workspace_of(int num_salient, int batch, int group, int ctas) {
+  const int rows = static_cast<int64_t>(num_salient) * group > kRows ? kManyRows : kRows;
+  return parts_offset(most_tiles(num_salient, batch, group), ctas) + 2ull * ctas * rows * (kD + 2) * sizeof(float);
 }
 
-template <bool PLAIN>
-int launch_few(const CUtensorMap& tk, const CUtensorMap& tv, const FewParams& p, int ctas, cudaStream_t s) {
-  static bool set[64] = {false};
+template <typename Kernel>
+int launch_rows(Kernel kernel, bool (&set)[64], int threads, uint32_t smem, const CUtensorMap& tk, const CUtensorMap& tv, const FewParams& p,
+                int ctas, cudaStream_t s) {
   int dev = 0;
   cudaGetDevice(&dev);
   dev = (dev < 0 || dev >= 64) ? 0 : dev;
   if (!set[dev]) {
-    if (cudaFuncSetAttribute(fp8_few_rows_kernel<PLAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(kFewSmem)) != cudaSuccess)
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
       return set_error(DYLLM_ERR_CUDA, "attention_salient_rows_fp8: cudaFuncSetAttribute failed: %s",
                        cudaGetErrorString(cudaGetLastError()));
     set[dev] = true;
   }
-  DYLLM_LAUNCH(fp8_few_rows_kernel<PLAIN>, ctas, kFewThreads, kFewSmem, s, tk, tv, p);
+  DYLLM_LAUNCH(kernel, ctas, threads, smem, s, tk, tv, p);
   return check_launch("attention_salient_rows_fp8");
+}
+template <bool PLAIN>
+int launch(bool many, const CUtensorMap& tk, const CUtensorMap& tv, const FewParams& p, int ctas, cudaStream_t s) {
+  static bool set[2][64] = {};
+  if (many)
+    return launch_rows(fp8_many_rows_kernel<PLAIN>, set[1], kManyThreads, kManySmem, tk, tv, p, ctas, s);
+  return launch_rows(fp8_few_rows_kernel<PLAIN>, set[0], kFewThreads, kFewSmem, tk, tv, p, ctas, s);
 }
 
 }  // namespace
@@ -1091,7 +1800,7 @@ extern "C" {
 size_t dyllm_attention_salient_rows_fp8_workspace_bytes(int num_salient, int batch, int num_heads, int num_kv_heads) {
   if (num_salient <= 0 || batch <= 0 || num_heads <= 0 || num_kv_heads <= 0)
     return 0;
-  return few_workspace(batch, sm_count());
+  return workspace_of(num_salient, batch, num_heads / num_kv_heads, sm_count());
 }
 
 int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, const void* k_codes, const float* k_scales,
@@ -1158,20 +1867,28 @@ int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, co
   const int ctas = sm_count();
   DYLLM_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, DYLLM_ERR_INVALID_ARGUMENT,
                 "attention_salient_rows_fp8: the workspace must be 16-byte aligned");
-  DYLLM_REQUIRE(workspace && workspace_bytes >= few_workspace(batch, ctas), DYLLM_ERR_WORKSPACE,
+  const int group = num_heads / num_kv_heads;
+  const int64_t tiles = most_tiles(num_salient, batch, group);
+  DYLLM_REQUIRE(workspace && workspace_bytes >= workspace_of(num_salient, batch, group, ctas), DYLLM_ERR_WORKSPACE,
                 "attention_salient_rows_fp8: workspace of %zu bytes is smaller than the %zu required", workspace_bytes,
-                few_workspace(batch, ctas));
+                workspace_of(num_salient, batch, group, ctas));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   f.a = p;
   f.tickets = reinterpret_cast<unsigned long long*>(ws);
   int2* spans = reinterpret_cast<int2*>(ws + ctas * sizeof(unsigned long long));
-  f.parts = reinterpret_cast<float*>(ws + few_parts_offset(batch, ctas));
+  f.parts = reinterpret_cast<float*>(ws + parts_offset(tiles, ctas));
   f.launch_id = next_launch_id() & ~0xffffull;
   f.status_word = device_status_word();
+  // a sequence with more rows than the bound says is served by either kernel; so is one with few beside others with many
+  const bool many = static_cast<int64_t>(max_rows_per_seq) * group > kRows && static_cast<int64_t>(num_salient) * group > kRows;
   if (p.ranges) {
     f.spans = spans;
-    DYLLM_LAUNCH(fp8_spans_kernel, cdiv_i(batch, 4), 128, 0, st, p, spans);
+    const unsigned blocks = static_cast<unsigned>((tiles + 3) / 4);
+    if (many)
+      DYLLM_LAUNCH(fp8_spans_kernel<kManyRows>, blocks, 128, 0, st, p, spans);
+    else
+      DYLLM_LAUNCH(fp8_spans_kernel<kRows>, blocks, 128, 0, st, p, spans);
   }
   CUtensorMap tk, tv;
   const uint64_t width = static_cast<uint64_t>(num_kv_heads) * kD;
@@ -1181,7 +1898,7 @@ int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, co
   if (rc != DYLLM_OK)
     return rc;
   const bool plain = softcap == 0.f && !slopes && !key_ranges;
-  return plain ? launch_few<true>(tk, tv, f, ctas, st) : launch_few<false>(tk, tv, f, ctas, st);
+  return plain ? launch<true>(many, tk, tv, f, ctas, st) : launch<false>(many, tk, tv, f, ctas, st);
 }
 
 }  // extern "C"

@@ -241,17 +241,17 @@ def _attend(b, heads, hkv, counts, mask=None, cap=0.0, slopes=False, scale=None,
 def _check(got, want, mag, big, floor, cap):
     """Half a step of bf16 for the result (2^-8).
 
-    A weight w <= 1 (its largest in the row is 1, the values' scales included), times 256 and in half precision (2^-11), is
-    e4m3 + e4m3(16 r) / 16 with the remainder r: |r| <= 2^-4 * 256 w (half a step of e4m3), rounded by 2^-4 of itself, or by
-    2^-10 / 16 where 16 r is below the normal numbers: off by at most (2^-8 + 2^-11) w or 2^-22.  The first moves the result by
-    as much of sum(weight * |v|); the second by 2^-22 of the largest weight for each key, times its codes, which are at most
-    twice the largest of the heaviest key.
+    A weight w <= 1 (its largest in the row is 1, the values' scales included) is held in half precision (2^-11) and split into
+    e4m3 and what that leaves, |r| <= 2^-4 w (half a step).  Few rows: r times 16 in e4m3, rounded by 2^-4 of itself, of 256 w;
+    many rows: r in e5m2, rounded by 2^-3 of itself, of 64 w: off by at most (2^-7 + 2^-11) w, or by half a step of the smallest
+    numbers, 2^-10 / 16 / 256 or 2^-17 / 64: 2^-22.  The first moves the result by as much of sum(weight * |v|); the second by
+    2^-22 of the largest weight for each key, times its codes, which are at most twice the largest of the heaviest key.
 
     The score is a sum of 128 products in fp32 (2^-24 a term, 2^-17 in all) of queries that are exact above 2^-18 of their row's
     largest and off by 2^-26 of it below, times a scale, capped and biased (a few 2^-24 of the cap and the bias): 2^-16 of what
     it is made of, which moves weights and sum by as much, relatively.  Exponential and quotient: 2^-20."""
     delta = 2.0 ** -16 * (big + cap).unsqueeze(-1)
-    tol = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -11 + 2.0 ** -20 + 2 * delta) * mag + 2.0 ** -21 * floor.unsqueeze(-1) + 1e-30
+    tol = 2.0 ** -8 * want.abs() + (2.0 ** -7 + 2.0 ** -11 + 2.0 ** -20 + 2 * delta) * mag + 2.0 ** -21 * floor.unsqueeze(-1) + 1e-30
     assert torch.equal(torch.isnan(got), torch.isnan(want))
     bad = (got - want).abs() > tol
     assert not bool(bad.any()), (int(bad.sum()), float(((got - want).abs() / tol).nan_to_num().max()))
