@@ -1120,22 +1120,6 @@ constexpr uint32_t kManySmem = (kManyRing + 4) * kTileBytes + 4 * kManyQBytes + 
 constexpr float kWeightLog2 = 6.f;                           // the reference's weight: 2^6
 constexpr float kHeadroom = 2.8f;                            // 2^(6 + 2.8) < 448
 
-__device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n .reg .b64 ra, rb, rc, rd;\n mov.b64 ra, {%2, %3};\n mov.b64 rb, {%4, %5};\n mov.b64 rc, {%6, %7};\n"
-      " fma.rn.f32x2 rd, ra, rb, rc;\n mov.b64 {%0, %1}, rd;\n}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-__device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n .reg .b64 ra, rb, rd;\n mov.b64 ra, {%2, %3};\n mov.b64 rb, {%4, %5};\n"
-      " add.rn.f32x2 rd, ra, rb;\n mov.b64 {%0, %1}, rd;\n}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -1159,8 +1143,8 @@ __device__ __forceinline__ bool join_many(const FewParams& p, int slot, int owne
   constexpr int kPart = kManyRows * kD + 2 * kManyRows;
   float* mine = p.parts + static_cast<int64_t>(slot) * kPart;
 #pragma unroll
-  for (int j = 0; j < 64; j += 4)
-    *reinterpret_cast<float4*>(mine + row * kD + c0 + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+  for (int j = 0; j < 64; ++j)      // [dimension][row]: a warp's rows lie side by side
+    mine[(c0 + j) * kManyRows + row] = o[j];
   if (c0 == 0) {
     mine[kManyRows * kD + row] = top;
     mine[kManyRows * kD + kManyRows + row] = l;
@@ -1189,18 +1173,14 @@ __device__ __forceinline__ bool join_many(const FewParams& p, int slot, int owne
     const float mul = exp2f(__ldcg(src + kManyRows * kD + row) - top);
     l += __ldcg(src + kManyRows * kD + kManyRows + row) * mul;
 #pragma unroll
-    for (int j = 0; j < 64; j += 4) {
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(src + row * kD + c0 + j));
-      o[j] = fmaf(x.x, mul, o[j]);
-      o[j + 1] = fmaf(x.y, mul, o[j + 1]);
-      o[j + 2] = fmaf(x.z, mul, o[j + 2]);
-      o[j + 3] = fmaf(x.w, mul, o[j + 3]);
-    }
+    for (int j = 0; j < 64; ++j)
+      o[j] = fmaf(__ldcg(src + (c0 + j) * kManyRows + row), mul, o[j]);
   }
   return true;
 }
 
-template <bool PLAIN>
+// CAP, BIAS: scores capped by a tanh, biased by their distance.
+template <bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kManyThreads, 1)
 fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const FewParams p) {
   pdl_wait();      // programmatic dependent launch: nothing before this reads an earlier kernel's data
@@ -1397,16 +1377,26 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         break;
       if (n >= 2)
         mbar_wait(&q_free[qb], ((n >> 1) - 1) & 1, &abort_flag, p.status_word, 511);
-      // queries: eight threads a row, 16 rows at a time, twice: the largest element, then the codes
+      // queries: eight threads a row, 16 rows at a time; all loads first (one after the other they took 13 us a part)
       if (tid == 0)
         s_amax[qb] = 0;
-      int row[8], head[8];
+      int row[8];
+      uint4 x0[8], x1[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const int t = w.t0 + 16 * k + (tid >> 3), i = t / group;
-        head[k] = w.hk * group + t - i * group;
-        row[k] = t < w.rows ? __ldg(a.idx + w.row0 + i) : -1;
+        const int t = w.t0 + 16 * k + (tid >> 3);
+        row[k] = t < w.rows ? __ldg(a.idx + w.row0 + t / group) : -1;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int t = w.t0 + 16 * k + (tid >> 3), head = w.hk * group + t % group;
         row[k] = row[k] >= a.total_q ? -1 : row[k];
+        x0[k] = x1[k] = make_uint4(0u, 0u, 0u, 0u);
+        if (row[k] >= 0) {
+          const uint4* src = reinterpret_cast<const uint4*>(a.q + row[k] * a.ldq + head * kD) + (tid & 7) * 2;
+          x0[k] = __ldg(src);
+          x1[k] = __ldg(src + 1);
+        }
       }
       loaders_sync();
       uint32_t finite = 0;
@@ -1414,20 +1404,7 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         uint32_t top = 0;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          uint4 x0 = make_uint4(0u, 0u, 0u, 0u), x1 = x0;
-          if (row[k] >= 0) {
-            const uint4* src = reinterpret_cast<const uint4*>(a.q + row[k] * a.ldq + head[k] * kD) + (tid & 7) * 2;
-            x0 = __ldg(src);
-            x1 = __ldg(src + 1);
-          }
-          float y[16];
-          bf16x8_to_float(x0, y);
-          bf16x8_to_float(x1, y + 8);
-          uint32_t m = 0;
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            m = max(m, __float_as_uint(y[j]) & 0x7fffffffu);
-          m = fp8_amax8(m);
+          const uint32_t m = fp8_amax8(max(bf16x8_amax(x0[k]), bf16x8_amax(x1[k])));
           if (m < 0x7f800000u) {
             finite |= 1u << k;
             top = max(top, m);
@@ -1444,40 +1421,47 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const int r = 16 * k + (tid >> 3), part = tid & 7;
-        uint4 x0 = make_uint4(0u, 0u, 0u, 0u), x1 = x0;
-        if (row[k] >= 0 && (finite >> k & 1)) {
-          const uint4* src = reinterpret_cast<const uint4*>(a.q + row[k] * a.ldq + head[k] * kD) + part * 2;
-          x0 = __ldg(src);
-          x1 = __ldg(src + 1);
-        }
+        if (!(finite >> k & 1))
+          x0[k] = x1[k] = make_uint4(0u, 0u, 0u, 0u);
         uint4 hi, lo;
-        split_query(x0, x1, inv, hi, lo);
+        split_query(x0[k], x1[k], inv, hi, lo);
         uint8_t* dst = q_dst + r * kD + ((part ^ (r & 7)) << 4);
         *reinterpret_cast<uint4*>(dst) = hi;
         *reinterpret_cast<uint4*>(dst + kManyQBytes) = lo;
-        if (part == 0) {
-          RowInfo v = {};
-          const int t = w.t0 + r;
-          v.out = t < w.rows ? (w.row0 + t / group) * a.H + head[k] : -1;
-          v.fix = row[k] < 0 ? 0.f : finite >> k & 1 ? 1.f : __uint_as_float(0x7fc00000u);
-          v.hi = row[k] < 0 ? 0 : w.len;
-          if (!PLAIN && row[k] >= 0) {
-            v.pos = __ldg(a.cu_k + w.b + 1) - __ldg(a.cu_k + w.b) - (__ldg(a.cu_q + w.b + 1) - row[k]);
-            v.slope = a.slopes ? __ldg(a.slopes + head[k]) * kLog2e : 0.f;
+      }
+      {
+        // one thread a row: what the softmax warps need to know of it
+        const int t = w.t0 + tid, i = t / group, head = w.hk * group + t - i * group;
+        RowInfo v = {};
+        v.out = -1;
+        if (t < w.rows) {
+          int at = __ldg(a.idx + w.row0 + i);
+          at = at >= a.total_q ? -1 : at;
+          v.out = (w.row0 + i) * a.H + head;
+          if (at >= 0) {
+            v.fix = 1.f;
+            v.hi = w.len;
+            v.pos = __ldg(a.cu_k + w.b + 1) - __ldg(a.cu_k + w.b) - (__ldg(a.cu_q + w.b + 1) - at);
+            v.slope = BIAS ? __ldg(a.slopes + head) * kLog2e : 0.f;
             if (a.ranges) {
-              const int2 range = __ldg(a.ranges + row[k]);
+              const int2 range = __ldg(a.ranges + at);
               v.lo = range.x;
               v.hi = min(range.y, w.len);
             }
           }
-          s_row[qb][r] = v;
         }
+        s_row[qb][tid] = v;
       }
+      loaders_sync();
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if ((tid & 7) == 0 && row[k] >= 0 && !(finite >> k & 1))
+          s_row[qb][16 * k + (tid >> 3)].fix = __uint_as_float(0x7fc00000u);
       fence_proxy_async_smem();
       warp_arrive(&q_full[qb]);
       // scales: thread = key, four tiles' loads at a time
       // scores come out times log2(e), or as twice the argument of the tanh that caps them
-      const float mul = a.scale * __uint_as_float(scale) * kLog2e * (a.cap > 0.f ? 2.f / a.cap : 1.f);
+      const float mul = a.scale * __uint_as_float(scale) * kLog2e * (CAP ? 2.f / a.cap : 1.f);
       const float* ks = a.k_scales + static_cast<int64_t>(w.k0) * a.Hkv + w.hk;
       const float* vs = a.v_scales + static_cast<int64_t>(w.v0) * a.Hkv + w.hk;
       for (int key = w.begin + tid; key - tid < w.end; key += 4 * kUnitKeys) {
@@ -1546,32 +1530,18 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
             uint32_t s[32];
             tmem_ld_32x32(t_s + c * 32, s);
             tmem_ld_wait();
-            float2* t = reinterpret_cast<float2*>(s);
-            if (PLAIN || a.cap == 0.f) {
+            float* t = reinterpret_cast<float*>(s);
+            const float d = away - static_cast<float>(c * 32);
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const float4 kk = *reinterpret_cast<const float4*>(sc + c * 32 + 4 * j);
-                const float4 ex = *reinterpret_cast<const float4*>(sc + kUnitKeys + c * 32 + 4 * j);
-                t[2 * j] = ffma2(t[2 * j], make_float2(kk.x, kk.y), make_float2(ex.x, ex.y));
-                t[2 * j + 1] = ffma2(t[2 * j + 1], make_float2(kk.z, kk.w), make_float2(ex.z, ex.w));
-              }
-            } else {
+            for (int j = 0; j < 32; j += 4) {
+              const float4 kk = *reinterpret_cast<const float4*>(sc + c * 32 + j);
+              const float4 ex = *reinterpret_cast<const float4*>(sc + kUnitKeys + c * 32 + j);
+              const float k4[4] = {kk.x, kk.y, kk.z, kk.w}, e4[4] = {ex.x, ex.y, ex.z, ex.w};
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const float4 kk = *reinterpret_cast<const float4*>(sc + c * 32 + 4 * j);
-                const float4 ex = *reinterpret_cast<const float4*>(sc + kUnitKeys + c * 32 + 4 * j);
-                t[2 * j].x = fmaf(capped(t[2 * j].x * kk.x, a.cap), kLog2e, ex.x);
-                t[2 * j].y = fmaf(capped(t[2 * j].y * kk.y, a.cap), kLog2e, ex.y);
-                t[2 * j + 1].x = fmaf(capped(t[2 * j + 1].x * kk.z, a.cap), kLog2e, ex.z);
-                t[2 * j + 1].y = fmaf(capped(t[2 * j + 1].y * kk.w, a.cap), kLog2e, ex.w);
-              }
-            }
-            if (!PLAIN && a.slopes) {
-              const float d = away - static_cast<float>(c * 32);
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                t[j].x = fmaf(-me.slope, fabsf(d - static_cast<float>(2 * j)), t[j].x);
-                t[j].y = fmaf(-me.slope, fabsf(d - static_cast<float>(2 * j + 1)), t[j].y);
+              for (int e = 0; e < 4; ++e) {
+                t[j + e] = CAP ? fmaf(capped(t[j + e] * k4[e], a.cap), kLog2e, e4[e]) : fmaf(t[j + e], k4[e], e4[e]);
+                if (BIAS)
+                  t[j + e] = fmaf(-me.slope, fabsf(d - static_cast<float>(j + e)), t[j + e]);
               }
             }
             if (cut) {
@@ -1581,7 +1551,7 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
             }
 #pragma unroll
             for (int j = 0; j < 16; ++j)
-              mx = fmax3(mx, t[j].x, t[j].y);
+              mx = fmax3(mx, t[2 * j], t[2 * j + 1]);
             tmem_st_32x32(t_s + c * 32, s);
           }
           tmem_st_wait();
@@ -1609,23 +1579,24 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
             }
             tmem_st_wait();
           }
-          const float2 shift = make_float2(kWeightLog2 - ref, kWeightLog2 - ref);
-          float2 sum = make_float2(l * old, 0.f);
+          const float shift = kWeightLog2 - ref;
+          float sum[2] = {l * old, 0.f};
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             uint32_t s[32];
             tmem_ld_32x32(t_s + c * 32, s);
             tmem_ld_wait();
-            float2* t = reinterpret_cast<float2*>(s);
             uint32_t hi4[8], lo4[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const float4 inv = *reinterpret_cast<const float4*>(sc + 2 * kUnitKeys + c * 32 + 4 * j);
-              float2 x = fadd2(t[2 * j], shift), y = fadd2(t[2 * j + 1], shift);
-              x = make_float2(exp2f(x.x), exp2f(x.y));
-              y = make_float2(exp2f(y.x), exp2f(y.y));
-              sum = ffma2(x, make_float2(inv.x, inv.y), sum);
-              sum = ffma2(y, make_float2(inv.z, inv.w), sum);
+              const uint32_t* u = s + 4 * j;
+              const float2 x = make_float2(exp2f(__uint_as_float(u[0]) + shift), exp2f(__uint_as_float(u[1]) + shift));
+              const float2 y = make_float2(exp2f(__uint_as_float(u[2]) + shift), exp2f(__uint_as_float(u[3]) + shift));
+              sum[0] = fmaf(x.x, inv.x, sum[0]);
+              sum[1] = fmaf(x.y, inv.y, sum[1]);
+              sum[0] = fmaf(y.x, inv.z, sum[0]);
+              sum[1] = fmaf(y.y, inv.w, sum[1]);
               split_weights_e5m2(x, y, hi4[j], lo4[j]);
             }
 #pragma unroll
@@ -1635,7 +1606,7 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
               *reinterpret_cast<uint4*>(p_dst + kTileBytes + chunk) = make_uint4(lo4[4 * h], lo4[4 * h + 1], lo4[4 * h + 2], lo4[4 * h + 3]);
             }
           }
-          l = sum.x + sum.y;
+          l = sum[0] + sum[1];
         }
         if (key0 + kUnitKeys > end) {
           // rows of V behind the last key may hold any byte, a NaN times a weight of zero among them
@@ -1783,11 +1754,14 @@ int launch_rows(Kernel kernel, bool (&set)[64], int threads, uint32_t smem, cons
   return check_launch("attention_salient_rows_fp8");
 }
 template <bool PLAIN>
-int launch(bool many, const CUtensorMap& tk, const CUtensorMap& tv, const FewParams& p, int ctas, cudaStream_t s) {
-  static bool set[2][64] = {};
-  if (many)
-    return launch_rows(fp8_many_rows_kernel<PLAIN>, set[1], kManyThreads, kManySmem, tk, tv, p, ctas, s);
-  return launch_rows(fp8_few_rows_kernel<PLAIN>, set[0], kFewThreads, kFewSmem, tk, tv, p, ctas, s);
+int launch_few(const CUtensorMap& tk, const CUtensorMap& tv, const FewParams& p, int ctas, cudaStream_t s) {
+  static bool set[64] = {};
+  return launch_rows(fp8_few_rows_kernel<PLAIN>, set, kFewThreads, kFewSmem, tk, tv, p, ctas, s);
+}
+template <bool CAP, bool BIAS>
+int launch_many(const CUtensorMap& tk, const CUtensorMap& tv, const FewParams& p, int ctas, cudaStream_t s) {
+  static bool set[64] = {};
+  return launch_rows(fp8_many_rows_kernel<CAP, BIAS>, set, kManyThreads, kManySmem, tk, tv, p, ctas, s);
 }
 
 }  // namespace
@@ -1897,8 +1871,13 @@ int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, co
     rc = encode_tmap_2d_u8(&tv, v_codes, v_rows ? v_rows : 1, width, width, 32, kD);
   if (rc != DYLLM_OK)
     return rc;
+  if (many) {
+    if (softcap > 0.f)
+      return slopes ? launch_many<true, true>(tk, tv, f, ctas, st) : launch_many<true, false>(tk, tv, f, ctas, st);
+    return slopes ? launch_many<false, true>(tk, tv, f, ctas, st) : launch_many<false, false>(tk, tv, f, ctas, st);
+  }
   const bool plain = softcap == 0.f && !slopes && !key_ranges;
-  return plain ? launch<true>(many, tk, tv, f, ctas, st) : launch<false>(many, tk, tv, f, ctas, st);
+  return plain ? launch_few<true>(tk, tv, f, ctas, st) : launch_few<false>(tk, tv, f, ctas, st);
 }
 
 }  // extern "C"

@@ -99,6 +99,12 @@ __device__ __forceinline__ void bf16x8_to_float(const uint4& v, float* x) {
     x[2 * j + 1] = f.y;
   }
 }
+// Bits of the largest magnitude of eight bf16 numbers, as those of a float.
+__device__ __forceinline__ uint32_t bf16x8_amax(const uint4& v) {
+  const uint32_t w[4] = {v.x & 0x7fff7fffu, v.y & 0x7fff7fffu, v.z & 0x7fff7fffu, v.w & 0x7fff7fffu};
+  const uint32_t m = __vmaxu2(__vmaxu2(w[0], w[1]), __vmaxu2(w[2], w[3]));
+  return max(m >> 16, m & 0xffffu) << 16;
+}
 __device__ __forceinline__ uint4 float_to_bf16x8(const float* x) {
   uint4 v;
   __nv_bfloat162* p = reinterpret_cast<__nv_bfloat162*>(&v);
