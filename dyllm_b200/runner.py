@@ -256,6 +256,7 @@ class StepRunner:
 
         self._graphs.clear()
         self._warm.clear()
+        self._graph_pool = None      # a memory pool ends with its last graph: the next capture opens another
         gc.collect()
         if self.device.type == "cuda":
             torch.cuda.synchronize(self.device)
