@@ -14,6 +14,7 @@ from typing import List, Optional
 
 import torch
 
+from . import ops
 from .cache import get_block_cuda, get_seqs_cuda, reset_block_cuda, reset_full_cuda, scatter_update_cuda
 from .context import get_context
 
@@ -103,18 +104,21 @@ class CacheManager:
         n = c.size(0)
         self._reserve(n)
         start = self._rows
-        self._arena[start : start + n].copy_(c)
+        self._store_rows(c, start)
         self._rows += n
         self._seq_to_start[seq_id] = start
         self._seq_to_len[seq_id] = n
         self.seq_start_gpu[seq_id] = start
         self.seq_len_gpu[seq_id] = n
 
+    def _store_rows(self, c: torch.Tensor, start: int) -> None:
+        self._arena[start : start + c.size(0)].copy_(c)
+
     def reset_seq(self, c: torch.Tensor, seq_id: int) -> None:
         if seq_id in self._seq_to_start:
             start, end = self.select_seq_range(seq_id)
             if end - start == c.size(0):
-                self._arena[start:end] = c
+                self._store_rows(c, start)
                 return
             self.remove_seq(seq_id)
         self.add_seq(c, seq_id)
@@ -125,7 +129,7 @@ class CacheManager:
         start, end = self.select_seq_range(seq_id)
         length = end - start
         if end < self._rows:
-            self._arena[start : self._rows - length] = self._arena[end : self._rows].clone()
+            self._close_gap(start, end)
         self._rows -= length
         moved = []
         for other, other_start in self._seq_to_start.items():
@@ -139,6 +143,9 @@ class CacheManager:
         del self._seq_to_len[seq_id]
         self.seq_start_gpu[seq_id] = -1
         self.seq_len_gpu[seq_id] = 0
+
+    def _close_gap(self, start: int, end: int) -> None:
+        self._arena[start : self._rows - (end - start)] = self._arena[end : self._rows].clone()
 
     def clear(self) -> None:
         """Forgets every sequence (the arena is kept for reuse)."""
@@ -184,6 +191,10 @@ class CacheManager:
                 new_lens.append(ctx.context_lens_cpu[i])
         if new_ids:
             self._allocate_new_seqs(new_ids, new_lens)
+        self._store_full(c, seq_ids)
+
+    def _store_full(self, c: torch.Tensor, seq_ids: torch.Tensor) -> None:
+        ctx = get_context()
         reset_full_cuda(self.cache, c, self.seq_start_gpu, ctx.cu_seqlens_q, seq_ids, ctx.total_seqlen)
 
     def reset_block(self, c: torch.Tensor, seq_ids: torch.Tensor) -> None:
@@ -204,3 +215,64 @@ class CacheManager:
         for sid in sorted(finished_seq_ids, key=lambda x: self._seq_to_start.get(x, -1), reverse=True):
             self.remove_seq(sid)
         return True
+
+
+class Fp8CacheManager(CacheManager):
+    """A cache of key or value heads in 8 bits (:func:`dyllm_b200.ops.fp8_cache_write`): 132 bytes instead of 256 per row and
+    head.  The sequences are kept as in :class:`CacheManager`; what comes in is quantised and what goes out is a bf16 copy, never
+    a view.  ``pair`` is what the operators on 8-bit caches take."""
+
+    def __init__(self, num_heads: int, head_dim: int = 128, max_num_seqs: int = 16384, device: torch.device = torch.device("cuda")):
+        if head_dim != 128:
+            raise ValueError(f"supported head dimension is 128; got {head_dim}")
+        super().__init__(num_heads * head_dim, max_num_seqs, torch.float8_e4m3fn, device)
+        self.num_heads = num_heads
+        self._scales = torch.empty((0, num_heads), dtype=torch.float32, device=device)
+
+    @property
+    def pair(self) -> tuple:
+        """``(codes [rows, heads * 128], scales [rows, heads])`` of the rows in use."""
+        return self._arena[: self._rows], self._scales[: self._rows]
+
+    def _reserve(self, extra_rows: int) -> None:
+        super()._reserve(extra_rows)
+        if self._arena.size(0) > self._scales.size(0):
+            scales = torch.empty((self._arena.size(0), self.num_heads), dtype=torch.float32, device=self.device)
+            scales[: self._rows].copy_(self._scales[: self._rows])
+            self._scales = scales
+
+    def _close_gap(self, start: int, end: int) -> None:
+        super()._close_gap(start, end)
+        self._scales[start : self._rows - (end - start)] = self._scales[end : self._rows].clone()
+
+    def _heads(self, c: torch.Tensor) -> torch.Tensor:
+        return c.reshape(c.size(0), self.num_heads, 128)
+
+    def _store_rows(self, c: torch.Tensor, start: int) -> None:
+        first, only = (torch.tensor([n], dtype=torch.long, device=self.device) for n in (start, 0))
+        cu = torch.tensor([0, c.size(0)], dtype=torch.int32, device=self.device)
+        ops.fp8_cache_write(self._heads(c), self._arena, self._scales, first, cu, only)
+
+    def _store_full(self, c: torch.Tensor, seq_ids: torch.Tensor) -> None:
+        ops.fp8_cache_write(self._heads(c), *self.pair, self.seq_start_gpu, get_context().cu_seqlens_q, seq_ids)
+
+    def reset_block(self, c: torch.Tensor, seq_ids: torch.Tensor) -> None:
+        ctx = get_context()
+        ops.fp8_cache_write(self._heads(c), *self.pair, self.seq_start_gpu, ctx.cu_seqlens_q, seq_ids,
+                            cu_seqlens_k=ctx.cu_seqlens_k)
+
+    def get_seqs(self, seq_ids: torch.Tensor, allow_view: bool = False,
+                 seq_ids_list: Optional[List[int]] = None) -> torch.Tensor:
+        ctx = get_context()
+        total = max(ctx.total_seqlen, ctx.total_seqlen_k)
+        return ops.fp8_cache_read(*self.pair, self.seq_start_gpu, ctx.cu_seqlens_k, seq_ids, total).view(total, self.hidden_dim)
+
+    def get_seqs_block(self, seq_ids: torch.Tensor, allow_view: bool = False,
+                       seq_ids_list: Optional[List[int]] = None) -> torch.Tensor:
+        ctx = get_context()
+        out = ops.fp8_cache_read(*self.pair, self.seq_start_gpu, ctx.cu_seqlens_q, seq_ids, ctx.total_seqlen,
+                                 cu_seqlens_k=ctx.cu_seqlens_k)
+        return out.view(ctx.total_seqlen, self.hidden_dim)
+
+    def scatter_update(self, seq_ids, row_idx, new, num_rows_dev=None) -> None:
+        raise RuntimeError("single rows of 8-bit caches are written by ops.fp8_kv_cache_update")

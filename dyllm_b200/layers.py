@@ -17,8 +17,8 @@ import torch.nn.functional as F
 from torch import nn
 
 from . import ops, profiling
-from .attention_ops import attention_salient_rows, attention_sparse_varlen
-from .cache_manager import CacheManager
+from .attention_ops import attention_salient_rows, attention_salient_rows_fp8, attention_sparse_varlen
+from .cache_manager import CacheManager, Fp8CacheManager
 from .context import get_context, get_metadata
 
 
@@ -186,6 +186,27 @@ def set_projection_backend(name: str) -> None:
     if name not in ("default", "cublas", "tcgen05"):
         raise ValueError(f"unknown projection backend {name!r}")
     _projection_backend = name
+
+
+# How the key and value caches of the attention blocks that are built from here on hold their rows.
+#   "bf16"   as the projections give them (the default);
+#   "fp8"    e4m3 codes with a power of two per row and head (ops.fp8_cache_write), 132 bytes instead of 256.  Dense steps
+#            attend over the exact keys and values; in sparse steps the exact attention of the salient rows reads the codes
+#            in place, delta-V is the change of what the cache holds, and the delta attention gets the keys as a bf16 copy.
+_kv_cache_dtype = "bf16"
+
+
+def set_kv_cache_dtype(name: str) -> None:
+    global _kv_cache_dtype
+    if name not in ("bf16", "fp8"):
+        raise ValueError(f"unknown K/V cache type {name!r}")
+    _kv_cache_dtype = name
+
+
+def kv_cache(num_kv_heads: int, head_dim: int) -> CacheManager:
+    if _kv_cache_dtype == "fp8":
+        return Fp8CacheManager(num_kv_heads, head_dim)
+    return CacheManager(num_kv_heads * head_dim)
 
 
 def _epilogue_bias(bias: torch.Tensor | None) -> torch.Tensor | None:
@@ -691,7 +712,7 @@ class Attention(nn.Module):
         self.threshold = threshold
         self.tp_size = _world_size()        # 1 under the sequence-sharded layout: this rank's rows are complete
         self.context_cache = CacheManager(self.num_heads * self.head_dim)
-        self.v_cache = CacheManager(self.num_kv_heads * self.head_dim)
+        self.v_cache = kv_cache(self.num_kv_heads, self.head_dim)
         self._hint_host = None      # pinned int32[1]: this layer's salient count, copied back without waiting
         self._hint = 0
 
@@ -715,10 +736,12 @@ class Attention(nn.Module):
         self._hint_host.copy_(count_dev, non_blocking=True)
         return min(self._hint, capacity) if self._hint else capacity
 
-    def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, dv: torch.Tensor | None = None) -> torch.Tensor:
+    def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, dv: torch.Tensor | None = None,
+                k_cache: Fp8CacheManager | None = None) -> torch.Tensor:
         """Dense step: q, k, v hold every row.  Sparse step: ``q`` every query row, ``k`` the packed full
         key tensor, ``v`` the new value rows of the step's salient tokens (reference convention).  ``dv``:
-        the caller has already formed delta-V and updated the value cache (``ops.kv_cache_update``)."""
+        the caller has already formed delta-V and updated the value cache (``ops.kv_cache_update``); with 8-bit
+        caches it always has, and brings the cache of the keys as ``k_cache``."""
         ctx, md = get_context(), get_metadata()
         q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
         seq_t = md.running_seqs_tensor
@@ -737,6 +760,9 @@ class Attention(nn.Module):
         cap = idx_q32.numel()            # capacity of the salient lists; the live count may be on the device
         n_dev, hint = ctx.num_salient_dev, ctx.salient_hint
         H, Hkv, D = self.num_heads, self.num_kv_heads, self.head_dim
+        fp8 = isinstance(self.v_cache, Fp8CacheManager)
+        if fp8 and (k_cache is None or dv is None and cap):
+            raise RuntimeError("8-bit caches are updated by the caller (ops.fp8_kv_cache_update): pass dv and k_cache")
 
         # delta-V and value-cache update in one pass over the salient rows (attention.py:67-74,89-96)
         if dv is None:
@@ -744,14 +770,23 @@ class Attention(nn.Module):
             if cap:
                 dest = ops.cache_dest_rows(rows_k, ctx.cu_seqlens_k, self.v_cache.seq_start_gpu, seq_t, n_dev)
                 ops.delta_v_update(v.view(cap, Hkv * D), self.v_cache.cache, dest, dv.view(cap, Hkv * D), n_dev)
-        v_full = self.v_cache.get_seqs(seq_t, allow_view=True, seq_ids_list=md.running_seqs).view(-1, Hkv, D)
+        if not fp8:
+            v_full = self.v_cache.get_seqs(seq_t, allow_view=True, seq_ids_list=md.running_seqs).view(-1, Hkv, D)
 
         # exact attention of the salient query rows (attention.py:76-87)
         max_rows = max(min(ctx.max_salient_per_seq, ctx.max_seqlen_q), 1)
         with profiling.region("salient_attention", 4.0 * (hint or cap) * ctx.max_seqlen_k * H * D,
-                              2.0 * ctx.total_seqlen_k * Hkv * D * 2 + 2.0 * (hint or cap) * H * D * 2):
-            o_sal = attention_salient_rows(q, k, v_full, ctx.cu_seqlens_k, ctx.cu_salientlens, idx_q32,
-                                           max_rows_per_seq=max_rows, num_salient=cap)
+                              2.0 * ctx.total_seqlen_k * Hkv * (D + 4 if fp8 else 2 * D) + 2.0 * (hint or cap) * H * D * 2):
+            if fp8:
+                # what the call is told decides between its two kernels: the estimate, where there is one
+                if hint:
+                    max_rows = min(max_rows, -(-hint // seq_t.numel()))
+                o_sal = attention_salient_rows_fp8(q, k_cache.pair, self.v_cache.pair, k_cache.seq_start_gpu,
+                                                   self.v_cache.seq_start_gpu, seq_t, ctx.cu_seqlens_q, ctx.cu_seqlens_k,
+                                                   ctx.cu_salientlens, idx_q32, max_rows_per_seq=max_rows)
+            else:
+                o_sal = attention_salient_rows(q, k, v_full, ctx.cu_seqlens_k, ctx.cu_salientlens, idx_q32,
+                                               max_rows_per_seq=max_rows, num_salient=cap)
 
         stats = torch.empty((ctx.total_seqlen, 3), dtype=torch.float32, device=q.device)   # overwritten (v_layout bit 2)
         mask = torch.empty((ctx.total_seqlen,), dtype=torch.bool, device=q.device)

@@ -18,7 +18,7 @@ import torch
 from torch import nn
 
 from . import layers, ops
-from .cache_manager import CacheManager
+from .cache_manager import CacheManager, Fp8CacheManager
 from .context import get_context, get_metadata
 from .layers import (Attention, ColumnParallelLinear, KVParallelLinear, LLaDAMLP, LLaDAMoESparseBlock, RMSNorm, salient_dest,
                      RotaryEmbedding, RowParallelLinear, _world_size, as_defined, attention_scope, unhooked)
@@ -77,7 +77,7 @@ class LLaDAAttention(nn.Module):
         # per-head RMSNorm of the projected queries and keys (LLaDA-MoE; ref: lladamoe.py:175-176,195-207)
         self.q_norm = RMSNorm(self.head_dim, eps=rms_norm_eps) if qk_layernorm else None
         self.k_norm = RMSNorm(self.head_dim, eps=rms_norm_eps) if qk_layernorm else None
-        self.k_cache = CacheManager(self.num_kv_heads * self.head_dim)
+        self.k_cache = layers.kv_cache(self.num_kv_heads, self.head_dim)
         assert rope_scaling is None
         self.rotary_emb = rotary_emb or RotaryEmbedding(self.head_dim, self.head_dim, max_position, rope_theta)
         self.attn = Attention(self.num_heads, self.head_dim, self.scaling, self.num_kv_heads, threshold)
@@ -128,17 +128,29 @@ class LLaDAAttention(nn.Module):
                     k_new = self.k_norm.forward_heads_(k_new.view(cap, Hkv, D), n_dev).view(cap, -1)
                 v_new = v_new.view(cap, Hkv, D)
                 # rotary embedding of the new keys, K-cache scatter, delta-V and V-cache update in one launch
-                dv = ops.kv_cache_update(k_new.view(cap, Hkv, D), v_new, rows_k, positions, ctx.idx_salient_row,
-                                         self.rotary_emb.cos_sin_cache.view(-1, D), ctx.cu_seqlens_k,
-                                         self.k_cache.seq_start_gpu, self.attn.v_cache.seq_start_gpu,
-                                         md.running_seqs_tensor, self.k_cache.cache, self.attn.v_cache.cache, n_dev)
+                dv = self._update_caches(k_new.view(cap, Hkv, D), v_new, rows_k, positions)
             else:
                 v_new = torch.empty((0, Hkv, D), dtype=q.dtype, device=q.device)
-            k_full = self.k_cache.get_seqs(md.running_seqs_tensor, allow_view=True, seq_ids_list=md.running_seqs)
-            o = self.attn(q, k_full.view(-1, Hkv, D), v_new, dv=dv)
+            o = self._sparse_attention(q, v_new, dv)
         out = self.o_proj(o.flatten(-2, -1))
         self.k_cache.finish(md.finished_seqs)
         return out
+
+
+    def _update_caches(self, k_new, v_new, rows_k, positions, dv=None) -> torch.Tensor:
+        """Rotary embedding of the salient rows' new keys, K and V into their caches; returns delta-V."""
+        ctx, md = get_context(), get_metadata()
+        args = (k_new, v_new, rows_k, positions, ctx.idx_salient_row, self.rotary_emb.cos_sin_cache.view(-1, self.head_dim),
+                ctx.cu_seqlens_k, self.k_cache.seq_start_gpu, self.attn.v_cache.seq_start_gpu, md.running_seqs_tensor)
+        if isinstance(self.k_cache, Fp8CacheManager):
+            return ops.fp8_kv_cache_update(*args, self.k_cache.pair, self.attn.v_cache.pair, ctx.num_salient_dev, dv=dv)
+        return ops.kv_cache_update(*args, self.k_cache.cache, self.attn.v_cache.cache, ctx.num_salient_dev, dv=dv)
+
+    def _sparse_attention(self, q, v_new, dv) -> torch.Tensor:
+        md = get_metadata()
+        k_full = self.k_cache.get_seqs(md.running_seqs_tensor, allow_view=True, seq_ids_list=md.running_seqs)
+        caches = {"k_cache": self.k_cache} if isinstance(self.k_cache, Fp8CacheManager) else {}
+        return self.attn(q, k_full.view(-1, self.num_kv_heads, self.head_dim), v_new, dv=dv, **caches)
 
 
 _side_streams: dict = {}
@@ -202,10 +214,7 @@ def _forward_sparse_overlapped(self, positions, hidden_states, salient_rows):
             k3 = k_new.view(cap, Hkv, D)
             if self.k_norm is not None:
                 k3 = self.k_norm.forward_heads_(k3, n_dev)
-            ops.kv_cache_update(k3, v_new.view(cap, Hkv, D), rows_k, positions, ctx.idx_salient_row,
-                                self.rotary_emb.cos_sin_cache.view(-1, D), ctx.cu_seqlens_k, self.k_cache.seq_start_gpu,
-                                self.attn.v_cache.seq_start_gpu, md.running_seqs_tensor, self.k_cache.cache,
-                                self.attn.v_cache.cache, n_dev, dv=dv)
+            self._update_caches(k3, v_new.view(cap, Hkv, D), rows_k, positions, dv)
 
     # A query projection of many rows is launched first: it fills the SMs, and what its last wave leaves idle is where the
     # other branch belongs.  (The other way round that branch takes SMs from the first wave, which then needs one wave more:
@@ -221,8 +230,7 @@ def _forward_sparse_overlapped(self, positions, hidden_states, salient_rows):
         kv_branch()
     q = _norm_and_rotate(self.rotary_emb, positions, q, self.q_norm)
     main.wait_stream(side)
-    k_full = self.k_cache.get_seqs(md.running_seqs_tensor, allow_view=True, seq_ids_list=md.running_seqs)
-    o = self.attn(q, k_full.view(-1, Hkv, D), v_new.view(cap, Hkv, D), dv=dv)
+    o = self._sparse_attention(q, v_new.view(cap, Hkv, D), dv)
     out = self.o_proj(o.flatten(-2, -1))
     self.k_cache.finish(md.finished_seqs)
     return out
