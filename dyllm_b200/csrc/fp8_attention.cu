@@ -102,6 +102,7 @@ struct FewParams {
   const int2* spans;           // per tile of rows: keys that any of them sees (null: all)
   unsigned long long* tickets; // one per CTA
   float* parts;                // two per CTA: [rows][128] sums, [rows] maxima, [rows] sums of weights
+  int* joins;                  // many rows, per CTA: parts of the tile that begins in it and goes on in others (0: none)
   unsigned long long launch_id;
   int* status_word;
 };
@@ -155,7 +156,7 @@ __device__ __forceinline__ SeqWork seq_work(const Fp8AttnParams& a, int b) {
 // A part of a tile as the scheduler hands it to the other warps.
 struct PartInfo {
   int begin, end;              // keys; end < 0: the share is done
-  int owner, parts, slot;      // several CTAs hold the tile (parts > 1): the first of them, how many, this CTA's slot
+  int owner, parts, slot, first;      // several CTAs hold the tile (parts > 1): the first of them, how many, this CTA's slot, it is the first
   int b, hk, row0, rows, t0;   // sequence, key head, the sequence's first listed row, its (row, head) pairs, the tile's first
   int k0, v0, len;             // the sequence's first rows in the caches, its keys
 };
@@ -323,11 +324,12 @@ struct Walk {
   // What the other warps need to know of the part.
   __device__ __forceinline__ PartInfo info() const {
     const int begin = span.x + first * kUnitKeys;
-    PartInfo v = {begin, min(span.y, span.x + last * kUnitKeys), 0, 1, 0, w.b, hk, w.row0, w.rows, tile * MROWS, w.k0, w.v0, w.len};
+    PartInfo v = {begin, min(span.y, span.x + last * kUnitKeys), 0, 1, 0, 0, w.b, hk, w.row0, w.rows, tile * MROWS, w.k0, w.v0, w.len};
     if (last - first < units) {
       v.owner = owner();
       v.parts = parts();
-      v.slot = 2 * static_cast<int>(blockIdx.x) + (first == 0 ? 1 : 0);
+      v.first = first == 0 ? 1 : 0;
+      v.slot = 2 * static_cast<int>(blockIdx.x) + v.first;
     }
     return v;
   }
@@ -1106,17 +1108,22 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
 // Tiles of 128 (listed row, query head) pairs, rows in the M = 128 of the products:
 //   S = Q K^T    A: the queries as e4m3 + e5m2 (two products into one accumulator), B: the K tile as loaded (K-major)
 //   O = P V      A: the weights as e4m3 + e5m2, B: the V tile as loaded (MN-major)
-// Two teams of four softmax warps take the key tiles in turn, thread = row, each with scores, sums and a maximum of its own, and
-// meet when the part ends.  A weight is 64 * 2^(t - reference); the reference follows the maximum in steps, so that the sums are
-// rescaled only where a score lies more than 2.8 (log2) above it.  A weight is off by 2^-7 of itself or by 2^-23 of the largest.
-// Four loader warps stage the queries of the next part and the scales of the next tiles.
+// Thread = row in four softmax warps.  A weight is 64 * 2^(t - reference); the reference follows the maximum in steps, so that the
+// sums are rescaled only where a score lies more than 2.8 (log2) above it.  A weight is off by 2^-7 of itself or by 2^-23 of the
+// largest.  Scores and weights share 128 columns of tensor memory (32 keys' weights, e4m3 then e5m2, lie in the first 16 of their
+// scores' 32 columns), so the steps of one tile follow one another; two CTAs per SM, each with parts of its own, fill each other's
+// waits, the ends of parts among them.  Four loader warps stage the queries of the next part and the scales of the next tiles.
 // ----------------------------------------------------------------------------------------------
 constexpr int kManyRows = 128;
 constexpr int kManyRing = 4;                                 // slots of one K or V tile
-constexpr int kScaleSlots = 8;                               // tiles whose scales are staged ahead
-constexpr int kTeamWarps = 4, kManyThreads = 32 * (3 + 2 * kTeamWarps + 4);
+constexpr int kScaleSlots = 2;                               // tiles whose scales are staged ahead
+constexpr int kManyWarps = 4, kManyThreads = 32 * (3 + kManyWarps + 4);
+constexpr int kManyCtas = 2;                                 // per SM
+constexpr uint32_t kManyTmemCols = 256;
+constexpr uint32_t kStageBytes = 32 * 64;                    // of a softmax warp: 32 head dimensions of its rows
 constexpr uint32_t kManyQBytes = kManyRows * kD;             // e4m3 or e5m2 part of the queries of a tile
-constexpr uint32_t kManySmem = (kManyRing + 4) * kTileBytes + 4 * kManyQBytes + kScaleSlots * 3 * kUnitKeys * sizeof(float) + 1024;
+constexpr uint32_t kManySmem = kManyRing * kTileBytes + 2 * kManyQBytes + kManyWarps * kStageBytes +
+                               kScaleSlots * 3 * kUnitKeys * sizeof(float) + 1024;
 constexpr float kWeightLog2 = 6.f;                           // the reference's weight: 2^6
 constexpr float kHeadroom = 2.8f;                            // 2^(6 + 2.8) < 448
 
@@ -1125,7 +1132,8 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-__device__ __forceinline__ void teams_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+// The lowest n bits.
+__device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
 // Four weights as codes, and what they leave in e5m2.  By way of half precision (2^-11).
 __device__ __forceinline__ void split_weights_e5m2(float2 a, float2 b, uint32_t& hi, uint32_t& lo) {
@@ -1137,67 +1145,44 @@ __device__ __forceinline__ void split_weights_e5m2(float2 a, float2 b, uint32_t&
   lo = __byte_perm(fp8_pack_half2_e5m2(*reinterpret_cast<const uint32_t*>(&r)), fp8_pack_half2_e5m2(*reinterpret_cast<const uint32_t*>(&s)), 0x5410);
 }
 
-// Joins the parts of a tile, as join_parts: a thread has its row and 64 head dimensions from c0 on.
-__device__ __forceinline__ bool join_many(const FewParams& p, int slot, int owner, int parts, int row, int c0, float& top, float& l,
-                                          float (&o)[64], int tid, int* joins) {
-  constexpr int kPart = kManyRows * kD + 2 * kManyRows;
-  float* mine = p.parts + static_cast<int64_t>(slot) * kPart;
-#pragma unroll
-  for (int j = 0; j < 64; ++j)      // [dimension][row]: a warp's rows lie side by side
-    mine[(c0 + j) * kManyRows + row] = o[j];
-  if (c0 == 0) {
-    mine[kManyRows * kD + row] = top;
-    mine[kManyRows * kD + kManyRows + row] = l;
-  }
-  __threadfence();
-  teams_sync();
-  if (tid == 0) {
-    open_join(p.tickets + owner, p.launch_id);
-    *joins = last_to_join(p.tickets + owner, parts) ? 1 : 0;
-  }
-  teams_sync();
-  if (!*joins)
-    return false;
-  __threadfence();
-  const float* one = p.parts + (2 * static_cast<int64_t>(owner) + 1) * kPart;
-  const float* rest = p.parts + 2 * static_cast<int64_t>(owner) * kPart;
-  top = kNothing;
-  l = 0.f;
-#pragma unroll
-  for (int j = 0; j < 64; ++j)
-    o[j] = 0.f;
-  for (int i = 0; i < parts; ++i)
-    top = fmaxf(top, __ldcg((i == 0 ? one : rest + 2 * static_cast<int64_t>(i) * kPart) + kManyRows * kD + row));
-  for (int i = 0; i < parts; ++i) {
-    const float* src = i == 0 ? one : rest + 2 * static_cast<int64_t>(i) * kPart;
-    const float mul = exp2f(__ldcg(src + kManyRows * kD + row) - top);
-    l += __ldcg(src + kManyRows * kD + kManyRows + row) * mul;
-#pragma unroll
-    for (int j = 0; j < 64; ++j)
-      o[j] = fmaf(__ldcg(src + (c0 + j) * kManyRows + row), mul, o[j]);
-  }
-  return true;
+// A part in the workspace: [dimension][row] sums, [row] references, sums of weights; of a first part also output rows and `fix`.
+constexpr int kManyPart = kManyRows * (kD + 4);
+
+// One step of a product whose A operand, 32 codes of a row in 8 columns, lies in tensor memory.
+__device__ __forceinline__ void umma_tile_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_addr, uint32_t idesc, uint32_t accumulate) {
+  constexpr uint32_t high = (1024u >> 4) | (1u << 14) | (2u << 29);      // as umma_tile
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      ".reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], b, %3, p;\n\t"
+      "}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "r"((b_addr >> 4) | (1u << 16)), "r"(idesc), "r"(accumulate), "n"(high)
+      : "memory");
 }
 
 // CAP, BIAS: scores capped by a tanh, biased by their distance.
 template <bool CAP, bool BIAS>
-__global__ void __launch_bounds__(kManyThreads, 1)
+__global__ void __launch_bounds__(kManyThreads, kManyCtas)
 fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const FewParams p) {
   pdl_wait();      // programmatic dependent launch: nothing before this reads an earlier kernel's data
   pdl_trigger();
   const Fp8AttnParams& a = p.a;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* p_smem = ring + kManyRing * kTileBytes;           // per team [128 rows][128 keys]: e4m3, then e5m2
-  uint8_t* q_smem = p_smem + 4 * kTileBytes;                 // two slots of [128 rows][128] e4m3, then e5m2
-  float* sc_smem = reinterpret_cast<float*>(q_smem + 4 * kManyQBytes);      // per tile: K scale * factors, V exponent, 1 / V scale
-  __shared__ uint64_t full[kManyRing], empty[kManyRing], part_full[kParts], part_done[kParts], q_full[2], q_free[2], s_full[2], s_free[2],
-      sc_full[kScaleSlots], sc_free[kScaleSlots], p_full[2], pv_done[2], o_free;
+  uint8_t* q_smem = ring + kManyRing * kTileBytes;           // [128 rows][128] e4m3, then e5m2
+  uint8_t* stage = q_smem + 2 * kManyQBytes;
+  float* sc_smem = reinterpret_cast<float*>(stage + kManyWarps * kStageBytes);      // per tile: K scale * factors, V exponent, 1 / V scale
+  __shared__ uint64_t full[kManyRing], empty[kManyRing], part_full[kParts], part_done[kParts], q_full, q_free, s_full, p_full, pv_done, o_free,
+      sc_full[kScaleSlots], sc_free[kScaleSlots];
   __shared__ PartInfo s_part[kParts];
   __shared__ uint32_t tmem_slot, s_amax[2];
-  __shared__ int abort_flag, joins;
-  __shared__ RowInfo s_row[2][kManyRows];
-  __shared__ float2 s_ml[2][2][kManyRows];   // of parts in turn, per team: reference and sum of weights
+  __shared__ int abort_flag;
+  __shared__ RowInfo s_row[kManyRows];
+  __shared__ int64_t s_src[kManyRows];
+  __shared__ uint32_t s_bad[4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -1207,33 +1192,30 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     }
     for (int i = 0; i < kParts; ++i) {
       mbar_init(&part_full[i], 1);
-      mbar_init(&part_done[i], 2 * kTeamWarps + 2 + 4);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 4);
-      mbar_init(&q_free[i], 2 * kTeamWarps);
-      mbar_init(&s_full[i], 1);
-      mbar_init(&s_free[i], kTeamWarps);
-      mbar_init(&p_full[i], kTeamWarps);
-      mbar_init(&pv_done[i], 1);
+      mbar_init(&part_done[i], kManyWarps + 2 + 4);
     }
     for (int i = 0; i < kScaleSlots; ++i) {
       mbar_init(&sc_full[i], 4);
-      mbar_init(&sc_free[i], kTeamWarps);
+      mbar_init(&sc_free[i], kManyWarps);
     }
-    mbar_init(&o_free, 2 * kTeamWarps);
+    mbar_init(&q_full, 4);
+    mbar_init(&q_free, kManyWarps);
+    mbar_init(&s_full, 1);
+    mbar_init(&p_full, kManyWarps);
+    mbar_init(&pv_done, 1);
+    mbar_init(&o_free, kManyWarps);
     fence_mbar_init();
     tma_prefetch_desc(&tmap_k);
     tma_prefetch_desc(&tmap_v);
   }
   if (warp == 1) {
-    tmem_alloc(&tmem_slot, kTmemCols);
+    tmem_alloc(&tmem_slot, kManyTmemCols);
     tmem_relinquish();
   }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem = tmem_slot;      // a team's S: columns 0 and 128, its O: 256 and 384
+  const uint32_t tmem = tmem_slot;      // scores and weights: columns 0 .. 127, sums: 128 .. 255
   const int group = a.H / a.Hkv;
 
   if (warp == 2) {
@@ -1242,10 +1224,6 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     walk.start(p);
     for (int n = 0;;) {
       const bool more = walk.next(p);
-      if (more && walk.span.y <= walk.span.x) {      // no keys: zeros
-        zero_rows(a, walk.w, walk.hk, walk.tile * kManyRows, kManyRows);
-        continue;
-      }
       const int slot = n % kParts;
       if (n >= kParts && !mbar_wait(&part_done[slot], (n / kParts - 1) & 1, &abort_flag, p.status_word, 500))
         break;
@@ -1262,7 +1240,7 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         break;
     }
   } else if (warp == 0) {
-    // ---------------------------------------------------------------- producer: K of a tile before V of the last
+    // ---------------------------------------------------------------- producer: K and V in turn
     int n = 0;
     auto load = [&](const CUtensorMap* map, int row, int left, int x) {
       const int slot = n % kManyRing;
@@ -1278,96 +1256,72 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       ++n;
     };
     Chunks c = {};
-    int v_row = 0, v_left = 0, v_x = 0;
-    bool owed = false;
     for (bool more = c.open(part_full, part_done, s_part, &abort_flag, p.status_word); more;) {
-      for (int i = 0; i < c.tiles; ++i) {
-        const int key = c.begin + i * kUnitKeys;
+      for (int key = c.begin; key < c.end; key += kUnitKeys) {
         load(&tmap_k, c.k0 + key, c.end - key, c.hk * kD);
-        if (owed)
-          load(&tmap_v, v_row, v_left, v_x);
-        owed = true;
-        v_row = c.v0 + key;
-        v_left = c.end - key;
-        v_x = c.hk * kD;
+        load(&tmap_v, c.v0 + key, c.end - key, c.hk * kD);
       }
       ++c.n;
       more = c.open(part_full, part_done, s_part, &abort_flag, p.status_word);
     }
-    if (owed)
-      load(&tmap_v, v_row, v_left, v_x);
     // a CTA may not end with copies on their way, also when a wait of another warp has given up
     for (int i = max(0, n - kManyRing); i < n; ++i)
       mbar_wait(&full[i % kManyRing], (i / kManyRing) & 1, &abort_flag, p.status_word, 502);
   } else if (warp == 1) {
-    // ---------------------------------------------------------------- MMA issuer: scores of a tile before the sums of the last
-    constexpr uint32_t idesc_hi = umma_idesc_f8(128, 128, 1 * 0, 0, 0, 0), idesc_lo = umma_idesc_f8(128, 128, 1, 0, 0, 0);
+    // ---------------------------------------------------------------- MMA issuer
+    constexpr uint32_t idesc_hi = umma_idesc_f8(128, 128, 0, 0, 0, 0), idesc_lo = umma_idesc_f8(128, 128, 1, 0, 0, 0);
     constexpr uint32_t idesc_pv = umma_idesc_f8(128, 128, 0, 0, 0, 1), idesc_pv_lo = umma_idesc_f8(128, 128, 1, 0, 0, 1);
-    const uint32_t ring_addr = smem_u32(ring), p_addr = smem_u32(p_smem), t_s = uniform(tmem), t_o = t_s + 256;
-    int n = 0, n_s = 0, n_p = 0;
-    auto sums = [&](int part, int tile) {      // P V of the tile before, the tile-th of its part
-      const int team = n_p & 1;
-      const int slot = n % kManyRing;
-      mbar_wait(&full[slot], (n / kManyRing) & 1, &abort_flag, p.status_word, 506);
-      if (tile == 0 && part > 0)
-        mbar_wait(&o_free, (part - 1) & 1, &abort_flag, p.status_word, 508);
-      mbar_wait(&p_full[team], (n_p >> 1) & 1, &abort_flag, p.status_word, 507);
-      tc_fence_after_sync();
-      if (elect_one()) {
-        const uint32_t v_addr = ring_addr + slot * kTileBytes;
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {      // 32 keys: 32 bytes of the weights' rows, 32 rows of V
-          const uint32_t w_addr = p_addr + team * 2 * kTileBytes + 32 * kk;
-          umma_tile(t_o + team * 128, w_addr, v_addr + kk * 4096, idesc_pv, tile < 2 && kk == 0 ? 0u : 1u);
-          umma_tile(t_o + team * 128, w_addr + kTileBytes, v_addr + kk * 4096, idesc_pv_lo, 1u);
-        }
-        umma_commit(&empty[slot]);
-        umma_commit(&pv_done[team]);
-      }
-      __syncwarp();
-      ++n;
-      ++n_p;
-    };
+    const uint32_t ring_addr = smem_u32(ring), q_addr = smem_u32(q_smem), t_s = uniform(tmem), t_o = t_s + 128;
+    int g = 0, live = 0;      // tiles, parts that have some
     Chunks c = {};
-    int owed_part = -1, owed_tile = 0;
     for (bool more = c.open(part_full, part_done, s_part, &abort_flag, p.status_word); more;) {
-      mbar_wait(&q_full[c.n & 1], (c.n >> 1) & 1, &abort_flag, p.status_word, 503);
-      const uint32_t q_addr = smem_u32(q_smem) + (c.n & 1) * 2 * kManyQBytes;
-      for (int i = 0; i < c.tiles; ++i) {
-        const int buf = n_s & 1, slot = n % kManyRing;
-        if (n_s >= 2)
-          mbar_wait(&s_free[buf], ((n_s >> 1) - 1) & 1, &abort_flag, p.status_word, 504);
-        mbar_wait(&full[slot], (n / kManyRing) & 1, &abort_flag, p.status_word, 505);
+      if (c.tiles)
+        mbar_wait(&q_full, live & 1, &abort_flag, p.status_word, 503);
+      for (int i = 0; i < c.tiles; ++i, ++g) {
+        const int ks = 2 * g % kManyRing, vs = ks + 1;
+        const uint32_t parity = (2 * g / kManyRing) & 1;
+        mbar_wait(&full[ks], parity, &abort_flag, p.status_word, 505);
+        if (g)
+          mbar_wait(&pv_done, (g - 1) & 1, &abort_flag, p.status_word, 504);      // the weights have been taken: their columns are free
         tc_fence_after_sync();
         if (elect_one()) {
-          const uint32_t k_addr = ring_addr + slot * kTileBytes;
+          const uint32_t k_addr = ring_addr + ks * kTileBytes;
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {      // 32 head dimensions = 32 bytes a step
-            umma_tile(t_s + buf * 128, q_addr + 32 * kk, k_addr + 32 * kk, idesc_hi, kk != 0 ? 1u : 0u);
-            umma_tile(t_s + buf * 128, q_addr + kManyQBytes + 32 * kk, k_addr + 32 * kk, idesc_lo, 1u);
+            umma_tile(t_s, q_addr + 32 * kk, k_addr + 32 * kk, idesc_hi, kk != 0 ? 1u : 0u);
+            umma_tile(t_s, q_addr + kManyQBytes + 32 * kk, k_addr + 32 * kk, idesc_lo, 1u);
           }
-          umma_commit(&empty[slot]);
-          umma_commit(&s_full[buf]);
+          umma_commit(&empty[ks]);
+          umma_commit(&s_full);
         }
         __syncwarp();
-        ++n;
-        ++n_s;
-        if (owed_part >= 0)
-          sums(owed_part, owed_tile);
-        owed_part = c.n;
-        owed_tile = i;
+        mbar_wait(&full[vs], parity, &abort_flag, p.status_word, 506);
+        if (i == 0 && live > 0)
+          mbar_wait(&o_free, (live - 1) & 1, &abort_flag, p.status_word, 508);
+        mbar_wait(&p_full, g & 1, &abort_flag, p.status_word, 507);
+        tc_fence_after_sync();
+        if (elect_one()) {
+          const uint32_t v_addr = ring_addr + vs * kTileBytes;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {      // 32 keys: 8 columns of weights, 32 rows of V
+            umma_tile_ts(t_o, t_s + 32 * kk, v_addr + kk * 4096, idesc_pv, i == 0 && kk == 0 ? 0u : 1u);
+            umma_tile_ts(t_o, t_s + 32 * kk + 8, v_addr + kk * 4096, idesc_pv_lo, 1u);
+          }
+          umma_commit(&empty[vs]);
+          umma_commit(&pv_done);
+        }
+        __syncwarp();
       }
+      live += c.tiles ? 1 : 0;
       ++c.n;
       more = c.open(part_full, part_done, s_part, &abort_flag, p.status_word);
     }
-    if (owed_part >= 0)
-      sums(owed_part, owed_tile);
-  } else if (warp >= 3 + 2 * kTeamWarps) {
+  } else if (warp >= 3 + kManyWarps) {
     // ---------------------------------------------------------------- loaders: queries of a part, scales of its tiles
-    const int tid = threadIdx.x - 32 * (3 + 2 * kTeamWarps);
-    int n_sc = 0;
+    const int tid = threadIdx.x - 32 * (3 + kManyWarps);
+    int n_sc = 0, live = 0;
     for (int n = 0;; ++n) {
-      const int slot = n % kParts, qb = n & 1;
+      const int slot = n % kParts, qb = live & 1;
       if (!mbar_wait(&part_full[slot], (n / kParts) & 1, &abort_flag, p.status_word, 510))
         break;
       const PartInfo w = s_part[slot];
@@ -1375,90 +1329,102 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       warp_arrive(&part_done[slot]);
       if (w.end < 0)
         break;
-      if (n >= 2)
-        mbar_wait(&q_free[qb], ((n >> 1) - 1) & 1, &abort_flag, p.status_word, 511);
-      // queries: eight threads a row, 16 rows at a time; all loads first (one after the other they took 13 us a part)
-      if (tid == 0)
-        s_amax[qb] = 0;
-      int row[8];
-      uint4 x0[8], x1[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int t = w.t0 + 16 * k + (tid >> 3);
-        row[k] = t < w.rows ? __ldg(a.idx + w.row0 + t / group) : -1;
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int t = w.t0 + 16 * k + (tid >> 3), head = w.hk * group + t % group;
-        row[k] = row[k] >= a.total_q ? -1 : row[k];
-        x0[k] = x1[k] = make_uint4(0u, 0u, 0u, 0u);
-        if (row[k] >= 0) {
-          const uint4* src = reinterpret_cast<const uint4*>(a.q + row[k] * a.ldq + head * kD) + (tid & 7) * 2;
-          x0[k] = __ldg(src);
-          x1[k] = __ldg(src + 1);
-        }
-      }
-      loaders_sync();
-      uint32_t finite = 0;
-      {
-        uint32_t top = 0;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t m = fp8_amax8(max(bf16x8_amax(x0[k]), bf16x8_amax(x1[k])));
-          if (m < 0x7f800000u) {
-            finite |= 1u << k;
-            top = max(top, m);
+      // thread = row: where its query lies, what the softmax warps need to know of it
+      const int t = w.t0 + tid, i = t / group, head = w.hk * group + t - i * group;
+      RowInfo v = {};
+      v.out = -1;
+      int64_t src = -1;
+      if (t < w.rows) {
+        v.out = (w.row0 + i) * a.H + head;
+        const int at = __ldg(a.idx + w.row0 + i);
+        if (at >= 0 && at < a.total_q) {
+          src = at * a.ldq + head * kD;
+          v.fix = 1.f;
+          v.hi = w.len;
+          v.pos = __ldg(a.cu_k + w.b + 1) - __ldg(a.cu_k + w.b) - (__ldg(a.cu_q + w.b + 1) - at);
+          v.slope = BIAS ? __ldg(a.slopes + head) * kLog2e : 0.f;
+          if (a.ranges) {
+            const int2 range = __ldg(a.ranges + at);
+            v.lo = range.x;
+            v.hi = min(range.y, w.len);
           }
         }
-        top = __reduce_max_sync(0xffffffffu, top);
-        if (lane == 0)
-          atomicMax(&s_amax[qb], top);
       }
+      if (w.end == w.begin) {      // no keys: zeros
+        s_src[tid] = v.out;
+        loaders_sync();
+#pragma unroll 1
+        for (int r = tid >> 4; r < kManyRows; r += 8)
+          if (s_src[r] >= 0)
+            *reinterpret_cast<uint4*>(a.out + s_src[r] * kD + (tid & 15) * 8) = make_uint4(0u, 0u, 0u, 0u);
+        loaders_sync();
+        continue;
+      }
+      s_src[tid] = src;
+      if (tid == 0)
+        s_amax[qb] = 0;
+      if (tid < 4)
+        s_bad[tid] = 0;
+      loaders_sync();
+      // queries: eight threads a row, 16 rows at a time, four times 16 in flight; first the largest element, then (from L1) the
+      // codes.  (Loops: straight-line code for 128 rows that runs once a part costs more in instruction fetches than it saves.)
+      uint4 x0[4], x1[4];
+      auto fetch = [&](int h) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int64_t from = s_src[64 * h + 16 * k + (tid >> 3)];
+          x0[k] = x1[k] = make_uint4(0u, 0u, 0u, 0u);
+          if (from >= 0) {
+            const uint4* q = reinterpret_cast<const uint4*>(a.q + from) + (tid & 7) * 2;
+            x0[k] = __ldg(q);
+            x1[k] = __ldg(q + 1);
+          }
+        }
+      };
+      uint32_t top = 0;
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        fetch(h);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = 64 * h + 16 * k + (tid >> 3);
+          const uint32_t m = fp8_amax8(max(bf16x8_amax(x0[k]), bf16x8_amax(x1[k])));
+          if (m < 0x7f800000u)
+            top = max(top, m);
+          else if ((tid & 7) == 0)
+            atomicOr(&s_bad[r >> 5], 1u << (r & 31));
+        }
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0)
+        atomicMax(&s_amax[qb], top);
       loaders_sync();
       const uint32_t scale = fp8_scale_bits(s_amax[qb]);
       const float inv = fp8_inverse(scale);
-      uint8_t* q_dst = q_smem + qb * 2 * kManyQBytes;
+      if (live > 0)
+        mbar_wait(&q_free, (live - 1) & 1, &abort_flag, p.status_word, 511);
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        fetch(h);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int r = 16 * k + (tid >> 3), part = tid & 7;
-        if (!(finite >> k & 1))
-          x0[k] = x1[k] = make_uint4(0u, 0u, 0u, 0u);
-        uint4 hi, lo;
-        split_query(x0[k], x1[k], inv, hi, lo);
-        uint8_t* dst = q_dst + r * kD + ((part ^ (r & 7)) << 4);
-        *reinterpret_cast<uint4*>(dst) = hi;
-        *reinterpret_cast<uint4*>(dst + kManyQBytes) = lo;
-      }
-      {
-        // one thread a row: what the softmax warps need to know of it
-        const int t = w.t0 + tid, i = t / group, head = w.hk * group + t - i * group;
-        RowInfo v = {};
-        v.out = -1;
-        if (t < w.rows) {
-          int at = __ldg(a.idx + w.row0 + i);
-          at = at >= a.total_q ? -1 : at;
-          v.out = (w.row0 + i) * a.H + head;
-          if (at >= 0) {
-            v.fix = 1.f;
-            v.hi = w.len;
-            v.pos = __ldg(a.cu_k + w.b + 1) - __ldg(a.cu_k + w.b) - (__ldg(a.cu_q + w.b + 1) - at);
-            v.slope = BIAS ? __ldg(a.slopes + head) * kLog2e : 0.f;
-            if (a.ranges) {
-              const int2 range = __ldg(a.ranges + at);
-              v.lo = range.x;
-              v.hi = min(range.y, w.len);
-            }
-          }
+        for (int k = 0; k < 4; ++k) {
+          const int r = 64 * h + 16 * k + (tid >> 3), part = tid & 7;
+          if (s_bad[r >> 5] >> (r & 31) & 1)
+            x0[k] = x1[k] = make_uint4(0u, 0u, 0u, 0u);
+          uint4 hi, lo;
+          split_query(x0[k], x1[k], inv, hi, lo);
+          uint8_t* dst = q_smem + r * kD + ((part ^ (r & 7)) << 4);
+          *reinterpret_cast<uint4*>(dst) = hi;
+          *reinterpret_cast<uint4*>(dst + kManyQBytes) = lo;
         }
-        s_row[qb][tid] = v;
       }
-      loaders_sync();
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if ((tid & 7) == 0 && row[k] >= 0 && !(finite >> k & 1))
-          s_row[qb][16 * k + (tid >> 3)].fix = __uint_as_float(0x7fc00000u);
+      if (s_bad[tid >> 5] >> (tid & 31) & 1)
+        v.fix = __uint_as_float(0x7fc00000u);
+      s_row[tid] = v;
       fence_proxy_async_smem();
-      warp_arrive(&q_full[qb]);
+      loaders_sync();
+      warp_arrive(&q_full);
+      ++live;
       // scales: thread = key, four tiles' loads at a time
       // scores come out times log2(e), or as twice the argument of the tanh that caps them
       const float mul = a.scale * __uint_as_float(scale) * kLog2e * (CAP ? 2.f / a.cap : 1.f);
@@ -1493,29 +1459,38 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     }
   } else {
     // ---------------------------------------------------------------- softmax: thread = row
-    const int quarter = warp & 3, team = (warp - 3) >> 2;
+    const int quarter = warp & 3;
     const int tid = threadIdx.x - 96;
     const int row = quarter * 32 + lane;
-    const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16), t_s = t_lane + team * 128, t_o = t_lane + 256;
-    uint8_t* p_dst = p_smem + team * 2 * kTileBytes + row * kD;
-    int n_tile = 0;                   // tiles so far, of both teams
-    bool more = mbar_wait(&part_full[0], 0, &abort_flag, p.status_word, 515) && s_part[0].end >= 0;
-    for (int n = 0; more; ++n) {
+    const uint32_t t_s = tmem + (static_cast<uint32_t>(quarter * 32) << 16), t_o = t_s + 128;
+    uint8_t* out_stage = stage + (warp - 3) * kStageBytes;
+    int g = 0;                        // tiles so far
+    bool owns = false;                // the first part of a tile that goes on in other CTAs
+    int live = 0;
+    for (int n = 0;; ++n) {
+      if (!mbar_wait(&part_full[n % kParts], (n / kParts) & 1, &abort_flag, p.status_word, 515))
+        break;
       const PartInfo& part = s_part[n % kParts];
-      const int qb = n & 1, begin = part.begin, end = part.end, tiles = (end - begin + kUnitKeys - 1) / kUnitKeys;
+      const int begin = part.begin, end = part.end;
       const bool alive = part.t0 + quarter * 32 < part.rows;
-      const int joined_slot = part.slot, joined_owner = part.owner, joined_parts = part.parts;
-      mbar_wait(&q_full[qb], (n >> 1) & 1, &abort_flag, p.status_word, 516);
-      const RowInfo me = s_row[qb][row];
+      const int joined_slot = part.slot, joined_parts = part.parts;
+      const bool joined_first = part.first != 0;
+      if (end <= begin) {
+        warp_arrive(&part_done[n % kParts]);
+        if (end < 0)
+          break;
+        continue;
+      }
+      mbar_wait(&q_full, live & 1, &abort_flag, p.status_word, 516);
+      const RowInfo me = s_row[row];
       warp_arrive(&part_done[n % kParts]);
-      more = mbar_wait(&part_full[(n + 1) % kParts], ((n + 1) / kParts) & 1, &abort_flag, p.status_word, 517) && s_part[(n + 1) % kParts].end >= 0;
+      ++live;
       float ref = kNothing, l = 0.f;
-      const int i0 = (n_tile ^ team) & 1;
-      for (int i = i0; i < tiles; i += 2) {
-        const int g = n_tile + i, sl = g % kScaleSlots, key0 = begin + i * kUnitKeys;
+      for (int key0 = begin; key0 < end; key0 += kUnitKeys, ++g) {
+        const int sl = g % kScaleSlots;
         const float* sc = sc_smem + sl * 3 * kUnitKeys;
         mbar_wait(&sc_full[sl], (g / kScaleSlots) & 1, &abort_flag, p.status_word, 518);
-        mbar_wait(&s_full[team], (g >> 1) & 1, &abort_flag, p.status_word, 519);
+        mbar_wait(&s_full, g & 1, &abort_flag, p.status_word, 519);      // and with it the product before
         tc_fence_after_sync();
         bool grown = false;
         float old = 1.f;
@@ -1523,36 +1498,42 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
           // scores (times log2 e, plus the exponents of the values' scales), in place of the products, and their maximum
           float mx = kNothing;
           const int lo = me.lo - key0, hi = min(me.hi, end) - key0;
-          const bool cut = __any_sync(0xffffffffu, me.out >= 0 && (lo > 0 || hi < kUnitKeys));
           const float away = static_cast<float>(me.pos - key0);
+          uint32_t s[2][16];
+          tmem_ld_32x16(t_s, s[0]);
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
-            uint32_t s[32];
-            tmem_ld_32x32(t_s + c * 32, s);
-            tmem_ld_wait();
-            float* t = reinterpret_cast<float*>(s);
-            const float d = away - static_cast<float>(c * 32);
+            const uint32_t seen = below(hi - c * 32) & ~below(lo - c * 32);      // of 32 keys
+            const bool cut = __any_sync(0xffffffffu, me.out >= 0 && seen != 0xffffffffu);
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const float4 kk = *reinterpret_cast<const float4*>(sc + c * 32 + j);
-              const float4 ex = *reinterpret_cast<const float4*>(sc + kUnitKeys + c * 32 + j);
-              const float k4[4] = {kk.x, kk.y, kk.z, kk.w}, e4[4] = {ex.x, ex.y, ex.z, ex.w};
+            for (int h = 0; h < 2; ++h) {
+              tmem_ld_wait();
+              if (h == 0 || c < 3)
+                tmem_ld_32x16(t_s + c * 32 + (h + 1) * 16, s[h ^ 1]);
+              float* t = reinterpret_cast<float*>(s[h]);
+              const float d = away - static_cast<float>(c * 32 + h * 16);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                t[j + e] = CAP ? fmaf(capped(t[j + e] * k4[e], a.cap), kLog2e, e4[e]) : fmaf(t[j + e], k4[e], e4[e]);
-                if (BIAS)
-                  t[j + e] = fmaf(-me.slope, fabsf(d - static_cast<float>(j + e)), t[j + e]);
+              for (int j = 0; j < 16; j += 4) {
+                const float4 kk = *reinterpret_cast<const float4*>(sc + c * 32 + h * 16 + j);
+                const float4 ex = *reinterpret_cast<const float4*>(sc + kUnitKeys + c * 32 + h * 16 + j);
+                const float k4[4] = {kk.x, kk.y, kk.z, kk.w}, e4[4] = {ex.x, ex.y, ex.z, ex.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  t[j + e] = CAP ? fmaf(capped(t[j + e] * k4[e], a.cap), kLog2e, e4[e]) : fmaf(t[j + e], k4[e], e4[e]);
+                  if (BIAS)
+                    t[j + e] = fmaf(-me.slope, fabsf(d - static_cast<float>(j + e)), t[j + e]);
+                }
               }
-            }
-            if (cut) {
+              if (cut) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
-                s[j] = c * 32 + j >= lo && c * 32 + j < hi ? s[j] : 0xff800000u;
-            }
+                for (int j = 0; j < 16; ++j)
+                  t[j] = seen >> (h * 16 + j) & 1 ? t[j] : -INFINITY;
+              }
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              mx = fmax3(mx, t[2 * j], t[2 * j + 1]);
-            tmem_st_32x32(t_s + c * 32, s);
+              for (int j = 0; j < 16; j += 2)
+                mx = fmax3(mx, t[j], t[j + 1]);
+              tmem_st_32x16(t_s + c * 32 + h * 16, s[h]);
+            }
           }
           tmem_st_wait();
           grown = mx > ref + kHeadroom;
@@ -1560,57 +1541,51 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
             old = exp2f(ref - mx);
             ref = mx;
           }
-        }
-        // the team's last weights have been taken
-        if (g >= 2)
-          mbar_wait(&pv_done[team], ((g >> 1) - 1) & 1, &abort_flag, p.status_word, 520);
-        if (alive) {
-          if (i >= 2 && __any_sync(0xffffffffu, grown)) {
-            tc_fence_after_sync();
+          if (key0 > begin && __any_sync(0xffffffffu, grown)) {
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
               uint32_t o[32];
-              tmem_ld_32x32(t_o + team * 128 + c * 32, o);
+              tmem_ld_32x32(t_o + c * 32, o);
               tmem_ld_wait();
 #pragma unroll
               for (int j = 0; j < 32; ++j)
                 o[j] = __float_as_uint(__uint_as_float(o[j]) * old);
-              tmem_st_32x32(t_o + team * 128 + c * 32, o);
+              tmem_st_32x32(t_o + c * 32, o);
             }
             tmem_st_wait();
           }
           const float shift = kWeightLog2 - ref;
           float sum[2] = {l * old, 0.f};
+          tmem_ld_32x16(t_s, s[0]);
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
-            uint32_t s[32];
-            tmem_ld_32x32(t_s + c * 32, s);
-            tmem_ld_wait();
-            uint32_t hi4[8], lo4[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float4 inv = *reinterpret_cast<const float4*>(sc + 2 * kUnitKeys + c * 32 + 4 * j);
-              const uint32_t* u = s + 4 * j;
-              const float2 x = make_float2(exp2f(__uint_as_float(u[0]) + shift), exp2f(__uint_as_float(u[1]) + shift));
-              const float2 y = make_float2(exp2f(__uint_as_float(u[2]) + shift), exp2f(__uint_as_float(u[3]) + shift));
-              sum[0] = fmaf(x.x, inv.x, sum[0]);
-              sum[1] = fmaf(x.y, inv.y, sum[1]);
-              sum[0] = fmaf(y.x, inv.z, sum[0]);
-              sum[1] = fmaf(y.y, inv.w, sum[1]);
-              split_weights_e5m2(x, y, hi4[j], lo4[j]);
-            }
+            uint32_t codes[16];      // e4m3 of 32 keys, then e5m2
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const int chunk = ((c * 2 + h) ^ (row & 7)) << 4;
-              *reinterpret_cast<uint4*>(p_dst + chunk) = make_uint4(hi4[4 * h], hi4[4 * h + 1], hi4[4 * h + 2], hi4[4 * h + 3]);
-              *reinterpret_cast<uint4*>(p_dst + kTileBytes + chunk) = make_uint4(lo4[4 * h], lo4[4 * h + 1], lo4[4 * h + 2], lo4[4 * h + 3]);
+              tmem_ld_wait();
+              if (h == 0 || c < 3)
+                tmem_ld_32x16(t_s + c * 32 + (h + 1) * 16, s[h ^ 1]);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float4 inv = *reinterpret_cast<const float4*>(sc + 2 * kUnitKeys + c * 32 + h * 16 + 4 * j);
+                const uint32_t* u = s[h] + 4 * j;
+                const float2 x = make_float2(exp2f(__uint_as_float(u[0]) + shift), exp2f(__uint_as_float(u[1]) + shift));
+                const float2 y = make_float2(exp2f(__uint_as_float(u[2]) + shift), exp2f(__uint_as_float(u[3]) + shift));
+                sum[0] = fmaf(x.x, inv.x, sum[0]);
+                sum[1] = fmaf(x.y, inv.y, sum[1]);
+                sum[0] = fmaf(y.x, inv.z, sum[0]);
+                sum[1] = fmaf(y.y, inv.w, sum[1]);
+                split_weights_e5m2(x, y, codes[h * 4 + j], codes[8 + h * 4 + j]);
+              }
             }
+            tmem_st_32x16(t_s + c * 32, codes);
           }
+          tmem_st_wait();
           l = sum[0] + sum[1];
         }
         if (key0 + kUnitKeys > end) {
           // rows of V behind the last key may hold any byte, a NaN times a weight of zero among them
-          const int use = 2 * g + 1 + (more ? 1 : 0);      // the order of the ring: K(0), K(1), V(0), K(2), V(1), ...
+          const int use = 2 * g + 1;
           mbar_wait(&full[use % kManyRing], (use / kManyRing) & 1, &abort_flag, p.status_word, 521);
           if (key0 + row >= end) {
             uint4* v = reinterpret_cast<uint4*>(ring + (use % kManyRing) * kTileBytes + row * kD);
@@ -1621,71 +1596,117 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         }
         tc_fence_before_sync();
         fence_proxy_async_smem();
-        warp_arrive(&p_full[team]);
-        warp_arrive(&s_free[team]);
+        warp_arrive(&p_full);
         warp_arrive(&sc_free[sl]);
       }
-      warp_arrive(&q_free[qb]);      // all scores of the part have been taken
-      // ---------------------------------------------------------------- the teams meet: a thread takes 64 head dimensions of its row
-      s_ml[n & 1][team][row] = make_float2(ref, l);
-      teams_sync();
-      const float2 a0 = s_ml[n & 1][0][row], a1 = s_ml[n & 1][1][row];
-      n_tile += tiles;
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int done = (n_tile + 1 - t) >> 1;      // products of team t so far
-        if (done > 0)
-          mbar_wait(&pv_done[t], (done - 1) & 1, &abort_flag, p.status_word, 522);
-      }
+      warp_arrive(&q_free);      // all scores of the part have been taken
+      // ---------------------------------------------------------------- the end of a part, 32 head dimensions at a time
+      mbar_wait(&pv_done, (g - 1) & 1, &abort_flag, p.status_word, 522);
       tc_fence_after_sync();
-      float top = fmaxf(a0.x, a1.x);
-      const float f0 = exp2f(a0.x - top), f1 = exp2f(a1.x - top);
-      l = a0.y * f0 + a1.y * f1;
-      float o[64];
-      if (alive) {
-        // a part of one tile has left nothing in the other team's columns
-        const bool both = tiles > 1;
-        const int sole = (n_tile - 1) & 1;
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          uint32_t u[16], v[16];
-          tmem_ld_32x16(t_o + (both ? 0 : sole * 128) + team * 64 + h * 16, u);
-          tmem_ld_32x16(t_o + 128 + team * 64 + h * 16, v);
+      if (joined_parts > 1) {
+        // the part goes to the workspace; fp8_join_kernel adds the parts of a tile up in their order
+        float* mine = p.parts + static_cast<int64_t>(joined_slot) * kManyPart;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          tmem_ld_32x32(t_o + c * 32, o);
           tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            o[h * 16 + j] = both ? fmaf(__uint_as_float(u[j]), f0, __uint_as_float(v[j]) * f1) : __uint_as_float(u[j]);
+          for (int j = 0; j < 32; ++j)      // a warp's rows lie side by side
+            mine[(c * 32 + j) * kManyRows + row] = __uint_as_float(o[j]);
         }
-        if (!both) {
-          top = sole ? a1.x : a0.x;
-          l = sole ? a1.y : a0.y;
+        mine += kManyRows * kD + row;
+        mine[0] = ref;
+        mine[kManyRows] = l;
+        if (joined_first) {
+          mine[2 * kManyRows] = __int_as_float(me.out);
+          mine[3 * kManyRows] = me.fix;
+          if (tid == 0)
+            p.joins[blockIdx.x] = joined_parts;
+          owns = true;
+        }
+      } else if (alive) {
+        const bool none = l == 0.f || me.fix == 0.f;
+        const float mul = __fdividef(me.fix, l);
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          tmem_ld_32x32(t_o + c * 32, o);
+          tmem_ld_wait();
+          // by way of shared memory: four lanes store the 64 bytes of a row
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              x[e] = none ? 0.f : __uint_as_float(o[8 * j + e]) * mul;
+            *reinterpret_cast<uint4*>(out_stage + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = float_to_bf16x8(x);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int r = j * 8 + (lane >> 2);
+            const int to = __shfl_sync(0xffffffffu, me.out, r);
+            const uint4 v = *reinterpret_cast<const uint4*>(out_stage + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
+            if (to >= 0)
+              *reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(to) * kD + c * 32 + (lane & 3) * 8) = v;
+          }
+          __syncwarp();
         }
       }
       tc_fence_before_sync();
       warp_arrive(&o_free);
-      if ((joined_parts == 1 || join_many(p, joined_slot, joined_owner, joined_parts, row, team * 64, top, l, o, tid, &joins)) && alive &&
-          me.out >= 0) {
-        const bool none = l == 0.f || me.fix == 0.f;
-        const float mul = __fdividef(me.fix, l);
-        uint4* dst = reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(me.out) * kD + team * 64);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float x[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            x[e] = none ? 0.f : o[8 * j + e] * mul;
-          dst[j] = float_to_bf16x8(x);
-        }
-      }
     }
+    if (tid == 0 && !owns)
+      p.joins[blockIdx.x] = 0;
   }
 
   tc_fence_before_sync();
   __syncthreads();
   if (warp == 1) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem, kTmemCols);
+    tmem_dealloc(tmem, kManyTmemCols);
   }
+}
+
+// Tiles whose parts lie in several CTAs of the many-rows kernel: the parts, in their order, added up.  A block has the tile that
+// begins in CTA blockIdx.x (if one goes on from there) and 32 head dimensions, a thread a row and 8 of them.  (The CTA that
+// finishes last took 76 us to do this alone with 19 parts.)
+constexpr int kJoinThreads = 512;
+__global__ void __launch_bounds__(kJoinThreads) fp8_join_kernel(const FewParams p) {
+  pdl_wait();
+  pdl_trigger();
+  const int owner = blockIdx.x, row = threadIdx.x & (kManyRows - 1), c0 = blockIdx.y * 32 + (threadIdx.x / kManyRows) * 8;
+  const int parts = __ldcg(p.joins + owner);
+  if (parts == 0)
+    return;
+  const float* one = p.parts + (2 * static_cast<int64_t>(owner) + 1) * kManyPart + row;
+  const float* rest = p.parts + 2 * static_cast<int64_t>(owner) * kManyPart + row;
+  auto part = [&](int i) { return i == 0 ? one : rest + 2 * static_cast<int64_t>(i) * kManyPart; };
+  constexpr int kRef = kManyRows * kD;
+  const int out = __float_as_int(__ldcg(one + kRef + 2 * kManyRows));
+  if (out < 0)
+    return;
+  float top = kNothing, l = 0.f, o[8] = {};
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i)
+    top = fmaxf(top, __ldcg(part(i) + kRef));
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) {
+    const float* src = part(i);
+    const float f = exp2f(__ldcg(src + kRef) - top);
+    l = fmaf(__ldcg(src + kRef + kManyRows), f, l);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      o[j] = fmaf(__ldcg(src + (c0 + j) * kManyRows), f, o[j]);
+  }
+  const float fix = __ldcg(one + kRef + 3 * kManyRows);
+  const bool none = l == 0.f || fix == 0.f;
+  const float mul = __fdividef(fix, l);
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    o[j] = none ? 0.f : o[j] * mul;
+  *reinterpret_cast<uint4*>(p.a.out + static_cast<int64_t>(out) * kD + c0) = float_to_bf16x8(o);
 }
 
 // Keys that any row of a tile sees; one warp per tile, numbered as Walk does.
@@ -1734,8 +1755,9 @@ __global__ void __launch_bounds__(128) fp8_spans_kernel(const Fp8AttnParams p, i
 int64_t most_tiles(int num_salient, int batch, int group) { return static_cast<int64_t>(num_salient) * group / kRows + batch; }
 size_t parts_offset(int64_t tiles, int ctas) { return (ctas * sizeof(unsigned long long) + tiles * sizeof(int2) + 255) / 256 * 256; }
 size_t workspace_of(int num_salient, int batch, int group, int ctas) {
-  const int rows = static_cast<int64_t>(num_salient) * group > kRows ? kManyRows : kRows;
-  return parts_offset(most_tiles(num_salient, batch, group), ctas) + 2ull * ctas * rows * (kD + 2) * sizeof(float);
+  const size_t few = 2ull * ctas * kRows * (kD + 2), many = 2ull * kManyCtas * ctas * kManyPart;
+  return parts_offset(most_tiles(num_salient, batch, group), kManyCtas * ctas) +
+         (static_cast<int64_t>(num_salient) * group > kRows ? max(few, many) : few) * sizeof(float);
 }
 
 template <typename Kernel>
@@ -1761,7 +1783,11 @@ int launch_few(const CUtensorMap& tk, const CUtensorMap& tv, const FewParams& p,
 template <bool CAP, bool BIAS>
 int launch_many(const CUtensorMap& tk, const CUtensorMap& tv, const FewParams& p, int ctas, cudaStream_t s) {
   static bool set[64] = {};
-  return launch_rows(fp8_many_rows_kernel<CAP, BIAS>, set, kManyThreads, kManySmem, tk, tv, p, ctas, s);
+  const int rc = launch_rows(fp8_many_rows_kernel<CAP, BIAS>, set, kManyThreads, kManySmem, tk, tv, p, kManyCtas * ctas, s);
+  if (rc != DYLLM_OK)
+    return rc;
+  DYLLM_LAUNCH(fp8_join_kernel, dim3(kManyCtas * ctas, kD / 32), kJoinThreads, 0, s, p);
+  return check_launch("attention_salient_rows_fp8");
 }
 
 }  // namespace
@@ -1849,9 +1875,10 @@ int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, co
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   f.a = p;
-  f.tickets = reinterpret_cast<unsigned long long*>(ws);
-  int2* spans = reinterpret_cast<int2*>(ws + ctas * sizeof(unsigned long long));
-  f.parts = reinterpret_cast<float*>(ws + parts_offset(tiles, ctas));
+  f.tickets = reinterpret_cast<unsigned long long*>(ws);      // few rows
+  f.joins = reinterpret_cast<int*>(ws);                       // many rows
+  int2* spans = reinterpret_cast<int2*>(ws + kManyCtas * ctas * sizeof(unsigned long long));
+  f.parts = reinterpret_cast<float*>(ws + parts_offset(tiles, kManyCtas * ctas));
   f.launch_id = next_launch_id() & ~0xffffull;
   f.status_word = device_status_word();
   // a sequence with more rows than the bound says is served by either kernel; so is one with few beside others with many
