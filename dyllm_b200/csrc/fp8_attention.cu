@@ -1132,6 +1132,32 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+// Pairs of floats in one instruction.
+__device__ __forceinline__ float2 get2(const float* x) { return make_float2(x[0], x[1]); }
+__device__ __forceinline__ void put2(float* x, float2 v) {
+  x[0] = v.x;
+  x[1] = v.y;
+}
+__device__ __forceinline__ uint64_t bits2(float2 v) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+  return r;
+}
+__device__ __forceinline__ float2 floats2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
+  return floats2(r);
+}
+__device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
+  return floats2(r);
+}
 // The lowest n bits.
 __device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
@@ -1516,11 +1542,18 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
               for (int j = 0; j < 16; j += 4) {
                 const float4 kk = *reinterpret_cast<const float4*>(sc + c * 32 + h * 16 + j);
                 const float4 ex = *reinterpret_cast<const float4*>(sc + kUnitKeys + c * 32 + h * 16 + j);
-                const float k4[4] = {kk.x, kk.y, kk.z, kk.w}, e4[4] = {ex.x, ex.y, ex.z, ex.w};
+                if (!CAP) {
+                  put2(t + j, ffma2(get2(t + j), make_float2(kk.x, kk.y), make_float2(ex.x, ex.y)));
+                  put2(t + j + 2, ffma2(get2(t + j + 2), make_float2(kk.z, kk.w), make_float2(ex.z, ex.w)));
+                } else {
+                  const float k4[4] = {kk.x, kk.y, kk.z, kk.w}, e4[4] = {ex.x, ex.y, ex.z, ex.w};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  t[j + e] = CAP ? fmaf(capped(t[j + e] * k4[e], a.cap), kLog2e, e4[e]) : fmaf(t[j + e], k4[e], e4[e]);
-                  if (BIAS)
+                  for (int e = 0; e < 4; ++e)
+                    t[j + e] = fmaf(capped(t[j + e] * k4[e], a.cap), kLog2e, e4[e]);
+                }
+                if (BIAS) {
+#pragma unroll
+                  for (int e = 0; e < 4; ++e)
                     t[j + e] = fmaf(-me.slope, fabsf(d - static_cast<float>(j + e)), t[j + e]);
                 }
               }
@@ -1555,7 +1588,8 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
             tmem_st_wait();
           }
           const float shift = kWeightLog2 - ref;
-          float sum[2] = {l * old, 0.f};
+          const float2 shift2 = make_float2(shift, shift);
+          float2 sum = make_float2(l * old, 0.f);
           tmem_ld_32x16(t_s, s[0]);
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
@@ -1568,20 +1602,19 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 const float4 inv = *reinterpret_cast<const float4*>(sc + 2 * kUnitKeys + c * 32 + h * 16 + 4 * j);
-                const uint32_t* u = s[h] + 4 * j;
-                const float2 x = make_float2(exp2f(__uint_as_float(u[0]) + shift), exp2f(__uint_as_float(u[1]) + shift));
-                const float2 y = make_float2(exp2f(__uint_as_float(u[2]) + shift), exp2f(__uint_as_float(u[3]) + shift));
-                sum[0] = fmaf(x.x, inv.x, sum[0]);
-                sum[1] = fmaf(x.y, inv.y, sum[1]);
-                sum[0] = fmaf(y.x, inv.z, sum[0]);
-                sum[1] = fmaf(y.y, inv.w, sum[1]);
+                const float* u = reinterpret_cast<const float*>(s[h]) + 4 * j;
+                float2 x = fadd2(get2(u), shift2), y = fadd2(get2(u + 2), shift2);
+                x = make_float2(exp2f(x.x), exp2f(x.y));
+                y = make_float2(exp2f(y.x), exp2f(y.y));
+                sum = ffma2(x, make_float2(inv.x, inv.y), sum);
+                sum = ffma2(y, make_float2(inv.z, inv.w), sum);
                 split_weights_e5m2(x, y, codes[h * 4 + j], codes[8 + h * 4 + j]);
               }
             }
             tmem_st_32x16(t_s + c * 32, codes);
           }
           tmem_st_wait();
-          l = sum[0] + sum[1];
+          l = sum.x + sum.y;
         }
         if (key0 + kUnitKeys > end) {
           // rows of V behind the last key may hold any byte, a NaN times a weight of zero among them
@@ -1670,13 +1703,13 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
 }
 
 // Tiles whose parts lie in several CTAs of the many-rows kernel: the parts, in their order, added up.  A block has the tile that
-// begins in CTA blockIdx.x (if one goes on from there) and 32 head dimensions, a thread a row and 8 of them.  (The CTA that
-// finishes last took 76 us to do this alone with 19 parts.)
-constexpr int kJoinThreads = 512;
-__global__ void __launch_bounds__(kJoinThreads) fp8_join_kernel(const FewParams p) {
+// begins in CTA blockIdx.x (if one goes on from there) and eight head dimensions, a thread a row.  (The CTA that finishes last
+// took 76 us to do this alone with 19 parts; blocks of 32 dimensions 15 us.)
+constexpr int kJoinDims = 8;
+__global__ void __launch_bounds__(kManyRows) fp8_join_kernel(const FewParams p) {
   pdl_wait();
   pdl_trigger();
-  const int owner = blockIdx.x, row = threadIdx.x & (kManyRows - 1), c0 = blockIdx.y * 32 + (threadIdx.x / kManyRows) * 8;
+  const int owner = blockIdx.x, row = threadIdx.x, c0 = blockIdx.y * kJoinDims;
   const int parts = __ldcg(p.joins + owner);
   if (parts == 0)
     return;
@@ -1687,7 +1720,7 @@ __global__ void __launch_bounds__(kJoinThreads) fp8_join_kernel(const FewParams 
   const int out = __float_as_int(__ldcg(one + kRef + 2 * kManyRows));
   if (out < 0)
     return;
-  float top = kNothing, l = 0.f, o[8] = {};
+  float top = kNothing, l = 0.f, o[kJoinDims] = {};
 #pragma unroll 4
   for (int i = 0; i < parts; ++i)
     top = fmaxf(top, __ldcg(part(i) + kRef));
@@ -1786,7 +1819,7 @@ int launch_many(const CUtensorMap& tk, const CUtensorMap& tv, const FewParams& p
   const int rc = launch_rows(fp8_many_rows_kernel<CAP, BIAS>, set, kManyThreads, kManySmem, tk, tv, p, kManyCtas * ctas, s);
   if (rc != DYLLM_OK)
     return rc;
-  DYLLM_LAUNCH(fp8_join_kernel, dim3(kManyCtas * ctas, kD / 32), kJoinThreads, 0, s, p);
+  DYLLM_LAUNCH(fp8_join_kernel, dim3(kManyCtas * ctas, kD / kJoinDims), kManyRows, 0, s, p);
   return check_launch("attention_salient_rows_fp8");
 }
 
