@@ -121,6 +121,25 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+_bound = None
+
+
+def native():
+    """The binding of the entry points on 8-bit caches (``csrc/bind.cpp``): it checks tensors, allocates and calls in one step."""
+    global _bound
+    if _bound is None:
+        lib = load()
+        try:
+            from . import _native
+        except ImportError as e:
+            raise RuntimeError(f"_native.so is missing or does not fit this torch ({e}): build it with `python -m dyllm_b200.build`") from e
+        _native.init(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            "dyllm_fp8_cache_write", "dyllm_fp8_cache_read", "dyllm_fp8_kv_cache_update", "dyllm_attention_salient_rows_fp8",
+            "dyllm_attention_salient_rows_fp8_workspace_bytes", "dyllm_last_error")))
+        _bound = _native
+    return _bound
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     """Device address of a tensor (None -> NULL)."""
     if t is None:
@@ -154,23 +173,3 @@ def require_cuda(t: torch.Tensor, name: str, dtype: torch.dtype | None = None, d
         raise RuntimeError(f"{name} must be {dim}-D, got {t.dim()}-D")
     if not t.is_contiguous():
         raise RuntimeError(f"{name} must be contiguous")
-
-
-def require_on(index: int, t: torch.Tensor, name: str, dtype: torch.dtype, dim: int) -> None:
-    """:func:`require_cuda` for the device with this index (one look at each property: calls of a few microseconds)."""
-    try:
-        if t.dtype is dtype and t.dim() == dim and t.get_device() == index and t.is_contiguous():
-            return
-    except AttributeError:
-        pass
-    require_cuda(t, name, dtype, dim)
-    raise RuntimeError(f"{name} must be on cuda:{index}, got {t.device}")
-
-
-def call_on(index: int, name: str, *args) -> None:
-    """:func:`call` with the current stream of device ``index`` as the last argument, and that device current."""
-    if torch._C._cuda_getDevice() == index:
-        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            call(name, *args, torch._C._cuda_getCurrentRawStream(index))

@@ -6,8 +6,8 @@ from __future__ import annotations
 
 import torch
 
-from . import ops
-from ._lib import call, call_on, load, ptr, require_on, stream_ptr
+from . import _lib as _lib_mod
+from ._lib import call, load, native, ptr, stream_ptr
 
 _EMPTY = None
 _workspaces: dict = {}
@@ -203,48 +203,9 @@ def attention_salient_rows_fp8(q, k_cache, v_cache, k_seq_starts, v_seq_starts, 
     (documents, block-causal prefixes, windows).  A row that sees no key gives zeros.  ``q`` may be a column slice of a wider
     product.  Returns ``[num_salient, heads, 128]`` in list order; rows past ``cu_salientlens[-1]`` are left untouched.
     """
-    index = ops._cuda_index(q, "q")
-    pitch = ops.require_rows(index, q, "q")
-    total_q, heads, head_dim = q.shape
-    kv_heads = k_cache[1].size(1)
-    if head_dim != 128:
-        raise RuntimeError(f"supported head dimension is 128; got {head_dim}")
-    if not (kv_heads > 0 and heads > 0 and heads % kv_heads == 0):
-        raise RuntimeError(f"query heads must be a positive multiple of KV heads; got {heads} and {kv_heads}")
-    k_codes, k_scales = ops.require_fp8_cache(index, k_cache, "k_cache", kv_heads, head_dim)
-    v_codes, v_scales = ops.require_fp8_cache(index, v_cache, "v_cache", kv_heads, head_dim)
-    batch = ops._require_sequences(index, k_seq_starts, cu_seqlens_q, seq_ids, cu_seqlens_k)
-    require_on(index, v_seq_starts, "v_seq_starts", torch.int64, 1)
-    require_on(index, cu_salientlens, "cu_salientlens", torch.int32, 1)
-    require_on(index, idx_salient_row, "idx_salient_row", torch.int32, 1)
-    if cu_salientlens.size(0) != batch + 1:
-        raise RuntimeError("cu_salientlens must have one entry more than seq_ids")
-    n = idx_salient_row.size(0) if num_salient is None else int(num_salient)
-    if not 0 <= n <= idx_salient_row.size(0):
-        raise RuntimeError("num_salient must fit idx_salient_row")
-    if slopes is not None:
-        require_on(index, slopes, "slopes", torch.float32, 1)
-        if slopes.size(0) != heads:
-            raise RuntimeError("slopes must have one value per query head")
-    if key_ranges is not None:
-        require_on(index, key_ranges, "key_ranges", torch.int32, 2)
-        if key_ranges.size(0) != total_q or key_ranges.size(1) != 2:
-            raise RuntimeError("key_ranges must be [q.size(0), 2]")
-    if out is None:
-        out = torch.empty((n, heads, head_dim), dtype=torch.bfloat16, device=q.device)
-    else:
-        require_on(index, out, "out", torch.bfloat16, 3)
-        if out.size(0) < n or out.size(1) != heads or out.size(2) != head_dim:
-            raise RuntimeError("out must be [num_salient, heads, 128]")
-    if n == 0 or max_rows_per_seq == 0 or batch == 0:
-        return out
-    ws = ops._scratch(load().dyllm_attention_salient_rows_fp8_workspace_bytes(n, batch, heads, kv_heads), q.device)
-    call_on(index, "dyllm_attention_salient_rows_fp8", q.data_ptr(), pitch, total_q, k_codes.data_ptr(), k_scales.data_ptr(),
-            k_codes.size(0), v_codes.data_ptr(), v_scales.data_ptr(), v_codes.size(0), k_seq_starts.data_ptr(),
-            v_seq_starts.data_ptr(), seq_ids.data_ptr(), out.data_ptr(), cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), batch,
-            int(max_rows_per_seq), heads, kv_heads, head_dim, cu_salientlens.data_ptr(), idx_salient_row.data_ptr(), n,
-            head_dim ** -0.5 if scale is None else float(scale), float(softcap), ptr(slopes), ptr(key_ranges), ws.data_ptr(),
-            ws.numel())
+    out = native().attention(q, k_cache, v_cache, k_seq_starts, v_seq_starts, seq_ids, cu_seqlens_q, cu_seqlens_k, cu_salientlens,
+                             idx_salient_row, max_rows_per_seq, scale, softcap, slopes, key_ranges, num_salient, out)
+    _lib_mod.launch_count += _lib_mod.KERNELS_PER_CALL["dyllm_attention_salient_rows_fp8"]
     return out
 
 

@@ -8,7 +8,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib as _lib_mod
-from ._lib import call, call_on, load, ptr, require_cuda, require_on, stream_ptr
+from ._lib import call, load, native, ptr, require_cuda, stream_ptr
 
 
 def _scratch(nbytes: int, device) -> torch.Tensor:
@@ -220,67 +220,18 @@ def kv_cache_update(k_new: torch.Tensor, v_new: torch.Tensor, rows_k: torch.Tens
     return dv
 
 
-_FP8 = torch.float8_e4m3fn
-
-
-def _cuda_index(t: torch.Tensor, name: str) -> int:
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise RuntimeError(f"{name} must be a CUDA tensor")
-    return t.get_device()
-
-
-def require_rows(index: int, x: torch.Tensor, name: str) -> int:
-    """Row pitch of ``x [rows, heads, 128]``: bf16, every row contiguous and 16-byte aligned (a slice of the columns of a wider
-    product is such a tensor)."""
-    if not isinstance(x, torch.Tensor) or x.get_device() != index or x.dtype is not torch.bfloat16 or x.dim() != 3:
-        raise RuntimeError(f"{name} must be a 3-D bfloat16 tensor on cuda:{index}")
-    heads, width = x.size(1), x.size(2)
-    rows, pitch = x.size(0), x.stride(0)
-    if (rows and heads and width) and (x.stride(2) != 1 or (heads > 1 and x.stride(1) != width)
-                                       or (rows > 1 and (pitch % 8 or pitch < heads * width)) or x.data_ptr() & 15):
-        raise RuntimeError(f"{name} must have contiguous, 16-byte aligned rows [heads, head_dim]")
-    return pitch if rows > 1 else heads * width
-
-
-def require_fp8_cache(index: int, cache, name: str, heads: int, head_dim: int) -> tuple:
-    """``(codes e4m3 [cache_rows, heads * head_dim], scales fp32 [cache_rows, heads])``."""
-    codes, scales = cache
-    require_on(index, codes, name + " codes", _FP8, 2)
-    require_on(index, scales, name + " scales", torch.float32, 2)
-    if codes.size(1) != heads * head_dim or scales.size(1) != heads or scales.size(0) != codes.size(0):
-        raise RuntimeError(f"{name} must be codes [cache_rows, {heads * head_dim}] with scales [cache_rows, {heads}]")
-    return codes, scales
-
-
-def _require_sequences(index, seq_starts, cu_seqlens, seq_ids, cu_seqlens_k=None):
-    require_on(index, seq_starts, "seq_starts", torch.int64, 1)
-    require_on(index, cu_seqlens, "cu_seqlens", torch.int32, 1)
-    require_on(index, seq_ids, "seq_ids", torch.int64, 1)
-    batch = seq_ids.size(0)
-    if cu_seqlens.size(0) != batch + 1:
-        raise RuntimeError("cu_seqlens must have one entry more than seq_ids")
-    if cu_seqlens_k is not None:
-        require_on(index, cu_seqlens_k, "cu_seqlens_k", torch.int32, 1)
-        if cu_seqlens_k.size(0) != batch + 1:
-            raise RuntimeError("cu_seqlens_k must have one entry more than seq_ids")
-    return batch
-
-
 def fp8_cache_write(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, seq_starts: torch.Tensor,
                     cu_seqlens: torch.Tensor, seq_ids: torch.Tensor, cu_seqlens_k: torch.Tensor | None = None) -> None:
-    """Quantises the packed rows ``x [rows, heads, 128]`` (bf16; the rows may lie in a wider product) into the 8-bit cache rows of
+    """Quantises the packed rows ``x [rows, heads, 128]`` (bf16; the rows may lie in a wider product: each contiguous and 16-byte
+    aligned) into the 8-bit cache rows of
     their sequences: from each sequence's first row on, or, with ``cu_seqlens_k``, its last rows.
 
     Per row and head 128 e4m3 ``codes`` ([cache_rows, heads * 128]) and a power of two in ``scales`` ([cache_rows, heads],
     fp32): the least with ``amax <= 448 * scale``, at least 2^-60; the value is their product, exact in bf16.  A head with a
     NaN or an infinity reads as NaN throughout.  8-bit counterpart of ``cache.reset_full_cuda`` / ``reset_block_cuda``.
     """
-    index = _cuda_index(x, "x")
-    pitch = require_rows(index, x, "x")
-    require_fp8_cache(index, (codes, scales), "cache", x.size(1), x.size(2))
-    batch = _require_sequences(index, seq_starts, cu_seqlens, seq_ids, cu_seqlens_k)
-    call_on(index, "dyllm_fp8_cache_write", x.data_ptr(), pitch, x.size(1), x.size(2), codes.data_ptr(), scales.data_ptr(),
-            codes.size(0), seq_starts.data_ptr(), cu_seqlens.data_ptr(), ptr(cu_seqlens_k), seq_ids.data_ptr(), batch, x.size(0))
+    native().cache_write(x, codes, scales, seq_starts, cu_seqlens, seq_ids, cu_seqlens_k)
+    _lib_mod.launch_count += _lib_mod.KERNELS_PER_CALL["dyllm_fp8_cache_write"]
 
 
 def fp8_cache_read(codes: torch.Tensor, scales: torch.Tensor, seq_starts: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -288,18 +239,8 @@ def fp8_cache_read(codes: torch.Tensor, scales: torch.Tensor, seq_starts: torch.
                    out: torch.Tensor | None = None) -> torch.Tensor:
     """Rows of an 8-bit cache (:func:`fp8_cache_write`) back as packed bf16 ``[total_rows, heads, 128]``; rows of ``out`` past
     ``cu_seqlens[-1]`` stay as they are.  8-bit counterpart of ``cache.get_seqs_cuda`` / ``get_block_cuda``."""
-    index = _cuda_index(codes, "codes")
-    heads = scales.size(1)
-    require_fp8_cache(index, (codes, scales), "cache", heads, 128)
-    batch = _require_sequences(index, seq_starts, cu_seqlens, seq_ids, cu_seqlens_k)
-    if out is None:
-        out = torch.empty((total_rows, heads, 128), dtype=torch.bfloat16, device=codes.device)
-    else:
-        require_on(index, out, "out", torch.bfloat16, 3)
-        if out.shape != (total_rows, heads, 128):
-            raise RuntimeError("out must be [total_rows, heads, 128]")
-    call_on(index, "dyllm_fp8_cache_read", codes.data_ptr(), scales.data_ptr(), codes.size(0), heads, 128, out.data_ptr(),
-            seq_starts.data_ptr(), cu_seqlens.data_ptr(), ptr(cu_seqlens_k), seq_ids.data_ptr(), batch, int(total_rows))
+    out = native().cache_read(codes, scales, seq_starts, cu_seqlens, seq_ids, total_rows, cu_seqlens_k, out)
+    _lib_mod.launch_count += _lib_mod.KERNELS_PER_CALL["dyllm_fp8_cache_read"]
     return out
 
 
@@ -311,37 +252,9 @@ def fp8_kv_cache_update(k_new: torch.Tensor, v_new: torch.Tensor, rows_k: torch.
     quantised into their caches, delta-V; returns dV ``[rows, kv_heads, 128]``, the difference between the values that the cache
     holds after and before (zero where the codes stay, so their rounding does not pile up in a context over the steps).
     ``k_new`` and ``v_new`` may be column slices of one product; ``rows_k`` lists no row twice."""
-    index = _cuda_index(k_new, "k_new")
-    ldk, ldv = require_rows(index, k_new, "k_new"), require_rows(index, v_new, "v_new")
-    n, heads, width = k_new.shape
-    if v_new.shape != k_new.shape:
-        raise RuntimeError("k_new and v_new must have the same shape")
-    require_on(index, rows_k, "rows_k", torch.int64, 1)
-    require_on(index, positions, "positions", torch.int64, 1)
-    require_on(index, cos_sin, "cos_sin", torch.float32, 2)
-    if pos_idx is not None:
-        require_on(index, pos_idx, "pos_idx", torch.int64, 1)
-    if rows_k.size(0) < n or (pos_idx if pos_idx is not None else positions).size(0) < n:
-        raise RuntimeError("rows_k and the positions must have an entry per new row")
-    if cos_sin.size(1) != 128:
-        raise RuntimeError("cos_sin must be [positions, 128]")
-    k_codes, k_scales = require_fp8_cache(index, k_cache, "k_cache", heads, width)
-    v_codes, v_scales = require_fp8_cache(index, v_cache, "v_cache", heads, width)
-    batch = _require_sequences(index, k_seq_starts, cu_seqlens_k, seq_ids)
-    require_on(index, v_seq_starts, "v_seq_starts", torch.int64, 1)
-    if num_rows_dev is not None:
-        require_on(index, num_rows_dev, "num_rows_dev", torch.int32, 1)
-    if dv is None:
-        dv = torch.empty((n, heads, width), dtype=torch.bfloat16, device=k_new.device)
-    else:
-        require_on(index, dv, "dv", torch.bfloat16, 3)
-        if dv.shape != k_new.shape:
-            raise RuntimeError("dv must have the shape of v_new")
-    call_on(index, "dyllm_fp8_kv_cache_update", k_new.data_ptr(), ldk, v_new.data_ptr(), ldv, rows_k.data_ptr(),
-            positions.data_ptr(), ptr(pos_idx), cos_sin.data_ptr(), cos_sin.size(0), cu_seqlens_k.data_ptr(),
-            k_seq_starts.data_ptr(), v_seq_starts.data_ptr(), seq_ids.data_ptr(), batch, n, ptr(num_rows_dev), heads, width,
-            k_codes.data_ptr(), k_scales.data_ptr(), k_codes.size(0), v_codes.data_ptr(), v_scales.data_ptr(), v_codes.size(0),
-            dv.data_ptr())
+    dv = native().kv_cache_update(k_new, v_new, rows_k, positions, pos_idx, cos_sin, cu_seqlens_k, k_seq_starts, v_seq_starts,
+                                  seq_ids, k_cache, v_cache, num_rows_dev, dv)
+    _lib_mod.launch_count += _lib_mod.KERNELS_PER_CALL["dyllm_fp8_kv_cache_update"]
     return dv
 
 
