@@ -534,12 +534,11 @@ struct QueryLoad {
     t = w.t0 + (tid >> 3);
     const int i = t / group;
     head = w.hk * group + t - i * group;
-    if (t < w.rows) {
-      row = __ldg(a.idx + w.row0 + i);
-      row = row >= a.total_q ? -1 : row;
-    }
+    if (t < w.rows)
+      row = __ldg(a.idx + w.row0 + i);      // looked at in data(), not while it is on its way
   }
   __device__ __forceinline__ void data(const Fp8AttnParams& a, int tid) {
+    row = row >= a.total_q ? -1 : row;
     x0 = x1 = make_uint4(0u, 0u, 0u, 0u);
     if (row >= 0) {
       const uint4* src = reinterpret_cast<const uint4*>(a.q + row * a.ldq + head * kD) + (tid & 7) * 2;
@@ -1784,13 +1783,18 @@ __global__ void __launch_bounds__(128) fp8_spans_kernel(const Fp8AttnParams p, i
     spans[before] = lo < hi ? make_int2(lo, hi) : make_int2(0, 0);
 }
 
+// Up to this many (listed row, query head) pairs a sequence and key head the few-rows kernel is the faster one, with a pass over
+// the keys for each 32 of them: 26 rows (16 x 512 keys, 32 heads) 43 us against 63; 64 rows (8 x 4096 keys, 16 heads, capped) 125
+// against 139; 128 rows (2 x 32011 keys, 8 key heads) 161 against 105.
+constexpr int kFewMost = 64;
+
 // Workspace: tickets, keys per tile (only with ranges), parts of tiles; for the kernel that needs most.
 int64_t most_tiles(int num_salient, int batch, int group) { return static_cast<int64_t>(num_salient) * group / kRows + batch; }
 size_t parts_offset(int64_t tiles, int ctas) { return (ctas * sizeof(unsigned long long) + tiles * sizeof(int2) + 255) / 256 * 256; }
 size_t workspace_of(int num_salient, int batch, int group, int ctas) {
   const size_t few = 2ull * ctas * kRows * (kD + 2), many = 2ull * kManyCtas * ctas * kManyPart;
   return parts_offset(most_tiles(num_salient, batch, group), kManyCtas * ctas) +
-         (static_cast<int64_t>(num_salient) * group > kRows ? max(few, many) : few) * sizeof(float);
+         (static_cast<int64_t>(num_salient) * group > kFewMost ? max(few, many) : few) * sizeof(float);
 }
 
 template <typename Kernel>
@@ -1915,7 +1919,7 @@ int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, co
   f.launch_id = next_launch_id() & ~0xffffull;
   f.status_word = device_status_word();
   // a sequence with more rows than the bound says is served by either kernel; so is one with few beside others with many
-  const bool many = static_cast<int64_t>(max_rows_per_seq) * group > kRows && static_cast<int64_t>(num_salient) * group > kRows;
+  const bool many = static_cast<int64_t>(max_rows_per_seq) * group > kFewMost && static_cast<int64_t>(num_salient) * group > kFewMost;
   if (p.ranges) {
     f.spans = spans;
     const unsigned blocks = static_cast<unsigned>((tiles + 3) / 4);

@@ -150,10 +150,10 @@ fp8_kv_cache_update_kernel(const uint4* __restrict__ k_new, int64_t ldk, const u
   for (int g = 0; g < G; ++g) {
     ka[g] = kb[g] = va[g] = vb[g] = make_uint4(0u, 0u, 0u, 0u);
     if (h0 + 4 * g < heads) {
-      ka[g] = __ldg(ksrc + g * 64);
-      kb[g] = __ldg(ksrc + g * 64 + 8);
-      va[g] = __ldg(vsrc + g * 64);
-      vb[g] = __ldg(vsrc + g * 64 + 8);
+      ka[g] = __ldcs(ksrc + g * 64);
+      kb[g] = __ldcs(ksrc + g * 64 + 8);
+      va[g] = __ldcs(vsrc + g * 64);
+      vb[g] = __ldcs(vsrc + g * 64 + 8);
     }
   }
   int64_t pos = __ldg(positions + (pos_idx ? __ldg(pos_idx + i) : i));
@@ -223,8 +223,8 @@ fp8_kv_cache_update_kernel(const uint4* __restrict__ k_new, int64_t ldk, const u
     }
     if (head) {
       uint4* dst = dv + (static_cast<int64_t>(i) * heads + h0 + 4 * g) * 16 + part;
-      dst[0] = float_to_bf16x8(x);
-      dst[8] = float_to_bf16x8(x + 8);
+      __stcs(dst, float_to_bf16x8(x));
+      __stcs(dst + 8, float_to_bf16x8(x + 8));
     }
   }
 }
