@@ -173,10 +173,13 @@ __device__ __forceinline__ int units_of(int2 span) { return max(1, (span.y - spa
 // Uniform over a warp.
 //
 // Shares are cut at total * i / ctas, but no part of a tile is shorter than kMinPart units: a cut nearer to an end of its
-// tile moves there.  (Joining the parts of a tile costs a CTA about 7 us, a unit 1 to 2.)
-constexpr int kMinPart = 4;
+// tile moves there.  Joining the parts of a tile costs a CTA of the few-rows kernel about 7 us, a unit 1 to 2.  With many rows a
+// unit takes 5 us and the join is a launch of its own: parts of at least 2 units against 4 take 34.6 us against 43.1 (32 x 601
+// keys, 28 heads on 4) and 163 against 166 (4 x 2048 rows of packed documents).
+constexpr int kMinPartFew = 4, kMinPartMany = 2;
 template <int MROWS>
 struct Walk {
+  static constexpr int kMinPart = MROWS == kRows ? kMinPartFew : kMinPartMany;
   SeqWork w;
   int64_t total, end;                   // units: of the launch, end of the share before its cut is moved
   int64_t tile_first;                   // first unit of the tile in the launch
