@@ -67,35 +67,12 @@ __device__ __forceinline__ float value_exponent(float scale) {
   return static_cast<float>(max(static_cast<int>(bits >> 23) - 127, kFp8MinExp));
 }
 
-// ----------------------------------------------------------------------------------------------
-// Few rows per sequence: bound by the bytes of the cache, which go from the TMA ring to the tensor cores as they are.
-//
-// The rows of a tile are the (listed row, query head) pairs of one sequence and key head, RN = 16 or 32 of them, so that
-// grouped query heads share one pass over their keys.  A unit of work is 128 keys of a tile; all units of the launch, in the
-// order (sequence, key head, tile, keys), are dealt out to the CTAs in equal contiguous shares that every CTA works out for
-// itself from the device-side counts.  A tile whose units lie in several CTAs is joined by the CTA that finishes last, in the
-// order of its parts.
-//
-// The products are transposed, keys (then head dimensions) in the M = 128 of tcgen05.mma.kind::f8f6f4:
-//   S^T = K Q^T         A: K tile as loaded (K-major), B: the queries as e4m3 + e5m2, two products into one accumulator
-//   O^T = V^T P^T       A: V tile as loaded (MN-major), B: the weights, 32 columns of e4m3 and 32 of their remainders
-// A query in bf16 (8 significant bits) is e4m3 (4 bits) plus a remainder of at most 3 bits, which e5m2 holds exactly down to
-// 2^-25 of the row's largest element.  A weight in [0, 1] is taken as e4m3(256 w) + e4m3(16 * remainder) / 16: off by at most
-// 2^-8 of itself, or 2^-22.  The codes of the cache are never widened.
-//
-// Softmax per chunk of up to kChunk tiles: thread = key, first the scores of all tiles of the chunk (kept in tensor memory in
-// place of the products) and their maxima, then weights tile by tile; the sums are rescaled between chunks.  Eight softmax
-// warps, two per quarter of the keys, each with half of the rows; a TMA warp and an MMA warp.  Two CTAs per SM.
-// ----------------------------------------------------------------------------------------------
-constexpr int kUnitKeys = 128;
-constexpr int kRows = 32, kGroup = 8;                        // rows of a tile, of a softmax warp
-constexpr int kChunk = 4;                                    // tiles whose scores are in registers at a time
-constexpr int kRing = 8;                                     // slots of one K or V tile
+constexpr int kUnitKeys = 128;                               // keys of a unit of work
+constexpr int kRows = 32;                                    // rows of a tile of the few-rows kernel
 constexpr int kParts = 4;                                    // slots of part descriptions
-constexpr uint32_t kTileBytes = kUnitKeys * kD, kQBytes = kRows * kD;
-constexpr int kSoftmaxWarps = 16, kFewThreads = 32 * (kSoftmaxWarps + 3);
-constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kFewSmem = (kRing + kChunk / 2) * kTileBytes + 4 * kQBytes + 2 * kChunk * 2 * kUnitKeys * sizeof(float) + 1024;
+constexpr uint32_t kTileBytes = kUnitKeys * kD;
+constexpr float kWeightLog2 = 6.f;                           // the reference's weight: 2^6
+constexpr float kHeadroom = 2.8f;                            // 2^(6 + 2.8) < 448
 
 struct FewParams {
   Fp8AttnParams a;
@@ -344,58 +321,11 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
   if ((threadIdx.x & 31) == 0)
     mbar_arrive(bar);
 }
-__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
-
-__device__ __forceinline__ void group_sync(int group) { asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory"); }
 __device__ __forceinline__ float warp_max(float x) {
   float r;
   asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
   return r;
 }
-__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-
-// Sum of each of N = 8 or 16 values over the lanes of a warp: lane l gets that of value l / (32 / N).
-template <int N>
-__device__ __forceinline__ float reduce_lanes(const float (&v)[N]) {
-  const int lane = threadIdx.x & 31;
-  float x[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    x[i] = v[i];
-  int bit = 16;
-#pragma unroll
-  for (int n = N / 2; n >= 1; n >>= 1, bit >>= 1) {
-    const bool up = lane & bit;
-#pragma unroll
-    for (int i = 0; i < N / 2; ++i)
-      if (i < n) {
-        const float keep = up ? x[i + n] : x[i], give = up ? x[i] : x[i + n];
-        x[i] = keep + __shfl_xor_sync(0xffffffffu, give, bit);
-      }
-  }
-#pragma unroll
-  for (int b = 16 / N; b >= 1; b >>= 1)
-    x[0] += __shfl_xor_sync(0xffffffffu, x[0], b);
-  return x[0];
-}
-
-// N consecutive floats of shared memory, 16-byte aligned, the same for all lanes
-template <int N>
-__device__ __forceinline__ void lds_row(float (&x)[N], const float* src) {
-#pragma unroll
-  for (int i = 0; i < N / 4; ++i) {
-    const float4 v = *reinterpret_cast<const float4*>(src + 4 * i);
-    x[4 * i] = v.x;
-    x[4 * i + 1] = v.y;
-    x[4 * i + 2] = v.z;
-    x[4 * i + 3] = v.w;
-  }
-}
-
 // One step of a product of 8-bit tiles with rows of 128 bytes (128-byte swizzle, groups of 8 rows 1024 bytes apart) at these
 // shared-memory addresses.  Only the low words of the descriptors vary: an issue costs few instructions.
 __device__ __forceinline__ void umma_tile(uint32_t d_tmem, uint32_t a_addr, uint32_t b_addr, uint32_t idesc, uint32_t accumulate) {
@@ -413,20 +343,42 @@ __device__ __forceinline__ void umma_tile(uint32_t d_tmem, uint32_t a_addr, uint
       : "memory");
 }
 
+// The same with B rows of 64 bytes (64-byte swizzle, groups of 8 rows 512 bytes apart).
+__device__ __forceinline__ void umma_tile_b64(uint32_t d_tmem, uint32_t a_addr, uint32_t b_addr, uint32_t idesc, uint32_t accumulate) {
+  constexpr uint32_t high = (1024u >> 4) | (1u << 14) | (2u << 29), high_b = (512u >> 4) | (1u << 14) | (4u << 29);
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      ".reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %5};\n\t"
+      "mov.b64 b, {%2, %6};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, p;\n\t"
+      "}\n" ::"r"(d_tmem),
+      "r"((a_addr >> 4) | (1u << 16)), "r"((b_addr >> 4) | (1u << 16)), "r"(idesc), "r"(accumulate), "n"(high), "n"(high_b)
+      : "memory");
+}
+
 // A value that all lanes share, in a register of the uniform datapath: what depends on it alone (loop counters, descriptors)
 // stays there, and an MMA issues every 33 cycles (its A operand's shared-memory read) instead of every 90.
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __reduce_max_sync(0xffffffffu, x); }
 
-__device__ __forceinline__ void loaders_sync() { asm volatile("bar.sync 7, 128;" ::: "memory"); }
-
-// Zeros for the rows t0 .. t0 + count - 1 of a sequence's (listed row, head) pairs; one warp.
-__device__ __forceinline__ void zero_rows(const Fp8AttnParams& a, const SeqWork& w, int hk, int t0, int count) {
-  const int group = a.H / a.Hkv;
-  for (int t = t0; t < min(t0 + count, w.rows); ++t) {
-    const int i = t / group;
-    __nv_bfloat16* dst = a.out + ((static_cast<int64_t>(w.row0) + i) * a.H + hk * group + t - i * group) * kD;
-    *reinterpret_cast<uint2*>(dst + (threadIdx.x & 31) * 4) = make_uint2(0u, 0u);
-  }
+// The 128 softmax threads of the few-rows kernel, or loader threads of the many-rows kernel, meet; any: whether the condition holds
+// for one of them (after a wait that has given up they all leave together: a barrier would wait for those that are gone).
+__device__ __forceinline__ void rows_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool rows_any(bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.or.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t"
+      "}\n"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(x))
+      : "memory");
+  return r != 0;
 }
 
 // Sixteen elements of a query times `inv` as codes: e4m3, and the rest in e5m2.
@@ -451,21 +403,6 @@ __device__ __forceinline__ void split_query(const uint4& x0, const uint4& x1, fl
 
 constexpr float kNothing = -1.0e30f;      // maximum of no scores (finite: it takes part in differences)
 
-// Four weights (times 256) as codes and the codes of 16 times what they leave.  By way of half precision (2^-11).
-__device__ __forceinline__ void split_weights(const float (&w)[4], uint32_t& hi, uint32_t& lo) {
-  uint32_t h[2], l[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const __half2 x = __floats2half2_rn(w[2 * i], w[2 * i + 1]);
-    h[i] = fp8_pack_half2(*reinterpret_cast<const uint32_t*>(&x));
-    const uint32_t back = fp8_to_half2(h[i]);
-    const __half2 rest = __hmul2(__hsub2(x, *reinterpret_cast<const __half2*>(&back)), __float2half2_rn(16.f));
-    l[i] = fp8_pack_half2(*reinterpret_cast<const uint32_t*>(&rest));
-  }
-  hi = h[0] | h[1] << 16;
-  lo = l[0] | l[1] << 16;
-}
-
 // What a tile's rows are to the softmax warps.
 struct RowInfo {
   int out;                     // output row, -1: none
@@ -474,134 +411,10 @@ struct RowInfo {
   int pos, lo, hi;             // the row's place in its sequence, the keys that it sees
 };
 
-// Joins the parts of a tile that several CTAs hold: every CTA leaves its part in the workspace, the last one to do so adds them
-// up in their order (true: for the caller to store).  Rows r0 .. r0 + 7, head dimension kl of a thread.
-__device__ __forceinline__ bool join_parts(const FewParams& p, const PartInfo& part, float (&top)[kGroup], float (&l)[kGroup],
-                                           float (&o)[kGroup], int r0, int kl, int tid, int* joins) {
-  constexpr int kPart = kRows * kD + 2 * kRows;
-  float* mine = p.parts + static_cast<int64_t>(part.slot) * kPart;
-#pragma unroll
-  for (int r = 0; r < kGroup; ++r)
-    mine[(r0 + r) * kD + kl] = o[r];
-  if (kl == 0) {
-#pragma unroll
-    for (int r = 0; r < kGroup; ++r) {
-      mine[kRows * kD + r0 + r] = top[r];
-      mine[kRows * kD + kRows + r0 + r] = l[r];
-    }
-  }
-  const int owner = part.owner, parts = part.parts;
-  __threadfence();
-  softmax_sync();
-  if (tid == 0) {
-    open_join(p.tickets + owner, p.launch_id);
-    *joins = last_to_join(p.tickets + owner, parts) ? 1 : 0;
-  }
-  softmax_sync();
-  if (!*joins)
-    return false;
-  __threadfence();
-  const float* first = p.parts + (2 * static_cast<int64_t>(owner) + 1) * kPart;
-  const float* rest = p.parts + 2 * static_cast<int64_t>(owner) * kPart;
-#pragma unroll
-  for (int r = 0; r < kGroup; ++r) {
-    top[r] = kNothing;
-    o[r] = l[r] = 0.f;
-  }
-  for (int i = 0; i < parts; ++i) {
-    const float* src = i == 0 ? first : rest + 2 * static_cast<int64_t>(i) * kPart;
-#pragma unroll
-    for (int r = 0; r < kGroup; ++r)
-      top[r] = fmaxf(top[r], __ldcg(src + kRows * kD + r0 + r));
-  }
-#pragma unroll 2
-  for (int i = 0; i < parts; ++i) {
-    const float* src = i == 0 ? first : rest + 2 * static_cast<int64_t>(i) * kPart;
-#pragma unroll
-    for (int r = 0; r < kGroup; ++r) {
-      const float mul = exp2f(__ldcg(src + kRows * kD + r0 + r) - top[r]);
-      l[r] += __ldcg(src + kRows * kD + kRows + r0 + r) * mul;
-      o[r] += __ldcg(src + (r0 + r) * kD + kl) * mul;
-    }
-  }
-  return true;
-}
-
-// The query rows of a tile on their way to shared memory: eight threads a row (the first 256 softmax threads), 16 elements each.
-struct QueryLoad {
-  uint4 x0, x1;
-  int row, head, t;
-  __device__ __forceinline__ void index(const Fp8AttnParams& a, const PartInfo& w, int tid) {
-    const int group = a.H / a.Hkv;
-    row = -1;
-    t = w.t0 + (tid >> 3);
-    const int i = t / group;
-    head = w.hk * group + t - i * group;
-    if (t < w.rows)
-      row = __ldg(a.idx + w.row0 + i);      // looked at in data(), not while it is on its way
-  }
-  __device__ __forceinline__ void data(const Fp8AttnParams& a, int tid) {
-    row = row >= a.total_q ? -1 : row;
-    x0 = x1 = make_uint4(0u, 0u, 0u, 0u);
-    if (row >= 0) {
-      const uint4* src = reinterpret_cast<const uint4*>(a.q + row * a.ldq + head * kD) + (tid & 7) * 2;
-      x0 = __ldg(src);
-      x1 = __ldg(src + 1);
-    }
-  }
-  // Codes next to the tile's largest element (an error of 2^-26 of it moves every score of the tile by as little), e4m3 and
-  // the e5m2 rest.
-  template <bool PLAIN>
-  __device__ __forceinline__ void store(const Fp8AttnParams& a, const PartInfo& w, int tid, uint8_t* q_smem, uint32_t* amax, RowInfo* info) {
-    float y[16];
-    bf16x8_to_float(x0, y);
-    bf16x8_to_float(x1, y + 8);
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      m = max(m, __float_as_uint(y[j]) & 0x7fffffffu);
-    m = fp8_amax8(m);
-    const bool finite = m < 0x7f800000u;
-    {
-      const uint32_t top = __reduce_max_sync(0xffffffffu, finite ? m : 0u);
-      if ((tid & 31) == 0)
-        atomicMax(amax, top);
-    }
-    asm volatile("bar.sync 6, 256;" ::: "memory");
-    const int r = tid >> 3, part = tid & 7;
-    const float inv = fp8_inverse(fp8_scale_bits(*amax));
-    uint4 hi, lo;
-    if (!finite)
-      x0 = x1 = make_uint4(0u, 0u, 0u, 0u);
-    split_query(x0, x1, inv, hi, lo);
-    uint8_t* dst = q_smem + r * kD + ((part ^ (r & 7)) << 4);
-    *reinterpret_cast<uint4*>(dst) = hi;
-    *reinterpret_cast<uint4*>(dst + kRows * kD) = lo;
-    if (part == 0) {
-      RowInfo v = {};
-      v.out = t < w.rows ? (w.row0 + t / (a.H / a.Hkv)) * a.H + head : -1;
-      v.fix = row < 0 ? 0.f : finite ? 1.f : __uint_as_float(0x7fc00000u);
-      if (!PLAIN && row >= 0) {
-        v.pos = __ldg(a.cu_k + w.b + 1) - __ldg(a.cu_k + w.b) - (__ldg(a.cu_q + w.b + 1) - row);
-        v.slope = a.slopes ? __ldg(a.slopes + head) * kLog2e : 0.f;
-        v.hi = w.len;
-        if (a.ranges) {
-          const int2 range = __ldg(a.ranges + row);
-          v.lo = range.x;
-          v.hi = min(range.y, w.len);
-        }
-      }
-      info[r] = v;
-    }
-    fence_proxy_async_smem();
-  }
-};
-
-// The chunks of a CTA's share one after the other, as the producer and the MMA warp walk over them.  Uniform over a warp.
-struct Chunks {
-  int n, c0, tiles;            // part, first tile of the chunk, tiles of the part
+// The parts of a CTA's share one after the other, as the producer and the MMA warp walk over them.  Uniform over a warp.
+struct PartWalk {
+  int n, tiles;                // part, its units
   int begin, end, hk, k0, v0;
-  __device__ __forceinline__ int count() const { return min(kChunk, tiles - c0); }
   __device__ __forceinline__ bool open(uint64_t* full, uint64_t* done, const PartInfo* parts, int* abort_flag, int* status) {
     const int slot = n % kParts;
     if (!mbar_wait(&full[slot], (n / kParts) & 1, abort_flag, status, 420))
@@ -613,521 +426,10 @@ struct Chunks {
     k0 = uniform(w.k0);
     v0 = uniform(w.v0);
     warp_arrive(&done[slot]);
-    c0 = 0;
     tiles = (end - begin + kUnitKeys - 1) / kUnitKeys;
     return end >= 0;
   }
-  __device__ __forceinline__ bool next(uint64_t* full, uint64_t* done, const PartInfo* parts, int* abort_flag, int* status) {
-    c0 += kChunk;
-    if (c0 < tiles)
-      return true;
-    ++n;
-    return open(full, done, parts, abort_flag, status);
-  }
 };
-
-template <bool PLAIN>
-__global__ void __launch_bounds__(kFewThreads, 1)
-fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const FewParams p) {
-  pdl_wait();      // programmatic dependent launch: nothing before this reads an earlier kernel's data
-  pdl_trigger();
-  const Fp8AttnParams& a = p.a;
-
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  // weights of a chunk: tile i in block i / 2; row = key, 64 bytes at 64 * (i % 2): kRows weights, then kRows remainders
-  uint8_t* p_smem = ring + kRing * kTileBytes;
-  uint8_t* q_smem = p_smem + kChunk / 2 * kTileBytes;        // two slots of [kRows][128] e4m3, then e5m2
-  float* sc_smem = reinterpret_cast<float*>(q_smem + 4 * kQBytes);      // two slots of [kChunk][K, V][128] scales
-  __shared__ uint64_t full[kRing], empty[kRing], part_full[kParts], part_done[kParts], q_full[2], s_full[2], s_free[2], p_full, pv_done;
-  __shared__ PartInfo s_part[kParts];
-  __shared__ uint32_t tmem_slot, s_amax[kParts];
-  __shared__ int abort_flag, joins;
-  __shared__ RowInfo s_row[2][kRows];
-  __shared__ __align__(16) float s_max[4][kRows], s_sum[4][kRows];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    abort_flag = 0;
-    for (int i = 0; i < kRing; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
-    }
-    for (int i = 0; i < kParts; ++i) {
-      mbar_init(&part_full[i], 1);
-      mbar_init(&part_done[i], kSoftmaxWarps + 2);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 8);
-      mbar_init(&s_full[i], 1);
-      mbar_init(&s_free[i], kSoftmaxWarps);
-    }
-    mbar_init(&p_full, kSoftmaxWarps);
-    mbar_init(&pv_done, 1);
-    fence_mbar_init();
-    tma_prefetch_desc(&tmap_k);
-    tma_prefetch_desc(&tmap_v);
-  }
-  if (warp == 1) {
-    tmem_alloc(&tmem_slot, kTmemCols);
-    tmem_relinquish();
-  }
-  tc_fence_before_sync();
-  __syncthreads();
-  tc_fence_after_sync();
-  const uint32_t tmem = tmem_slot;      // S^T of two chunks, then O^T: kRows columns of 256 w, kRows of remainders
-
-  if (warp == kSoftmaxWarps + 2) {
-    // ---------------------------------------------------------------- scheduler: the parts of this CTA's share
-    Walk<kRows> walk;
-    walk.start(p);
-    for (int n = 0;;) {
-      const bool more = walk.next(p);
-      if (more && walk.span.y <= walk.span.x) {      // no keys: zeros
-        zero_rows(a, walk.w, walk.hk, walk.tile * kRows, kRows);
-        continue;
-      }
-      const int slot = n % kParts;
-      if (n >= kParts && !mbar_wait(&part_done[slot], (n / kParts - 1) & 1, &abort_flag, p.status_word, 400))
-        break;
-      if (lane == 0) {
-        PartInfo v = {};
-        v.end = -1;
-        if (more)
-          v = walk.info();
-        s_part[slot] = v;
-        s_amax[slot] = 0;
-      }
-      warp_arrive(&part_full[slot]);
-      ++n;
-      if (!more)
-        break;
-    }
-  } else if (warp == 0) {
-    // ---------------------------------------------------------------- producer: the K tiles of a chunk before the V tiles of the last
-    int n = 0;
-    auto load = [&](const CUtensorMap* map, const Chunks& c, int row0) {
-      for (int i = 0; i < c.count(); ++i, ++n) {
-        const int slot = n % kRing, key = c.begin + (c.c0 + i) * kUnitKeys;
-        if (n >= kRing)
-          mbar_wait(&empty[slot], (n / kRing - 1) & 1, &abort_flag, p.status_word, 401);
-        if (elect_one()) {
-          const int boxes = min(4, (c.end - key + 31) / 32);      // no box of keys that do not belong to the part
-          mbar_arrive_expect_tx(&full[slot], boxes * 32 * kD);
-          for (int j = 0; j < boxes; ++j)
-            tma_load_2d(ring + slot * kTileBytes + j * 32 * kD, map, &full[slot], c.hk * kD, row0 + key + 32 * j);
-        }
-        __syncwarp();
-      }
-    };
-    Chunks ahead = {};
-    bool more = ahead.open(part_full, part_done, s_part, &abort_flag, p.status_word);
-    if (more)
-      load(&tmap_k, ahead, ahead.k0);
-    while (more) {
-      const Chunks now = ahead;
-      more = ahead.next(part_full, part_done, s_part, &abort_flag, p.status_word);
-      if (more)
-        load(&tmap_k, ahead, ahead.k0);
-      load(&tmap_v, now, now.v0);
-    }
-    // a CTA may not end with copies on their way, also when a wait of another warp has given up
-    for (int i = max(0, n - kRing); i < n; ++i)
-      mbar_wait(&full[i % kRing], (i / kRing) & 1, &abort_flag, p.status_word, 402);
-  } else if (warp == 1) {
-    // ---------------------------------------------------------------- MMA issuer: the scores of a chunk before the sums of the last
-    constexpr uint32_t idesc_hi = umma_idesc_f8(128, kRows, 0, 0, 0, 0), idesc_lo = umma_idesc_f8(128, kRows, 0, 1, 0, 0);
-    constexpr uint32_t idesc_pv = umma_idesc_f8(128, 2 * kRows, 0, 0, 1, 1);
-    const uint32_t ring_addr = smem_u32(ring), p_addr = smem_u32(p_smem), t_s = uniform(tmem), t_o = t_s + 2 * kChunk * kRows;
-    int n = 0, n_s = 0, n_p = 0;
-    auto scores = [&](const Chunks& c) {
-      const int buf = n_s & 1;
-      if (c.c0 == 0)
-        mbar_wait(&q_full[c.n & 1], (c.n >> 1) & 1, &abort_flag, p.status_word, 403);
-      if (n_s >= 2)
-        mbar_wait(&s_free[buf], ((n_s >> 1) - 1) & 1, &abort_flag, p.status_word, 404);
-      const uint32_t q_addr = smem_u32(q_smem) + (c.n & 1) * 2 * kQBytes;
-      const int nt = c.count();
-      for (int i = 0; i < nt; ++i, ++n) {
-        const int slot = n % kRing;
-        mbar_wait(&full[slot], (n / kRing) & 1, &abort_flag, p.status_word, 405);
-        tc_fence_after_sync();
-        if (elect_one()) {
-          const uint32_t k_addr = ring_addr + slot * kTileBytes, d = t_s + (buf * kChunk + i) * kRows;
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {      // 32 head dimensions = 32 bytes a step
-            umma_tile(d, k_addr + 32 * kk, q_addr + 32 * kk, idesc_hi, kk != 0 ? 1u : 0u);
-            umma_tile(d, k_addr + 32 * kk, q_addr + kQBytes + 32 * kk, idesc_lo, 1u);
-          }
-          umma_commit(&empty[slot]);
-          if (i == nt - 1)
-            umma_commit(&s_full[buf]);
-        }
-        __syncwarp();
-      }
-      ++n_s;
-    };
-    Chunks ahead = {};
-    bool more = ahead.open(part_full, part_done, s_part, &abort_flag, p.status_word);
-    if (more)
-      scores(ahead);
-    while (more) {
-      const Chunks now = ahead;
-      more = ahead.next(part_full, part_done, s_part, &abort_flag, p.status_word);
-      if (more)
-        scores(ahead);
-      const int nt = now.count();
-      mbar_wait(&p_full, n_p & 1, &abort_flag, p.status_word, 407);
-      ++n_p;
-      for (int i = 0; i < nt; ++i, ++n) {
-        const int slot = n % kRing;
-        mbar_wait(&full[slot], (n / kRing) & 1, &abort_flag, p.status_word, 406);
-        tc_fence_after_sync();
-        if (elect_one()) {
-          const uint32_t v_addr = ring_addr + slot * kTileBytes, w_addr = p_addr + (i >> 1) * kTileBytes + (i & 1) * 64;
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)        // 32 keys = 32 rows of 128 bytes a step
-            umma_tile(t_o, v_addr + kk * 4096, w_addr + kk * 4096, idesc_pv, (now.c0 | i | kk) != 0 ? 1u : 0u);
-          umma_commit(&empty[slot]);
-          if (i == nt - 1)
-            umma_commit(&pv_done);
-        }
-        __syncwarp();
-      }
-    }
-  } else {
-    // ---------------------------------------------------------------- softmax over the keys, epilogue
-    const int rg = (warp - 2) >> 2;                // rows kGroup * rg ..
-    const int quarter = warp & 3;                  // tensor-memory lanes: keys (head dimensions) 32 * quarter ..
-    const int tid = threadIdx.x - 64;
-    const int kl = quarter * 32 + lane;            // key of a tile, or head dimension
-    const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    const uint32_t t_o = t_lane + 2 * kChunk * kRows;
-    const int r0 = rg * kGroup;
-    const bool stages = warp < 10;                 // takes part in staging the queries
-    const float key_mul = a.scale * (PLAIN ? kLog2e : 1.f);
-    uint8_t* p_dst = p_smem + kl * kD + (rg & 1) * 8;
-
-    // Scales of the keys of a chunk, copied ahead of their use: K's by the first half of the threads, V's by the second.  The
-    // heads of a key lie side by side: CTAs that work on them at the same time start at different tiles.
-    auto request_scales = [&](const PartInfo& w, int key, int slot) {
-      const bool of_v = tid >= 256;
-      const float* src = (of_v ? a.v_scales + static_cast<int64_t>(w.v0) * a.Hkv : a.k_scales + static_cast<int64_t>(w.k0) * a.Hkv) + w.hk;
-      float* dst = sc_smem + slot * kChunk * 2 * kUnitKeys + (of_v ? kUnitKeys : 0) + (tid & 127);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int i = (2 * j + ((tid >> 7) & 1) + w.hk) & (kChunk - 1), at = key + i * kUnitKeys + (tid & 127);
-        if (at < w.end)
-          cp_async4(dst + i * 2 * kUnitKeys, src + static_cast<int64_t>(at) * a.Hkv);
-      }
-      cp_async_commit();
-    };
-    auto wait_part = [&](int n) {
-      return mbar_wait(&part_full[n % kParts], (n / kParts) & 1, &abort_flag, p.status_word, 415) && s_part[n % kParts].end >= 0;
-    };
-    auto stage = [&](int n, QueryLoad& ql) {
-      if (stages) {
-        ql.template store<PLAIN>(a, s_part[n % kParts], tid, q_smem + (n & 1) * 2 * kQBytes, &s_amax[n % kParts], s_row[n & 1]);
-        warp_arrive(&q_full[n & 1]);
-      }
-    };
-
-    QueryLoad ql;
-    int n_chunk = 0, ring_at = 0;
-    bool more = wait_part(0), after = false;       // whether the part at hand and the one after it exist
-    if (more) {
-      request_scales(s_part[0], s_part[0].begin, 0);
-      if (stages) {
-        ql.index(a, s_part[0], tid);
-        ql.data(a, tid);
-      }
-      stage(0, ql);
-      after = wait_part(1);
-      if (after && stages) {
-        ql.index(a, s_part[1], tid);
-        ql.data(a, tid);
-      }
-      cp_async_wait_all();
-      softmax_sync();
-      ring_at = min(kChunk, (s_part[0].end - s_part[0].begin + kUnitKeys - 1) / kUnitKeys);
-    }
-    for (int n = 0; more; ++n) {
-      const PartInfo& part = s_part[n % kParts];
-      const RowInfo* rows = &s_row[n & 1][r0];
-      const int end = part.end, tiles = (end - part.begin + kUnitKeys - 1) / kUnitKeys;
-      const bool alive = rows[0].out >= 0;         // rows are filled from the first on
-      bool then = false;                           // whether the part after the next exists
-      float top[kGroup], l[kGroup];
-#pragma unroll
-      for (int r = 0; r < kGroup; ++r) {
-        top[r] = kNothing;
-        l[r] = 0.f;
-      }
-      for (int c0 = 0; c0 < tiles; c0 += kChunk, ++n_chunk) {
-        const int nt = min(kChunk, tiles - c0), buf = n_chunk & 1;
-        const bool last = c0 + kChunk >= tiles;
-        const int key0 = part.begin + c0 * kUnitKeys + kl;
-        float kk[kChunk], ex[kChunk];
-        {
-          const float* sc = sc_smem + buf * kChunk * 2 * kUnitKeys + kl;
-          const float mul = key_mul * __uint_as_float(fp8_scale_bits(s_amax[n % kParts]));
-#pragma unroll
-          for (int i = 0; i < kChunk; ++i) {
-            kk[i] = sc[i * 2 * kUnitKeys] * mul;
-            ex[i] = value_exponent(sc[(i * 2 + 1) * kUnitKeys]);
-          }
-        }
-        // products of the chunk; tensor memory is free for the next one
-        mbar_wait(&s_full[buf], (n_chunk >> 1) & 1, &abort_flag, p.status_word, 409);
-        tc_fence_after_sync();
-        uint32_t s[kChunk][kGroup];
-#pragma unroll
-        for (int i = 0; i < kChunk; ++i)
-          if (i < nt)
-            tmem_ld_32x8(t_lane + (buf * kChunk + i) * kRows + r0, s[i]);
-        tmem_ld_wait();
-        tc_fence_before_sync();
-        warp_arrive(&s_free[buf]);
-        // what the next chunk needs
-        int next_tiles = 0;
-        if (!last) {
-          request_scales(part, part.begin + (c0 + kChunk) * kUnitKeys, buf ^ 1);
-          next_tiles = min(kChunk, tiles - c0 - kChunk);
-        } else if (after) {
-          stage(n + 1, ql);
-          const PartInfo& w = s_part[(n + 1) % kParts];
-          request_scales(w, w.begin, buf ^ 1);
-          next_tiles = min(kChunk, (w.end - w.begin + kUnitKeys - 1) / kUnitKeys);
-          then = wait_part(n + 2);
-          if (then && stages)
-            ql.index(a, s_part[(n + 2) % kParts], tid);
-        }
-        const int v_at = ring_at + next_tiles;      // the chunk's V tiles in the order of the ring
-        ring_at = v_at + nt;
-
-        float mx[kGroup];
-#pragma unroll
-        for (int r = 0; r < kGroup; ++r)
-          mx[r] = top[r];
-        if (alive) {
-          // scores (times log2 e, plus the exponents of the values' scales) and their maxima
-          if (PLAIN) {
-#pragma unroll
-            for (int i = 0; i < kChunk; ++i)
-              if (key0 + i * kUnitKeys < end) {
-#pragma unroll
-                for (int r = 0; r < kGroup; ++r) {
-                  const float t = fmaf(__uint_as_float(s[i][r]), kk[i], ex[i]);
-                  s[i][r] = __float_as_uint(t);
-                  mx[r] = fmaxf(mx[r], t);
-                }
-              }
-          } else {
-#pragma unroll
-            for (int i = 0; i < kChunk; ++i)
-#pragma unroll
-              for (int r = 0; r < kGroup; ++r)
-                s[i][r] = __float_as_uint(__uint_as_float(s[i][r]) * kk[i]);
-            if (a.cap > 0.f) {
-              const float to = 2.f * kLog2e / a.cap;
-#pragma unroll
-              for (int i = 0; i < kChunk; ++i)
-#pragma unroll
-                for (int r = 0; r < kGroup; ++r)
-                  s[i][r] = __float_as_uint(capped(__uint_as_float(s[i][r]) * to, a.cap));
-            }
-#pragma unroll
-            for (int r = 0; r < kGroup; ++r) {
-              const float slope = rows[r].slope;
-              const int pos = rows[r].pos, lo = rows[r].lo, hi = min(rows[r].hi, end);
-#pragma unroll
-              for (int i = 0; i < kChunk; ++i) {
-                const int at = key0 + i * kUnitKeys;
-                float t = fmaf(__uint_as_float(s[i][r]), kLog2e, ex[i]) - slope * static_cast<float>(abs(pos - at));
-                t = at >= lo && at < hi ? t : -INFINITY;
-                s[i][r] = __float_as_uint(t);
-                mx[r] = fmaxf(mx[r], t);
-              }
-            }
-          }
-#pragma unroll
-          for (int r = 0; r < kGroup; ++r)
-            mx[r] = warp_max(mx[r]);
-          if (lane == 0) {
-#pragma unroll
-            for (int r = 0; r < kGroup; r += 4)
-              *reinterpret_cast<float4*>(&s_max[quarter][r0 + r]) = make_float4(mx[r], mx[r + 1], mx[r + 2], mx[r + 3]);
-          }
-          group_sync(rg);
-#pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-            float x[kGroup];
-            lds_row(x, s_max[q4] + r0);
-#pragma unroll
-            for (int r = 0; r < kGroup; ++r)
-              mx[r] = fmaxf(mx[r], x[r]);
-          }
-        }
-        // the weights of the last chunk have been taken; the sums are rescaled where a maximum has grown
-        if (n_chunk > 0)
-          mbar_wait(&pv_done, (n_chunk - 1) & 1, &abort_flag, p.status_word, 410);
-        if (alive) {
-          bool grown = false;
-#pragma unroll
-          for (int r = 0; r < kGroup; ++r)
-            grown = grown || mx[r] > top[r];
-          if (c0 > 0 && grown) {      // the same rows in all four quarters
-            float old[kGroup];
-#pragma unroll
-            for (int r = 0; r < kGroup; ++r) {
-              old[r] = exp2f(top[r] - mx[r]);
-              l[r] *= old[r];
-            }
-            tc_fence_after_sync();
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              uint32_t o[kGroup];
-              tmem_ld_32x8(t_o + j * kRows + r0, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int r = 0; r < kGroup; ++r)
-                o[r] = __float_as_uint(__uint_as_float(o[r]) * old[r]);
-              tmem_st_32x8(t_o + j * kRows + r0, o);
-            }
-            tmem_st_wait();
-          }
-#pragma unroll
-          for (int r = 0; r < kGroup; ++r) {
-            top[r] = mx[r];
-            mx[r] = 8.f - mx[r];      // weights are taken times 256
-          }
-#pragma unroll
-          for (int i = 0; i < kChunk; ++i)
-            if (i < nt) {
-              uint32_t hi[2] = {0u, 0u}, lo[2] = {0u, 0u};
-              if (key0 + i * kUnitKeys < end) {
-                // the weight of a NaN is a NaN where its key is seen, else zero
-                const float inv = ex[i] == ex[i] ? exp2f(-ex[i]) : 1.f;
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                  float w4[4];
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) {
-                    w4[e] = exp2f(__uint_as_float(s[i][4 * j + e]) + mx[4 * j + e]);
-                    l[4 * j + e] = fmaf(w4[e], inv, l[4 * j + e]);
-                  }
-                  split_weights(w4, hi[j], lo[j]);
-                }
-              }
-              uint8_t* dst = p_dst + (i >> 1) * kTileBytes;
-              *reinterpret_cast<uint2*>(dst + (((4 * (i & 1) + (rg >> 1)) ^ (kl & 7)) << 4)) = make_uint2(hi[0], hi[1]);
-              *reinterpret_cast<uint2*>(dst + (((4 * (i & 1) + 2 + (rg >> 1)) ^ (kl & 7)) << 4)) = make_uint2(lo[0], lo[1]);
-            }
-        }
-        if (last && end - (key0 - kl) < nt * kUnitKeys && rg == 0) {
-          // rows behind the last key may hold any byte, a NaN times a weight of zero among them
-          const int use = v_at + nt - 1;
-          mbar_wait(&full[use % kRing], (use / kRing) & 1, &abort_flag, p.status_word, 412);
-          if (key0 + (nt - 1) * kUnitKeys >= end) {
-            uint4* v = reinterpret_cast<uint4*>(ring + (use % kRing) * kTileBytes + kl * kD);
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              v[j] = make_uint4(0u, 0u, 0u, 0u);
-          }
-        }
-        tc_fence_before_sync();
-        fence_proxy_async_smem();
-        warp_arrive(&p_full);
-        if (!last) {
-          cp_async_wait_all();
-          softmax_sync();      // everybody's scales of the next chunk are there
-        }
-      }
-
-      // ---------------------------------------------------------------- thread = head dimension kl of kGroup rows
-      if (then && stages)
-        ql.data(a, tid);
-      {
-        const float v = reduce_lanes<kGroup>(l);
-        if (lane % (32 / kGroup) == 0)
-          s_sum[quarter][r0 + lane / (32 / kGroup)] = v;
-      }
-      int dst[kGroup];
-      float fix[kGroup];
-#pragma unroll
-      for (int r = 0; r < kGroup; ++r) {
-        dst[r] = rows[r].out;
-        fix[r] = rows[r].fix;
-      }
-      const PartInfo joined = part;
-      cp_async_wait_all();
-      softmax_sync();          // the sums and the next part's scales and rows are there; this part's descriptions are not read again
-      warp_arrive(&part_done[n % kParts]);
-#pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        float x[kGroup];
-        lds_row(x, s_sum[q4] + r0);
-#pragma unroll
-        for (int r = 0; r < kGroup; ++r)
-          l[r] = q4 == 0 ? x[r] : l[r] + x[r];
-      }
-      mbar_wait(&pv_done, (n_chunk - 1) & 1, &abort_flag, p.status_word, 413);
-      tc_fence_after_sync();
-      float o[kGroup];
-      {
-        uint32_t u[kGroup], v[kGroup];
-        tmem_ld_32x8(t_o + r0, u);
-        tmem_ld_32x8(t_o + kRows + r0, v);
-        tmem_ld_wait();
-#pragma unroll
-        for (int r = 0; r < kGroup; ++r)
-          o[r] = fmaf(__uint_as_float(v[r]), 0.0625f, __uint_as_float(u[r]));
-      }
-      tc_fence_before_sync();
-      if (joined.parts == 1 || join_parts(p, joined, top, l, o, r0, kl, tid, &joins)) {
-#pragma unroll
-        for (int r = 0; r < kGroup; ++r)
-          if (dst[r] >= 0)
-            a.out[static_cast<int64_t>(dst[r]) * kD + kl] =
-                __float2bfloat16_rn(l[r] == 0.f || fix[r] == 0.f ? 0.f : o[r] * __fdividef(fix[r], l[r]));
-      }
-      more = after;
-      after = then;
-    }
-  }
-
-  tc_fence_before_sync();
-  __syncthreads();
-  if (warp == 1) {
-    tc_fence_after_sync();
-    tmem_dealloc(tmem, kTmemCols);
-  }
-}
-
-// ----------------------------------------------------------------------------------------------
-// Many rows per sequence: bound by the exponentials and the instructions around them (a tile of 128 rows x 128 keys takes the
-// tensor cores 950 cycles, its exponentials 1024).
-//
-// Tiles of 128 (listed row, query head) pairs, rows in the M = 128 of the products:
-//   S = Q K^T    A: the queries as e4m3 + e5m2 (two products into one accumulator), B: the K tile as loaded (K-major)
-//   O = P V      A: the weights as e4m3 + e5m2, B: the V tile as loaded (MN-major)
-// Thread = row in four softmax warps.  A weight is 64 * 2^(t - reference); the reference follows the maximum in steps, so that the
-// sums are rescaled only where a score lies more than 2.8 (log2) above it.  A weight is off by 2^-7 of itself or by 2^-23 of the
-// largest.  Scores and weights share 128 columns of tensor memory (32 keys' weights, e4m3 then e5m2, lie in the first 16 of their
-// scores' 32 columns), so the steps of one tile follow one another; two CTAs per SM, each with parts of its own, fill each other's
-// waits, the ends of parts among them.  Four loader warps stage the queries of the next part and the scales of the next tiles.
-// ----------------------------------------------------------------------------------------------
-constexpr int kManyRows = 128;
-constexpr int kManyRing = 4;                                 // slots of one K or V tile
-constexpr int kScaleSlots = 2;                               // tiles whose scales are staged ahead
-constexpr int kManyWarps = 4, kManyThreads = 32 * (3 + kManyWarps + 4);
-constexpr int kManyCtas = 2;                                 // per SM
-constexpr uint32_t kManyTmemCols = 256;
-constexpr uint32_t kStageBytes = 32 * 64;                    // of a softmax warp: 32 head dimensions of its rows
-constexpr uint32_t kManyQBytes = kManyRows * kD;             // e4m3 or e5m2 part of the queries of a tile
-constexpr uint32_t kManySmem = kManyRing * kTileBytes + 2 * kManyQBytes + kManyWarps * kStageBytes +
-                               kScaleSlots * 3 * kUnitKeys * sizeof(float) + 1024;
-constexpr float kWeightLog2 = 6.f;                           // the reference's weight: 2^6
-constexpr float kHeadroom = 2.8f;                            // 2^(6 + 2.8) < 448
 
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
   float d;
@@ -1172,6 +474,543 @@ __device__ __forceinline__ void split_weights_e5m2(float2 a, float2 b, uint32_t&
   hi = __byte_perm(h0, h1, 0x5410);
   lo = __byte_perm(fp8_pack_half2_e5m2(*reinterpret_cast<const uint32_t*>(&r)), fp8_pack_half2_e5m2(*reinterpret_cast<const uint32_t*>(&s)), 0x5410);
 }
+
+// ----------------------------------------------------------------------------------------------
+// Few rows per sequence: bound by the bytes of the cache, which go from the TMA ring to the tensor cores as they are, and by the
+// chain of steps from the lists of a sequence to its result.
+//
+// The rows of a tile are up to 32 (listed row, query head) pairs of one sequence and key head, so that grouped query heads share
+// one pass over their keys.  A unit of work is 128 keys of a tile; all units of the launch, in the order (sequence, tile, key head,
+// keys), are dealt out to the CTAs in equal contiguous shares that every CTA works out for itself from the device-side counts.  A
+// tile whose units lie in several CTAs is joined by the CTA that finishes last, in the order of its parts.
+//
+// The products are transposed, keys (then head dimensions) in the M = 128 of tcgen05.mma.kind::f8f6f4:
+//   S^T = K Q^T         A: K tile as loaded (K-major), B: the queries as e4m3 + e5m2, two products into one accumulator
+//   O^T = V^T P^T       A: V tile as loaded (MN-major), B: the weights as e4m3 + e5m2, two products into one accumulator
+// A query in bf16 (8 significant bits) is e4m3 (4 bits) plus a remainder of at most 3 bits, which e5m2 holds exactly down to
+// 2^-25 of the tile's largest element.  A weight is 64 * 2^(t - reference), as with many rows: off by 2^-7 of itself or by 2^-23 of
+// the largest.  The codes of the cache are never widened.
+//
+// Four softmax warps, thread = key with the scores of all rows in registers; a row's reference is in shared memory and follows the
+// maximum in steps, so that a unit costs one barrier (does any score exceed its reference by more than 2.8?) and the maxima are
+// looked for only where one does.  Three CTAs per SM, each with parts of its own, fill each other's waits: 16 x 512 keys, 32
+// heads, 26 rows take 43 us with one CTA of sixteen softmax warps.
+// ----------------------------------------------------------------------------------------------
+constexpr int kFewRing = 2;                                  // slots of one K or V tile
+constexpr int kFewCtas = 4;                                  // per SM
+constexpr int kFewWarps = 4, kFewThreads = 32 * (3 + kFewWarps);
+constexpr uint32_t kFewTmemCols = 128, kQBytes = kRows * kD, kPBytes = kUnitKeys * 64;
+constexpr uint32_t kFewSmem = kFewRing * kTileBytes + kPBytes + 2 * kQBytes + 1024;
+
+// Rows of a part in the workspace: [dimension][row] sums, [row] references, [row] sums of weights.
+constexpr int kFewPart = kRows * (kD + 2);
+
+// Sum of each of 32 values over the lanes of a warp: lane l gets that of value l.
+__device__ __forceinline__ float sum_lanes(float (&v)[32]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int half = 16; half; half >>= 1) {
+    const bool upper = lane & half;
+#pragma unroll
+    for (int i = 0; i < half; ++i) {
+      const float give = upper ? v[i] : v[i + half], keep = upper ? v[i + half] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, half);
+    }
+  }
+  return v[0];
+}
+
+template <bool PLAIN>
+__global__ void __launch_bounds__(kFewThreads, kFewCtas)
+fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const FewParams p) {
+  pdl_wait();      // programmatic dependent launch: nothing before this reads an earlier kernel's data
+  pdl_trigger();
+  const Fp8AttnParams& a = p.a;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* p_smem = ring + kFewRing * kTileBytes;            // [128 keys][32 e4m3, 32 e5m2], 64-byte swizzle
+  uint8_t* q_smem = p_smem + kPBytes;                        // [32 rows][128] e4m3, then e5m2
+  __shared__ uint64_t full[kFewRing], empty[kFewRing], part_full[kParts], part_done[kParts], q_full, s_full[2], p_full, pv_done, o_free;
+  __shared__ PartInfo s_part[kParts];
+  __shared__ uint32_t tmem_slot, s_top[kFewWarps];
+  __shared__ int abort_flag, joins;
+  __shared__ RowInfo s_row[kRows];
+  __shared__ __align__(16) float s_max[kFewWarps][kRows], s_ref[kRows], s_old[kRows];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < kFewRing; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < kParts; ++i) {
+      mbar_init(&part_full[i], 1);
+      mbar_init(&part_done[i], kFewWarps + 2);
+    }
+    mbar_init(&s_full[0], 1);
+    mbar_init(&s_full[1], 1);
+    mbar_init(&p_full, kFewWarps);
+    mbar_init(&pv_done, 1);
+    mbar_init(&q_full, kFewWarps);
+    mbar_init(&o_free, kFewWarps);
+    fence_mbar_init();
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, kFewTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;      // S^T of two units, 32 columns each, then O^T
+
+  if (warp == 2) {
+    // ---------------------------------------------------------------- scheduler: the parts of this CTA's share
+    Walk<kRows> walk;
+    walk.start(p);
+    for (int n = 0;;) {
+      const bool more = walk.next(p);
+      const int slot = n % kParts;
+      if (n >= kParts && !mbar_wait(&part_done[slot], (n / kParts - 1) & 1, &abort_flag, p.status_word, 400))
+        break;
+      if (lane == 0) {
+        PartInfo v = {};
+        v.end = -1;
+        if (more)
+          v = walk.info();
+        s_part[slot] = v;
+      }
+      warp_arrive(&part_full[slot]);
+      ++n;
+      if (!more)
+        break;
+    }
+  } else if (warp == 0) {
+    // ---------------------------------------------------------------- producer: K of a unit before V of the last
+    int n = 0;
+    PartWalk c = {};
+    auto load = [&](const CUtensorMap* map, int row0, int key) {
+      const int slot = n % kFewRing;
+      if (n >= kFewRing)
+        mbar_wait(&empty[slot], (n / kFewRing - 1) & 1, &abort_flag, p.status_word, 401);
+      if (elect_one()) {
+        const int boxes = min(4, (c.end - key + 31) / 32);      // no box of keys that do not belong to the part
+        mbar_arrive_expect_tx(&full[slot], boxes * 32 * kD);
+        for (int j = 0; j < boxes; ++j)
+          tma_load_2d(ring + slot * kTileBytes + j * 32 * kD, map, &full[slot], c.hk * kD, row0 + key + 32 * j);
+      }
+      __syncwarp();
+      ++n;
+    };
+    for (bool more = c.open(part_full, part_done, s_part, &abort_flag, p.status_word); more;) {
+      if (c.tiles)
+        load(&tmap_k, c.k0, c.begin);
+      for (int key = c.begin; key < c.end; key += kUnitKeys) {
+        if (key + kUnitKeys < c.end)
+          load(&tmap_k, c.k0, key + kUnitKeys);
+        load(&tmap_v, c.v0, key);
+      }
+      ++c.n;
+      more = c.open(part_full, part_done, s_part, &abort_flag, p.status_word);
+    }
+    // a CTA may not end with copies on their way, also when a wait of another warp has given up
+    for (int i = max(0, n - kFewRing); i < n; ++i)
+      mbar_wait(&full[i % kFewRing], (i / kFewRing) & 1, &abort_flag, p.status_word, 402);
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer: scores of a unit before the sums of the last
+    constexpr uint32_t idesc_hi = umma_idesc_f8(128, kRows, 0, 0, 0, 0), idesc_lo = umma_idesc_f8(128, kRows, 0, 1, 0, 0);
+    constexpr uint32_t idesc_pv = umma_idesc_f8(128, kRows, 0, 0, 1, 1), idesc_pv_lo = umma_idesc_f8(128, kRows, 0, 1, 1, 1);
+    const uint32_t ring_addr = smem_u32(ring), p_addr = smem_u32(p_smem), q_addr = smem_u32(q_smem), t_s = uniform(tmem), t_o = t_s + 64;
+    int n = 0, u0 = 0, live = 0;      // tiles of the ring, units before the part, parts that have some
+    PartWalk c = {};
+    auto scores = [&](int i) {
+      const int slot = n % kFewRing, u = u0 + i;
+      mbar_wait(&full[slot], (n / kFewRing) & 1, &abort_flag, p.status_word, 405);
+      tc_fence_after_sync();
+      if (elect_one()) {
+        const uint32_t k_addr = ring_addr + slot * kTileBytes, d = t_s + (u & 1) * kRows;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {      // 32 head dimensions = 32 bytes a step
+          umma_tile(d, k_addr + 32 * kk, q_addr + 32 * kk, idesc_hi, kk != 0 ? 1u : 0u);
+          umma_tile(d, k_addr + 32 * kk, q_addr + kQBytes + 32 * kk, idesc_lo, 1u);
+        }
+        umma_commit(&empty[slot]);
+        umma_commit(&s_full[u & 1]);
+      }
+      __syncwarp();
+      ++n;
+    };
+    for (bool more = c.open(part_full, part_done, s_part, &abort_flag, p.status_word); more;) {
+      if (c.tiles) {
+        mbar_wait(&q_full, live & 1, &abort_flag, p.status_word, 403);
+        scores(0);
+      }
+      for (int i = 0; i < c.tiles; ++i) {
+        if (i + 1 < c.tiles)
+          scores(i + 1);      // into the columns whose scores became the weights that the last product took
+        const int slot = n % kFewRing, u = u0 + i;
+        mbar_wait(&full[slot], (n / kFewRing) & 1, &abort_flag, p.status_word, 406);
+        if (i == 0 && live > 0)
+          mbar_wait(&o_free, (live - 1) & 1, &abort_flag, p.status_word, 408);
+        mbar_wait(&p_full, u & 1, &abort_flag, p.status_word, 407);
+        tc_fence_after_sync();
+        if (elect_one()) {
+          const uint32_t v_addr = ring_addr + slot * kTileBytes;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {      // 32 keys: 32 rows of V and of the weights
+            umma_tile_b64(t_o, v_addr + kk * 4096, p_addr + kk * 2048, idesc_pv, (i | kk) != 0 ? 1u : 0u);
+            umma_tile_b64(t_o, v_addr + kk * 4096, p_addr + 32 + kk * 2048, idesc_pv_lo, 1u);
+          }
+          umma_commit(&empty[slot]);
+          umma_commit(&pv_done);
+        }
+        __syncwarp();
+        ++n;
+      }
+      live += c.tiles ? 1 : 0;
+      u0 += c.tiles;
+      ++c.n;
+      more = c.open(part_full, part_done, s_part, &abort_flag, p.status_word);
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax over the keys, epilogue
+    const int quarter = warp & 3;                  // tensor-memory lanes: keys (head dimensions) 32 * quarter ..
+    const int tid = threadIdx.x - 96;
+    const int kl = quarter * 32 + lane;            // key of a unit, or head dimension
+    const int group = a.H / a.Hkv;
+    const uint32_t t_s = tmem + (static_cast<uint32_t>(quarter * 32) << 16), t_o = t_s + 64;
+    int u = 0, n_ring = 0;                         // units and tiles of the ring so far
+    // the list on its way while the scheduler works out the share: behind the first tiles of K and V it takes 2 us
+    for (int i = tid * 32; i < min(a.num_salient, 128 * 32); i += 128 * 32)
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(a.idx + i));
+    for (int n = 0;; ++n) {
+      if (rows_any(!mbar_wait(&part_full[n % kParts], (n / kParts) & 1, &abort_flag, p.status_word, 415)))
+        break;
+      const PartInfo part = s_part[n % kParts];
+      warp_arrive(&part_done[n % kParts]);
+      const int begin = part.begin, end = part.end;
+      if (end < 0)
+        break;
+      if (end == begin) {      // no keys: zeros
+        for (int t = part.t0 + (tid >> 4); t < min(part.t0 + kRows, part.rows); t += 8) {
+          const int i = t / group;
+          const int64_t row = (static_cast<int64_t>(part.row0) + i) * a.H + part.hk * group + t - i * group;
+          *reinterpret_cast<uint4*>(a.out + row * kD + (tid & 15) * 8) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        continue;
+      }
+      const float* k_scale = a.k_scales + static_cast<int64_t>(part.k0) * a.Hkv + part.hk;
+      const float* v_scale = a.v_scales + static_cast<int64_t>(part.v0) * a.Hkv + part.hk;
+      float ks_next = 1.f, vs_next = 1.f;
+      if (begin + kl < end) {
+        ks_next = __ldg(k_scale + static_cast<int64_t>(begin + kl) * a.Hkv);
+        vs_next = __ldg(v_scale + static_cast<int64_t>(begin + kl) * a.Hkv);
+      }
+      // queries: eight threads a row, rows tid / 8 and 16 + tid / 8; codes next to the tile's largest element (an error of 2^-26
+      // of it moves every score of the tile by as little), e4m3 and the e5m2 rest
+      float q_scale;
+      {
+        uint4 x0[2], x1[2];
+        int at[2], head[2], t[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          t[h] = part.t0 + 16 * h + (tid >> 3);
+          const int i = t[h] / group;
+          head[h] = part.hk * group + t[h] - i * group;
+          at[h] = t[h] < part.rows ? __ldg(a.idx + part.row0 + i) : -1;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          at[h] = at[h] >= a.total_q ? -1 : at[h];
+          x0[h] = x1[h] = make_uint4(0u, 0u, 0u, 0u);
+          if (at[h] >= 0) {
+            const uint4* src = reinterpret_cast<const uint4*>(a.q + at[h] * a.ldq + head[h] * kD) + (tid & 7) * 2;
+            x0[h] = __ldg(src);
+            x1[h] = __ldg(src + 1);
+          }
+        }
+        bool finite[2];
+        uint32_t top = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t m = fp8_amax8(max(bf16x8_amax(x0[h]), bf16x8_amax(x1[h])));
+          finite[h] = m < 0x7f800000u;
+          top = max(top, finite[h] ? m : 0u);
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (lane == 0)
+          s_top[quarter] = top;
+        rows_sync();
+        const uint32_t scale = fp8_scale_bits(max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3])));
+        const float inv = fp8_inverse(scale);
+        q_scale = __uint_as_float(scale);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = 16 * h + (tid >> 3);
+          if (!finite[h])
+            x0[h] = x1[h] = make_uint4(0u, 0u, 0u, 0u);
+          uint4 hi, lo;
+          split_query(x0[h], x1[h], inv, hi, lo);
+          uint8_t* dst = q_smem + r * kD + (((tid & 7) ^ (r & 7)) << 4);
+          *reinterpret_cast<uint4*>(dst) = hi;
+          *reinterpret_cast<uint4*>(dst + kQBytes) = lo;
+          if ((tid & 7) == 0) {
+            RowInfo v = {};
+            v.out = t[h] < part.rows ? (part.row0 + t[h] / group) * a.H + head[h] : -1;
+            v.fix = at[h] < 0 ? 0.f : finite[h] ? 1.f : __uint_as_float(0x7fc00000u);
+            if (!PLAIN && at[h] >= 0) {
+              v.pos = __ldg(a.cu_k + part.b + 1) - __ldg(a.cu_k + part.b) - (__ldg(a.cu_q + part.b + 1) - at[h]);
+              v.slope = a.slopes ? __ldg(a.slopes + head[h]) * kLog2e : 0.f;
+              v.hi = part.len;
+              if (a.ranges) {
+                const int2 range = __ldg(a.ranges + at[h]);
+                v.lo = range.x;
+                v.hi = min(range.y, part.len);
+              }
+            }
+            s_row[r] = v;
+            s_ref[r] = kNothing;
+          }
+        }
+        fence_proxy_async_smem();
+        warp_arrive(&q_full);
+        rows_sync();
+      }
+      const float key_mul = a.scale * (PLAIN ? kLog2e : 1.f) * q_scale, to_cap = a.cap > 0.f ? 2.f * kLog2e / a.cap : 0.f;
+      const int tiles = (end - begin + kUnitKeys - 1) / kUnitKeys;
+      float l = 0.f;                               // lane = row: sum of the weights of this quarter's keys
+      for (int i = 0; i < tiles; ++i, ++u) {
+        const int at = begin + i * kUnitKeys + kl, buf = u & 1;
+        const float kk = ks_next * key_mul, ex = value_exponent(vs_next);
+        if (at + kUnitKeys < end) {
+          ks_next = __ldg(k_scale + static_cast<int64_t>(at + kUnitKeys) * a.Hkv);
+          vs_next = __ldg(v_scale + static_cast<int64_t>(at + kUnitKeys) * a.Hkv);
+        }
+        mbar_wait(&s_full[buf], (u >> 1) & 1, &abort_flag, p.status_word, 409);
+        tc_fence_after_sync();
+        uint32_t s[kRows];
+        float* t = reinterpret_cast<float*>(s);
+        tmem_ld_32x32(t_s + buf * kRows, s);
+        tmem_ld_wait();
+        // scores (times log2 e, plus the exponents of the values' scales)
+        if (PLAIN) {
+#pragma unroll
+          for (int r = 0; r < kRows; r += 2)
+            put2(t + r, ffma2(get2(t + r), make_float2(kk, kk), make_float2(ex, ex)));
+          if (at >= end) {
+#pragma unroll
+            for (int r = 0; r < kRows; ++r)
+              t[r] = -INFINITY;
+          }
+        } else {
+          if (a.cap > 0.f) {
+#pragma unroll
+            for (int r = 0; r < kRows; ++r)
+              t[r] = capped(t[r] * kk * to_cap, a.cap);
+          } else {
+#pragma unroll
+            for (int r = 0; r < kRows; ++r)
+              t[r] *= kk;
+          }
+#pragma unroll
+          for (int r = 0; r < kRows; ++r) {
+            const RowInfo& row = s_row[r];
+            t[r] = fmaf(t[r], kLog2e, ex) - row.slope * static_cast<float>(abs(row.pos - at));
+            t[r] = at >= row.lo && at < row.hi && at < end ? t[r] : -INFINITY;
+          }
+        }
+        // does any lie above its reference by more than the weights' codes can take?
+        float above = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < kRows; r += 4) {
+          const float4 ref = *reinterpret_cast<const float4*>(s_ref + r);
+          above = fmax3(above, t[r] - ref.x, t[r + 1] - ref.y);
+          above = fmax3(above, t[r + 2] - ref.z, t[r + 3] - ref.w);
+        }
+        if (rows_any(above > kHeadroom)) {
+          float mx = 0.f;
+#pragma unroll
+          for (int r = 0; r < kRows; ++r) {
+            const float m = warp_max(t[r]);
+            mx = lane == r ? m : mx;
+          }
+          s_max[quarter][lane] = mx;
+          rows_sync();
+          const float was = s_ref[lane];
+          mx = fmaxf(fmaxf(s_max[0][lane], s_max[1][lane]), fmaxf(s_max[2][lane], s_max[3][lane]));
+          const float ref = mx > was + kHeadroom ? mx : was, old = exp2f(was - ref);
+          l *= old;
+          rows_sync();
+          if (quarter == 0) {
+            s_ref[lane] = ref;
+            s_old[lane] = old;
+          }
+          rows_sync();
+          if (i > 0) {
+            mbar_wait(&pv_done, (u - 1) & 1, &abort_flag, p.status_word, 410);
+            tc_fence_after_sync();
+#pragma unroll 1
+            for (int c = 0; c < kRows; c += 8) {
+              uint32_t o[8];
+              tmem_ld_32x8(t_o + c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int r = 0; r < 8; ++r)
+                o[r] = __float_as_uint(__uint_as_float(o[r]) * s_old[c + r]);
+              tmem_st_32x8(t_o + c, o);
+            }
+            tmem_st_wait();
+          }
+        }
+        // weights
+        if (u > 0)
+          mbar_wait(&pv_done, (u - 1) & 1, &abort_flag, p.status_word, 411);      // the last ones have been taken
+        uint8_t* dst = p_smem + kl * 64;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int r = 16 * h + 4 * j;
+            const float4 ref = *reinterpret_cast<const float4*>(s_ref + r);
+            t[r] = exp2f(t[r] - ref.x + kWeightLog2);
+            t[r + 1] = exp2f(t[r + 1] - ref.y + kWeightLog2);
+            t[r + 2] = exp2f(t[r + 2] - ref.z + kWeightLog2);
+            t[r + 3] = exp2f(t[r + 3] - ref.w + kWeightLog2);
+            split_weights_e5m2(make_float2(t[r], t[r + 1]), make_float2(t[r + 2], t[r + 3]), hi[j], lo[j]);
+          }
+          *reinterpret_cast<uint4*>(dst + ((h ^ (kl >> 1 & 3)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(dst + (((2 + h) ^ (kl >> 1 & 3)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+        if (at - kl + kUnitKeys > end) {
+          // rows of V behind the last key may hold any byte, a NaN times a weight of zero among them
+          const int use = n_ring + 2 * i + 1;      // the part's last tile in the ring
+          mbar_wait(&full[use % kFewRing], (use / kFewRing) & 1, &abort_flag, p.status_word, 412);
+          if (at >= end) {
+            uint4* v = reinterpret_cast<uint4*>(ring + (use % kFewRing) * kTileBytes + kl * kD);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              v[j] = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+        tc_fence_before_sync();
+        fence_proxy_async_smem();
+        warp_arrive(&p_full);
+        // the weight of a NaN is a NaN where its key is seen, else zero
+        const float inv = ex == ex ? exp2f(-ex) : 1.f;
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+          t[r] *= inv;
+        float (&w)[kRows] = *reinterpret_cast<float (*)[kRows]>(s);
+        l += sum_lanes(w);
+      }
+      n_ring += 2 * tiles;
+
+      // ---------------------------------------------------------------- thread = head dimension kl of all rows
+      s_max[quarter][lane] = l;
+      const RowInfo me = s_row[lane];
+      float top = s_ref[lane];
+      mbar_wait(&pv_done, (u - 1) & 1, &abort_flag, p.status_word, 413);
+      tc_fence_after_sync();
+      uint32_t ou[kRows];
+      float* o = reinterpret_cast<float*>(ou);
+      tmem_ld_32x32(t_o, ou);
+      tmem_ld_wait();
+      tc_fence_before_sync();
+      warp_arrive(&o_free);
+      rows_sync();
+      l = (s_max[0][lane] + s_max[1][lane]) + (s_max[2][lane] + s_max[3][lane]);
+      bool store = true;
+      if (part.parts > 1) {
+        float* mine = p.parts + static_cast<int64_t>(part.slot) * kFewPart;
+#pragma unroll
+        for (int r = 0; r < kRows; r += 4)
+          *reinterpret_cast<float4*>(mine + kl * kRows + r) = make_float4(o[r], o[r + 1], o[r + 2], o[r + 3]);
+        if (quarter == 0) {
+          mine[kRows * kD + lane] = top;
+          mine[kRows * kD + kRows + lane] = l;
+        }
+        __threadfence();
+        rows_sync();
+        if (tid == 0) {
+          open_join(p.tickets + part.owner, p.launch_id);
+          joins = last_to_join(p.tickets + part.owner, part.parts) ? 1 : 0;
+        }
+        rows_sync();
+        store = joins != 0;
+        if (store) {
+          __threadfence();
+          const float* first = p.parts + (2 * static_cast<int64_t>(part.owner) + 1) * kFewPart;
+          const float* rest = p.parts + 2 * static_cast<int64_t>(part.owner) * kFewPart;
+          top = kNothing;
+          l = 0.f;
+#pragma unroll
+          for (int r = 0; r < kRows; ++r)
+            o[r] = 0.f;
+          for (int i = 0; i < part.parts; ++i)
+            top = fmaxf(top, __ldcg((i == 0 ? first : rest + 2 * static_cast<int64_t>(i) * kFewPart) + kRows * kD + lane));
+          for (int i = 0; i < part.parts; ++i) {
+            const float* src = i == 0 ? first : rest + 2 * static_cast<int64_t>(i) * kFewPart;
+            const float f = exp2f(__ldcg(src + kRows * kD + lane) - top);
+            l = fmaf(__ldcg(src + kRows * kD + kRows + lane), f, l);
+#pragma unroll
+            for (int r = 0; r < kRows; r += 4) {
+              const float4 v = __ldcg(reinterpret_cast<const float4*>(src + kl * kRows + r));
+              o[r] = fmaf(v.x, __shfl_sync(0xffffffffu, f, r), o[r]);
+              o[r + 1] = fmaf(v.y, __shfl_sync(0xffffffffu, f, r + 1), o[r + 1]);
+              o[r + 2] = fmaf(v.z, __shfl_sync(0xffffffffu, f, r + 2), o[r + 2]);
+              o[r + 3] = fmaf(v.w, __shfl_sync(0xffffffffu, f, r + 3), o[r + 3]);
+            }
+          }
+        }
+      }
+      if (store) {
+        const float mul = l == 0.f || me.fix == 0.f ? 0.f : __fdividef(me.fix, l);
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+          const int out = __shfl_sync(0xffffffffu, me.out, r);
+          const float m = __shfl_sync(0xffffffffu, mul, r);
+          if (out >= 0)
+            a.out[static_cast<int64_t>(out) * kD + kl] = __float2bfloat16_rn(m == 0.f ? 0.f : o[r] * m);
+        }
+      }
+      rows_sync();      // nobody overwrites what describes the rows while another warp reads it
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, kFewTmemCols);
+  }
+}
+
+// ----------------------------------------------------------------------------------------------
+// Many rows per sequence: bound by the exponentials and the instructions around them (a tile of 128 rows x 128 keys takes the
+// tensor cores 950 cycles, its exponentials 1024).
+//
+// Tiles of 128 (listed row, query head) pairs, rows in the M = 128 of the products:
+//   S = Q K^T    A: the queries as e4m3 + e5m2 (two products into one accumulator), B: the K tile as loaded (K-major)
+//   O = P V      A: the weights as e4m3 + e5m2, B: the V tile as loaded (MN-major)
+// Thread = row in four softmax warps.  A weight is 64 * 2^(t - reference); the reference follows the maximum in steps, so that the
+// sums are rescaled only where a score lies more than 2.8 (log2) above it.  A weight is off by 2^-7 of itself or by 2^-23 of the
+// largest.  Scores and weights share 128 columns of tensor memory (32 keys' weights, e4m3 then e5m2, lie in the first 16 of their
+// scores' 32 columns), so the steps of one tile follow one another; two CTAs per SM, each with parts of its own, fill each other's
+// waits, the ends of parts among them.  Four loader warps stage the queries of the next part and the scales of the next tiles.
+// ----------------------------------------------------------------------------------------------
+constexpr int kManyRows = 128;
+constexpr int kManyRing = 4;                                 // slots of one K or V tile
+constexpr int kScaleSlots = 2;                               // tiles whose scales are staged ahead
+constexpr int kManyWarps = 4, kManyThreads = 32 * (3 + kManyWarps + 4);
+constexpr int kManyCtas = 2;                                 // per SM
+constexpr uint32_t kManyTmemCols = 256;
+constexpr uint32_t kStageBytes = 32 * 64;                    // of a softmax warp: 32 head dimensions of its rows
+constexpr uint32_t kManyQBytes = kManyRows * kD;             // e4m3 or e5m2 part of the queries of a tile
+constexpr uint32_t kManySmem = kManyRing * kTileBytes + 2 * kManyQBytes + kManyWarps * kStageBytes +
+                               kScaleSlots * 3 * kUnitKeys * sizeof(float) + 1024;
 
 // A part in the workspace: [dimension][row] sums, [row] references, sums of weights; of a first part also output rows and `fix`.
 constexpr int kManyPart = kManyRows * (kD + 4);
@@ -1283,7 +1122,7 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       __syncwarp();
       ++n;
     };
-    Chunks c = {};
+    PartWalk c = {};
     for (bool more = c.open(part_full, part_done, s_part, &abort_flag, p.status_word); more;) {
       for (int key = c.begin; key < c.end; key += kUnitKeys) {
         load(&tmap_k, c.k0 + key, c.end - key, c.hk * kD);
@@ -1301,7 +1140,7 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     constexpr uint32_t idesc_pv = umma_idesc_f8(128, 128, 0, 0, 0, 1), idesc_pv_lo = umma_idesc_f8(128, 128, 1, 0, 0, 1);
     const uint32_t ring_addr = smem_u32(ring), q_addr = smem_u32(q_smem), t_s = uniform(tmem), t_o = t_s + 128;
     int g = 0, live = 0;      // tiles, parts that have some
-    Chunks c = {};
+    PartWalk c = {};
     for (bool more = c.open(part_full, part_done, s_part, &abort_flag, p.status_word); more;) {
       if (c.tiles)
         mbar_wait(&q_full, live & 1, &abort_flag, p.status_word, 503);
@@ -1350,10 +1189,10 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     int n_sc = 0, live = 0;
     for (int n = 0;; ++n) {
       const int slot = n % kParts, qb = live & 1;
-      if (!mbar_wait(&part_full[slot], (n / kParts) & 1, &abort_flag, p.status_word, 510))
+      if (rows_any(!mbar_wait(&part_full[slot], (n / kParts) & 1, &abort_flag, p.status_word, 510)))
         break;
       const PartInfo w = s_part[slot];
-      loaders_sync();
+      rows_sync();
       warp_arrive(&part_done[slot]);
       if (w.end < 0)
         break;
@@ -1380,12 +1219,12 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       }
       if (w.end == w.begin) {      // no keys: zeros
         s_src[tid] = v.out;
-        loaders_sync();
+        rows_sync();
 #pragma unroll 1
         for (int r = tid >> 4; r < kManyRows; r += 8)
           if (s_src[r] >= 0)
             *reinterpret_cast<uint4*>(a.out + s_src[r] * kD + (tid & 15) * 8) = make_uint4(0u, 0u, 0u, 0u);
-        loaders_sync();
+        rows_sync();
         continue;
       }
       s_src[tid] = src;
@@ -1393,7 +1232,7 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         s_amax[qb] = 0;
       if (tid < 4)
         s_bad[tid] = 0;
-      loaders_sync();
+      rows_sync();
       // queries: eight threads a row, 16 rows at a time, four times 16 in flight; first the largest element, then (from L1) the
       // codes.  (Loops: straight-line code for 128 rows that runs once a part costs more in instruction fetches than it saves.)
       uint4 x0[4], x1[4];
@@ -1426,7 +1265,7 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       top = __reduce_max_sync(0xffffffffu, top);
       if (lane == 0)
         atomicMax(&s_amax[qb], top);
-      loaders_sync();
+      rows_sync();
       const uint32_t scale = fp8_scale_bits(s_amax[qb]);
       const float inv = fp8_inverse(scale);
       if (live > 0)
@@ -1450,7 +1289,7 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         v.fix = __uint_as_float(0x7fc00000u);
       s_row[tid] = v;
       fence_proxy_async_smem();
-      loaders_sync();
+      rows_sync();
       warp_arrive(&q_full);
       ++live;
       // scales: thread = key, four tiles' loads at a time
@@ -1792,11 +1631,12 @@ __global__ void __launch_bounds__(128) fp8_spans_kernel(const Fp8AttnParams p, i
 constexpr int kFewMost = 64;
 
 // Workspace: tickets, keys per tile (only with ranges), parts of tiles; for the kernel that needs most.
+constexpr int kMostCtas = kFewCtas > kManyCtas ? kFewCtas : kManyCtas;
 int64_t most_tiles(int num_salient, int batch, int group) { return static_cast<int64_t>(num_salient) * group / kRows + batch; }
 size_t parts_offset(int64_t tiles, int ctas) { return (ctas * sizeof(unsigned long long) + tiles * sizeof(int2) + 255) / 256 * 256; }
 size_t workspace_of(int num_salient, int batch, int group, int ctas) {
-  const size_t few = 2ull * ctas * kRows * (kD + 2), many = 2ull * kManyCtas * ctas * kManyPart;
-  return parts_offset(most_tiles(num_salient, batch, group), kManyCtas * ctas) +
+  const size_t few = 2ull * kFewCtas * ctas * kFewPart, many = 2ull * kManyCtas * ctas * kManyPart;
+  return parts_offset(most_tiles(num_salient, batch, group), kMostCtas * ctas) +
          (static_cast<int64_t>(num_salient) * group > kFewMost ? max(few, many) : few) * sizeof(float);
 }
 
@@ -1818,7 +1658,7 @@ int launch_rows(Kernel kernel, bool (&set)[64], int threads, uint32_t smem, cons
 template <bool PLAIN>
 int launch_few(const CUtensorMap& tk, const CUtensorMap& tv, const FewParams& p, int ctas, cudaStream_t s) {
   static bool set[64] = {};
-  return launch_rows(fp8_few_rows_kernel<PLAIN>, set, kFewThreads, kFewSmem, tk, tv, p, ctas, s);
+  return launch_rows(fp8_few_rows_kernel<PLAIN>, set, kFewThreads, kFewSmem, tk, tv, p, kFewCtas * ctas, s);
 }
 template <bool CAP, bool BIAS>
 int launch_many(const CUtensorMap& tk, const CUtensorMap& tv, const FewParams& p, int ctas, cudaStream_t s) {
@@ -1917,8 +1757,8 @@ int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, co
   f.a = p;
   f.tickets = reinterpret_cast<unsigned long long*>(ws);      // few rows
   f.joins = reinterpret_cast<int*>(ws);                       // many rows
-  int2* spans = reinterpret_cast<int2*>(ws + kManyCtas * ctas * sizeof(unsigned long long));
-  f.parts = reinterpret_cast<float*>(ws + parts_offset(tiles, kManyCtas * ctas));
+  int2* spans = reinterpret_cast<int2*>(ws + kMostCtas * ctas * sizeof(unsigned long long));
+  f.parts = reinterpret_cast<float*>(ws + parts_offset(tiles, kMostCtas * ctas));
   f.launch_id = next_launch_id() & ~0xffffull;
   f.status_word = device_status_word();
   // a sequence with more rows than the bound says is served by either kernel; so is one with few beside others with many
