@@ -771,7 +771,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
               }
             }
             s_row[r] = v;
-            s_ref[r] = kNothing;
+            s_ref[r] = kNothing;      // less kWeightLog2, as all that follow
           }
         }
         fence_proxy_async_smem();
@@ -829,7 +829,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
           above = fmax3(above, t[r] - ref.x, t[r + 1] - ref.y);
           above = fmax3(above, t[r + 2] - ref.z, t[r + 3] - ref.w);
         }
-        if (rows_any(above > kHeadroom)) {
+        if (rows_any(above > kHeadroom + kWeightLog2)) {
           float mx = 0.f;
 #pragma unroll
           for (int r = 0; r < kRows; ++r) {
@@ -840,7 +840,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
           rows_sync();
           const float was = s_ref[lane];
           mx = fmaxf(fmaxf(s_max[0][lane], s_max[1][lane]), fmaxf(s_max[2][lane], s_max[3][lane]));
-          const float ref = mx > was + kHeadroom ? mx : was, old = exp2f(was - ref);
+          const float ref = mx > was + (kHeadroom + kWeightLog2) ? mx - kWeightLog2 : was, old = exp2f(was - ref);
           l *= old;
           rows_sync();
           if (quarter == 0) {
@@ -875,10 +875,10 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
           for (int j = 0; j < 4; ++j) {
             const int r = 16 * h + 4 * j;
             const float4 ref = *reinterpret_cast<const float4*>(s_ref + r);
-            t[r] = exp2f(t[r] - ref.x + kWeightLog2);
-            t[r + 1] = exp2f(t[r + 1] - ref.y + kWeightLog2);
-            t[r + 2] = exp2f(t[r + 2] - ref.z + kWeightLog2);
-            t[r + 3] = exp2f(t[r + 3] - ref.w + kWeightLog2);
+            t[r] = exp2f(t[r] - ref.x);
+            t[r + 1] = exp2f(t[r + 1] - ref.y);
+            t[r + 2] = exp2f(t[r + 2] - ref.z);
+            t[r + 3] = exp2f(t[r + 3] - ref.w);
             split_weights_e5m2(make_float2(t[r], t[r + 1]), make_float2(t[r + 2], t[r + 3]), hi[j], lo[j]);
           }
           *reinterpret_cast<uint4*>(dst + ((h ^ (kl >> 1 & 3)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
@@ -967,16 +967,30 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
         }
       }
       if (store) {
-        const float mul = l == 0.f || me.fix == 0.f ? 0.f : __fdividef(me.fix, l);
+        // by way of shared memory, where weights and queries were: 16 threads store the 256 bytes of a row
+        float* lines = reinterpret_cast<float*>(p_smem);
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) {
-          const int out = __shfl_sync(0xffffffffu, me.out, r);
-          const float m = __shfl_sync(0xffffffffu, mul, r);
-          if (out >= 0)
-            a.out[static_cast<int64_t>(out) * kD + kl] = __float2bfloat16_rn(m == 0.f ? 0.f : o[r] * m);
+        for (int r = 0; r < kRows; ++r)
+          lines[r * kD + kl] = o[r];
+        if (quarter == 0)
+          s_old[lane] = l == 0.f || me.fix == 0.f ? 0.f : __fdividef(me.fix, l);
+        rows_sync();
+#pragma unroll
+        for (int r = tid >> 4; r < kRows; r += 8) {
+          const int out = s_row[r].out;
+          const float mul = s_old[r];
+          if (out >= 0) {
+            float x[8];
+            *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(lines + r * kD + (tid & 15) * 8);
+            *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(lines + r * kD + (tid & 15) * 8 + 4);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              x[e] = mul == 0.f ? 0.f : x[e] * mul;
+            *reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(out) * kD + (tid & 15) * 8) = float_to_bf16x8(x);
+          }
         }
       }
-      rows_sync();      // nobody overwrites what describes the rows while another warp reads it
+      rows_sync();      // nobody overwrites the rows or what describes them while another warp reads it
     }
   }
 
