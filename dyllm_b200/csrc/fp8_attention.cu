@@ -493,8 +493,9 @@ __device__ __forceinline__ void split_weights_e5m2(float2 a, float2 b, uint32_t&
 //
 // Four softmax warps, thread = key with the scores of all rows in registers; a row's reference is in shared memory and follows the
 // maximum in steps, so that a unit costs one barrier (does any score exceed its reference by more than 2.8?) and the maxima are
-// looked for only where one does.  Three CTAs per SM, each with parts of its own, fill each other's waits: 16 x 512 keys, 32
-// heads, 26 rows take 43 us with one CTA of sixteen softmax warps.
+// looked for only where one does.  A part of four units takes 14 us from its description to its result, nearly all of it waits
+// along that chain, so four CTAs per SM with parts of their own take turns: 16 x 512 keys, 32 heads, 26 rows take 30 us (2.5 TB/s
+// of the cache); 41 us with three CTAs, where 68 of 512 tiles wait for a second turn; 43 us with one CTA of sixteen softmax warps.
 // ----------------------------------------------------------------------------------------------
 constexpr int kFewRing = 2;                                  // slots of one K or V tile
 constexpr int kFewCtas = 4;                                  // per SM
@@ -520,7 +521,8 @@ __device__ __forceinline__ float sum_lanes(float (&v)[32]) {
   return v[0];
 }
 
-template <bool PLAIN>
+// CAP, BIAS: scores capped by a tanh, biased by their distance.
+template <bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kFewThreads, kFewCtas)
 fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const FewParams p) {
   pdl_wait();      // programmatic dependent launch: nothing before this reads an earlier kernel's data
@@ -534,8 +536,10 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
   __shared__ PartInfo s_part[kParts];
   __shared__ uint32_t tmem_slot, s_top[kFewWarps];
   __shared__ int abort_flag, joins;
-  __shared__ RowInfo s_row[kRows];
-  __shared__ __align__(16) float s_max[kFewWarps][kRows], s_ref[kRows], s_old[kRows];
+  __shared__ int s_out[kRows];                               // output row, -1: none
+  __shared__ int2 s_sees[kRows], s_all[kFewWarps];           // keys that a row sees, that all rows see (of a quarter of them)
+  __shared__ __align__(16) float2 s_bias[kRows];             // slope times log2(e), place in the sequence counted from the part's first key
+  __shared__ __align__(16) float s_fix[kRows], s_max[kFewWarps][kRows], s_ref[kRows], s_old[kRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -746,6 +750,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
         const uint32_t scale = fp8_scale_bits(max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3])));
         const float inv = fp8_inverse(scale);
         q_scale = __uint_as_float(scale);
+        int2 sees = make_int2(0, end);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int r = 16 * h + (tid >> 3);
@@ -757,33 +762,43 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
           *reinterpret_cast<uint4*>(dst) = hi;
           *reinterpret_cast<uint4*>(dst + kQBytes) = lo;
           if ((tid & 7) == 0) {
-            RowInfo v = {};
-            v.out = t[h] < part.rows ? (part.row0 + t[h] / group) * a.H + head[h] : -1;
-            v.fix = at[h] < 0 ? 0.f : finite[h] ? 1.f : __uint_as_float(0x7fc00000u);
-            if (!PLAIN && at[h] >= 0) {
-              v.pos = __ldg(a.cu_k + part.b + 1) - __ldg(a.cu_k + part.b) - (__ldg(a.cu_q + part.b + 1) - at[h]);
-              v.slope = a.slopes ? __ldg(a.slopes + head[h]) * kLog2e : 0.f;
-              v.hi = part.len;
-              if (a.ranges) {
-                const int2 range = __ldg(a.ranges + at[h]);
-                v.lo = range.x;
-                v.hi = min(range.y, part.len);
-              }
-            }
-            s_row[r] = v;
+            s_out[r] = t[h] < part.rows ? (part.row0 + t[h] / group) * a.H + head[h] : -1;
+            // 1; 0: the row does not exist in q; NaN: the query is not finite
+            s_fix[r] = at[h] < 0 ? 0.f : finite[h] ? 1.f : __uint_as_float(0x7fc00000u);
             s_ref[r] = kNothing;      // less kWeightLog2, as all that follow
+            if (BIAS && at[h] >= 0) {
+              const int pos = __ldg(a.cu_k + part.b + 1) - __ldg(a.cu_k + part.b) - (__ldg(a.cu_q + part.b + 1) - at[h]);
+              s_bias[r] = make_float2(__ldg(a.slopes + head[h]) * kLog2e, static_cast<float>(pos - begin));
+            } else {
+              s_bias[r] = make_float2(0.f, 0.f);
+            }
+            if (a.ranges && at[h] >= 0) {
+              const int2 range = __ldg(a.ranges + at[h]);
+              s_sees[r] = make_int2(range.x, min(range.y, end));
+              sees.x = max(sees.x, range.x);
+              sees.y = min(sees.y, range.y);
+            } else {
+              s_sees[r] = make_int2(0, end);
+            }
           }
         }
+        sees.x = __reduce_max_sync(0xffffffffu, sees.x);
+        sees.y = __reduce_min_sync(0xffffffffu, sees.y);
+        if (lane == 0)
+          s_all[quarter] = sees;
         fence_proxy_async_smem();
         warp_arrive(&q_full);
         rows_sync();
       }
-      const float key_mul = a.scale * (PLAIN ? kLog2e : 1.f) * q_scale, to_cap = a.cap > 0.f ? 2.f * kLog2e / a.cap : 0.f;
+      // scores come out times log2(e), or as twice the argument of the tanh that caps them
+      const float key_mul = a.scale * q_scale * kLog2e * (CAP ? 2.f / a.cap : 1.f);
+      const int all_from = max(max(s_all[0].x, s_all[1].x), max(s_all[2].x, s_all[3].x));
+      const int all_to = min(min(s_all[0].y, s_all[1].y), min(s_all[2].y, s_all[3].y));
       const int tiles = (end - begin + kUnitKeys - 1) / kUnitKeys;
       float l = 0.f;                               // lane = row: sum of the weights of this quarter's keys
       for (int i = 0; i < tiles; ++i, ++u) {
         const int at = begin + i * kUnitKeys + kl, buf = u & 1;
-        const float kk = ks_next * key_mul, ex = value_exponent(vs_next);
+        const float kk = ks_next * key_mul, ex = value_exponent(vs_next), place = static_cast<float>(at - begin);
         if (at + kUnitKeys < end) {
           ks_next = __ldg(k_scale + static_cast<int64_t>(at + kUnitKeys) * a.Hkv);
           vs_next = __ldg(v_scale + static_cast<int64_t>(at + kUnitKeys) * a.Hkv);
@@ -795,30 +810,25 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
         tmem_ld_32x32(t_s + buf * kRows, s);
         tmem_ld_wait();
         // scores (times log2 e, plus the exponents of the values' scales)
-        if (PLAIN) {
 #pragma unroll
-          for (int r = 0; r < kRows; r += 2)
-            put2(t + r, ffma2(get2(t + r), make_float2(kk, kk), make_float2(ex, ex)));
-          if (at >= end) {
-#pragma unroll
-            for (int r = 0; r < kRows; ++r)
-              t[r] = -INFINITY;
-          }
-        } else {
-          if (a.cap > 0.f) {
-#pragma unroll
-            for (int r = 0; r < kRows; ++r)
-              t[r] = capped(t[r] * kk * to_cap, a.cap);
+        for (int r = 0; r < kRows; r += 2) {
+          if (CAP) {
+            t[r] = fmaf(capped(t[r] * kk, a.cap), kLog2e, ex);
+            t[r + 1] = fmaf(capped(t[r + 1] * kk, a.cap), kLog2e, ex);
           } else {
-#pragma unroll
-            for (int r = 0; r < kRows; ++r)
-              t[r] *= kk;
+            put2(t + r, ffma2(get2(t + r), make_float2(kk, kk), make_float2(ex, ex)));
           }
+          if (BIAS) {
+            const float4 row = *reinterpret_cast<const float4*>(s_bias + r);
+            t[r] = fmaf(-row.x, fabsf(row.y - place), t[r]);
+            t[r + 1] = fmaf(-row.z, fabsf(row.w - place), t[r + 1]);
+          }
+        }
+        if (at - kl < all_from || at - kl + kUnitKeys > all_to) {      // not all rows see all keys
 #pragma unroll
           for (int r = 0; r < kRows; ++r) {
-            const RowInfo& row = s_row[r];
-            t[r] = fmaf(t[r], kLog2e, ex) - row.slope * static_cast<float>(abs(row.pos - at));
-            t[r] = at >= row.lo && at < row.hi && at < end ? t[r] : -INFINITY;
+            const int2 sees = s_sees[r];
+            t[r] = at >= sees.x && at < sees.y ? t[r] : -INFINITY;
           }
         }
         // does any lie above its reference by more than the weights' codes can take?
@@ -910,7 +920,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
 
       // ---------------------------------------------------------------- thread = head dimension kl of all rows
       s_max[quarter][lane] = l;
-      const RowInfo me = s_row[lane];
+      const float fix = s_fix[lane];
       float top = s_ref[lane];
       mbar_wait(&pv_done, (u - 1) & 1, &abort_flag, p.status_word, 413);
       tc_fence_after_sync();
@@ -973,11 +983,11 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
         for (int r = 0; r < kRows; ++r)
           lines[r * kD + kl] = o[r];
         if (quarter == 0)
-          s_old[lane] = l == 0.f || me.fix == 0.f ? 0.f : __fdividef(me.fix, l);
+          s_old[lane] = l == 0.f || fix == 0.f ? 0.f : __fdividef(fix, l);
         rows_sync();
 #pragma unroll
         for (int r = tid >> 4; r < kRows; r += 8) {
-          const int out = s_row[r].out;
+          const int out = s_out[r];
           const float mul = s_old[r];
           if (out >= 0) {
             float x[8];
@@ -1003,8 +1013,10 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
 }
 
 // ----------------------------------------------------------------------------------------------
-// Many rows per sequence: bound by the exponentials and the instructions around them (a tile of 128 rows x 128 keys takes the
-// tensor cores 950 cycles, its exponentials 1024).
+// Many rows per sequence: bound by the instructions around the exponentials.  A unit of 128 rows x 128 keys takes the tensor cores
+// 1000 cycles, its exponentials 1024, the scales of its keys (three words a key for each of four warps) 1536 of shared memory; with
+// all else it takes an SM 4800 (2 x 32011 keys, 128 pairs a key head: 105 us, of which 9 for lists and queries, 8 for the join).
+// Without the reads of the scales it would take 93 us, without the scores' pass 89, without the weights' pass 90.
 //
 // Tiles of 128 (listed row, query head) pairs, rows in the M = 128 of the products:
 //   S = Q K^T    A: the queries as e4m3 + e5m2 (two products into one accumulator), B: the K tile as loaded (K-major)
@@ -1639,9 +1651,9 @@ __global__ void __launch_bounds__(128) fp8_spans_kernel(const Fp8AttnParams p, i
     spans[before] = lo < hi ? make_int2(lo, hi) : make_int2(0, 0);
 }
 
-// Up to this many (listed row, query head) pairs a sequence and key head the few-rows kernel is the faster one, with a pass over
-// the keys for each 32 of them: 26 rows (16 x 512 keys, 32 heads) 43 us against 63; 64 rows (8 x 4096 keys, 16 heads, capped) 125
-// against 139; 128 rows (2 x 32011 keys, 8 key heads) 161 against 105.
+// Up to this many (listed row, query head) pairs a sequence and key head the few-rows kernel is taken, with a pass over the keys for
+// each 32 of them.  Few against many, us: 26 pairs (16 x 512 keys, 32 heads) 30 : 63; 64 pairs there 52 : 68, capped over 8 x 4096
+// keys 90 : 139, but over 2 x 32011 keys 129 : 102; 96 pairs, 2 x 1001 keys 25 : 27, 2 x 4001 51 : 37, 2 x 32011 148 : 104.
 constexpr int kFewMost = 64;
 
 // Workspace: tickets, keys per tile (only with ranges), parts of tiles; for the kernel that needs most.
@@ -1669,10 +1681,10 @@ int launch_rows(Kernel kernel, bool (&set)[64], int threads, uint32_t smem, cons
   DYLLM_LAUNCH(kernel, ctas, threads, smem, s, tk, tv, p);
   return check_launch("attention_salient_rows_fp8");
 }
-template <bool PLAIN>
+template <bool CAP, bool BIAS>
 int launch_few(const CUtensorMap& tk, const CUtensorMap& tv, const FewParams& p, int ctas, cudaStream_t s) {
   static bool set[64] = {};
-  return launch_rows(fp8_few_rows_kernel<PLAIN>, set, kFewThreads, kFewSmem, tk, tv, p, kFewCtas * ctas, s);
+  return launch_rows(fp8_few_rows_kernel<CAP, BIAS>, set, kFewThreads, kFewSmem, tk, tv, p, kFewCtas * ctas, s);
 }
 template <bool CAP, bool BIAS>
 int launch_many(const CUtensorMap& tk, const CUtensorMap& tv, const FewParams& p, int ctas, cudaStream_t s) {
@@ -1792,13 +1804,14 @@ int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, co
     rc = encode_tmap_2d_u8(&tv, v_codes, v_rows ? v_rows : 1, width, width, 32, kD);
   if (rc != DYLLM_OK)
     return rc;
-  if (many) {
-    if (softcap > 0.f)
-      return slopes ? launch_many<true, true>(tk, tv, f, ctas, st) : launch_many<true, false>(tk, tv, f, ctas, st);
-    return slopes ? launch_many<false, true>(tk, tv, f, ctas, st) : launch_many<false, false>(tk, tv, f, ctas, st);
+  if (softcap > 0.f) {
+    if (slopes)
+      return many ? launch_many<true, true>(tk, tv, f, ctas, st) : launch_few<true, true>(tk, tv, f, ctas, st);
+    return many ? launch_many<true, false>(tk, tv, f, ctas, st) : launch_few<true, false>(tk, tv, f, ctas, st);
   }
-  const bool plain = softcap == 0.f && !slopes && !key_ranges;
-  return plain ? launch_few<true>(tk, tv, f, ctas, st) : launch_few<false>(tk, tv, f, ctas, st);
+  if (slopes)
+    return many ? launch_many<false, true>(tk, tv, f, ctas, st) : launch_few<false, true>(tk, tv, f, ctas, st);
+  return many ? launch_many<false, false>(tk, tv, f, ctas, st) : launch_few<false, false>(tk, tv, f, ctas, st);
 }
 
 }  // extern "C"
