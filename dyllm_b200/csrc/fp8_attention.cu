@@ -532,14 +532,14 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* p_smem = ring + kFewRing * kTileBytes;            // [128 keys][32 e4m3, 32 e5m2], 64-byte swizzle
   uint8_t* q_smem = p_smem + kPBytes;                        // [32 rows][128] e4m3, then e5m2
-  __shared__ uint64_t full[kFewRing], empty[kFewRing], part_full[kParts], part_done[kParts], q_full, s_full[2], p_full, pv_done, o_free;
+  __shared__ uint64_t full[kFewRing], empty[kFewRing], part_full[kParts], part_done[kParts], q_asked, q_full, s_full[2], p_full, pv_done, o_free;
   __shared__ PartInfo s_part[kParts];
   __shared__ uint32_t tmem_slot, s_top[kFewWarps];
   __shared__ int abort_flag, joins;
   __shared__ int s_out[kRows];                               // output row, -1: none
   __shared__ int2 s_sees[kRows], s_all[kFewWarps];           // keys that a row sees, that all rows see (of a quarter of them)
   __shared__ __align__(16) float2 s_bias[kRows];             // slope times log2(e), place in the sequence counted from the part's first key
-  __shared__ __align__(16) float s_fix[kRows], s_max[kFewWarps][kRows], s_ref[kRows], s_old[kRows];
+  __shared__ __align__(16) float s_fix[kRows], s_max[kFewWarps][kRows], s_sum[kFewWarps][kRows], s_ref[kFewWarps][kRows], s_old[kFewWarps][kRows];      // a copy for each warp
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -555,6 +555,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
     mbar_init(&s_full[1], 1);
     mbar_init(&p_full, kFewWarps);
     mbar_init(&pv_done, 1);
+    mbar_init(&q_asked, kFewWarps);
     mbar_init(&q_full, kFewWarps);
     mbar_init(&o_free, kFewWarps);
     fence_mbar_init();
@@ -594,6 +595,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
   } else if (warp == 0) {
     // ---------------------------------------------------------------- producer: K of a unit before V of the last
     int n = 0;
+    bool asked = false;
     PartWalk c = {};
     auto load = [&](const CUtensorMap* map, int row0, int key) {
       const int slot = n % kFewRing;
@@ -609,6 +611,11 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
       ++n;
     };
     for (bool more = c.open(part_full, part_done, s_part, &abort_flag, p.status_word); more;) {
+      if (c.tiles && !asked) {
+        // the first part's rows before the tiles, which would hold them up (8 x 4096 keys, 64 rows 93.0 -> 90.8 us)
+        asked = true;
+        mbar_wait(&q_asked, 0, &abort_flag, p.status_word, 403);
+      }
       if (c.tiles)
         load(&tmap_k, c.k0, c.begin);
       for (int key = c.begin; key < c.end; key += kUnitKeys) {
@@ -686,9 +693,6 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
     const int group = a.H / a.Hkv;
     const uint32_t t_s = tmem + (static_cast<uint32_t>(quarter * 32) << 16), t_o = t_s + 64;
     int u = 0, n_ring = 0;                         // units and tiles of the ring so far
-    // the list on its way while the scheduler works out the share: behind the first tiles of K and V it takes 2 us
-    for (int i = tid * 32; i < min(a.num_salient, 128 * 32); i += 128 * 32)
-      asm volatile("prefetch.global.L1 [%0];" ::"l"(a.idx + i));
     for (int n = 0;; ++n) {
       if (rows_any(!mbar_wait(&part_full[n % kParts], (n / kParts) & 1, &abort_flag, p.status_word, 415)))
         break;
@@ -735,6 +739,8 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
             x1[h] = __ldg(src + 1);
           }
         }
+        if (u == 0)
+          warp_arrive(&q_asked);
         bool finite[2];
         uint32_t top = 0;
 #pragma unroll
@@ -765,7 +771,6 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
             s_out[r] = t[h] < part.rows ? (part.row0 + t[h] / group) * a.H + head[h] : -1;
             // 1; 0: the row does not exist in q; NaN: the query is not finite
             s_fix[r] = at[h] < 0 ? 0.f : finite[h] ? 1.f : __uint_as_float(0x7fc00000u);
-            s_ref[r] = kNothing;      // less kWeightLog2, as all that follow
             if (BIAS && at[h] >= 0) {
               const int pos = __ldg(a.cu_k + part.b + 1) - __ldg(a.cu_k + part.b) - (__ldg(a.cu_q + part.b + 1) - at[h]);
               s_bias[r] = make_float2(__ldg(a.slopes + head[h]) * kLog2e, static_cast<float>(pos - begin));
@@ -796,6 +801,8 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
       const int all_to = min(min(s_all[0].y, s_all[1].y), min(s_all[2].y, s_all[3].y));
       const int tiles = (end - begin + kUnitKeys - 1) / kUnitKeys;
       float l = 0.f;                               // lane = row: sum of the weights of this quarter's keys
+      float was = kNothing;                        // lane = row: reference less kWeightLog2, as in s_ref
+      float* my_ref = s_ref[quarter];
       for (int i = 0; i < tiles; ++i, ++u) {
         const int at = begin + i * kUnitKeys + kl, buf = u & 1;
         const float kk = ks_next * key_mul, ex = value_exponent(vs_next), place = static_cast<float>(at - begin);
@@ -832,14 +839,18 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
           }
         }
         // does any lie above its reference by more than the weights' codes can take?
-        float above = -INFINITY;
+        bool moves = i == 0;
+        if (!moves) {
+          float above = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < kRows; r += 4) {
-          const float4 ref = *reinterpret_cast<const float4*>(s_ref + r);
-          above = fmax3(above, t[r] - ref.x, t[r + 1] - ref.y);
-          above = fmax3(above, t[r + 2] - ref.z, t[r + 3] - ref.w);
+          for (int r = 0; r < kRows; r += 4) {
+            const float4 ref = *reinterpret_cast<const float4*>(my_ref + r);
+            above = fmax3(above, t[r] - ref.x, t[r + 1] - ref.y);
+            above = fmax3(above, t[r + 2] - ref.z, t[r + 3] - ref.w);
+          }
+          moves = rows_any(above > kHeadroom + kWeightLog2);
         }
-        if (rows_any(above > kHeadroom + kWeightLog2)) {
+        if (moves) {
           float mx = 0.f;
 #pragma unroll
           for (int r = 0; r < kRows; ++r) {
@@ -848,16 +859,13 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
           }
           s_max[quarter][lane] = mx;
           rows_sync();
-          const float was = s_ref[lane];
           mx = fmaxf(fmaxf(s_max[0][lane], s_max[1][lane]), fmaxf(s_max[2][lane], s_max[3][lane]));
           const float ref = mx > was + (kHeadroom + kWeightLog2) ? mx - kWeightLog2 : was, old = exp2f(was - ref);
           l *= old;
-          rows_sync();
-          if (quarter == 0) {
-            s_ref[lane] = ref;
-            s_old[lane] = old;
-          }
-          rows_sync();
+          was = ref;
+          my_ref[lane] = ref;
+          s_old[quarter][lane] = old;
+          __syncwarp();
           if (i > 0) {
             mbar_wait(&pv_done, (u - 1) & 1, &abort_flag, p.status_word, 410);
             tc_fence_after_sync();
@@ -868,7 +876,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
               tmem_ld_wait();
 #pragma unroll
               for (int r = 0; r < 8; ++r)
-                o[r] = __float_as_uint(__uint_as_float(o[r]) * s_old[c + r]);
+                o[r] = __float_as_uint(__uint_as_float(o[r]) * s_old[quarter][c + r]);
               tmem_st_32x8(t_o + c, o);
             }
             tmem_st_wait();
@@ -884,7 +892,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int r = 16 * h + 4 * j;
-            const float4 ref = *reinterpret_cast<const float4*>(s_ref + r);
+            const float4 ref = *reinterpret_cast<const float4*>(my_ref + r);
             t[r] = exp2f(t[r] - ref.x);
             t[r + 1] = exp2f(t[r + 1] - ref.y);
             t[r + 2] = exp2f(t[r + 2] - ref.z);
@@ -919,9 +927,9 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
       n_ring += 2 * tiles;
 
       // ---------------------------------------------------------------- thread = head dimension kl of all rows
-      s_max[quarter][lane] = l;
+      s_sum[quarter][lane] = l;
       const float fix = s_fix[lane];
-      float top = s_ref[lane];
+      float top = was;
       mbar_wait(&pv_done, (u - 1) & 1, &abort_flag, p.status_word, 413);
       tc_fence_after_sync();
       uint32_t ou[kRows];
@@ -931,7 +939,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
       tc_fence_before_sync();
       warp_arrive(&o_free);
       rows_sync();
-      l = (s_max[0][lane] + s_max[1][lane]) + (s_max[2][lane] + s_max[3][lane]);
+      l = (s_sum[0][lane] + s_sum[1][lane]) + (s_sum[2][lane] + s_sum[3][lane]);
       bool store = true;
       if (part.parts > 1) {
         float* mine = p.parts + static_cast<int64_t>(part.slot) * kFewPart;
@@ -983,12 +991,12 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
         for (int r = 0; r < kRows; ++r)
           lines[r * kD + kl] = o[r];
         if (quarter == 0)
-          s_old[lane] = l == 0.f || fix == 0.f ? 0.f : __fdividef(fix, l);
+          s_old[0][lane] = l == 0.f || fix == 0.f ? 0.f : __fdividef(fix, l);
         rows_sync();
 #pragma unroll
         for (int r = tid >> 4; r < kRows; r += 8) {
           const int out = s_out[r];
-          const float mul = s_old[r];
+          const float mul = s_old[0][r];
           if (out >= 0) {
             float x[8];
             *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(lines + r * kD + (tid & 15) * 8);

@@ -241,11 +241,11 @@ def _attend(b, heads, hkv, counts, mask=None, cap=0.0, slopes=False, scale=None,
 def _check(got, want, mag, big, floor, cap):
     """Half a step of bf16 for the result (2^-8).
 
-    A weight w <= 1 (its largest in the row is 1, the values' scales included) is held in half precision (2^-11) and split into
-    e4m3 and what that leaves, |r| <= 2^-4 w (half a step).  Few rows: r times 16 in e4m3, rounded by 2^-4 of itself, of 256 w;
-    many rows: r in e5m2, rounded by 2^-3 of itself, of 64 w: off by at most (2^-7 + 2^-11) w, or by half a step of the smallest
-    numbers, 2^-10 / 16 / 256 or 2^-17 / 64: 2^-22.  The first moves the result by as much of sum(weight * |v|); the second by
-    2^-22 of the largest weight for each key, times its codes, which are at most twice the largest of the heaviest key.
+    A weight w (within 2^2.8 of its row's largest, 1, the values' scales included) is taken as 64 w in half precision (2^-11) and
+    split into e4m3 and what that leaves, |r| <= 2^-4 of it (half a step), in e5m2, rounded by 2^-3 of itself: off by at most
+    (2^-7 + 2^-11) w, or by half a step of the smallest numbers, 2^-17 / 64 <= 2^-22.  The first moves the result by as much of
+    sum(weight * |v|); the second by 2^-22 of the largest weight for each key, times its codes, which are at most twice the largest
+    of the heaviest key.
 
     The score is a sum of 128 products in fp32 (2^-24 a term, 2^-17 in all) of queries that are exact above 2^-18 of their row's
     largest and off by 2^-26 of it below, times a scale, capped and biased (a few 2^-24 of the cap and the bias): 2^-16 of what
