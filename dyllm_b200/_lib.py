@@ -84,7 +84,8 @@ SIGNATURES: dict[str, tuple] = {
     "dyllm_tp_allreduce_f32": (I, [P, P, I, P]),
 }
 
-# kernels of this library launched by one call of each entry point (for launch accounting)
+# kernels of this library launched by one call of each entry point (for launch accounting; the attention over 8-bit caches: at
+# least one, another with key ranges, another with many rows)
 KERNELS_PER_CALL = {
     "dyllm_context_stats": 1, "dyllm_cosine_mask": 1, "dyllm_salient_select": 1, "dyllm_salient_select_static": 1,
     "dyllm_fused_offset": 1,

@@ -50,8 +50,11 @@ const at::Tensor& require(int device, PyObject* o, const char* name, at::ScalarT
     refuse("%s must be on cuda:%d, got cuda:%d", name, device, static_cast<int>(t.get_device()));
   return t;
 }
-const void* require_or_null(int device, PyObject* o, const char* name, at::ScalarType type, int dim) {
-  return o == Py_None ? nullptr : require(device, o, name, type, dim).const_data_ptr();
+// Sizes that the entry points take in 32 bits.
+int size32(int64_t n, const char* name) {
+  if (n > INT32_MAX)
+    refuse("%s has %lld entries: too many", name, static_cast<long long>(n));
+  return static_cast<int>(n);
 }
 template <typename T>
 const T* data(const at::Tensor& t) {
@@ -112,7 +115,7 @@ Sequences require_sequences(int device, PyObject* starts, PyObject* cu_, PyObjec
   const at::Tensor& ids = require(device, ids_, "seq_ids", at::kLong, 1);
   s.cu = data<int32_t>(cu);
   s.ids = data<int64_t>(ids);
-  s.batch = static_cast<int>(ids.size(0));
+  s.batch = size32(ids.size(0), "seq_ids");
   if (cu.size(0) != ids.size(0) + 1)
     refuse("cu_seqlens must have one entry more than seq_ids");
   if (cu_k != Py_None) {
@@ -138,13 +141,6 @@ float to_float(PyObject* o) {
     throw Refused();
   return static_cast<float>(v);
 }
-// Sizes that the entry points take in 32 bits.
-int size32(int64_t n, const char* name) {
-  if (n > INT32_MAX)
-    refuse("%s has %lld entries: too many", name, static_cast<long long>(n));
-  return static_cast<int>(n);
-}
-
 at::Tensor empty_rows(int device, int64_t rows, int64_t heads) {
   return at::empty({rows, heads, 128}, at::TensorOptions().dtype(at::kBFloat16).device(at::kCUDA, device));
 }
@@ -263,7 +259,13 @@ PyObject* kv_cache_update(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   const Cache kc = require_cache(device, a[10], "k_cache", k.heads, k.width), vc = require_cache(device, a[11], "v_cache", k.heads, k.width);
   const Sequences s = require_sequences(device, a[7], a[6], a[9], Py_None);
   const int64_t* v_starts = data<int64_t>(require(device, a[8], "v_seq_starts", at::kLong, 1));
-  const void* count = require_or_null(device, a[12], "num_rows_dev", at::kInt, 1);
+  const int32_t* count = nullptr;
+  if (a[12] != Py_None) {
+    const at::Tensor& t = require(device, a[12], "num_rows_dev", at::kInt, 1);
+    if (t.size(0) < 1)
+      refuse("num_rows_dev must have an entry");
+    count = data<int32_t>(t);
+  }
   const int rows = size32(k.rows, "k_new"), heads = size32(k.heads, "k_new"), width = size32(k.width, "k_new");
   const int angles = size32(cos_sin.size(0), "cos_sin");
   at::Tensor dv;
@@ -276,7 +278,7 @@ PyObject* kv_cache_update(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   }
   on(device, "dyllm_fp8_kv_cache_update", [&](void* stream) {
     return g_update(k.ptr, k.pitch, v.ptr, v.pitch, data<int64_t>(rows_k), data<int64_t>(positions), pos_idx, data<float>(cos_sin), angles,
-                    s.cu, s.starts, v_starts, s.ids, s.batch, rows, static_cast<const int32_t*>(count), heads, width, kc.codes, kc.scales,
+                    s.cu, s.starts, v_starts, s.ids, s.batch, rows, count, heads, width, kc.codes, kc.scales,
                     kc.rows, vc.codes, vc.scales, vc.rows, dv.data_ptr(), stream);
   });
   return THPVariable_Wrap(std::move(dv));

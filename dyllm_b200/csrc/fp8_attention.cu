@@ -150,7 +150,7 @@ __device__ __forceinline__ int units_of(int2 span) { return max(1, (span.y - spa
 // Uniform over a warp.
 //
 // Shares are cut at total * i / ctas, but no part of a tile is shorter than kMinPart units: a cut nearer to an end of its
-// tile moves there.  Joining the parts of a tile costs a CTA of the few-rows kernel about 7 us, a unit 1 to 2.  With many rows a
+// tile moves there.  Joining the parts of a tile costs a CTA of the few-rows kernel about 5 us, a unit 3.  With many rows a
 // unit takes 5 us and the join is a launch of its own: parts of at least 2 units against 4 take 34.6 us against 43.1 (32 x 601
 // keys, 28 heads on 4) and 163 against 166 (4 x 2048 rows of packed documents).
 constexpr int kMinPartFew = 4, kMinPartMany = 2;
@@ -779,7 +779,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
             }
             if (a.ranges && at[h] >= 0) {
               const int2 range = __ldg(a.ranges + at[h]);
-              s_sees[r] = make_int2(range.x, min(range.y, end));
+              s_sees[r] = make_int2(max(range.x, 0), min(range.y, end));
               sees.x = max(sees.x, range.x);
               sees.y = min(sees.y, range.y);
             } else {
@@ -1245,9 +1245,9 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
           v.pos = __ldg(a.cu_k + w.b + 1) - __ldg(a.cu_k + w.b) - (__ldg(a.cu_q + w.b + 1) - at);
           v.slope = BIAS ? __ldg(a.slopes + head) * kLog2e : 0.f;
           if (a.ranges) {
-            const int2 range = __ldg(a.ranges + at);
-            v.lo = range.x;
-            v.hi = min(range.y, w.len);
+            const int2 range = __ldg(a.ranges + at);      // cut: differences with keys must not wrap
+            v.lo = max(range.x, 0);
+            v.hi = max(min(range.y, w.len), 0);
           }
         }
       }
@@ -1732,7 +1732,8 @@ int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, co
   DYLLM_REQUIRE(num_heads > 0 && num_kv_heads > 0 && num_heads % num_kv_heads == 0, DYLLM_ERR_INVALID_ARGUMENT,
                 "attention_salient_rows_fp8: query heads (%d) must be a positive multiple of KV heads (%d)", num_heads,
                 num_kv_heads);
-  DYLLM_REQUIRE(scale == scale && softcap >= 0.f && softcap <= 3.0e38f, DYLLM_ERR_INVALID_ARGUMENT,
+  // a smaller cap: its quotient may be infinite, and a score of zero times that is no number
+  DYLLM_REQUIRE(scale == scale && (softcap == 0.f || softcap >= 1e-6f) && softcap <= 3.0e38f, DYLLM_ERR_INVALID_ARGUMENT,
                 "attention_salient_rows_fp8: scale %g softcap %g", static_cast<double>(scale), static_cast<double>(softcap));
   if (batch == 0 || num_salient == 0 || max_rows_per_seq == 0)
     return DYLLM_OK;

@@ -91,7 +91,7 @@ ATTEND = dict(q=SOME, ldq=1024, tq=8, kc=SOME, ks=SOME, kr=64, vc=SOME, vs=SOME,
 @pytest.mark.parametrize("change,text", [
     (dict(dim=64), "head_dim 64"), (dict(heads=6), "positive multiple"), (dict(heads=0), "positive multiple"), (dict(kv=0), "positive multiple"),
     (dict(n=-1), "rows -1"), (dict(batch=-1), "batch -1"), (dict(most=-1), "max rows -1"), (dict(tq=-1), "Tq -1"), (dict(kr=-1), "batch"),
-    (dict(cap=-1.0), "softcap -1"), (dict(cap=float("nan")), "softcap"), (dict(cap=float("inf")), "softcap"),
+    (dict(cap=-1.0), "softcap -1"), (dict(cap=1e-9), "softcap"), (dict(cap=float("nan")), "softcap"), (dict(cap=float("inf")), "softcap"),
     (dict(scale=float("nan")), "scale"), (dict(q=None), "null"), (dict(idx=None), "null"), (dict(cu_r=None), "null"), (dict(vs=None), "null"),
     (dict(q=SOME + 8), "16-byte"), (dict(vc=SOME + 8), "16-byte"), (dict(out=SOME + 2), "16-byte"), (dict(ldq=1020), "row pitch"),
     (dict(ldq=512), "row pitch"), (dict(ranges=SOME + 4), "key_ranges"),

@@ -194,6 +194,9 @@ def _ranges(kind, b, g):
             r[::2] = torch.tensor([5, 5])
             r[1::4] = torch.tensor([2 ** 31 - 1, -2 ** 31])
             got.append(r)
+        elif kind == "extremes":
+            ends = torch.tensor([[-2 ** 31, length // 2], [0, -2 ** 31], [-2 ** 31, 2 ** 31 - 1], [length // 3, 2 ** 31 - 1]])
+            got.append(ends[torch.arange(q) % 4])
         else:
             a = torch.randint(0, max(length, 1), (q,), generator=g)
             got.append(torch.stack([a, a + torch.randint(0, length + 2, (q,), generator=g)], 1))
@@ -272,6 +275,11 @@ SHAPES = [
 @pytest.mark.parametrize("mask", [None, "prefix", "window", "empty", "random"])
 def test_attention(cuda_device, lens, qlens, counts, heads, hkv, mask):
     _check(*_attend(Batch(lens, qlens, seed=len(lens) + heads), heads, hkv, counts, mask))
+
+
+@pytest.mark.parametrize("lens,qlens,counts,heads,hkv", SHAPES[2:])
+def test_attention_with_ranges_at_the_ends_of_their_type(cuda_device, lens, qlens, counts, heads, hkv):
+    _check(*_attend(Batch(lens, qlens, seed=11), heads, hkv, counts, "extremes"))
 
 
 @pytest.mark.parametrize("lens,qlens,counts,heads,hkv", SHAPES[1:6])
