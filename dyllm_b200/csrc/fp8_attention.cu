@@ -1659,10 +1659,20 @@ __global__ void __launch_bounds__(128) fp8_spans_kernel(const Fp8AttnParams p, i
     spans[before] = lo < hi ? make_int2(lo, hi) : make_int2(0, 0);
 }
 
-// Up to this many (listed row, query head) pairs a sequence and key head the few-rows kernel is taken, with a pass over the keys for
-// each 32 of them.  Few against many, us: 26 pairs (16 x 512 keys, 32 heads) 30 : 63; 64 pairs there 52 : 68, capped over 8 x 4096
-// keys 90 : 139, but over 2 x 32011 keys 129 : 102; 96 pairs, 2 x 1001 keys 25 : 27, 2 x 4001 51 : 37, 2 x 32011 148 : 104.
+// The kernel for a call.  Up to kFewMost (listed row, query head) pairs a sequence and key head the few-rows kernel is taken, with a
+// pass over the keys for each 32 of them; so it is for more of them where the caches are short (their rows are all that the host
+// knows of the keys): tiles of up to 8 units, which it does not split, and at most ten units a CTA.  Few against many, us:
+//   26 pairs (16 x 512 keys, 32 heads) 30 : 63; 64 there 52 : 68; 64, capped, over 8 x 4096 keys 90 : 139; 64 over 2 x 32011 129 : 102
+//   77 (175 keys, 4 key heads) 13 : 30; 84 (32 x 601, 4) 31 : 35; 140 there 36 : 44; 96 (2 x 1001, 8) 25 : 27
+//   96 (2 x 4001 keys, 8 key heads) 51 : 37; 90 (16 x 512, 32) 73 : 71; 128 there 96 : 74
 constexpr int kFewMost = 64;
+bool takes_many(int64_t max_rows, int64_t num_salient, int64_t batch, int64_t group, int64_t kv_heads, int64_t cache_rows, int64_t ctas) {
+  const int64_t most = min(max_rows, num_salient) * group;
+  if (most <= kFewMost)
+    return false;
+  const int64_t tiles = (min(most, (num_salient * group + batch - 1) / batch) + kRows - 1) / kRows;
+  return cache_rows > 8 * kUnitKeys * batch || (cache_rows / kUnitKeys + batch) * tiles * kv_heads > 10 * kFewCtas * ctas;
+}
 
 // Workspace: tickets, keys per tile (only with ranges), parts of tiles; for the kernel that needs most.
 constexpr int kMostCtas = kFewCtas > kManyCtas ? kFewCtas : kManyCtas;
@@ -1797,7 +1807,7 @@ int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, co
   f.launch_id = next_launch_id() & ~0xffffull;
   f.status_word = device_status_word();
   // a sequence with more rows than the bound says is served by either kernel; so is one with few beside others with many
-  const bool many = static_cast<int64_t>(max_rows_per_seq) * group > kFewMost && static_cast<int64_t>(num_salient) * group > kFewMost;
+  const bool many = takes_many(max_rows_per_seq, num_salient, batch, group, num_kv_heads, k_rows, ctas);
   if (p.ranges) {
     f.spans = spans;
     const unsigned blocks = static_cast<unsigned>((tiles + 3) / 4);

@@ -50,6 +50,12 @@ class Batch:
         return _cum([len(r) for r in rows]), torch.cat(rows).int(), torch.cat(rows_k).long()
 
 
+def _far(b, code, scale):
+    """The same cache with rows of nobody behind it: more than 1024 a sequence, so that the call cannot take it for a short one."""
+    n = 1025 * b.n
+    return torch.cat([code, torch.zeros(n, *code.shape[1:]).double()]), torch.cat([scale, torch.ones(n, scale.size(1)).double()])
+
+
 def _to_cache(code, scale):
     return code.flatten(1).float().cuda().to(FP8), scale.float().cuda()
 
@@ -204,7 +210,7 @@ def _ranges(kind, b, g):
 
 
 def _attend(b, heads, hkv, counts, mask=None, cap=0.0, slopes=False, scale=None, seed=0, q_size=1.0, spread=0.5, sliced=False,
-            most=None, edit=None):
+            most=None, edit=None, far=False):
     from dyllm_b200 import _lib
     from dyllm_b200.attention_ops import attention_salient_rows_fp8
 
@@ -214,6 +220,8 @@ def _attend(b, heads, hkv, counts, mask=None, cap=0.0, slopes=False, scale=None,
     (kc, ks), (vc, vs) = b.cache(hkv, spread), b.cache(hkv, spread)
     if edit:
         edit(b, kc, ks, vc, vs)
+    if far:
+        (kc, ks), (vc, vs) = _far(b, kc, ks), _far(b, vc, vs)
     ranges = None if mask is None else _ranges(mask, b, b.g)
     slope = 2.0 ** -torch.arange(1, heads + 1).float() if slopes else None
     qd = q.cuda()
@@ -273,13 +281,22 @@ SHAPES = [
 
 @pytest.mark.parametrize("lens,qlens,counts,heads,hkv", SHAPES)
 @pytest.mark.parametrize("mask", [None, "prefix", "window", "empty", "random"])
-def test_attention(cuda_device, lens, qlens, counts, heads, hkv, mask):
-    _check(*_attend(Batch(lens, qlens, seed=len(lens) + heads), heads, hkv, counts, mask))
+@pytest.mark.parametrize("far", [False, True])
+def test_attention(cuda_device, lens, qlens, counts, heads, hkv, mask, far):
+    _check(*_attend(Batch(lens, qlens, seed=len(lens) + heads), heads, hkv, counts, mask, far=far))
+
+
+@pytest.mark.parametrize("counts", [[10, 2, 7], [40, 2, 33]])                              # pairs: 20, 80 a sequence and key head
+@pytest.mark.parametrize("mask,slopes", [(None, False), (None, True), ("prefix", False), ("random", True)])
+def test_attention_of_sequences_that_many_ctas_hold(cuda_device, counts, mask, slopes):
+    """Hundreds of parts, joined in their order; a short sequence between long ones."""
+    _check(*_attend(Batch([20011, 5, 9000], [64, 5, 300], seed=13), 4, 2, counts, mask, slopes=slopes))
 
 
 @pytest.mark.parametrize("lens,qlens,counts,heads,hkv", SHAPES[2:])
-def test_attention_with_ranges_at_the_ends_of_their_type(cuda_device, lens, qlens, counts, heads, hkv):
-    _check(*_attend(Batch(lens, qlens, seed=11), heads, hkv, counts, "extremes"))
+@pytest.mark.parametrize("far", [False, True])
+def test_attention_with_ranges_at_the_ends_of_their_type(cuda_device, lens, qlens, counts, heads, hkv, far):
+    _check(*_attend(Batch(lens, qlens, seed=11), heads, hkv, counts, "extremes", far=far))
 
 
 @pytest.mark.parametrize("lens,qlens,counts,heads,hkv", SHAPES[1:6])
@@ -287,32 +304,36 @@ def test_attention_with_ranges_at_the_ends_of_their_type(cuda_device, lens, qlen
     (None, 20.0, False, None, False), (None, 0.0, True, None, True), ("prefix", 30.0, True, 0.2, True), (None, 5.0, False, -0.1, False),
     (None, 0.0, False, 0.0, False),
 ])
-def test_attention_scores(cuda_device, lens, qlens, counts, heads, hkv, mask, cap, slopes, scale, sliced):
-    _check(*_attend(Batch(lens, qlens, seed=7), heads, hkv, counts, mask, cap, slopes, scale, sliced=sliced))
+@pytest.mark.parametrize("far", [False, True])
+def test_attention_scores(cuda_device, lens, qlens, counts, heads, hkv, mask, cap, slopes, scale, sliced, far):
+    _check(*_attend(Batch(lens, qlens, seed=7), heads, hkv, counts, mask, cap, slopes, scale, sliced=sliced, far=far))
 
 
 @pytest.mark.parametrize("heads,hkv,counts", [(4, 4, [6, 20]), (8, 2, [9, 30]), (2, 1, [100, 70])])
 @pytest.mark.parametrize("q_size,spread", [(8.0, 3.0), (1e-3, 0.0), (1e4, 0.5), (30.0, 6.0)])
-def test_attention_with_peaked_scores_and_values_of_all_sizes(cuda_device, heads, hkv, counts, q_size, spread):
+@pytest.mark.parametrize("far", [False, True])
+def test_attention_with_peaked_scores_and_values_of_all_sizes(cuda_device, heads, hkv, counts, q_size, spread, far):
     _check(*_attend(Batch([400, 333], [200, 100], seed=3), heads, hkv, counts, q_size=q_size, spread=spread,
-                    scale=128 ** -0.5 / max(q_size / 8.0, 1.0)))
+                    scale=128 ** -0.5 / max(q_size / 8.0, 1.0), far=far))
 
 
 @pytest.mark.parametrize("counts", [[3, 5], [60, 90]])
 @pytest.mark.parametrize("most", [1, 1000])
-def test_the_bound_of_listed_rows_only_chooses_kernels(cuda_device, counts, most):
-    _check(*_attend(Batch([210, 340], [100, 340], seed=5), 4, 2, counts, most=most))
+@pytest.mark.parametrize("far", [False, True])
+def test_the_bound_of_listed_rows_only_chooses_kernels(cuda_device, counts, most, far):
+    _check(*_attend(Batch([210, 340], [100, 340], seed=5), 4, 2, counts, most=most, far=far))
 
 
 @pytest.mark.parametrize("counts", [[4], [100]])
-def test_nan_of_unseen_keys_stays_unseen(cuda_device, counts):
+@pytest.mark.parametrize("far", [False, True])
+def test_nan_of_unseen_keys_stays_unseen(cuda_device, counts, far):
     """Keys 20.. of the sequence hold NaN in K or V; the rows of a window that ends before them are finite, the others NaN."""
     def edit(b, kc, ks, vc, vs):
         k0, v0 = int(b.k_starts[b.ids[0]]), int(b.v_starts[b.ids[0]])
         kc[k0 + 150], ks[k0 + 150] = 0.0, math.nan
         vc[v0 + 170], vs[v0 + 170] = 0.0, math.nan
 
-    got, want, mag, big, floor, cap = _attend(Batch([200], [200], seed=2), 2, 2, counts, "window", edit=edit)
+    got, want, mag, big, floor, cap = _attend(Batch([200], [200], seed=2), 2, 2, counts, "window", edit=edit, far=far)
     bad = torch.isnan(got).any(-1).any(-1)
     assert bool(bad.any()) == bool(torch.isnan(want).any()) and not bool(bad.all())
     fine = ~torch.isnan(want)
@@ -321,11 +342,12 @@ def test_nan_of_unseen_keys_stays_unseen(cuda_device, counts):
 
 
 @pytest.mark.parametrize("counts", [[4], [100]])
-def test_rows_of_nobody_may_hold_any_byte(cuda_device, counts):
+@pytest.mark.parametrize("gap", [150, 1100])
+def test_rows_of_nobody_may_hold_any_byte(cuda_device, counts, gap):
     """Rows between the sequences are never part of a result, be they NaN codes (an arena comes uninitialised)."""
     from dyllm_b200.attention_ops import attention_salient_rows_fp8
 
-    b = Batch([133], [133], seed=4, gap=150)
+    b = Batch([133], [133], seed=4, gap=gap)
     cu, rows, _ = b.picks(counts)
     (kc, ks), (vc, vs) = b.cache(2), b.cache(2)
     q = b.randn(133, 2, 128).bfloat16().cuda()
@@ -345,17 +367,23 @@ def test_rows_of_nobody_may_hold_any_byte(cuda_device, counts):
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
 
 
-def test_sequences_without_a_cache_and_rows_out_of_range_give_zeros(cuda_device):
+@pytest.mark.parametrize("times,far", [(1, False), (30, False), (30, True)])
+def test_sequences_without_a_cache_and_rows_out_of_range_give_zeros(cuda_device, times, far):
     from dyllm_b200.attention_ops import attention_salient_rows_fp8
 
     b = Batch([40, 50], seed=6)
     (kc, ks), (vc, vs) = b.cache(2), b.cache(2)
+    if far:
+        (kc, ks), (vc, vs) = _far(b, kc, ks), _far(b, vc, vs)
     q = b.randn(90, 4, 128).bfloat16().cuda()
     b.v_starts[b.ids[1]] = -1
-    cu, rows = torch.tensor([0, 3, 5], dtype=torch.int32), torch.tensor([0, -4, 90, 41, 60], dtype=torch.int32)
-    out = attention_salient_rows_fp8(q, _to_cache(kc, ks), _to_cache(vc, vs),
-                                     *_cuda(b.k_starts, b.v_starts, b.ids, b.cu_q, b.cu_k, cu, rows), max_rows_per_seq=3)
-    assert bool((out[0] != 0).any(-1).all()) and bool((out[1:] == 0).all())
+    cu, rows = torch.tensor([0, 3 * times, 5 * times], dtype=torch.int32), torch.tensor([0, -4, 90] * times + [41, 60] * times, dtype=torch.int32)
+    out = torch.full((5 * times, 4, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    attention_salient_rows_fp8(q, _to_cache(kc, ks), _to_cache(vc, vs), *_cuda(b.k_starts, b.v_starts, b.ids, b.cu_q, b.cu_k, cu, rows),
+                               max_rows_per_seq=3 * times, out=out)
+    there = torch.zeros(5 * times, dtype=torch.bool)
+    there[0 : 3 * times : 3] = True
+    assert bool((out[there.cuda()] != 0).any(-1).all()) and bool((out[~there.cuda()] == 0).all())
 
 
 def test_python_refusals(cuda_device):

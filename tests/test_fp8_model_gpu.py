@@ -210,10 +210,10 @@ def test_two_captured_graphs_on_two_streams_keep_apart(cuda_device):
     """Two generations' operators captured over shared caches, replayed at the same time on two streams: same bits as alone."""
     from dyllm_b200 import ops
     from dyllm_b200.attention_ops import attention_salient_rows_fp8
-    from tests.test_fp8_cache_gpu import Batch, _to_cache
+    from tests.test_fp8_cache_gpu import Batch, _far, _to_cache
 
     b = Batch([900, 333, 64], [300, 333, 64], seed=8)
-    kc, vc = _to_cache(*b.cache(2)), _to_cache(*b.cache(2))
+    kc, vc = _to_cache(*_far(b, *b.cache(2))), _to_cache(*_far(b, *b.cache(2)))
     ks, vs, ids, cu_q, cu_k = (t.cuda() for t in (b.k_starts, b.v_starts, b.ids, b.cu_q, b.cu_k))
     jobs = []
     for counts in ([7, 2, 9], [250, 333, 64]):
