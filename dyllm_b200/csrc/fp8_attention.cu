@@ -1756,8 +1756,9 @@ int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, co
                 "attention_salient_rows_fp8: scale %g softcap %g", static_cast<double>(scale), static_cast<double>(softcap));
   if (batch == 0 || num_salient == 0 || max_rows_per_seq == 0)
     return DYLLM_OK;
-  DYLLM_REQUIRE(q && k_codes && k_scales && v_codes && v_scales && k_seq_starts && v_seq_starts && seq_ids && out &&
-                    cu_seqlens_q && cu_seqlens_k && cu_salientlens && idx_salient_row,
+  // empty tensors have no address, and nothing reads them
+  DYLLM_REQUIRE((q || total_q == 0) && ((k_codes && k_scales) || k_rows == 0) && ((v_codes && v_scales) || v_rows == 0) && k_seq_starts &&
+                    v_seq_starts && seq_ids && out && cu_seqlens_q && cu_seqlens_k && cu_salientlens && idx_salient_row,
                 DYLLM_ERR_INVALID_ARGUMENT, "attention_salient_rows_fp8: null pointer");
   for (const void* p16 : {q, k_codes, v_codes, static_cast<const void*>(out)})
     DYLLM_REQUIRE((reinterpret_cast<uintptr_t>(p16) & 15) == 0, DYLLM_ERR_INVALID_ARGUMENT,
@@ -1827,9 +1828,10 @@ int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, co
   }
   CUtensorMap tk, tv;
   const uint64_t width = static_cast<uint64_t>(num_kv_heads) * kD;
-  int rc = encode_tmap_2d_u8(&tk, k_codes, k_rows ? k_rows : 1, width, width, 32, kD);
+  // (a cache without rows: a descriptor that no copy uses)
+  int rc = encode_tmap_2d_u8(&tk, k_rows ? k_codes : out, k_rows ? k_rows : 1, width, width, 32, kD);
   if (rc == DYLLM_OK)
-    rc = encode_tmap_2d_u8(&tv, v_codes, v_rows ? v_rows : 1, width, width, 32, kD);
+    rc = encode_tmap_2d_u8(&tv, v_rows ? v_codes : out, v_rows ? v_rows : 1, width, width, 32, kD);
   if (rc != DYLLM_OK)
     return rc;
   if (softcap > 0.f) {

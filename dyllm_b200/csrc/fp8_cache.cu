@@ -274,7 +274,7 @@ int dyllm_fp8_cache_write(const void* x, int64_t ldx, int heads, int head_dim, v
     return rc;
   if ((rc = check_stride("fp8_cache_write", "x", x, ldx, heads)) != DYLLM_OK)
     return rc;
-  DYLLM_REQUIRE(codes && scales && seq_starts && cu_seqlens && seq_ids, DYLLM_ERR_INVALID_ARGUMENT,
+  DYLLM_REQUIRE(((codes && scales) || cache_rows == 0) && seq_starts && cu_seqlens && seq_ids, DYLLM_ERR_INVALID_ARGUMENT,
                 "fp8_cache_write: null pointer");
   DYLLM_REQUIRE(aligned(codes, 16) && aligned(scales, 4), DYLLM_ERR_INVALID_ARGUMENT,
                 "fp8_cache_write: codes must be 16-byte aligned");
@@ -293,7 +293,7 @@ int dyllm_fp8_cache_read(const void* codes, const float* scales, int64_t cache_r
   int rc = check_heads("fp8_cache_read", heads, head_dim, batch, total_rows, cache_rows);
   if (rc <= 0)
     return rc;
-  DYLLM_REQUIRE(codes && scales && out && seq_starts && cu_seqlens && seq_ids, DYLLM_ERR_INVALID_ARGUMENT,
+  DYLLM_REQUIRE(((codes && scales) || cache_rows == 0) && out && seq_starts && cu_seqlens && seq_ids, DYLLM_ERR_INVALID_ARGUMENT,
                 "fp8_cache_read: null pointer");
   DYLLM_REQUIRE(aligned(codes, 16) && aligned(scales, 4) && aligned(out, 16), DYLLM_ERR_INVALID_ARGUMENT,
                 "fp8_cache_read: codes and out must be 16-byte aligned");
@@ -319,8 +319,8 @@ int dyllm_fp8_kv_cache_update(const void* k_new, int64_t ldk, const void* v_new,
       (rc = check_stride("fp8_kv_cache_update", "v_new", v_new, ldv, kv_heads)) != DYLLM_OK)
     return rc;
   DYLLM_REQUIRE(max_pos > 0, DYLLM_ERR_INVALID_ARGUMENT, "fp8_kv_cache_update: an angle table of %d positions", max_pos);
-  DYLLM_REQUIRE(rows_k && positions && cos_sin && cu_seqlens_k && k_seq_starts && v_seq_starts && seq_ids && k_codes &&
-                    k_scales && v_codes && v_scales && dv,
+  DYLLM_REQUIRE(rows_k && positions && cos_sin && cu_seqlens_k && k_seq_starts && v_seq_starts && seq_ids &&
+                    ((k_codes && k_scales) || k_rows == 0) && ((v_codes && v_scales) || v_rows == 0) && dv,
                 DYLLM_ERR_INVALID_ARGUMENT, "fp8_kv_cache_update: null pointer");
   DYLLM_REQUIRE(aligned(k_codes, 16) && aligned(v_codes, 16) && aligned(dv, 16) && aligned(cos_sin, 16) &&
                     aligned(k_scales, 4) && aligned(v_scales, 4),

@@ -386,6 +386,27 @@ def test_sequences_without_a_cache_and_rows_out_of_range_give_zeros(cuda_device,
     assert bool((out[there.cuda()] != 0).any(-1).all()) and bool((out[~there.cuda()] == 0).all())
 
 
+@pytest.mark.parametrize("listed", [3, 200])
+def test_caches_without_rows_and_batches_without_queries(cuda_device, listed):
+    """An arena that holds nobody yet: nothing is written, everything reads as zeros; lists of a batch that has no query rows."""
+    from dyllm_b200 import _lib, ops
+    from dyllm_b200.attention_ops import attention_salient_rows_fp8
+
+    cache = torch.empty(0, 256, device="cuda").to(FP8), torch.empty(0, 2, device="cuda")
+    starts, ids, cu = _cuda(torch.tensor([0, -1]), torch.tensor([0, 1]), torch.tensor([0, listed, listed + 2], dtype=torch.int32))
+    x = torch.ones(listed + 2, 2, 128, dtype=torch.bfloat16, device="cuda")
+    ops.fp8_cache_write(x, *cache, starts, cu, ids)
+    assert bool((ops.fp8_cache_read(*cache, starts, cu, ids, listed + 2) == 0).all())
+    rows = torch.arange(listed + 2, device="cuda")
+    dv = ops.fp8_kv_cache_update(x, x, rows, rows, None, torch.ones(listed + 2, 128, device="cuda"), cu, starts, starts, ids, cache, cache)
+    assert bool((dv == 0).all())
+    for q in (x, x[:0]):
+        out = torch.full_like(x, 5.0)
+        got = attention_salient_rows_fp8(q, cache, cache, starts, starts, ids, cu if len(q) else cu * 0, cu, cu, rows.int(), listed, out=out)
+        assert got is out and bool((out == 0).all())
+    assert _lib.load().dyllm_device_status() == 0
+
+
 def test_python_refusals(cuda_device):
     from dyllm_b200 import ops
     from dyllm_b200.attention_ops import attention_salient_rows_fp8
