@@ -386,6 +386,105 @@ def test_sequences_without_a_cache_and_rows_out_of_range_give_zeros(cuda_device,
     assert bool((out[there.cuda()] != 0).any(-1).all()) and bool((out[~there.cuda()] == 0).all())
 
 
+@pytest.mark.parametrize("far", [False, True])
+@pytest.mark.parametrize("most", [3, 60])
+def test_attention_of_a_batch_of_more_than_a_warps_sequences(cuda_device, most, far):
+    g = torch.Generator().manual_seed(21)
+    lens = torch.randint(0, 300, (75,), generator=g).tolist()
+    counts = [min(n, int(torch.randint(0, most + 1, (1,), generator=g))) for n in lens]
+    _check(*_attend(Batch(lens, seed=21), 4, 2, counts, far=far))
+    _check(*_attend(Batch(lens, seed=22), 4, 2, counts, "window", far=far))
+
+
+@pytest.mark.parametrize("far", [False, True])
+@pytest.mark.parametrize("heads,hkv", [(160, 1), (66, 2), (33, 33)])
+def test_attention_of_more_heads_than_a_tile_has_rows(cuda_device, heads, hkv, far):
+    _check(*_attend(Batch([70, 3, 140], seed=17), heads, hkv, [2, 1, 3], "prefix", far=far))
+
+
+@pytest.mark.parametrize("far", [False, True])
+def test_a_replayed_call_follows_the_lists(cuda_device, far):
+    """Captured with lists of one length and replayed with others: counts, rows and sequences are read on the device."""
+    from dyllm_b200 import ops
+    from dyllm_b200.attention_ops import attention_salient_rows_fp8
+
+    b = Batch([500, 90, 333], [200, 90, 100], seed=19)
+    total_q, heads, hkv = sum(b.qlens), 6, 2
+    caches = [_to_cache(*(_far(b, *c) if far else c)) for c in (b.cache(hkv), b.cache(hkv))]
+    q = b.randn(total_q, heads, 128).bfloat16().cuda()
+    ks, vs, ids, cu_q, cu_k = _cuda(b.k_starts, b.v_starts, b.ids, b.cu_q, b.cu_k)
+    k_new, v_new = (b.randn(total_q, hkv, 128).bfloat16().cuda() for _ in range(2))
+    angle = torch.outer(torch.arange(600).double(), 10000.0 ** (-torch.arange(64).double() / 64))
+    cos_sin = torch.cat([angle.cos(), angle.sin()], -1).float().cuda()
+    cu, rows = torch.zeros(4, dtype=torch.int32, device="cuda"), torch.zeros(total_q, dtype=torch.int32, device="cuda")
+    rows_k, count = torch.zeros(total_q, dtype=torch.int64, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    positions = torch.arange(total_q, device="cuda")
+
+    def fill(counts):
+        c, r, rk = b.picks(counts)
+        cu.copy_(c)
+        rows[: len(r)], rows_k[: len(rk)] = r.cuda(), rk.cuda()
+        count.fill_(len(r))
+
+    def run(caches):
+        dv = torch.zeros_like(v_new)
+        ops.fp8_kv_cache_update(k_new, v_new, rows_k, positions, None, cos_sin, cu_k, ks, vs, ids, *caches, num_rows_dev=count, dv=dv)
+        out = torch.zeros(total_q, heads, 128, dtype=torch.bfloat16, device="cuda")
+        attention_salient_rows_fp8(q, *caches, ks, vs, ids, cu_q, cu_k, cu, rows, max_rows_per_seq=200, out=out)
+        return dv, out, ops.fp8_cache_read(*caches[0], ks, cu_k, ids, sum(b.lens))
+
+    def copy():
+        return [tuple(t.clone() for t in c) for c in caches]
+
+    fill([3, 1, 2])
+    run(copy())
+    torch.cuda.synchronize()
+    mine = copy()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(mine)
+    for counts in ([3, 1, 2], [200, 90, 100], [0, 0, 0], [0, 17, 1], [150, 0, 0], [1, 1, 1]):
+        fill(counts)
+        for m, c in zip(mine, caches):
+            for x, y in zip(m, c):
+                x.copy_(y)
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(got, run(copy())):
+            assert torch.equal(x, y)
+
+
+def test_calls_from_two_threads_on_two_streams(cuda_device):
+    import threading
+
+    from dyllm_b200 import _lib
+    from dyllm_b200.attention_ops import attention_salient_rows_fp8
+
+    jobs, results = [], {}
+    for n, counts in enumerate(([9, 4], [130, 90])):
+        b = Batch([300, 1500], [300, 200], seed=23 + n)
+        kc, vc = _to_cache(*b.cache(2)), _to_cache(*b.cache(2))
+        cu, rows, _ = b.picks(counts)
+        args = (b.randn(500, 4, 128).bfloat16().cuda(), kc, vc, *_cuda(b.k_starts, b.v_starts, b.ids, b.cu_q, b.cu_k, cu, rows), max(counts))
+        jobs.append((args, attention_salient_rows_fp8(*args)))
+    torch.cuda.synchronize()
+
+    def work(n):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            results[n] = [attention_salient_rows_fp8(*jobs[n][0]) for _ in range(40)]
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert _lib.load().dyllm_device_status() == 0
+    for n, (_, want) in enumerate(jobs):
+        assert len(results[n]) == 40 and all(torch.equal(got, want) for got in results[n])
+
+
 @pytest.mark.parametrize("listed", [3, 200])
 def test_caches_without_rows_and_batches_without_queries(cuda_device, listed):
     """An arena that holds nobody yet: nothing is written, everything reads as zeros; lists of a batch that has no query rows."""
