@@ -1261,6 +1261,14 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         rows_sync();
         continue;
       }
+      // the first tile's scales are on their way with the queries
+      const float* ks = a.k_scales + static_cast<int64_t>(w.k0) * a.Hkv + w.hk;
+      const float* vs = a.v_scales + static_cast<int64_t>(w.v0) * a.Hkv + w.hk;
+      float first_k = 1.f, first_v = 1.f;
+      if (w.begin + tid < w.end) {
+        first_k = __ldg(ks + static_cast<int64_t>(w.begin + tid) * a.Hkv);
+        first_v = __ldg(vs + static_cast<int64_t>(w.begin + tid) * a.Hkv);
+      }
       s_src[tid] = src;
       if (tid == 0)
         s_amax[qb] = 0;
@@ -1302,6 +1310,21 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       rows_sync();
       const uint32_t scale = fp8_scale_bits(s_amax[qb]);
       const float inv = fp8_inverse(scale);
+      // scores come out times log2(e), or as twice the argument of the tanh that caps them
+      const float mul = a.scale * __uint_as_float(scale) * kLog2e * (CAP ? 2.f / a.cap : 1.f);
+      auto deposit = [&](float k, float v) {
+        const int sl = n_sc % kScaleSlots;
+        if (n_sc >= kScaleSlots)
+          mbar_wait(&sc_free[sl], (n_sc / kScaleSlots - 1) & 1, &abort_flag, p.status_word, 512);
+        const float ex = value_exponent(v);
+        float* dst = sc_smem + sl * 3 * kUnitKeys + tid;
+        dst[0] = k * mul;
+        dst[kUnitKeys] = ex;
+        dst[2 * kUnitKeys] = ex == ex ? exp2f(-ex) : 1.f;      // the weight of a NaN is a NaN where its key is seen, else zero
+        warp_arrive(&sc_full[sl]);
+        ++n_sc;
+      };
+      deposit(first_k, first_v);
       if (live > 0)
         mbar_wait(&q_free, (live - 1) & 1, &abort_flag, p.status_word, 511);
 #pragma unroll 1
@@ -1326,12 +1349,8 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       rows_sync();
       warp_arrive(&q_full);
       ++live;
-      // scales: thread = key, four tiles' loads at a time
-      // scores come out times log2(e), or as twice the argument of the tanh that caps them
-      const float mul = a.scale * __uint_as_float(scale) * kLog2e * (CAP ? 2.f / a.cap : 1.f);
-      const float* ks = a.k_scales + static_cast<int64_t>(w.k0) * a.Hkv + w.hk;
-      const float* vs = a.v_scales + static_cast<int64_t>(w.v0) * a.Hkv + w.hk;
-      for (int key = w.begin + tid; key - tid < w.end; key += 4 * kUnitKeys) {
+      // scales of the other tiles: thread = key, four tiles' loads at a time
+      for (int key = w.begin + kUnitKeys + tid; key - tid < w.end; key += 4 * kUnitKeys) {
         float x[4], y[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -1344,18 +1363,8 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (key - tid + i * kUnitKeys < w.end) {
-            const int sl = n_sc % kScaleSlots;
-            if (n_sc >= kScaleSlots)
-              mbar_wait(&sc_free[sl], (n_sc / kScaleSlots - 1) & 1, &abort_flag, p.status_word, 512);
-            const float ex = value_exponent(y[i]);
-            float* dst = sc_smem + sl * 3 * kUnitKeys + tid;
-            dst[0] = x[i] * mul;
-            dst[kUnitKeys] = ex;
-            dst[2 * kUnitKeys] = ex == ex ? exp2f(-ex) : 1.f;      // the weight of a NaN is a NaN where its key is seen, else zero
-            warp_arrive(&sc_full[sl]);
-            ++n_sc;
-          }
+          if (key - tid + i * kUnitKeys < w.end)
+            deposit(x[i], y[i]);
       }
     }
   } else {
