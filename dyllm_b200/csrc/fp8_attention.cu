@@ -1023,7 +1023,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
 // ----------------------------------------------------------------------------------------------
 // Many rows per sequence: bound by the instructions around the exponentials.  A unit of 128 rows x 128 keys takes the tensor cores
 // 1000 cycles, its exponentials 1024, the scales of its keys (three words a key for each of four warps) 1536 of shared memory; with
-// all else it takes an SM 4800 (2 x 32011 keys, 128 pairs a key head: 105 us, of which 9 for lists and queries, 8 for the join).
+// all else it takes an SM 4800 (2 x 32011 keys, 128 pairs a key head: 105 us, of which 9 for lists and queries, 5 for the join).
 // Without the reads of the scales it would take 93 us, without the scores' pass 89, without the weights' pass 90.
 //
 // Tiles of 128 (listed row, query head) pairs, rows in the M = 128 of the products:
