@@ -71,6 +71,10 @@ constexpr int kUnitKeys = 128;                               // keys of a unit o
 constexpr int kRows = 32;                                    // rows of a tile of the few-rows kernel
 constexpr int kParts = 4;                                    // slots of part descriptions
 constexpr uint32_t kTileBytes = kUnitKeys * kD;
+constexpr int kManyRows = 128;                               // and of the many-rows kernel
+// A part in the workspace: [dimension][row] sums, [row] references, sums of weights; of a first part also output rows and `fix`.
+__host__ __device__ constexpr int part_floats(int rows) { return rows * (kD + 4); }
+constexpr int kFewPart = part_floats(kRows), kManyPart = part_floats(kManyRows);
 constexpr float kWeightLog2 = 6.f;                           // the reference's weight: 2^6
 constexpr float kHeadroom = 2.8f;                            // 2^(6 + 2.8) < 448
 
@@ -79,7 +83,8 @@ struct FewParams {
   const int2* spans;           // per tile of rows: keys that any of them sees (null: all)
   unsigned long long* tickets; // one per CTA
   float* parts;                // two per CTA: [rows][128] sums, [rows] maxima, [rows] sums of weights
-  int* joins;                  // many rows, per CTA: parts of the tile that begins in it and goes on in others (0: none)
+  int* joins;                  // per CTA: parts of the tile that begins in it and goes on in others (0: none); for fp8_join_kernel
+  bool later;                  // few rows: that kernel joins them
   unsigned long long launch_id;
   int* status_word;
 };
@@ -482,7 +487,8 @@ __device__ __forceinline__ void split_weights_e5m2(float2 a, float2 b, uint32_t&
 // The rows of a tile are up to 32 (listed row, query head) pairs of one sequence and key head, so that grouped query heads share
 // one pass over their keys.  A unit of work is 128 keys of a tile; all units of the launch, in the order (sequence, tile, key head,
 // keys), are dealt out to the CTAs in equal contiguous shares that every CTA works out for itself from the device-side counts.  A
-// tile whose units lie in several CTAs is joined by the CTA that finishes last, in the order of its parts.
+// tile whose units lie in several CTAs is joined by the CTA that finishes last, or where there will be many parts by a launch of
+// its own, in the order of its parts.
 //
 // The products are transposed, keys (then head dimensions) in the M = 128 of tcgen05.mma.kind::f8f6f4:
 //   S^T = K Q^T         A: K tile as loaded (K-major), B: the queries as e4m3 + e5m2, two products into one accumulator
@@ -502,9 +508,6 @@ constexpr int kFewCtas = 4;                                  // per SM
 constexpr int kFewWarps = 4, kFewThreads = 32 * (3 + kFewWarps);
 constexpr uint32_t kFewTmemCols = 128, kQBytes = kRows * kD, kPBytes = kUnitKeys * 64;
 constexpr uint32_t kFewSmem = kFewRing * kTileBytes + kPBytes + 2 * kQBytes + 1024;
-
-// Rows of a part in the workspace: [dimension][row] sums, [row] references, [row] sums of weights.
-constexpr int kFewPart = kRows * (kD + 2);
 
 // Sum of each of 32 values over the lanes of a warp: lane l gets that of value l.
 __device__ __forceinline__ float sum_lanes(float (&v)[32]) {
@@ -693,6 +696,8 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
     const int group = a.H / a.Hkv;
     const uint32_t t_s = tmem + (static_cast<uint32_t>(quarter * 32) << 16), t_o = t_s + 64;
     int u = 0, n_ring = 0;                         // units and tiles of the ring so far
+    if (p.later && tid == 0)
+      p.joins[blockIdx.x] = 0;                     // unless a tile begins here that goes on in other CTAs
     for (int n = 0;; ++n) {
       if (rows_any(!mbar_wait(&part_full[n % kParts], (n / kParts) & 1, &abort_flag, p.status_word, 415)))
         break;
@@ -950,14 +955,24 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
           mine[kRows * kD + lane] = top;
           mine[kRows * kD + kRows + lane] = l;
         }
-        __threadfence();
-        rows_sync();
-        if (tid == 0) {
-          open_join(p.tickets + part.owner, p.launch_id);
-          joins = last_to_join(p.tickets + part.owner, part.parts) ? 1 : 0;
+        if (p.later) {
+          store = false;
+          if (part.first && quarter == 0) {
+            mine[kRows * kD + 2 * kRows + lane] = __int_as_float(s_out[lane]);
+            mine[kRows * kD + 3 * kRows + lane] = fix;
+          }
+          if (part.first && tid == 0)
+            p.joins[blockIdx.x] = part.parts;
+        } else {
+          __threadfence();
+          rows_sync();
+          if (tid == 0) {
+            open_join(p.tickets + part.owner, p.launch_id);
+            joins = last_to_join(p.tickets + part.owner, part.parts) ? 1 : 0;
+          }
+          rows_sync();
+          store = joins != 0;
         }
-        rows_sync();
-        store = joins != 0;
         if (store) {
           __threadfence();
           const float* first = p.parts + (2 * static_cast<int64_t>(part.owner) + 1) * kFewPart;
@@ -1035,7 +1050,6 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
 // scores' 32 columns), so the steps of one tile follow one another; two CTAs per SM, each with parts of its own, fill each other's
 // waits, the ends of parts among them.  Four loader warps stage the queries of the next part and the scales of the next tiles.
 // ----------------------------------------------------------------------------------------------
-constexpr int kManyRows = 128;
 constexpr int kManyRing = 4;                                 // slots of one K or V tile
 constexpr int kScaleSlots = 2;                               // tiles whose scales are staged ahead
 constexpr int kManyWarps = 4, kManyThreads = 32 * (3 + kManyWarps + 4);
@@ -1046,8 +1060,6 @@ constexpr uint32_t kManyQBytes = kManyRows * kD;             // e4m3 or e5m2 par
 constexpr uint32_t kManySmem = kManyRing * kTileBytes + 2 * kManyQBytes + kManyWarps * kStageBytes +
                                kScaleSlots * 3 * kUnitKeys * sizeof(float) + 1024;
 
-// A part in the workspace: [dimension][row] sums, [row] references, sums of weights; of a first part also output rows and `fix`.
-constexpr int kManyPart = kManyRows * (kD + 4);
 
 // One step of a product whose A operand, 32 codes of a row in 8 columns, lies in tensor memory.
 __device__ __forceinline__ void umma_tile_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_addr, uint32_t idesc, uint32_t accumulate) {
@@ -1375,7 +1387,8 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     const uint32_t t_s = tmem + (static_cast<uint32_t>(quarter * 32) << 16), t_o = t_s + 128;
     uint8_t* out_stage = stage + (warp - 3) * kStageBytes;
     int g = 0;                        // tiles so far
-    bool owns = false;                // the first part of a tile that goes on in other CTAs
+    if (tid == 0)
+      p.joins[blockIdx.x] = 0;        // unless a tile begins here that goes on in other CTAs
     int live = 0;
     for (int n = 0;; ++n) {
       if (!mbar_wait(&part_full[n % kParts], (n / kParts) & 1, &abort_flag, p.status_word, 515))
@@ -1540,7 +1553,6 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
           mine[3 * kManyRows] = me.fix;
           if (tid == 0)
             p.joins[blockIdx.x] = joined_parts;
-          owns = true;
         }
       } else if (alive) {
         const bool none = l == 0.f || me.fix == 0.f;
@@ -1574,8 +1586,6 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       tc_fence_before_sync();
       warp_arrive(&o_free);
     }
-    if (tid == 0 && !owns)
-      p.joins[blockIdx.x] = 0;
   }
 
   tc_fence_before_sync();
@@ -1586,22 +1596,24 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
   }
 }
 
-// Tiles whose parts lie in several CTAs of the many-rows kernel: the parts, in their order, added up.  A block has the tile that
-// begins in CTA blockIdx.x (if one goes on from there) and eight head dimensions, a thread a row.  (The CTA that finishes last
-// took 76 us to do this alone with 19 parts; blocks of 32 dimensions 15 us.)
-constexpr int kJoinDims = 8;
-__global__ void __launch_bounds__(kManyRows) fp8_join_kernel(const FewParams p) {
+// Tiles whose parts lie in several CTAs: the parts, in their order, added up.  A block has the tile that begins in CTA blockIdx.x
+// (if one goes on from there), a thread a row and eight head dimensions.  (The CTA that finishes last took 76 us to do this alone
+// with 19 parts of 128 rows; blocks of 32 dimensions 15 us.)
+constexpr int kJoinThreads = 128, kJoinDims = 8;
+template <int ROWS>
+__global__ void __launch_bounds__(kJoinThreads) fp8_join_kernel(const FewParams p) {
   pdl_wait();
   pdl_trigger();
-  const int owner = blockIdx.x, row = threadIdx.x, c0 = blockIdx.y * kJoinDims;
+  constexpr int kPart = part_floats(ROWS);
+  const int owner = blockIdx.x, row = threadIdx.x % ROWS, c0 = (blockIdx.y * (kJoinThreads / ROWS) + threadIdx.x / ROWS) * kJoinDims;
   const int parts = __ldcg(p.joins + owner);
   if (parts == 0)
     return;
-  const float* one = p.parts + (2 * static_cast<int64_t>(owner) + 1) * kManyPart + row;
-  const float* rest = p.parts + 2 * static_cast<int64_t>(owner) * kManyPart + row;
-  auto part = [&](int i) { return i == 0 ? one : rest + 2 * static_cast<int64_t>(i) * kManyPart; };
-  constexpr int kRef = kManyRows * kD;
-  const int out = __float_as_int(__ldcg(one + kRef + 2 * kManyRows));
+  const float* one = p.parts + (2 * static_cast<int64_t>(owner) + 1) * kPart + row;
+  const float* rest = p.parts + 2 * static_cast<int64_t>(owner) * kPart + row;
+  auto part = [&](int i) { return i == 0 ? one : rest + 2 * static_cast<int64_t>(i) * kPart; };
+  constexpr int kRef = ROWS * kD;
+  const int out = __float_as_int(__ldcg(one + kRef + 2 * ROWS));
   if (out < 0)
     return;
   float top = kNothing, l = 0.f, o[kJoinDims] = {};
@@ -1612,12 +1624,12 @@ __global__ void __launch_bounds__(kManyRows) fp8_join_kernel(const FewParams p) 
   for (int i = 0; i < parts; ++i) {
     const float* src = part(i);
     const float f = exp2f(__ldcg(src + kRef) - top);
-    l = fmaf(__ldcg(src + kRef + kManyRows), f, l);
+    l = fmaf(__ldcg(src + kRef + ROWS), f, l);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      o[j] = fmaf(__ldcg(src + (c0 + j) * kManyRows), f, o[j]);
+      o[j] = fmaf(__ldcg(src + (c0 + j) * ROWS), f, o[j]);
   }
-  const float fix = __ldcg(one + kRef + 3 * kManyRows);
+  const float fix = __ldcg(one + kRef + 3 * ROWS);
   const bool none = l == 0.f || fix == 0.f;
   const float mul = __fdividef(fix, l);
 #pragma unroll
@@ -1671,9 +1683,9 @@ __global__ void __launch_bounds__(128) fp8_spans_kernel(const Fp8AttnParams p, i
 // The kernel for a call.  Up to kFewMost (listed row, query head) pairs a sequence and key head the few-rows kernel is taken, with a
 // pass over the keys for each 32 of them; so it is for more of them where the caches are short (their rows are all that the host
 // knows of the keys): tiles of up to 8 units, which it does not split, and at most ten units a CTA.  Few against many, us:
-//   26 pairs (16 x 512 keys, 32 heads) 30 : 63; 64 there 52 : 68; 64, capped, over 8 x 4096 keys 90 : 139; 64 over 2 x 32011 129 : 102
+//   26 pairs (16 x 512 keys, 32 heads) 30 : 63; 64 there 52 : 68; 64 over 8 x 4096 keys 88 : 101, capped 92 : 139; over 2 x 32011 84 : 96
 //   77 (175 keys, 4 key heads) 13 : 30; 84 (32 x 601, 4) 31 : 35; 140 there 36 : 44; 96 (2 x 1001, 8) 25 : 27
-//   96 (2 x 4001 keys, 8 key heads) 51 : 37; 90 (16 x 512, 32) 73 : 71; 128 there 96 : 74
+//   96 (2 x 32011 keys, 8 key heads) 103 : 98, biased 128 : 103; 90 (16 x 512, 32) 74 : 70; 128 there 96 : 74
 constexpr int kFewMost = 64;
 bool takes_many(int64_t max_rows, int64_t num_salient, int64_t batch, int64_t group, int64_t kv_heads, int64_t cache_rows, int64_t ctas) {
   const int64_t most = min(max_rows, num_salient) * group;
@@ -1681,6 +1693,15 @@ bool takes_many(int64_t max_rows, int64_t num_salient, int64_t batch, int64_t gr
     return false;
   const int64_t tiles = (min(most, (num_salient * group + batch - 1) / batch) + kRows - 1) / kRows;
   return cache_rows > 8 * kUnitKeys * batch || (cache_rows / kUnitKeys + batch) * tiles * kv_heads > 10 * kFewCtas * ctas;
+}
+
+// Whether the few-rows kernel leaves the joins to a launch: where a tile of average length will have more than six parts.  The CTA
+// that finishes last adds them up in 1 us each: 2 x 32011 keys, 8 key heads, 32 pairs (37 parts) 121 us against 72 with the launch,
+// 64 pairs (18 parts) 112 against 84.
+bool joins_later(int64_t max_rows, int64_t num_salient, int64_t batch, int64_t group, int64_t kv_heads, int64_t cache_rows, int64_t ctas) {
+  const int64_t most = min(min(max_rows, num_salient) * group, (num_salient * group + batch - 1) / batch);
+  const int64_t tiles = (most + kRows - 1) / kRows * batch * kv_heads;
+  return min(cache_rows / kUnitKeys / batch / kMinPartFew, kFewCtas * ctas / tiles) > 6;
 }
 
 // Workspace: tickets, keys per tile (only with ranges), parts of tiles; for the kernel that needs most.
@@ -1716,20 +1737,24 @@ int launch_rows(Kernel kernel, bool (&set)[64], int threads, uint32_t smem, cons
   DYLLM_LAUNCH(kernel, ctas, threads, smem, s, tk, tv, p);
   return check_launch("attention_salient_rows_fp8");
 }
+template <int ROWS>
+int launch_join(const FewParams& p, int ctas, cudaStream_t s) {
+  DYLLM_LAUNCH(fp8_join_kernel<ROWS>, dim3(ctas, kD / kJoinDims * ROWS / kJoinThreads), kJoinThreads, 0, s, p);
+  return check_launch("attention_salient_rows_fp8");
+}
 template <bool CAP, bool BIAS>
 int launch_few(const CUtensorMap& tk, const CUtensorMap& tv, const FewParams& p, int ctas, cudaStream_t s) {
   static bool set[64] = {};
-  return launch_rows(fp8_few_rows_kernel<CAP, BIAS>, set, kFewThreads, kFewSmem, tk, tv, p, grid_of(p.a, kRows, kMinPartFew, kFewCtas * ctas), s);
+  const int grid = grid_of(p.a, kRows, kMinPartFew, kFewCtas * ctas);
+  const int rc = launch_rows(fp8_few_rows_kernel<CAP, BIAS>, set, kFewThreads, kFewSmem, tk, tv, p, grid, s);
+  return rc == DYLLM_OK && p.later ? launch_join<kRows>(p, grid, s) : rc;
 }
 template <bool CAP, bool BIAS>
 int launch_many(const CUtensorMap& tk, const CUtensorMap& tv, const FewParams& p, int ctas, cudaStream_t s) {
   static bool set[64] = {};
   const int grid = grid_of(p.a, kManyRows, kMinPartMany, kManyCtas * ctas);
   const int rc = launch_rows(fp8_many_rows_kernel<CAP, BIAS>, set, kManyThreads, kManySmem, tk, tv, p, grid, s);
-  if (rc != DYLLM_OK)
-    return rc;
-  DYLLM_LAUNCH(fp8_join_kernel, dim3(grid, kD / kJoinDims), kManyRows, 0, s, p);
-  return check_launch("attention_salient_rows_fp8");
+  return rc == DYLLM_OK ? launch_join<kManyRows>(p, grid, s) : rc;
 }
 
 }  // namespace
@@ -1819,13 +1844,14 @@ int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, co
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   f.a = p;
-  f.tickets = reinterpret_cast<unsigned long long*>(ws);      // few rows
-  f.joins = reinterpret_cast<int*>(ws);                       // many rows
+  f.tickets = reinterpret_cast<unsigned long long*>(ws);
+  f.joins = reinterpret_cast<int*>(ws);                       // or these
   int2* spans = reinterpret_cast<int2*>(ws + kMostCtas * ctas * sizeof(unsigned long long));
   f.parts = reinterpret_cast<float*>(ws + parts_offset(tiles, kMostCtas * ctas));
   f.launch_id = next_launch_id() & ~0xffffull;
   f.status_word = device_status_word();
   // a sequence with more rows than the bound says is served by either kernel; so is one with few beside others with many
+  f.later = joins_later(max_rows_per_seq, num_salient, batch, group, num_kv_heads, k_rows, ctas);
   const bool many = takes_many(max_rows_per_seq, num_salient, batch, group, num_kv_heads, k_rows, ctas);
   if (p.ranges) {
     f.spans = spans;
