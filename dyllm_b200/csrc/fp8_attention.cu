@@ -412,6 +412,7 @@ constexpr float kNothing = -1.0e30f;      // maximum of no scores (finite: it ta
 struct RowInfo {
   int out;                     // output row, -1: none
   float fix;                   // 1; 0: the row does not exist in q; NaN: the query is not finite
+  float mul;                   // scale of the query's codes (bits of its largest magnitude until that is worked out)
   float slope;                 // times log2(e)
   int pos, lo, hi;             // the row's place in its sequence, the keys that it sees
 };
@@ -462,6 +463,11 @@ __device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
   return floats2(r);
 }
+__device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
+  return floats2(r);
+}
 __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
@@ -493,8 +499,9 @@ __device__ __forceinline__ void split_weights_e5m2(float2 a, float2 b, uint32_t&
 // The products are transposed, keys (then head dimensions) in the M = 128 of tcgen05.mma.kind::f8f6f4:
 //   S^T = K Q^T         A: K tile as loaded (K-major), B: the queries as e4m3 + e5m2, two products into one accumulator
 //   O^T = V^T P^T       A: V tile as loaded (MN-major), B: the weights as e4m3 + e5m2, two products into one accumulator
-// A query in bf16 (8 significant bits) is e4m3 (4 bits) plus a remainder of at most 3 bits, which e5m2 holds exactly down to
-// 2^-25 of the tile's largest element.  A weight is 64 * 2^(t - reference), as with many rows: off by 2^-7 of itself or by 2^-23 of
+// A query in bf16 (8 significant bits) is e4m3 (4 bits) plus a remainder of at most 3 bits in e5m2, next to a power of two of its own
+// row: exact down to 2^-14.8 of the row's largest element (below that e4m3 runs out of bits), off by 2^-21.8 of it at most.  A
+// weight is 64 * 2^(t - reference), as with many rows: off by 2^-7 of itself or by 2^-23 of
 // the largest.  The codes of the cache are never widened.
 //
 // Four softmax warps, thread = key with the scores of all rows in registers; a row's reference is in shared memory and follows the
@@ -537,12 +544,12 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
   uint8_t* q_smem = p_smem + kPBytes;                        // [32 rows][128] e4m3, then e5m2
   __shared__ uint64_t full[kFewRing], empty[kFewRing], part_full[kParts], part_done[kParts], q_asked, q_full, s_full[2], p_full, pv_done, o_free;
   __shared__ PartInfo s_part[kParts];
-  __shared__ uint32_t tmem_slot, s_top[kFewWarps];
+  __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag, joins;
   __shared__ int s_out[kRows];                               // output row, -1: none
   __shared__ int2 s_sees[kRows], s_all[kFewWarps];           // keys that a row sees, that all rows see (of a quarter of them)
   __shared__ __align__(16) float2 s_bias[kRows];             // slope times log2(e), place in the sequence counted from the part's first key
-  __shared__ __align__(16) float s_fix[kRows], s_max[kFewWarps][kRows], s_sum[kFewWarps][kRows], s_ref[kFewWarps][kRows], s_old[kFewWarps][kRows];      // a copy for each warp
+  __shared__ __align__(16) float s_fix[kRows], s_mul[kRows], s_max[kFewWarps][kRows], s_sum[kFewWarps][kRows], s_ref[kFewWarps][kRows], s_old[kFewWarps][kRows];      // a copy for each warp
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -721,9 +728,8 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
         ks_next = __ldg(k_scale + static_cast<int64_t>(begin + kl) * a.Hkv);
         vs_next = __ldg(v_scale + static_cast<int64_t>(begin + kl) * a.Hkv);
       }
-      // queries: eight threads a row, rows tid / 8 and 16 + tid / 8; codes next to the tile's largest element (an error of 2^-26
-      // of it moves every score of the tile by as little), e4m3 and the e5m2 rest
-      float q_scale;
+      // queries: eight threads a row, rows tid / 8 and 16 + tid / 8; codes next to the row's own largest element, e4m3 and the e5m2
+      // rest
       {
         uint4 x0[2], x1[2];
         int at[2], head[2], t[2];
@@ -746,36 +752,27 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
         }
         if (u == 0)
           warp_arrive(&q_asked);
-        bool finite[2];
-        uint32_t top = 0;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t m = fp8_amax8(max(bf16x8_amax(x0[h]), bf16x8_amax(x1[h])));
-          finite[h] = m < 0x7f800000u;
-          top = max(top, finite[h] ? m : 0u);
-        }
-        top = __reduce_max_sync(0xffffffffu, top);
-        if (lane == 0)
-          s_top[quarter] = top;
-        rows_sync();
-        const uint32_t scale = fp8_scale_bits(max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3])));
-        const float inv = fp8_inverse(scale);
-        q_scale = __uint_as_float(scale);
         int2 sees = make_int2(0, end);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int r = 16 * h + (tid >> 3);
-          if (!finite[h])
+          uint32_t top = fp8_amax8(max(bf16x8_amax(x0[h]), bf16x8_amax(x1[h])));
+          const bool finite = top < 0x7f800000u;
+          if (!finite) {
             x0[h] = x1[h] = make_uint4(0u, 0u, 0u, 0u);
+            top = 0;
+          }
+          const uint32_t scale = fp8_scale_bits(top);
           uint4 hi, lo;
-          split_query(x0[h], x1[h], inv, hi, lo);
+          split_query(x0[h], x1[h], fp8_inverse(scale), hi, lo);
           uint8_t* dst = q_smem + r * kD + (((tid & 7) ^ (r & 7)) << 4);
           *reinterpret_cast<uint4*>(dst) = hi;
           *reinterpret_cast<uint4*>(dst + kQBytes) = lo;
           if ((tid & 7) == 0) {
             s_out[r] = t[h] < part.rows ? (part.row0 + t[h] / group) * a.H + head[h] : -1;
             // 1; 0: the row does not exist in q; NaN: the query is not finite
-            s_fix[r] = at[h] < 0 ? 0.f : finite[h] ? 1.f : __uint_as_float(0x7fc00000u);
+            s_fix[r] = at[h] < 0 ? 0.f : finite ? 1.f : __uint_as_float(0x7fc00000u);
+            s_mul[r] = __uint_as_float(scale);
             if (BIAS && at[h] >= 0) {
               const int pos = __ldg(a.cu_k + part.b + 1) - __ldg(a.cu_k + part.b) - (__ldg(a.cu_q + part.b + 1) - at[h]);
               s_bias[r] = make_float2(__ldg(a.slopes + head[h]) * kLog2e, static_cast<float>(pos - begin));
@@ -801,7 +798,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
         rows_sync();
       }
       // scores come out times log2(e), or as twice the argument of the tanh that caps them
-      const float key_mul = a.scale * q_scale * kLog2e * (CAP ? 2.f / a.cap : 1.f);
+      const float key_mul = a.scale * kLog2e * (CAP ? 2.f / a.cap : 1.f);
       const int all_from = max(max(s_all[0].x, s_all[1].x), max(s_all[2].x, s_all[3].x));
       const int all_to = min(min(s_all[0].y, s_all[1].y), min(s_all[2].y, s_all[3].y));
       const int tiles = (end - begin + kUnitKeys - 1) / kUnitKeys;
@@ -823,17 +820,26 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
         tmem_ld_wait();
         // scores (times log2 e, plus the exponents of the values' scales)
 #pragma unroll
-        for (int r = 0; r < kRows; r += 2) {
+        for (int r = 0; r < kRows; r += 4) {
+          // the factors of row and key first: their product is within the type's range wherever the score is
+          const float4 row = *reinterpret_cast<const float4*>(s_mul + r);
+          const float2 m0 = fmul2(make_float2(row.x, row.y), make_float2(kk, kk)), m1 = fmul2(make_float2(row.z, row.w), make_float2(kk, kk));
           if (CAP) {
-            t[r] = fmaf(capped(t[r] * kk, a.cap), kLog2e, ex);
-            t[r + 1] = fmaf(capped(t[r + 1] * kk, a.cap), kLog2e, ex);
+            t[r] = fmaf(capped(t[r] * m0.x, a.cap), kLog2e, ex);
+            t[r + 1] = fmaf(capped(t[r + 1] * m0.y, a.cap), kLog2e, ex);
+            t[r + 2] = fmaf(capped(t[r + 2] * m1.x, a.cap), kLog2e, ex);
+            t[r + 3] = fmaf(capped(t[r + 3] * m1.y, a.cap), kLog2e, ex);
           } else {
-            put2(t + r, ffma2(get2(t + r), make_float2(kk, kk), make_float2(ex, ex)));
+            put2(t + r, ffma2(get2(t + r), m0, make_float2(ex, ex)));
+            put2(t + r + 2, ffma2(get2(t + r + 2), m1, make_float2(ex, ex)));
           }
           if (BIAS) {
-            const float4 row = *reinterpret_cast<const float4*>(s_bias + r);
-            t[r] = fmaf(-row.x, fabsf(row.y - place), t[r]);
-            t[r + 1] = fmaf(-row.z, fabsf(row.w - place), t[r + 1]);
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+              const float4 b = *reinterpret_cast<const float4*>(s_bias + r + e);
+              t[r + e] = fmaf(-b.x, fabsf(b.y - place), t[r + e]);
+              t[r + e + 1] = fmaf(-b.z, fabsf(b.w - place), t[r + e + 1]);
+            }
           }
         }
         if (at - kl < all_from || at - kl + kUnitKeys > all_to) {      // not all rows see all keys
@@ -1054,6 +1060,7 @@ constexpr int kManyRing = 4;                                 // slots of one K o
 constexpr int kScaleSlots = 2;                               // tiles whose scales are staged ahead
 constexpr int kManyWarps = 4, kManyThreads = 32 * (3 + kManyWarps + 4);
 constexpr int kManyCtas = 2;                                 // per SM
+// (Dynamic, static and the system's shared memory of two CTAs leave 128 bytes: more of it, and there is one CTA per SM, 157 us for 110.)
 constexpr uint32_t kManyTmemCols = 256;
 constexpr uint32_t kStageBytes = 32 * 64;                    // of a softmax warp: 32 head dimensions of its rows
 constexpr uint32_t kManyQBytes = kManyRows * kD;             // e4m3 or e5m2 part of the queries of a tile
@@ -1091,11 +1098,10 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
   __shared__ uint64_t full[kManyRing], empty[kManyRing], part_full[kParts], part_done[kParts], q_full, q_free, s_full, p_full, pv_done, o_free,
       sc_full[kScaleSlots], sc_free[kScaleSlots];
   __shared__ PartInfo s_part[kParts];
-  __shared__ uint32_t tmem_slot, s_amax[2];
+  __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   __shared__ RowInfo s_row[kManyRows];
   __shared__ int64_t s_src[kManyRows];
-  __shared__ uint32_t s_bad[4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -1234,7 +1240,7 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     const int tid = threadIdx.x - 32 * (3 + kManyWarps);
     int n_sc = 0, live = 0;
     for (int n = 0;; ++n) {
-      const int slot = n % kParts, qb = live & 1;
+      const int slot = n % kParts;
       if (rows_any(!mbar_wait(&part_full[slot], (n / kParts) & 1, &abort_flag, p.status_word, 510)))
         break;
       const PartInfo w = s_part[slot];
@@ -1282,13 +1288,9 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         first_v = __ldg(vs + static_cast<int64_t>(w.begin + tid) * a.Hkv);
       }
       s_src[tid] = src;
-      if (tid == 0)
-        s_amax[qb] = 0;
-      if (tid < 4)
-        s_bad[tid] = 0;
       rows_sync();
-      // queries: eight threads a row, 16 rows at a time, four times 16 in flight; first the largest element, then (from L1) the
-      // codes.  (Loops: straight-line code for 128 rows that runs once a part costs more in instruction fetches than it saves.)
+      // queries: eight threads a row, 16 rows at a time, four times 16 in flight; codes next to the row's own largest element.
+      // (Loops: straight-line code for 128 rows that runs once a part costs more in instruction fetches than it saves.)
       uint4 x0[4], x1[4];
       auto fetch = [&](int h) {
 #pragma unroll
@@ -1302,28 +1304,8 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
           }
         }
       };
-      uint32_t top = 0;
-#pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
-        fetch(h);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int r = 64 * h + 16 * k + (tid >> 3);
-          const uint32_t m = fp8_amax8(max(bf16x8_amax(x0[k]), bf16x8_amax(x1[k])));
-          if (m < 0x7f800000u)
-            top = max(top, m);
-          else if ((tid & 7) == 0)
-            atomicOr(&s_bad[r >> 5], 1u << (r & 31));
-        }
-      }
-      top = __reduce_max_sync(0xffffffffu, top);
-      if (lane == 0)
-        atomicMax(&s_amax[qb], top);
-      rows_sync();
-      const uint32_t scale = fp8_scale_bits(s_amax[qb]);
-      const float inv = fp8_inverse(scale);
-      // scores come out times log2(e), or as twice the argument of the tanh that caps them
-      const float mul = a.scale * __uint_as_float(scale) * kLog2e * (CAP ? 2.f / a.cap : 1.f);
+      // scores come out times log2(e), or as twice the argument of the tanh that caps them, but for the row's factor
+      const float mul = a.scale * kLog2e * (CAP ? 2.f / a.cap : 1.f);
       auto deposit = [&](float k, float v) {
         const int sl = n_sc % kScaleSlots;
         if (n_sc >= kScaleSlots)
@@ -1336,26 +1318,34 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         warp_arrive(&sc_full[sl]);
         ++n_sc;
       };
+      fetch(0);
       deposit(first_k, first_v);
       if (live > 0)
         mbar_wait(&q_free, (live - 1) & 1, &abort_flag, p.status_word, 511);
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {
-        fetch(h);
+        if (h)
+          fetch(h);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int r = 64 * h + 16 * k + (tid >> 3), part = tid & 7;
-          if (s_bad[r >> 5] >> (r & 31) & 1)
+          const uint32_t top = fp8_amax8(max(bf16x8_amax(x0[k]), bf16x8_amax(x1[k])));
+          if (part == 0)
+            s_row[r].mul = __uint_as_float(top);
+          if (top >= 0x7f800000u)
             x0[k] = x1[k] = make_uint4(0u, 0u, 0u, 0u);
           uint4 hi, lo;
-          split_query(x0[k], x1[k], inv, hi, lo);
+          split_query(x0[k], x1[k], fp8_inverse(fp8_scale_bits(top)), hi, lo);
           uint8_t* dst = q_smem + r * kD + ((part ^ (r & 7)) << 4);
           *reinterpret_cast<uint4*>(dst) = hi;
           *reinterpret_cast<uint4*>(dst + kManyQBytes) = lo;
         }
       }
-      if (s_bad[tid >> 5] >> (tid & 31) & 1)
+      rows_sync();
+      const uint32_t top = __float_as_uint(s_row[tid].mul);
+      if (top >= 0x7f800000u)
         v.fix = __uint_as_float(0x7fc00000u);
+      v.mul = __uint_as_float(fp8_scale_bits(top >= 0x7f800000u ? 0u : top));
       s_row[tid] = v;
       fence_proxy_async_smem();
       rows_sync();
@@ -1439,11 +1429,13 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
               for (int j = 0; j < 16; j += 4) {
                 const float4 kk = *reinterpret_cast<const float4*>(sc + c * 32 + h * 16 + j);
                 const float4 ex = *reinterpret_cast<const float4*>(sc + kUnitKeys + c * 32 + h * 16 + j);
+                // the factors of row and key first: their product is within the type's range wherever the score is
+                const float2 f = fmul2(make_float2(kk.x, kk.y), make_float2(me.mul, me.mul)), g2 = fmul2(make_float2(kk.z, kk.w), make_float2(me.mul, me.mul));
                 if (!CAP) {
-                  put2(t + j, ffma2(get2(t + j), make_float2(kk.x, kk.y), make_float2(ex.x, ex.y)));
-                  put2(t + j + 2, ffma2(get2(t + j + 2), make_float2(kk.z, kk.w), make_float2(ex.z, ex.w)));
+                  put2(t + j, ffma2(get2(t + j), f, make_float2(ex.x, ex.y)));
+                  put2(t + j + 2, ffma2(get2(t + j + 2), g2, make_float2(ex.z, ex.w)));
                 } else {
-                  const float k4[4] = {kk.x, kk.y, kk.z, kk.w}, e4[4] = {ex.x, ex.y, ex.z, ex.w};
+                  const float k4[4] = {f.x, f.y, g2.x, g2.y}, e4[4] = {ex.x, ex.y, ex.z, ex.w};
 #pragma unroll
                   for (int e = 0; e < 4; ++e)
                     t[j + e] = fmaf(capped(t[j + e] * k4[e], a.cap), kLog2e, e4[e]);
