@@ -204,6 +204,9 @@ def attention_salient_rows_fp8(q, k_cache, v_cache, k_seq_starts, v_seq_starts, 
     product.  ``max_rows_per_seq``: bound (or estimate) of a sequence's listed rows; it chooses between two kernels, which serve
     any number (0: nothing is computed).  Returns ``[num_salient, heads, 128]`` in list order; rows past ``cu_salientlens[-1]``
     are left untouched.
+
+    Scores and sums are in fp32, a weight in half precision (2^-11 of itself, or 2^-28 of the row's largest); an element of a
+    query below 2^-14.8 of the row's largest is off by up to 2^-21.8 of that.
     """
     out = native().attention(q, k_cache, v_cache, k_seq_starts, v_seq_starts, seq_ids, cu_seqlens_q, cu_seqlens_k, cu_salientlens,
                              idx_salient_row, max_rows_per_seq, scale, softcap, slopes, key_ranges, num_salient, out)

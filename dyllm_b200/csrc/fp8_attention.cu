@@ -75,8 +75,8 @@ constexpr int kManyRows = 128;                               // and of the many-
 // A part in the workspace: [dimension][row] sums, [row] references, sums of weights; of a first part also output rows and `fix`.
 __host__ __device__ constexpr int part_floats(int rows) { return rows * (kD + 4); }
 constexpr int kFewPart = part_floats(kRows), kManyPart = part_floats(kManyRows);
-constexpr float kWeightLog2 = 6.f;                           // the reference's weight: 2^6
-constexpr float kHeadroom = 2.8f;                            // 2^(6 + 2.8) < 448
+constexpr float kWeightLog2 = 12.f;                          // the reference's weight: 2^12
+constexpr float kHeadroom = 2.8f;                            // 2^(12 + 2.8) < 57344, the largest e5m2 number
 
 struct FewParams {
   Fp8AttnParams a;
@@ -473,17 +473,34 @@ __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
   return floats2(r);
 }
+// A row's reference for scores up to mx: weights are 2^(t - reference).  2^12 for the largest, but 1 where mx is so large (2^27) that
+// their difference would be rounded up past the largest e5m2 number.
+__device__ __forceinline__ float reference(float mx) {
+  const float ref = mx - kWeightLog2;
+  return mx - ref > kHeadroom + kWeightLog2 ? mx : ref;
+}
 // The lowest n bits.
 __device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
-// Four weights as codes, and what they leave in e5m2.  By way of half precision (2^-11).
-__device__ __forceinline__ void split_weights_e5m2(float2 a, float2 b, uint32_t& hi, uint32_t& lo) {
-  const __half2 x = __floats2half2_rn(a.x, a.y), y = __floats2half2_rn(b.x, b.y);
-  const uint32_t h0 = fp8_pack_half2(*reinterpret_cast<const uint32_t*>(&x)), h1 = fp8_pack_half2(*reinterpret_cast<const uint32_t*>(&y));
-  const uint32_t u = fp8_to_half2(h0), v = fp8_to_half2(h1);
-  const __half2 r = __hsub2(x, *reinterpret_cast<const __half2*>(&u)), s = __hsub2(y, *reinterpret_cast<const __half2*>(&v));
-  hi = __byte_perm(h0, h1, 0x5410);
-  lo = __byte_perm(fp8_pack_half2_e5m2(*reinterpret_cast<const uint32_t*>(&r)), fp8_pack_half2_e5m2(*reinterpret_cast<const uint32_t*>(&s)), 0x5410);
+// Four weights, rounded to half precision (2^-11), as three codes in e5m2 each, which are the high bytes of half-precision numbers:
+// the number, what that leaves, what that leaves, the first two rounded by adding half a step.  Eleven bits in three codes of three
+// bits and two signs: their sum is the half-precision number, exactly down to 2^-6 (below, the last one's steps of 2^-16).
+__device__ __forceinline__ void split_weights(float2 a, float2 b, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+  const __half2 x[2] = {__floats2half2_rn(a.x, a.y), __floats2half2_rn(b.x, b.y)};
+  uint32_t h[2], m[2], l[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    h[i] = *reinterpret_cast<const uint32_t*>(&x[i]) + 0x00800080u;
+    const uint32_t u = h[i] & 0xff00ff00u;
+    const __half2 r = __hsub2(x[i], *reinterpret_cast<const __half2*>(&u));
+    m[i] = *reinterpret_cast<const uint32_t*>(&r) + 0x00800080u;
+    const uint32_t v = m[i] & 0xff00ff00u;
+    const __half2 q = __hsub2(r, *reinterpret_cast<const __half2*>(&v));      // a NaN ends up here
+    l[i] = *reinterpret_cast<const uint32_t*>(&q);
+  }
+  hi = __byte_perm(h[0], h[1], 0x7531);
+  mid = __byte_perm(m[0], m[1], 0x7531);
+  lo = __byte_perm(l[0], l[1], 0x7531);
 }
 
 // ----------------------------------------------------------------------------------------------
@@ -498,11 +515,13 @@ __device__ __forceinline__ void split_weights_e5m2(float2 a, float2 b, uint32_t&
 //
 // The products are transposed, keys (then head dimensions) in the M = 128 of tcgen05.mma.kind::f8f6f4:
 //   S^T = K Q^T         A: K tile as loaded (K-major), B: the queries as e4m3 + e5m2, two products into one accumulator
-//   O^T = V^T P^T       A: V tile as loaded (MN-major), B: the weights as e4m3 + e5m2, two products into one accumulator
+//   O^T = V^T P^T       A: V tile as loaded (MN-major), B: the weights as three codes in e5m2, three products into one accumulator
 // A query in bf16 (8 significant bits) is e4m3 (4 bits) plus a remainder of at most 3 bits in e5m2, next to a power of two of its own
 // row: exact down to 2^-14.8 of the row's largest element (below that e4m3 runs out of bits), off by 2^-21.8 of it at most.  A
-// weight is 64 * 2^(t - reference), as with many rows: off by 2^-7 of itself or by 2^-23 of
-// the largest.  The codes of the cache are never widened.
+// weight is 2^12 * 2^(t - reference) in half precision, as with many rows: off by 2^-11 of itself or by 2^-28 of the largest.  (As
+// e4m3 + e5m2 it was off by 2^-8 of itself, or by 2^-20 of the largest: percents of what many small weights beside a large one make
+// up together; 32.0 us for 34.4 at the size below.  Codes cut instead of rounded, 2^-8.4 of a weight: 32.8; conversion instructions
+// instead of added half steps: 34.8.)  The codes of the cache are never widened.
 //
 // Four softmax warps, thread = key with the scores of all rows in registers; a row's reference is in shared memory and follows the
 // maximum in steps, so that a unit costs one barrier (does any score exceed its reference by more than 2.8?) and the maxima are
@@ -514,7 +533,8 @@ constexpr int kFewRing = 2;                                  // slots of one K o
 constexpr int kFewCtas = 4;                                  // per SM
 constexpr int kFewWarps = 4, kFewThreads = 32 * (3 + kFewWarps);
 constexpr uint32_t kFewTmemCols = 128, kQBytes = kRows * kD, kPBytes = kUnitKeys * 64;
-constexpr uint32_t kFewSmem = kFewRing * kTileBytes + kPBytes + 2 * kQBytes + 1024;
+constexpr uint32_t kP3Bytes = kPBytes / 2;
+constexpr uint32_t kFewSmem = kFewRing * kTileBytes + kPBytes + 2 * kQBytes + kP3Bytes + 1024;      // four CTAs per SM have 55 KB each with the static part
 
 // Sum of each of 32 values over the lanes of a warp: lane l gets that of value l.
 __device__ __forceinline__ float sum_lanes(float (&v)[32]) {
@@ -540,8 +560,9 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
   const Fp8AttnParams& a = p.a;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* p_smem = ring + kFewRing * kTileBytes;            // [128 keys][32 e4m3, 32 e5m2], 64-byte swizzle
+  uint8_t* p_smem = ring + kFewRing * kTileBytes;            // first and second codes of the weights: [128 keys][32, 32], 64-byte swizzle
   uint8_t* q_smem = p_smem + kPBytes;                        // [32 rows][128] e4m3, then e5m2
+  uint8_t* p3_smem = q_smem + 2 * kQBytes;                   // third codes of the weights: [64][keys 0 .., keys 64 .. of 32], 64-byte swizzle
   __shared__ uint64_t full[kFewRing], empty[kFewRing], part_full[kParts], part_done[kParts], q_asked, q_full, s_full[2], p_full, pv_done, o_free;
   __shared__ PartInfo s_part[kParts];
   __shared__ uint32_t tmem_slot;
@@ -549,7 +570,8 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
   __shared__ int s_out[kRows];                               // output row, -1: none
   __shared__ int2 s_sees[kRows], s_all[kFewWarps];           // keys that a row sees, that all rows see (of a quarter of them)
   __shared__ __align__(16) float2 s_bias[kRows];             // slope times log2(e), place in the sequence counted from the part's first key
-  __shared__ __align__(16) float s_fix[kRows], s_mul[kRows], s_max[kFewWarps][kRows], s_sum[kFewWarps][kRows], s_ref[kFewWarps][kRows], s_old[kFewWarps][kRows];      // a copy for each warp
+  __shared__ __align__(16) float s_fix[kRows], s_mul[kRows], s_max[kFewWarps][kRows], s_ref[kFewWarps][kRows], s_old[kFewWarps][kRows];      // a copy for each warp
+  float (&s_sum)[kFewWarps][kRows] = s_max;                  // the maxima have been read once a part's last unit has been multiplied
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -642,8 +664,8 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer: scores of a unit before the sums of the last
     constexpr uint32_t idesc_hi = umma_idesc_f8(128, kRows, 0, 0, 0, 0), idesc_lo = umma_idesc_f8(128, kRows, 0, 1, 0, 0);
-    constexpr uint32_t idesc_pv = umma_idesc_f8(128, kRows, 0, 0, 1, 1), idesc_pv_lo = umma_idesc_f8(128, kRows, 0, 1, 1, 1);
-    const uint32_t ring_addr = smem_u32(ring), p_addr = smem_u32(p_smem), q_addr = smem_u32(q_smem), t_s = uniform(tmem), t_o = t_s + 64;
+    constexpr uint32_t idesc_pv = umma_idesc_f8(128, kRows, 0, 1, 1, 1);
+    const uint32_t ring_addr = smem_u32(ring), p_addr = smem_u32(p_smem), q_addr = smem_u32(q_smem), p3_addr = smem_u32(p3_smem), t_s = uniform(tmem), t_o = t_s + 64;
     int n = 0, u0 = 0, live = 0;      // tiles of the ring, units before the part, parts that have some
     PartWalk c = {};
     auto scores = [&](int i) {
@@ -682,7 +704,8 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {      // 32 keys: 32 rows of V and of the weights
             umma_tile_b64(t_o, v_addr + kk * 4096, p_addr + kk * 2048, idesc_pv, (i | kk) != 0 ? 1u : 0u);
-            umma_tile_b64(t_o, v_addr + kk * 4096, p_addr + 32 + kk * 2048, idesc_pv_lo, 1u);
+            umma_tile_b64(t_o, v_addr + kk * 4096, p_addr + 32 + kk * 2048, idesc_pv, 1u);
+            umma_tile_b64(t_o, v_addr + kk * 4096, p3_addr + 32 * (kk >> 1) + (kk & 1) * 2048, idesc_pv, 1u);
           }
           umma_commit(&empty[slot]);
           umma_commit(&pv_done);
@@ -803,7 +826,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
       const int all_to = min(min(s_all[0].y, s_all[1].y), min(s_all[2].y, s_all[3].y));
       const int tiles = (end - begin + kUnitKeys - 1) / kUnitKeys;
       float l = 0.f;                               // lane = row: sum of the weights of this quarter's keys
-      float was = kNothing;                        // lane = row: reference less kWeightLog2, as in s_ref
+      float was = kNothing;                        // lane = row: reference, as in s_ref
       float* my_ref = s_ref[quarter];
       for (int i = 0; i < tiles; ++i, ++u) {
         const int at = begin + i * kUnitKeys + kl, buf = u & 1;
@@ -871,7 +894,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
           s_max[quarter][lane] = mx;
           rows_sync();
           mx = fmaxf(fmaxf(s_max[0][lane], s_max[1][lane]), fmaxf(s_max[2][lane], s_max[3][lane]));
-          const float ref = mx > was + (kHeadroom + kWeightLog2) ? mx - kWeightLog2 : was, old = exp2f(was - ref);
+          const float ref = mx - was > kHeadroom + kWeightLog2 ? reference(mx) : was, old = exp2f(was - ref);
           l *= old;
           was = ref;
           my_ref[lane] = ref;
@@ -897,9 +920,10 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
         if (u > 0)
           mbar_wait(&pv_done, (u - 1) & 1, &abort_flag, p.status_word, 411);      // the last ones have been taken
         uint8_t* dst = p_smem + kl * 64;
+        uint8_t* dst3 = p3_smem + (kl & 63) * 64;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          uint32_t hi[4], lo[4];
+          uint32_t hi[4], mid[4], lo[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int r = 16 * h + 4 * j;
@@ -908,10 +932,11 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
             t[r + 1] = exp2f(t[r + 1] - ref.y);
             t[r + 2] = exp2f(t[r + 2] - ref.z);
             t[r + 3] = exp2f(t[r + 3] - ref.w);
-            split_weights_e5m2(make_float2(t[r], t[r + 1]), make_float2(t[r + 2], t[r + 3]), hi[j], lo[j]);
+            split_weights(make_float2(t[r], t[r + 1]), make_float2(t[r + 2], t[r + 3]), hi[j], mid[j], lo[j]);
           }
           *reinterpret_cast<uint4*>(dst + ((h ^ (kl >> 1 & 3)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4*>(dst + (((2 + h) ^ (kl >> 1 & 3)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          *reinterpret_cast<uint4*>(dst + (((2 + h) ^ (kl >> 1 & 3)) << 4)) = make_uint4(mid[0], mid[1], mid[2], mid[3]);
+          *reinterpret_cast<uint4*>(dst3 + (((2 * (kl >> 6) + h) ^ (kl >> 1 & 3)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
         if (at - kl + kUnitKeys > end) {
           // rows of V behind the last key may hold any byte, a NaN times a weight of zero among them
@@ -938,11 +963,11 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
       n_ring += 2 * tiles;
 
       // ---------------------------------------------------------------- thread = head dimension kl of all rows
-      s_sum[quarter][lane] = l;
       const float fix = s_fix[lane];
       float top = was;
       mbar_wait(&pv_done, (u - 1) & 1, &abort_flag, p.status_word, 413);
       tc_fence_after_sync();
+      s_sum[quarter][lane] = l;
       uint32_t ou[kRows];
       float* o = reinterpret_cast<float*>(ou);
       tmem_ld_32x32(t_o, ou);
@@ -1049,10 +1074,10 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
 //
 // Tiles of 128 (listed row, query head) pairs, rows in the M = 128 of the products:
 //   S = Q K^T    A: the queries as e4m3 + e5m2 (two products into one accumulator), B: the K tile as loaded (K-major)
-//   O = P V      A: the weights as e4m3 + e5m2, B: the V tile as loaded (MN-major)
-// Thread = row in four softmax warps.  A weight is 64 * 2^(t - reference); the reference follows the maximum in steps, so that the
-// sums are rescaled only where a score lies more than 2.8 (log2) above it.  A weight is off by 2^-7 of itself or by 2^-23 of the
-// largest.  Scores and weights share 128 columns of tensor memory (32 keys' weights, e4m3 then e5m2, lie in the first 16 of their
+//   O = P V      A: the weights as three codes in e5m2, B: the V tile as loaded (MN-major)
+// Thread = row in four softmax warps.  A weight is 2^12 * 2^(t - reference); the reference follows the maximum in steps, so that the
+// sums are rescaled only where a score lies more than 2.8 (log2) above it.  A weight is off by 2^-11 of itself or by 2^-28 of the
+// largest.  Scores and weights share 128 columns of tensor memory (the three codes of 32 keys' weights lie in the first 24 of their
 // scores' 32 columns), so the steps of one tile follow one another; two CTAs per SM, each with parts of its own, fill each other's
 // waits, the ends of parts among them.  Four loader warps stage the queries of the next part and the scales of the next tiles.
 // ----------------------------------------------------------------------------------------------
@@ -1189,7 +1214,7 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer
     constexpr uint32_t idesc_hi = umma_idesc_f8(128, 128, 0, 0, 0, 0), idesc_lo = umma_idesc_f8(128, 128, 1, 0, 0, 0);
-    constexpr uint32_t idesc_pv = umma_idesc_f8(128, 128, 0, 0, 0, 1), idesc_pv_lo = umma_idesc_f8(128, 128, 1, 0, 0, 1);
+    constexpr uint32_t idesc_pv = umma_idesc_f8(128, 128, 1, 0, 0, 1);
     const uint32_t ring_addr = smem_u32(ring), q_addr = smem_u32(q_smem), t_s = uniform(tmem), t_o = t_s + 128;
     int g = 0, live = 0;      // tiles, parts that have some
     PartWalk c = {};
@@ -1222,9 +1247,10 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         if (elect_one()) {
           const uint32_t v_addr = ring_addr + vs * kTileBytes;
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {      // 32 keys: 8 columns of weights, 32 rows of V
+          for (int kk = 0; kk < 4; ++kk) {      // 32 keys: three times 8 columns of weights, 32 rows of V
             umma_tile_ts(t_o, t_s + 32 * kk, v_addr + kk * 4096, idesc_pv, i == 0 && kk == 0 ? 0u : 1u);
-            umma_tile_ts(t_o, t_s + 32 * kk + 8, v_addr + kk * 4096, idesc_pv_lo, 1u);
+            umma_tile_ts(t_o, t_s + 32 * kk + 8, v_addr + kk * 4096, idesc_pv, 1u);
+            umma_tile_ts(t_o, t_s + 32 * kk + 16, v_addr + kk * 4096, idesc_pv, 1u);
           }
           umma_commit(&empty[vs]);
           umma_commit(&pv_done);
@@ -1458,10 +1484,11 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
             }
           }
           tmem_st_wait();
-          grown = mx > ref + kHeadroom;
+          grown = mx - ref > kHeadroom + kWeightLog2;
           if (grown) {
-            old = exp2f(ref - mx);
-            ref = mx;
+            old = ref;
+            ref = reference(mx);
+            old = exp2f(old - ref);
           }
           if (key0 > begin && __any_sync(0xffffffffu, grown)) {
 #pragma unroll 1
@@ -1476,13 +1503,12 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
             }
             tmem_st_wait();
           }
-          const float shift = kWeightLog2 - ref;
-          const float2 shift2 = make_float2(shift, shift);
+          const float2 shift2 = make_float2(-ref, -ref);
           float2 sum = make_float2(l * old, 0.f);
           tmem_ld_32x16(t_s, s[0]);
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
-            uint32_t codes[16];      // e4m3 of 32 keys, then e5m2
+            uint32_t codes[16], third[8];      // first codes of 32 keys, second, third
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               tmem_ld_wait();
@@ -1497,10 +1523,11 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
                 y = make_float2(exp2f(y.x), exp2f(y.y));
                 sum = ffma2(x, make_float2(inv.x, inv.y), sum);
                 sum = ffma2(y, make_float2(inv.z, inv.w), sum);
-                split_weights_e5m2(x, y, codes[h * 4 + j], codes[8 + h * 4 + j]);
+                split_weights(x, y, codes[h * 4 + j], codes[8 + h * 4 + j], third[h * 4 + j]);
               }
             }
             tmem_st_32x16(t_s + c * 32, codes);
+            tmem_st_32x8(t_s + c * 32 + 16, third);
           }
           tmem_st_wait();
           l = sum.x + sum.y;

@@ -23,17 +23,6 @@ __device__ __forceinline__ uint32_t fp8_pack2(float lo, float hi) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(hi), "f"(lo));
   return d;
 }
-// Two half-precision numbers to two codes.
-__device__ __forceinline__ uint32_t fp8_pack_half2(uint32_t h) {
-  uint16_t d;
-  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(d) : "r"(h));
-  return d;
-}
-__device__ __forceinline__ uint32_t fp8_pack_half2_e5m2(uint32_t h) {
-  uint16_t d;
-  asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(d) : "r"(h));
-  return d;
-}
 // Two floats to two codes in e5m2.
 __device__ __forceinline__ uint32_t fp8_pack2_e5m2(float lo, float hi) {
   uint16_t d;
