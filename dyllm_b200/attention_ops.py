@@ -197,7 +197,7 @@ def attention_salient_rows_fp8(q, k_cache, v_cache, k_seq_starts, v_seq_starts, 
     """Exact attention of the listed query rows over the 8-bit keys and values of their sequence (``ops.fp8_cache_write``),
     read in place in the caches: pairs ``(codes, scales)`` whose rows start at ``k_seq_starts`` / ``v_seq_starts[seq_ids[b]]``.
 
-    ``s_j = scale * q . k_j`` (``scale`` None: 1/sqrt(128)); with ``softcap`` > 0 (at least 1e-6) ``s_j = softcap * tanh(s_j / softcap)``; with
+    ``s_j = scale * q . k_j`` (``scale`` None: 1/sqrt(128)); with ``softcap`` > 0 (from 1e-6 to 2^125) ``s_j = softcap * tanh(s_j / softcap)``; with
     ``slopes`` (fp32 ``[heads]``) ``s_j -= slopes[h] * |pos - j|``, where the queries of a sequence are its last rows;
     ``key_ranges`` (int32 ``[total_q, 2]``): the keys ``[begin, end)`` that each query row sees, as places in its sequence
     (documents, block-causal prefixes, windows).  A row that sees no key gives zeros.  ``q`` may be a column slice of a wider

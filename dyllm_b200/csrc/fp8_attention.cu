@@ -34,7 +34,7 @@ struct Fp8AttnParams {
   const int32_t* cu_sal;
   const int32_t* idx;
   int num_salient, batch, H, Hkv;
-  float scale, cap;
+  float scale, cap, inv_cap;   // cap in powers of two (times log2(e)), 1 / that
   const float* slopes;
   const int2* ranges;
 };
@@ -54,10 +54,6 @@ __device__ __forceinline__ KeyRange keys_of(const Fp8AttnParams& p, int b) {
   r.len = r.k0 < 0 || r.v0 < 0 || len < 0 ? 0 : static_cast<int>(len);
   return r;
 }
-
-// cap * tanh(s / cap) from z = 2 log2(e) s / cap: tanh(x) = 1 - 2 / (1 + e^2x), absolute error a few 2^-24 (the hardware tanh
-// has 2^-11).
-__device__ __forceinline__ float capped(float z, float cap) { return cap - 2.f * cap * __fdividef(1.f, 1.f + exp2f(z)); }
 
 // Exponent of a value's scale (a power of two by definition).
 __device__ __forceinline__ float value_exponent(float scale) {
@@ -473,6 +469,18 @@ __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
   return floats2(r);
 }
+// cap * tanh(s / cap).  With x = s / cap, below 1/4 (and for every score where the cap is large) the odd polynomial, of which
+// 62/2835 x^8 < 2^-21 is left out; above, tanh(x) = 1 - 2 / (1 + e^2x), off by a few 2^-23, 2^-18 of a score at x = -1/4 and less
+// further out.  (The hardware tanh has 2^-11; the second form alone is off by that much of the cap.)
+__device__ __forceinline__ float2 capped(float2 s, float cap, float inv_cap) {
+  const auto both = [](float v) { return make_float2(v, v); };
+  const float2 x = fmul2(s, both(inv_cap)), u = fmul2(x, x), z = fmul2(x, both(2.f * kLog2e));
+  float2 poly = ffma2(u, both(-17.f / 315.f), both(2.f / 15.f));
+  poly = fmul2(ffma2(ffma2(poly, u, both(-1.f / 3.f)), u, both(1.f)), s);
+  const float2 rest = make_float2(__fdividef(1.f, 1.f + exp2f(z.x)), __fdividef(1.f, 1.f + exp2f(z.y)));
+  const float2 wide = ffma2(rest, both(-2.f * cap), both(cap));
+  return make_float2(u.x < 0.0625f ? poly.x : wide.x, u.y < 0.0625f ? poly.y : wide.y);
+}
 // A row's reference for scores up to mx: weights are 2^(t - reference).  2^12 for the largest, but 1 where mx is so large (2^27) that
 // their difference would be rounded up past the largest e5m2 number.
 __device__ __forceinline__ float reference(float mx) {
@@ -820,8 +828,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
         warp_arrive(&q_full);
         rows_sync();
       }
-      // scores come out times log2(e), or as twice the argument of the tanh that caps them
-      const float key_mul = a.scale * kLog2e * (CAP ? 2.f / a.cap : 1.f);
+      const float key_mul = a.scale * kLog2e;      // scores and caps are taken times log2(e)
       const int all_from = max(max(s_all[0].x, s_all[1].x), max(s_all[2].x, s_all[3].x));
       const int all_to = min(min(s_all[0].y, s_all[1].y), min(s_all[2].y, s_all[3].y));
       const int tiles = (end - begin + kUnitKeys - 1) / kUnitKeys;
@@ -848,10 +855,8 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
           const float4 row = *reinterpret_cast<const float4*>(s_mul + r);
           const float2 m0 = fmul2(make_float2(row.x, row.y), make_float2(kk, kk)), m1 = fmul2(make_float2(row.z, row.w), make_float2(kk, kk));
           if (CAP) {
-            t[r] = fmaf(capped(t[r] * m0.x, a.cap), kLog2e, ex);
-            t[r + 1] = fmaf(capped(t[r + 1] * m0.y, a.cap), kLog2e, ex);
-            t[r + 2] = fmaf(capped(t[r + 2] * m1.x, a.cap), kLog2e, ex);
-            t[r + 3] = fmaf(capped(t[r + 3] * m1.y, a.cap), kLog2e, ex);
+            put2(t + r, fadd2(capped(fmul2(get2(t + r), m0), a.cap, a.inv_cap), make_float2(ex, ex)));
+            put2(t + r + 2, fadd2(capped(fmul2(get2(t + r + 2), m1), a.cap, a.inv_cap), make_float2(ex, ex)));
           } else {
             put2(t + r, ffma2(get2(t + r), m0, make_float2(ex, ex)));
             put2(t + r + 2, ffma2(get2(t + r + 2), m1, make_float2(ex, ex)));
@@ -1330,8 +1335,7 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
           }
         }
       };
-      // scores come out times log2(e), or as twice the argument of the tanh that caps them, but for the row's factor
-      const float mul = a.scale * kLog2e * (CAP ? 2.f / a.cap : 1.f);
+      const float mul = a.scale * kLog2e;      // scores (but for the row's factor) and caps are taken times log2(e)
       auto deposit = [&](float k, float v) {
         const int sl = n_sc % kScaleSlots;
         if (n_sc >= kScaleSlots)
@@ -1461,10 +1465,8 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
                   put2(t + j, ffma2(get2(t + j), f, make_float2(ex.x, ex.y)));
                   put2(t + j + 2, ffma2(get2(t + j + 2), g2, make_float2(ex.z, ex.w)));
                 } else {
-                  const float k4[4] = {f.x, f.y, g2.x, g2.y}, e4[4] = {ex.x, ex.y, ex.z, ex.w};
-#pragma unroll
-                  for (int e = 0; e < 4; ++e)
-                    t[j + e] = fmaf(capped(t[j + e] * k4[e], a.cap), kLog2e, e4[e]);
+                  put2(t + j, fadd2(capped(fmul2(get2(t + j), f), a.cap, a.inv_cap), make_float2(ex.x, ex.y)));
+                  put2(t + j + 2, fadd2(capped(fmul2(get2(t + j + 2), g2), a.cap, a.inv_cap), make_float2(ex.z, ex.w)));
                 }
                 if (BIAS) {
 #pragma unroll
@@ -1804,8 +1806,8 @@ int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, co
   DYLLM_REQUIRE(num_heads > 0 && num_kv_heads > 0 && num_heads % num_kv_heads == 0, DYLLM_ERR_INVALID_ARGUMENT,
                 "attention_salient_rows_fp8: query heads (%d) must be a positive multiple of KV heads (%d)", num_heads,
                 num_kv_heads);
-  // a smaller cap: its quotient may be infinite, and a score of zero times that is no number
-  DYLLM_REQUIRE(scale == scale && (softcap == 0.f || softcap >= 1e-6f) && softcap <= 3.0e38f, DYLLM_ERR_INVALID_ARGUMENT,
+  // a smaller cap: its quotient may be infinite, and a score of zero times that is no number; a larger one: its quotient is not normal
+  DYLLM_REQUIRE(scale == scale && (softcap == 0.f || softcap >= 1e-6f) && softcap <= 0x1p125f, DYLLM_ERR_INVALID_ARGUMENT,
                 "attention_salient_rows_fp8: scale %g softcap %g", static_cast<double>(scale), static_cast<double>(softcap));
   if (batch == 0 || num_salient == 0 || max_rows_per_seq == 0)
     return DYLLM_OK;
@@ -1848,7 +1850,8 @@ int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, co
   p.H = num_heads;
   p.Hkv = num_kv_heads;
   p.scale = scale;
-  p.cap = softcap;
+  p.cap = softcap * kLog2e;
+  p.inv_cap = softcap > 0.f ? 1.f / p.cap : 0.f;
   p.slopes = slopes;
   p.ranges = reinterpret_cast<const int2*>(key_ranges);
   FewParams f = {};

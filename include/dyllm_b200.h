@@ -452,7 +452,7 @@ size_t dyllm_attention_salient_rows_fp8_workspace_bytes(int num_salient, int bat
 
 /* Exact attention of the listed query rows over the 8-bit keys and values of their sequence, read in place:
  *   out[i] = sum_j softmax_j(s_j) v_j,  s_j = scale * q[idx_salient_row[i]] . k_j,
- *   softcap > 0 (1e-6 at least): s_j = softcap * tanh(s_j / softcap);  then slopes ([num_heads], nullable): s_j -= slopes[h] * |pos - j|,
+ *   softcap > 0 (from 1e-6 to 2^125): s_j = softcap * tanh(s_j / softcap);  then slopes ([num_heads], nullable): s_j -= slopes[h] * |pos - j|,
  * pos the row's place in its sequence (the queries of a sequence are its last len_q rows).  key_ranges (int32 [total_q, 2],
  * nullable) gives every query row the keys [begin, end) that it sees, as places in its sequence, cut to [0, len_k): documents,
  * prefixes, windows.  A row that sees no key gives zeros.  q: [total_q, num_heads, 128] bf16, row pitch ldq (a multiple of

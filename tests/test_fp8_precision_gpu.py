@@ -76,3 +76,15 @@ def test_many_keys_of_small_weights_beside_a_heavy_one(cuda_device, rows, cache_
     tol = (2.0 ** -8 + 2.0 ** -11 + 2.0 ** -18 + 2.0 ** -14) * want
     err = (out.view(batch, rows, heads, 128).cpu().double() - want).abs()
     assert bool((err <= tol).all()), float((err / want).max())
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# capped scores
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("lens,qlens,counts,heads,hkv", [SHAPES[1], SHAPES[4], SHAPES[6]])
+@pytest.mark.parametrize("cap,q_size", [(1e-6, 1.0), (0.5, 1.0), (5.0, 3.0), (50.0, 8.0), (1e4, 3.0), (1e6, 3.0), (1e9, 3.0), (1e30, 3.0), (4e37, 3.0)])
+@pytest.mark.parametrize("far", [False, True])
+def test_a_cap_of_any_size_costs_its_scores_no_digits(cuda_device, lens, qlens, counts, heads, hkv, cap, q_size, far):
+    """The bound of a score's error is that of the score: the cap takes no part (tanh by itself: 2^-18 of the score)."""
+    got, want, mag, big, floor, _ = _attend(Batch(lens, qlens, seed=47), heads, hkv, counts, cap=cap, q_size=q_size, far=far)
+    _check(got, want, mag, big, floor, 0.0)
