@@ -167,10 +167,12 @@ fp8_kv_cache_update_kernel(const uint4* __restrict__ k_new, int64_t ldk, const u
   }
   const int64_t r = __ldg(rows_k + i);
   const int b = min(seq_of_row(cu_k, batch, r), batch - 1);
-  const int64_t off = r - static_cast<int64_t>(__ldg(cu_k + b)), sid = __ldg(seq_ids + b);
+  const int32_t first = __ldg(cu_k + b);
+  const int64_t off = r - first, length = __ldg(cu_k + b + 1) - first, sid = __ldg(seq_ids + b);
   const int64_t krow = __ldg(k_starts + sid) + off, vrow = __ldg(v_starts + sid) + off;
-  // a row that no cache holds (a sequence without one, an index out of range) changes nothing: its delta-V is zero
-  const bool held = off >= 0 && krow >= off && krow < k_rows && vrow >= off && vrow < v_rows;
+  // a row that no cache holds (a sequence without one, an index out of range) changes nothing: its delta-V is zero.  Behind the
+  // batch's last row the caches may go on, with sequences of others.
+  const bool held = off >= 0 && off < length && krow >= off && krow < k_rows && vrow >= off && vrow < v_rows;
   uint2 olo[G], ohi[G];
   float oscale[G];
 #pragma unroll

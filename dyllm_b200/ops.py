@@ -251,7 +251,8 @@ def fp8_kv_cache_update(k_new: torch.Tensor, v_new: torch.Tensor, rows_k: torch.
     """:func:`kv_cache_update` on 8-bit caches (pairs ``(codes, scales)``): rotary embedding of the new K rows, both halves
     quantised into their caches, delta-V; returns dV ``[rows, kv_heads, 128]``, the difference between the values that the cache
     holds after and before (zero where the codes stay, so their rounding does not pile up in a context over the steps).
-    ``k_new`` and ``v_new`` may be column slices of one product; ``rows_k`` lists no row twice."""
+    ``k_new`` and ``v_new`` may be column slices of one product; ``rows_k`` lists no row twice; a row outside the batch's
+    sequences changes nothing (its dV is zero)."""
     dv = native().kv_cache_update(k_new, v_new, rows_k, positions, pos_idx, cos_sin, cu_seqlens_k, k_seq_starts, v_seq_starts,
                                   seq_ids, k_cache, v_cache, num_rows_dev, dv)
     _lib_mod.launch_count += _lib_mod.KERNELS_PER_CALL["dyllm_fp8_kv_cache_update"]

@@ -439,7 +439,8 @@ int dyllm_fp8_cache_read(const void* codes, const float* scales, int64_t cache_r
  *   dv[i] = bf16(new - old) of the values that V row row_v(i) holds after and before;  V row row_v(i) = quantised v_new[i]
  * The difference is taken between what the cache holds, so a value whose codes do not change adds nothing to a context (the
  * rounding of the codes does not pile up over the steps).  k_new, v_new: [num_rows, kv_heads, 128] bf16 with row pitches ldk,
- * ldv (multiples of 8); dv packed; rows_k without repetitions. */
+ * ldv (multiples of 8); dv packed; rows_k without repetitions.  A row outside the batch's sequences, or that a cache does not
+ * hold, changes nothing: dv[i] = 0. */
 int dyllm_fp8_kv_cache_update(const void* k_new, int64_t ldk, const void* v_new, int64_t ldv, const int64_t* rows_k,
                               const int64_t* positions, const int64_t* pos_idx, const float* cos_sin, int max_pos,
                               const int32_t* cu_seqlens_k, const int64_t* k_seq_starts, const int64_t* v_seq_starts,

@@ -1,0 +1,24 @@
+"""Calls on 8-bit caches that the formulas allow and few programs make."""
+import pytest
+import torch
+
+from tests.test_fp8_cache_gpu import FP8, _cuda
+
+pytestmark = pytest.mark.gpu
+
+
+def test_update_of_rows_behind_the_last_sequence_of_the_batch(cuda_device):
+    """The caches go on behind it, with a sequence of another batch: its rows stay, delta-V is zero."""
+    from dyllm_b200 import ops
+
+    cache = [(torch.full((12, 128), 2.0).cuda().to(FP8), torch.ones(12, 1).cuda()) for _ in range(2)]
+    starts, cu, ids = _cuda(torch.tensor([5, 0, 8]), torch.tensor([0, 3, 6], dtype=torch.int32), torch.tensor([0, 1]))
+    rows_k, positions = _cuda(torch.tensor([6, 2, 7, 5, 2 ** 40, 10]), torch.zeros(6, dtype=torch.int64))
+    cos_sin = torch.cat([torch.ones(4, 64), torch.zeros(4, 64)], 1).cuda()
+    x = torch.full((6, 1, 128), 8.0).bfloat16().cuda()
+    dv = ops.fp8_kv_cache_update(x, x, rows_k, positions, None, cos_sin, cu, starts, starts, ids, *cache)
+    assert dv[:, 0, 0].tolist() == [0.0, 6.0, 0.0, 6.0, 0.0, 0.0]
+    want = torch.full((12,), 2.0)
+    want[[7, 2]] = 8.0
+    for codes, scales in cache:
+        assert torch.equal((codes.float() * scales).cpu(), want.unsqueeze(1).expand(12, 128))
