@@ -202,7 +202,7 @@ def attention_salient_rows_fp8(q, k_cache, v_cache, k_seq_starts, v_seq_starts, 
     ``key_ranges`` (int32 ``[total_q, 2]``): the keys ``[begin, end)`` that each query row sees, as places in its sequence
     (documents, block-causal prefixes, windows).  A row that sees no key gives zeros.  ``q`` may be a column slice of a wider
     product.  ``max_rows_per_seq``: bound (or estimate) of a sequence's listed rows; it chooses between two kernels, which serve
-    any number (0: nothing is computed).  Returns ``[num_salient, heads, 128]`` in list order; rows past ``cu_salientlens[-1]``
+    any number.  Returns ``[num_salient, heads, 128]`` in list order; rows past ``cu_salientlens[-1]``
     are left untouched.
 
     Scores and sums are in fp32, a weight in half precision (2^-11 of itself, or 2^-28 of the row's largest); an element of a

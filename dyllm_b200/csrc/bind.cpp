@@ -308,7 +308,9 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   if (cu_rows.size(0) != static_cast<int64_t>(s.batch) + 1)
     refuse("cu_salientlens must have one entry more than seq_ids");
   const int total_q = size32(q.rows, "q"), heads = size32(q.heads, "q"), kv_heads = size32(kc.heads, "k_cache");
-  const int most = to_int(a[10], "max_rows_per_seq");
+  int most = to_int(a[10], "max_rows_per_seq");
+  if (most == 0)
+    most = 1;      // whether rows are listed after all is known on the device alone
   const int n = a[15] == Py_None ? size32(idx.size(0), "idx_salient_row") : to_int(a[15], "num_salient");
   if (n < 0 || n > idx.size(0))
     refuse("num_salient must fit idx_salient_row");
@@ -339,7 +341,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   // two calls share it
   size_t bytes = 0;
   at::Tensor ws;
-  if (n && most && s.batch) {
+  if (n && s.batch) {
     const c10::cuda::CUDAGuard guard(device);      // its size depends on the device
     bytes = g_attention_workspace(n, s.batch, heads, kv_heads);
     ws = at::empty({static_cast<int64_t>(bytes)}, first.options().dtype(at::kByte));

@@ -459,8 +459,8 @@ size_t dyllm_attention_salient_rows_fp8_workspace_bytes(int num_salient, int bat
  * prefixes, windows.  A row that sees no key gives zeros.  q: [total_q, num_heads, 128] bf16, row pitch ldq (a multiple of
  * 8); out: [num_salient, num_heads, 128] bf16, of which the rows up to cu_salientlens[batch] (the live count, read on the
  * device) are written; a listed row outside [0, total_q) gives zeros.  max_rows_per_seq: upper bound of the listed rows of
- * one sequence; it chooses the kernels (a wrong bound costs time, not rows); 0: none are listed, nothing is written.  workspace: 16-byte aligned, need not be
- * cleared; calls that may overlap on the GPU need different ones. */
+ * one sequence; it chooses the kernels (a wrong bound above 0 costs time, not rows); 0: none are listed, nothing is written.
+ * workspace: 16-byte aligned, need not be cleared; calls that may overlap on the GPU need different ones. */
 int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, const void* k_codes, const float* k_scales,
                                      int64_t k_rows, const void* v_codes, const float* v_scales, int64_t v_rows,
                                      const int64_t* k_seq_starts, const int64_t* v_seq_starts, const int64_t* seq_ids,

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from tests.test_fp8_cache_gpu import FP8, _cuda
+from tests.test_fp8_cache_gpu import FP8, Batch, _cuda, _to_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -22,3 +22,16 @@ def test_update_of_rows_behind_the_last_sequence_of_the_batch(cuda_device):
     want[[7, 2]] = 8.0
     for codes, scales in cache:
         assert torch.equal((codes.float() * scales).cpu(), want.unsqueeze(1).expand(12, 128))
+
+
+def test_a_bound_of_no_rows_loses_none(cuda_device):
+    from dyllm_b200.attention_ops import attention_salient_rows_fp8
+
+    b = Batch([70, 90], [70, 90], seed=53)
+    kc, vc = _to_cache(*b.cache(2)), _to_cache(*b.cache(2))
+    cu, rows, _ = b.picks([5, 3])
+    args = (b.randn(160, 4, 128).bfloat16().cuda(), kc, vc, *_cuda(b.k_starts, b.v_starts, b.ids, b.cu_q, b.cu_k, cu, rows))
+    want = attention_salient_rows_fp8(*args, max_rows_per_seq=5)
+    out = torch.full_like(want, 7.0)
+    assert attention_salient_rows_fp8(*args, max_rows_per_seq=0, out=out) is out
+    assert torch.equal(out, want)
