@@ -62,6 +62,7 @@ SIGNATURES: dict[str, tuple] = {
     "dyllm_fp8_cache_read": (I, [P, P, L, I, I, P, P, P, P, P, I, I, P]),
     "dyllm_fp8_kv_cache_update": (I, [P, L, P, L, P, P, P, P, I, P, P, P, P, I, I, P, I, I, P, P, L, P, P, L, P, P]),
     "dyllm_attention_salient_rows_fp8_workspace_bytes": (Z, [I, I, I, I]),
+    "dyllm_attention_salient_rows_fp8_launches": (I, [I, I, I, I, I, L, I]),
     "dyllm_attention_salient_rows_fp8": (I, [P, L, I, P, P, L, P, P, L, P, P, P, P, P, P, I, I, I, I, I, P, P, I, F, F, P, P, P, Z, P]),
     "dyllm_tp_comm_create": (I, [I, I, Z, P]),
     "dyllm_tp_comm_region_bytes": (Z, [P]),
@@ -84,8 +85,8 @@ SIGNATURES: dict[str, tuple] = {
     "dyllm_tp_allreduce_f32": (I, [P, P, I, P]),
 }
 
-# kernels of this library launched by one call of each entry point (for launch accounting; the attention over 8-bit caches: at
-# least one, another with key ranges, another with many rows)
+# kernels of this library launched by one call of each entry point (for launch accounting; the attention over 8-bit caches says
+# for each call how many)
 KERNELS_PER_CALL = {
     "dyllm_context_stats": 1, "dyllm_cosine_mask": 1, "dyllm_salient_select": 1, "dyllm_salient_select_static": 1,
     "dyllm_fused_offset": 1,
@@ -97,7 +98,6 @@ KERNELS_PER_CALL = {
     "dyllm_tp_reduce_f32": 1, "dyllm_tp_allreduce_f32": 2, "dyllm_tp_gather_rows": 2, "dyllm_tp_gather_push": 1,
     "dyllm_tp_gather_finish": 1, "dyllm_tp_scatter_push": 1,
     "dyllm_fp8_cache_write": 1, "dyllm_fp8_cache_read": 1, "dyllm_fp8_kv_cache_update": 1,
-    "dyllm_attention_salient_rows_fp8": 1,
 }
 launch_count = 0
 
@@ -136,7 +136,7 @@ def native():
             raise RuntimeError(f"_native.so is missing or does not fit this torch ({e}): build it with `python -m dyllm_b200.build`") from e
         _native.init(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
             "dyllm_fp8_cache_write", "dyllm_fp8_cache_read", "dyllm_fp8_kv_cache_update", "dyllm_attention_salient_rows_fp8",
-            "dyllm_attention_salient_rows_fp8_workspace_bytes", "dyllm_last_error")))
+            "dyllm_attention_salient_rows_fp8_workspace_bytes", "dyllm_attention_salient_rows_fp8_launches", "dyllm_last_error")))
         _bound = _native
     return _bound
 

@@ -208,9 +208,10 @@ def attention_salient_rows_fp8(q, k_cache, v_cache, k_seq_starts, v_seq_starts, 
     Scores and sums are in fp32, a weight in half precision (2^-11 of itself, or 2^-28 of the row's largest); an element of a
     query below 2^-14.8 of the row's largest is off by up to 2^-21.8 of that.
     """
-    out = native().attention(q, k_cache, v_cache, k_seq_starts, v_seq_starts, seq_ids, cu_seqlens_q, cu_seqlens_k, cu_salientlens,
-                             idx_salient_row, max_rows_per_seq, scale, softcap, slopes, key_ranges, num_salient, out)
-    _lib_mod.launch_count += _lib_mod.KERNELS_PER_CALL["dyllm_attention_salient_rows_fp8"]
+    out, launches = native().attention(q, k_cache, v_cache, k_seq_starts, v_seq_starts, seq_ids, cu_seqlens_q, cu_seqlens_k,
+                                       cu_salientlens, idx_salient_row, max_rows_per_seq, scale, softcap, slopes, key_ranges,
+                                       num_salient, out)
+    _lib_mod.launch_count += launches
     return out
 
 

@@ -28,6 +28,7 @@ decltype(&dyllm_fp8_cache_read) g_read;
 decltype(&dyllm_fp8_kv_cache_update) g_update;
 decltype(&dyllm_attention_salient_rows_fp8) g_attention;
 decltype(&dyllm_attention_salient_rows_fp8_workspace_bytes) g_attention_workspace;
+decltype(&dyllm_attention_salient_rows_fp8_launches) g_attention_launches;
 decltype(&dyllm_last_error) g_last_error;
 
 const at::Tensor& cuda_tensor(PyObject* o, const char* name) {
@@ -171,12 +172,13 @@ void on(int device, const char* name, Call call) {
   END_HANDLE_TH_ERRORS
 
 PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
-  if (n_args != 6) {
-    PyErr_SetString(PyExc_RuntimeError, "init takes six addresses");
+  constexpr int kEntries = 7;
+  if (n_args != kEntries) {
+    PyErr_SetString(PyExc_RuntimeError, "init takes seven addresses");
     return nullptr;
   }
-  void* at[6];
-  for (int i = 0; i < 6; ++i) {
+  void* at[kEntries];
+  for (int i = 0; i < kEntries; ++i) {
     at[i] = PyLong_AsVoidPtr(a[i]);
     if (!at[i]) {
       if (!PyErr_Occurred())
@@ -188,7 +190,8 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   g_update = reinterpret_cast<decltype(g_update)>(at[2]);
   g_attention = reinterpret_cast<decltype(g_attention)>(at[3]);
   g_attention_workspace = reinterpret_cast<decltype(g_attention_workspace)>(at[4]);
-  g_last_error = reinterpret_cast<decltype(g_last_error)>(at[5]);
+  g_attention_launches = reinterpret_cast<decltype(g_attention_launches)>(at[5]);
+  g_last_error = reinterpret_cast<decltype(g_last_error)>(at[6]);
   g_write = reinterpret_cast<decltype(g_write)>(at[0]);
   Py_RETURN_NONE;
 }
@@ -286,7 +289,8 @@ PyObject* kv_cache_update(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 }
 
 // q, k_cache, v_cache, k_seq_starts, v_seq_starts, seq_ids, cu_seqlens_q, cu_seqlens_k, cu_salientlens, idx_salient_row,
-// max_rows_per_seq, scale or None, softcap, slopes or None, key_ranges or None, num_salient or None, out or None
+// max_rows_per_seq, scale or None, softcap, slopes or None, key_ranges or None, num_salient or None, out or None; returns the result
+// and the number of kernels launched
 PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   BEGIN(17)
   const at::Tensor& first = cuda_tensor(a[0], "q");
@@ -340,10 +344,12 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   // workspace: from and to the caching allocator in the order of the stream, or of the graph that is being captured, so that no
   // two calls share it
   size_t bytes = 0;
+  int launches = 0;
   at::Tensor ws;
   if (n && s.batch) {
-    const c10::cuda::CUDAGuard guard(device);      // its size depends on the device
+    const c10::cuda::CUDAGuard guard(device);      // its size and the choice of the kernels depend on the device
     bytes = g_attention_workspace(n, s.batch, heads, kv_heads);
+    launches = g_attention_launches(n, s.batch, most, heads, kv_heads, kc.rows, ranges != nullptr);
     ws = at::empty({static_cast<int64_t>(bytes)}, first.options().dtype(at::kByte));
   }
   on(device, "dyllm_attention_salient_rows_fp8", [&](void* stream) {
@@ -351,7 +357,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                        out.data_ptr(), s.cu, s.cu_k, s.batch, most, heads, kv_heads, 128, data<int32_t>(cu_rows), data<int32_t>(idx), n,
                        scale, softcap, slopes, ranges, bytes ? ws.data_ptr() : nullptr, bytes, stream);
   });
-  return THPVariable_Wrap(std::move(out));
+  return Py_BuildValue("(Ni)", THPVariable_Wrap(std::move(out)), launches);
   END
 }
 

@@ -1725,6 +1725,17 @@ bool joins_later(int64_t max_rows, int64_t num_salient, int64_t batch, int64_t g
   return min(cache_rows / kUnitKeys / batch / kMinPartFew, kFewCtas * ctas / tiles) > 6;
 }
 
+// The kernels of a call: the few-rows or the many-rows one, that of the spans, that of the joins.
+struct Kernels {
+  bool many, spans, join;
+  int count() const { return 1 + spans + join; }
+};
+Kernels kernels_of(int num_salient, int batch, int max_rows, int heads, int kv_heads, int64_t cache_rows, bool ranges, int ctas) {
+  // a sequence with more rows than the bound says is served by either kernel; so is one with few beside others with many
+  const bool many = takes_many(max_rows, num_salient, batch, heads / kv_heads, kv_heads, cache_rows, ctas);
+  return {many, ranges, many || joins_later(max_rows, num_salient, batch, heads / kv_heads, kv_heads, cache_rows, ctas)};
+}
+
 // Workspace: tickets, keys per tile (only with ranges), parts of tiles; for the kernel that needs most.
 constexpr int kMostCtas = kFewCtas > kManyCtas ? kFewCtas : kManyCtas;
 int64_t most_tiles(int num_salient, int batch, int group) { return static_cast<int64_t>(num_salient) * group / kRows + batch; }
@@ -1789,6 +1800,13 @@ size_t dyllm_attention_salient_rows_fp8_workspace_bytes(int num_salient, int bat
   if (num_salient <= 0 || batch <= 0 || num_heads <= 0 || num_kv_heads <= 0)
     return 0;
   return workspace_of(num_salient, batch, num_heads / num_kv_heads, sm_count());
+}
+
+int dyllm_attention_salient_rows_fp8_launches(int num_salient, int batch, int max_rows_per_seq, int num_heads, int num_kv_heads,
+                                              int64_t k_rows, int has_key_ranges) {
+  if (num_salient <= 0 || batch <= 0 || max_rows_per_seq <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0)
+    return 0;
+  return kernels_of(num_salient, batch, max_rows_per_seq, num_heads, num_kv_heads, k_rows, has_key_ranges != 0, sm_count()).count();
 }
 
 int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, const void* k_codes, const float* k_scales,
@@ -1872,10 +1890,10 @@ int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, co
   f.parts = reinterpret_cast<float*>(ws + parts_offset(tiles, kMostCtas * ctas));
   f.launch_id = next_launch_id() & ~0xffffull;
   f.status_word = device_status_word();
-  // a sequence with more rows than the bound says is served by either kernel; so is one with few beside others with many
-  f.later = joins_later(max_rows_per_seq, num_salient, batch, group, num_kv_heads, k_rows, ctas);
-  const bool many = takes_many(max_rows_per_seq, num_salient, batch, group, num_kv_heads, k_rows, ctas);
-  if (p.ranges) {
+  const Kernels kernels = kernels_of(num_salient, batch, max_rows_per_seq, num_heads, num_kv_heads, k_rows, p.ranges != nullptr, ctas);
+  const bool many = kernels.many;
+  f.later = kernels.join;
+  if (kernels.spans) {
     f.spans = spans;
     const unsigned blocks = static_cast<unsigned>((tiles + 3) / 4);
     if (many)

@@ -451,6 +451,10 @@ int dyllm_fp8_kv_cache_update(const void* k_new, int64_t ldk, const void* v_new,
 /* Bytes of workspace dyllm_attention_salient_rows_fp8 needs. */
 size_t dyllm_attention_salient_rows_fp8_workspace_bytes(int num_salient, int batch, int num_heads, int num_kv_heads);
 
+/* Kernels that a call of dyllm_attention_salient_rows_fp8 with these arguments launches on the current device. */
+int dyllm_attention_salient_rows_fp8_launches(int num_salient, int batch, int max_rows_per_seq, int num_heads, int num_kv_heads,
+                                              int64_t k_rows, int has_key_ranges);
+
 /* Exact attention of the listed query rows over the 8-bit keys and values of their sequence, read in place:
  *   out[i] = sum_j softmax_j(s_j) v_j,  s_j = scale * q[idx_salient_row[i]] . k_j,
  *   softcap > 0 (from 1e-6 to 2^125): s_j = softcap * tanh(s_j / softcap);  then slopes ([num_heads], nullable): s_j -= slopes[h] * |pos - j|,

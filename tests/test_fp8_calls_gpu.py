@@ -35,3 +35,50 @@ def test_a_bound_of_no_rows_loses_none(cuda_device):
     out = torch.full_like(want, 7.0)
     assert attention_salient_rows_fp8(*args, max_rows_per_seq=0, out=out) is out
     assert torch.equal(out, want)
+
+
+def _launches(call):
+    """Kernels that a call launches, as a graph holds them."""
+    import ctypes
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        call()
+    n = ctypes.c_size_t()
+    runtime = ctypes.CDLL("libcudart.so.12")
+    assert runtime.cudaGraphGetNodes(ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(n)) == 0
+    return n.value
+
+
+@pytest.mark.parametrize("lens,counts,heads,hkv,ranges,launches", [
+    ([300, 64], [5, 3], 4, 2, False, 1),                  # few rows
+    ([300, 64], [5, 3], 4, 2, True, 2),                   # and keys per tile
+    ([32011, 900], [32, 3], 4, 4, False, 2),              # a tile in many parts: joined by a launch
+    ([1500, 900], [200, 90], 4, 2, False, 2),             # many rows
+    ([1500, 900], [200, 90], 4, 2, True, 3),
+    ([300, 64], [0, 0], 4, 2, False, 1),                  # lists that turn out empty on the device
+])
+def test_launches_are_counted(cuda_device, lens, counts, heads, hkv, ranges, launches):
+    from dyllm_b200 import _lib
+    from dyllm_b200.attention_ops import attention_salient_rows_fp8
+
+    b = Batch(lens, [min(n, 400) for n in lens], seed=59)
+    kc, vc = _to_cache(*b.cache(hkv)), _to_cache(*b.cache(hkv))
+    cu, rows, _ = b.picks(counts)
+    total_q = sum(b.qlens)
+    rows = torch.cat([rows, torch.zeros(3, dtype=torch.int32)])
+    args = (b.randn(total_q, heads, 128).bfloat16().cuda(), kc, vc, *_cuda(b.k_starts, b.v_starts, b.ids, b.cu_q, b.cu_k, cu, rows))
+    seen = torch.tensor([[0, 200]], dtype=torch.int32).repeat(total_q, 1).cuda() if ranges else None
+
+    def call():
+        return attention_salient_rows_fp8(*args, max_rows_per_seq=max(max(counts), 1), key_ranges=seen)
+
+    assert _launches(call) == launches
+    before = _lib.launch_count
+    call()
+    assert _lib.launch_count - before == launches
+    empty = torch.zeros(0, dtype=torch.int32, device="cuda")
+    attention_salient_rows_fp8(*args[:-1], empty, max_rows_per_seq=1)
+    assert _lib.launch_count - before == launches
