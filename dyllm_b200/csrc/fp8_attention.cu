@@ -145,15 +145,15 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
     return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
   return a / b;
 }
-__device__ __forceinline__ int units_of(int2 span) { return max(1, (span.y - span.x + kUnitKeys - 1) / kUnitKeys); }
-
 // Walks over the parts of tiles that a CTA's share of the units consists of, in the order (sequence, tile, key head, keys).
 // Uniform over a warp.
 //
 // Shares are cut at total * i / ctas, but no part of a tile is shorter than kMinPart units: a cut nearer to an end of its
-// tile moves there.  Joining the parts of a tile costs a CTA of the few-rows kernel about 5 us, a unit 3.  With many rows a
-// unit takes 5 us and the join is a launch of its own: parts of at least 2 units against 4 take 34.6 us against 43.1 (32 x 601
-// keys, 28 heads on 4) and 163 against 166 (4 x 2048 rows of packed documents).
+// tile moves there, and a tile counts as kMinPart units at least (what it costs, too: most of a part's time passes before its second
+// unit), so that no share is smaller: one sequence of 8192 keys among 70 of 100, 8 key heads, 46.7 us against 63.6 with 34 parts of one
+// or two units; 32 x 601 ragged keys, 28 heads on 4, 28.6 against 35.0.  Joining the parts of a tile costs a CTA of the few-rows
+// kernel about 5 us, a unit 3.  With many rows a unit takes 5 us and the join is a launch of its own: parts of at least 2 units
+// against 4 take 34.6 us against 43.1 (32 x 601 keys, 28 heads on 4) and 163 against 166 (4 x 2048 rows of packed documents).
 constexpr int kMinPartFew = 4, kMinPartMany = 2;
 template <int MROWS>
 struct Walk {
@@ -181,6 +181,7 @@ struct Walk {
     }
     return x;
   }
+  static __device__ __forceinline__ int units_of(int2 span) { return max(kMinPart, (span.y - span.x + kUnitKeys - 1) / kUnitKeys); }
   // Units of a sequence's tiles, for one key head.
   static __device__ __forceinline__ int64_t seq_units(const FewParams& p, const SeqWork& x, int base) {
     if (!p.spans)
@@ -213,7 +214,7 @@ struct Walk {
     for (int s = 16; s; s >>= 1)
       sum += __shfl_xor_sync(0xffffffffu, sum, s);
     total = sum * p.a.Hkv;
-    ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), max(static_cast<int64_t>(all_tiles) * p.a.Hkv, total / kMinPart)));
+    ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total / kMinPart));
     end = tile_first = 0;
     first = 0;
     begun = false;

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from tests.test_fp8_cache_gpu import FP8, Batch, _cuda, _to_cache
+from tests.test_fp8_cache_gpu import FP8, Batch, _attend, _check, _cuda, _to_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -82,3 +82,10 @@ def test_launches_are_counted(cuda_device, lens, counts, heads, hkv, ranges, lau
     empty = torch.zeros(0, dtype=torch.int32, device="cuda")
     attention_salient_rows_fp8(*args[:-1], empty, max_rows_per_seq=1)
     assert _lib.launch_count - before == launches
+
+
+@pytest.mark.parametrize("rows,far", [(2, False), (70, True)])
+def test_a_long_sequence_among_many_short_ones(cuda_device, rows, far):
+    """Tiles of one unit by the hundred, and between them some that are cut into parts."""
+    lens = [100, 1, 0, 90] * 9 + [5003] + [100] * 34
+    _check(*_attend(Batch(lens, seed=61), 8, 8, [min(n, rows) for n in lens], far=far))
