@@ -403,7 +403,7 @@ __device__ __forceinline__ void split_query(const uint4& x0, const uint4& x1, fl
   lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
-constexpr float kNothing = -1.0e30f;      // maximum of no scores (finite: it takes part in differences)
+constexpr float kNothing = -3.0e38f;      // maximum of no scores (finite: it takes part in differences; below every score)
 
 // What a tile's rows are to the softmax warps.
 struct RowInfo {

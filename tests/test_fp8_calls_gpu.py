@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from tests.test_fp8_cache_gpu import FP8, Batch, _attend, _check, _cuda, _to_cache
+from tests.test_fp8_cache_gpu import FP8, Batch, _attend, _check, _cuda, _far, _to_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +89,24 @@ def test_a_long_sequence_among_many_short_ones(cuda_device, rows, far):
     """Tiles of one unit by the hundred, and between them some that are cut into parts."""
     lens = [100, 1, 0, 90] * 9 + [5003] + [100] * 34
     _check(*_attend(Batch(lens, seed=61), 8, 8, [min(n, rows) for n in lens], far=far))
+
+
+@pytest.mark.parametrize("rows,far", [(5, False), (90, True)])
+@pytest.mark.parametrize("size", [-1e20, -1e13, 1.0, 1e13, 1e20])
+def test_a_key_that_is_alone_has_all_the_weight(cuda_device, rows, far, size):
+    """However far below zero its score is: rows of a window of one key give that key's value."""
+    from dyllm_b200.attention_ops import attention_salient_rows_fp8
+
+    b = Batch([100], [100], seed=67)
+    (_, _), (vc, vs) = b.cache(2), b.cache(2)
+    kc, ks = torch.ones(b.rows, 2, 128).double(), torch.full((b.rows, 2), 2.0 ** 50).double()
+    caches = [_to_cache(*(_far(b, *c) if far else c)) for c in ((kc, ks), (vc, vs))]
+    q = torch.full((100, 4, 128), size).bfloat16()
+    pos = torch.arange(100, dtype=torch.int32)
+    cu, idx = torch.tensor([0, rows], dtype=torch.int32), pos[:rows].flip(0)
+    out = attention_salient_rows_fp8(q.cuda(), *caches, *_cuda(b.k_starts, b.v_starts, b.ids, b.cu_q, b.cu_k, cu, idx), rows,
+                                     key_ranges=torch.stack([pos, pos + 1], 1).cuda())
+    at = int(b.v_starts[b.ids[0]]) + idx.long()
+    want = (vc[at] * vs[at].unsqueeze(-1)).repeat_interleave(2, 1)
+    # a weight of 2^12 exactly, over its own sum: the quotient's rounding, and a value that bf16 holds
+    assert bool(((out.cpu().double() - want).abs() <= 2.0 ** -8 * want.abs()).all())
