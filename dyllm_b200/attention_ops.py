@@ -197,13 +197,13 @@ def attention_salient_rows_fp8(q, k_cache, v_cache, k_seq_starts, v_seq_starts, 
     """Exact attention of the listed query rows over the 8-bit keys and values of their sequence (``ops.fp8_cache_write``),
     read in place in the caches: pairs ``(codes, scales)`` whose rows start at ``k_seq_starts`` / ``v_seq_starts[seq_ids[b]]``.
 
-    ``s_j = scale * q . k_j`` (``scale`` None: 1/sqrt(128)); with ``softcap`` > 0 (from 1e-6 to 2^125) ``s_j = softcap * tanh(s_j / softcap)``; with
-    ``slopes`` (fp32 ``[heads]``) ``s_j -= slopes[h] * |pos - j|``, where the queries of a sequence are its last rows;
-    ``key_ranges`` (int32 ``[total_q, 2]``): the keys ``[begin, end)`` that each query row sees, as places in its sequence
-    (documents, block-causal prefixes, windows).  A row that sees no key gives zeros.  ``q`` may be a column slice of a wider
-    product.  ``max_rows_per_seq``: bound (or estimate) of a sequence's listed rows; it chooses between two kernels, which serve
-    any number.  Returns ``[num_salient, heads, 128]`` in list order; rows past ``cu_salientlens[-1]``
-    are left untouched.
+    ``s_j = scale * q . k_j`` (``scale`` None: 1/sqrt(128)); with ``softcap`` > 0 (from 1e-6 to 2^125)
+    ``s_j = softcap * tanh(s_j / softcap)``; with ``slopes`` (fp32 ``[heads]``) ``s_j -= slopes[h] * |pos - j|``, where the
+    queries of a sequence are its last rows; ``key_ranges`` (int32 ``[total_q, 2]``): the keys ``[begin, end)`` that each query row
+    sees, as places in its sequence (documents, block-causal prefixes, windows).  A row that sees no key gives zeros.  ``q`` may be
+    a column slice of a wider product.  ``max_rows_per_seq``: bound (or estimate) of a sequence's listed rows; it chooses between
+    two kernels, which serve any number.  Returns ``[num_salient, heads, 128]`` in list order; rows past ``cu_salientlens[-1]`` are
+    left untouched.
 
     Scores and sums are in fp32, a weight in half precision (2^-11 of itself, or 2^-28 of the row's largest); an element of a
     query below 2^-14.8 of the row's largest is off by up to 2^-21.8 of that.

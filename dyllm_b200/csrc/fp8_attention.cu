@@ -74,13 +74,13 @@ constexpr int kFewPart = part_floats(kRows), kManyPart = part_floats(kManyRows);
 constexpr float kWeightLog2 = 12.f;                          // the reference's weight: 2^12
 constexpr float kHeadroom = 2.8f;                            // 2^(12 + 2.8) < 57344, the largest e5m2 number
 
-struct FewParams {
+struct WorkParams {
   Fp8AttnParams a;
   const int2* spans;           // per tile of rows: keys that any of them sees (null: all)
   unsigned long long* tickets; // one per CTA
   float* parts;                // two per CTA: [rows][128] sums, [rows] maxima, [rows] sums of weights
   int* joins;                  // per CTA: parts of the tile that begins in it and goes on in others (0: none); for fp8_join_kernel
-  bool later;                  // few rows: that kernel joins them
+  bool later;                  // that kernel joins them (of few rows: only where there are many parts)
   unsigned long long launch_id;
   int* status_word;
 };
@@ -183,7 +183,7 @@ struct Walk {
   }
   static __device__ __forceinline__ int units_of(int2 span) { return max(kMinPart, (span.y - span.x + kUnitKeys - 1) / kUnitKeys); }
   // Units of a sequence's tiles, for one key head.
-  static __device__ __forceinline__ int64_t seq_units(const FewParams& p, const SeqWork& x, int base) {
+  static __device__ __forceinline__ int64_t seq_units(const WorkParams& p, const SeqWork& x, int base) {
     if (!p.spans)
       return static_cast<int64_t>(x.tiles) * units_of(make_int2(0, x.len));
     int64_t sum = 0;
@@ -191,11 +191,11 @@ struct Walk {
       sum += units_of(__ldg(p.spans + base + t));
     return sum;
   }
-  __device__ __forceinline__ void open(const FewParams& p) {
+  __device__ __forceinline__ void open(const WorkParams& p) {
     span = p.spans ? __ldg(p.spans + tile_base + tile) : make_int2(0, w.len);
     units = units_of(span);
   }
-  __device__ __forceinline__ void start(const FewParams& p) {
+  __device__ __forceinline__ void start(const WorkParams& p) {
     const int lane = threadIdx.x & 31;
     int64_t sum = 0;
     int all_tiles = 0;
@@ -270,7 +270,7 @@ struct Walk {
     first = moved(static_cast<int>(at - tile_first), units);
   }
   // The next part, false at the end of the share.
-  __device__ __forceinline__ bool next(const FewParams& p) {
+  __device__ __forceinline__ bool next(const WorkParams& p) {
     if (tile_first >= end)
       return false;
     if (begun || first == units) {
@@ -365,10 +365,10 @@ __device__ __forceinline__ void umma_tile_b64(uint32_t d_tmem, uint32_t a_addr, 
 // stays there, and an MMA issues every 33 cycles (its A operand's shared-memory read) instead of every 90.
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __reduce_max_sync(0xffffffffu, x); }
 
-// The 128 softmax threads of the few-rows kernel, or loader threads of the many-rows kernel, meet; any: whether the condition holds
+// The team of 128 threads that works on a tile's rows (softmax of the few-rows kernel, loaders of the many-rows kernel) meets; any: whether the condition holds
 // for one of them (after a wait that has given up they all leave together: a barrier would wait for those that are gone).
-__device__ __forceinline__ void rows_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
-__device__ __forceinline__ bool rows_any(bool x) {
+__device__ __forceinline__ void team_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool team_any(bool x) {
   uint32_t r;
   asm volatile(
       "{\n\t"
@@ -535,8 +535,9 @@ __device__ __forceinline__ void split_weights(float2 a, float2 b, uint32_t& hi, 
 // Four softmax warps, thread = key with the scores of all rows in registers; a row's reference is in shared memory and follows the
 // maximum in steps, so that a unit costs one barrier (does any score exceed its reference by more than 2.8?) and the maxima are
 // looked for only where one does.  A part of four units takes 14 us from its description to its result, nearly all of it waits
-// along that chain, so four CTAs per SM with parts of their own take turns: 16 x 512 keys, 32 heads, 26 rows take 30 us (2.5 TB/s
-// of the cache); 41 us with three CTAs, where 68 of 512 tiles wait for a second turn; 43 us with one CTA of sixteen softmax warps.
+// along that chain, so four CTAs per SM with parts of their own take turns: 16 x 512 keys, 32 heads, 26 rows take 33 us (2.3 TB/s
+// of the cache).  With the weights of before 30 us, and then 41 us with three CTAs, where 68 of 512 tiles wait for a second turn, 43 us
+// with one CTA of sixteen softmax warps.
 // ----------------------------------------------------------------------------------------------
 constexpr int kFewRing = 2;                                  // slots of one K or V tile
 constexpr int kFewCtas = 4;                                  // per SM
@@ -563,7 +564,7 @@ __device__ __forceinline__ float sum_lanes(float (&v)[32]) {
 // CAP, BIAS: scores capped by a tanh, biased by their distance.
 template <bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kFewThreads, kFewCtas)
-fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const FewParams p) {
+fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const WorkParams p) {
   pdl_wait();      // programmatic dependent launch: nothing before this reads an earlier kernel's data
   pdl_trigger();
   const Fp8AttnParams& a = p.a;
@@ -738,7 +739,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
     if (p.later && tid == 0)
       p.joins[blockIdx.x] = 0;                     // unless a tile begins here that goes on in other CTAs
     for (int n = 0;; ++n) {
-      if (rows_any(!mbar_wait(&part_full[n % kParts], (n / kParts) & 1, &abort_flag, p.status_word, 415)))
+      if (team_any(!mbar_wait(&part_full[n % kParts], (n / kParts) & 1, &abort_flag, p.status_word, 415)))
         break;
       const PartInfo part = s_part[n % kParts];
       warp_arrive(&part_done[n % kParts]);
@@ -827,7 +828,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
           s_all[quarter] = sees;
         fence_proxy_async_smem();
         warp_arrive(&q_full);
-        rows_sync();
+        team_sync();
       }
       const float key_mul = a.scale * kLog2e;      // scores and caps are taken times log2(e)
       const int all_from = max(max(s_all[0].x, s_all[1].x), max(s_all[2].x, s_all[3].x));
@@ -888,7 +889,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
             above = fmax3(above, t[r] - ref.x, t[r + 1] - ref.y);
             above = fmax3(above, t[r + 2] - ref.z, t[r + 3] - ref.w);
           }
-          moves = rows_any(above > kHeadroom + kWeightLog2);
+          moves = team_any(above > kHeadroom + kWeightLog2);
         }
         if (moves) {
           float mx = 0.f;
@@ -898,7 +899,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
             mx = lane == r ? m : mx;
           }
           s_max[quarter][lane] = mx;
-          rows_sync();
+          team_sync();
           mx = fmaxf(fmaxf(s_max[0][lane], s_max[1][lane]), fmaxf(s_max[2][lane], s_max[3][lane]));
           const float ref = mx - was > kHeadroom + kWeightLog2 ? reference(mx) : was, old = exp2f(was - ref);
           l *= old;
@@ -980,7 +981,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
       tmem_ld_wait();
       tc_fence_before_sync();
       warp_arrive(&o_free);
-      rows_sync();
+      team_sync();
       l = (s_sum[0][lane] + s_sum[1][lane]) + (s_sum[2][lane] + s_sum[3][lane]);
       bool store = true;
       if (part.parts > 1) {
@@ -1002,12 +1003,12 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
             p.joins[blockIdx.x] = part.parts;
         } else {
           __threadfence();
-          rows_sync();
+          team_sync();
           if (tid == 0) {
             open_join(p.tickets + part.owner, p.launch_id);
             joins = last_to_join(p.tickets + part.owner, part.parts) ? 1 : 0;
           }
-          rows_sync();
+          team_sync();
           store = joins != 0;
         }
         if (store) {
@@ -1044,7 +1045,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
           lines[r * kD + kl] = o[r];
         if (quarter == 0)
           s_old[0][lane] = l == 0.f || fix == 0.f ? 0.f : __fdividef(fix, l);
-        rows_sync();
+        team_sync();
 #pragma unroll
         for (int r = tid >> 4; r < kRows; r += 8) {
           const int out = s_out[r];
@@ -1060,7 +1061,7 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
           }
         }
       }
-      rows_sync();      // nobody overwrites the rows or what describes them while another warp reads it
+      team_sync();      // nobody overwrites the rows or what describes them while another warp reads it
     }
   }
 
@@ -1073,10 +1074,11 @@ fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_con
 }
 
 // ----------------------------------------------------------------------------------------------
-// Many rows per sequence: bound by the instructions around the exponentials.  A unit of 128 rows x 128 keys takes the tensor cores
-// 1000 cycles, its exponentials 1024, the scales of its keys (three words a key for each of four warps) 1536 of shared memory; with
-// all else it takes an SM 4800 (2 x 32011 keys, 128 pairs a key head: 105 us, of which 9 for lists and queries, 5 for the join).
-// Without the reads of the scales it would take 93 us, without the scores' pass 89, without the weights' pass 90.
+// Many rows per sequence: bound by the passes over tensor memory and the instructions around the exponentials.  A unit of 128 rows x
+// 128 keys takes the tensor cores 1250 cycles, its exponentials 1024, the scales of its keys (three words a key for each of four
+// warps) 1536 of shared memory; with all else it takes an SM 5100 (2 x 32011 keys, 128 pairs a key head: 112 us, of which 9 for lists
+// and queries, 5 for the join).  Without the reads of the scales it would take 89 us, without the scores' pass 86, without the
+// weights' pass 86, without the products of the third codes 110.
 //
 // Tiles of 128 (listed row, query head) pairs, rows in the M = 128 of the products:
 //   S = Q K^T    A: the queries as e4m3 + e5m2 (two products into one accumulator), B: the K tile as loaded (K-major)
@@ -1117,7 +1119,7 @@ __device__ __forceinline__ void umma_tile_ts(uint32_t d_tmem, uint32_t a_tmem, u
 // CAP, BIAS: scores capped by a tanh, biased by their distance.
 template <bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kManyThreads, kManyCtas)
-fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const FewParams p) {
+fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const WorkParams p) {
   pdl_wait();      // programmatic dependent launch: nothing before this reads an earlier kernel's data
   pdl_trigger();
   const Fp8AttnParams& a = p.a;
@@ -1273,10 +1275,10 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     int n_sc = 0, live = 0;
     for (int n = 0;; ++n) {
       const int slot = n % kParts;
-      if (rows_any(!mbar_wait(&part_full[slot], (n / kParts) & 1, &abort_flag, p.status_word, 510)))
+      if (team_any(!mbar_wait(&part_full[slot], (n / kParts) & 1, &abort_flag, p.status_word, 510)))
         break;
       const PartInfo w = s_part[slot];
-      rows_sync();
+      team_sync();
       warp_arrive(&part_done[slot]);
       if (w.end < 0)
         break;
@@ -1303,12 +1305,12 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       }
       if (w.end == w.begin) {      // no keys: zeros
         s_src[tid] = v.out;
-        rows_sync();
+        team_sync();
 #pragma unroll 1
         for (int r = tid >> 4; r < kManyRows; r += 8)
           if (s_src[r] >= 0)
             *reinterpret_cast<uint4*>(a.out + s_src[r] * kD + (tid & 15) * 8) = make_uint4(0u, 0u, 0u, 0u);
-        rows_sync();
+        team_sync();
         continue;
       }
       // the first tile's scales are on their way with the queries
@@ -1320,7 +1322,7 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         first_v = __ldg(vs + static_cast<int64_t>(w.begin + tid) * a.Hkv);
       }
       s_src[tid] = src;
-      rows_sync();
+      team_sync();
       // queries: eight threads a row, 16 rows at a time, four times 16 in flight; codes next to the row's own largest element.
       // (Loops: straight-line code for 128 rows that runs once a part costs more in instruction fetches than it saves.)
       uint4 x0[4], x1[4];
@@ -1372,14 +1374,14 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
           *reinterpret_cast<uint4*>(dst + kManyQBytes) = lo;
         }
       }
-      rows_sync();
+      team_sync();
       const uint32_t top = __float_as_uint(s_row[tid].mul);
       if (top >= 0x7f800000u)
         v.fix = __uint_as_float(0x7fc00000u);
       v.mul = __uint_as_float(fp8_scale_bits(top >= 0x7f800000u ? 0u : top));
       s_row[tid] = v;
       fence_proxy_async_smem();
-      rows_sync();
+      team_sync();
       warp_arrive(&q_full);
       ++live;
       // scales of the other tiles: thread = key, four tiles' loads at a time
@@ -1623,7 +1625,7 @@ fp8_many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
 // with 19 parts of 128 rows; blocks of 32 dimensions 15 us.)
 constexpr int kJoinThreads = 128, kJoinDims = 8;
 template <int ROWS>
-__global__ void __launch_bounds__(kJoinThreads) fp8_join_kernel(const FewParams p) {
+__global__ void __launch_bounds__(kJoinThreads) fp8_join_kernel(const WorkParams p) {
   pdl_wait();
   pdl_trigger();
   constexpr int kPart = part_floats(ROWS);
@@ -1705,9 +1707,9 @@ __global__ void __launch_bounds__(128) fp8_spans_kernel(const Fp8AttnParams p, i
 // The kernel for a call.  Up to kFewMost (listed row, query head) pairs a sequence and key head the few-rows kernel is taken, with a
 // pass over the keys for each 32 of them; so it is for more of them where the caches are short (their rows are all that the host
 // knows of the keys): tiles of up to 8 units, which it does not split, and at most ten units a CTA.  Few against many, us:
-//   26 pairs (16 x 512 keys, 32 heads) 30 : 63; 64 there 52 : 68; 64 over 8 x 4096 keys 88 : 101, capped 92 : 139; over 2 x 32011 84 : 96
-//   77 (175 keys, 4 key heads) 13 : 30; 84 (32 x 601, 4) 31 : 35; 140 there 36 : 44; 96 (2 x 1001, 8) 25 : 27
-//   96 (2 x 32011 keys, 8 key heads) 103 : 98, biased 128 : 103; 90 (16 x 512, 32) 74 : 70; 128 there 96 : 74
+//   26 pairs (16 x 512 keys, 32 heads) 33 : 66; 64 there 57 : 72; 64 over 8 x 4096 keys 97 : 109, capped 111 : 150; over 2 x 32011 92 : 103
+//   77 (175 keys, 4 key heads) 13 : 21; 84 (32 x 601, 4) 27 : 36; 140 there 43 : 46; 96 (2 x 1001, 8) 25 : 26
+//   96 (2 x 32011 keys, 8 key heads) 119 : 105, biased 133 : 110; 90 (16 x 512, 32) 82 : 74; 128 there 106 : 77
 constexpr int kFewMost = 64;
 bool takes_many(int64_t max_rows, int64_t num_salient, int64_t batch, int64_t group, int64_t kv_heads, int64_t cache_rows, int64_t ctas) {
   const int64_t most = min(max_rows, num_salient) * group;
@@ -1756,7 +1758,7 @@ int grid_of(const Fp8AttnParams& a, int tile_rows, int min_part, int most) {
 }
 
 template <typename Kernel>
-int launch_rows(Kernel kernel, bool (&set)[64], int threads, uint32_t smem, const CUtensorMap& tk, const CUtensorMap& tv, const FewParams& p,
+int launch_rows(Kernel kernel, bool (&set)[64], int threads, uint32_t smem, const CUtensorMap& tk, const CUtensorMap& tv, const WorkParams& p,
                 int ctas, cudaStream_t s) {
   int dev = 0;
   cudaGetDevice(&dev);
@@ -1771,19 +1773,19 @@ int launch_rows(Kernel kernel, bool (&set)[64], int threads, uint32_t smem, cons
   return check_launch("attention_salient_rows_fp8");
 }
 template <int ROWS>
-int launch_join(const FewParams& p, int ctas, cudaStream_t s) {
+int launch_join(const WorkParams& p, int ctas, cudaStream_t s) {
   DYLLM_LAUNCH(fp8_join_kernel<ROWS>, dim3(ctas, kD / kJoinDims * ROWS / kJoinThreads), kJoinThreads, 0, s, p);
   return check_launch("attention_salient_rows_fp8");
 }
 template <bool CAP, bool BIAS>
-int launch_few(const CUtensorMap& tk, const CUtensorMap& tv, const FewParams& p, int ctas, cudaStream_t s) {
+int launch_few(const CUtensorMap& tk, const CUtensorMap& tv, const WorkParams& p, int ctas, cudaStream_t s) {
   static bool set[64] = {};
   const int grid = grid_of(p.a, kRows, kMinPartFew, kFewCtas * ctas);
   const int rc = launch_rows(fp8_few_rows_kernel<CAP, BIAS>, set, kFewThreads, kFewSmem, tk, tv, p, grid, s);
   return rc == DYLLM_OK && p.later ? launch_join<kRows>(p, grid, s) : rc;
 }
 template <bool CAP, bool BIAS>
-int launch_many(const CUtensorMap& tk, const CUtensorMap& tv, const FewParams& p, int ctas, cudaStream_t s) {
+int launch_many(const CUtensorMap& tk, const CUtensorMap& tv, const WorkParams& p, int ctas, cudaStream_t s) {
   static bool set[64] = {};
   const int grid = grid_of(p.a, kManyRows, kMinPartMany, kManyCtas * ctas);
   const int rc = launch_rows(fp8_many_rows_kernel<CAP, BIAS>, set, kManyThreads, kManySmem, tk, tv, p, grid, s);
@@ -1873,7 +1875,7 @@ int dyllm_attention_salient_rows_fp8(const void* q, int64_t ldq, int total_q, co
   p.inv_cap = softcap > 0.f ? 1.f / p.cap : 0.f;
   p.slopes = slopes;
   p.ranges = reinterpret_cast<const int2*>(key_ranges);
-  FewParams f = {};
+  WorkParams f = {};
   const int ctas = sm_count();
   DYLLM_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, DYLLM_ERR_INVALID_ARGUMENT,
                 "attention_salient_rows_fp8: the workspace must be 16-byte aligned");

@@ -413,8 +413,9 @@ int dyllm_rope_neox(void* x, const int64_t* positions, const int64_t* pos_idx, c
  *
  * Per row and key/value head a cache holds 128 codes in e4m3 ([cache_rows, heads * 128] bytes, 16-byte aligned) and one fp32
  * scale ([cache_rows, heads]): scale = 2^e, e the least integer >= -60 with amax <= 448 * 2^e; a value is code * scale,
- * which bf16 holds exactly.  A head of a row with a NaN or an infinity gets codes of zero and a NaN scale: it reads as NaN,
- * and a key that a row does not see never reaches its result.  Sequences lie in both arrays as in the bf16 caches:
+ * which bf16 holds exactly (codes that round to 2^128, of magnitudes above 3.2e38, read as infinity).  A head of a row with a
+ * NaN or an infinity gets codes of zero and a NaN scale: it reads as NaN, and a key that a row does not see never reaches its
+ * result.  Sequences lie in both arrays as in the bf16 caches:
  * seq_starts[seq_ids[b]] is the first row of batch entry b.  A row that lies outside [0, cache_rows), or whose sequence has
  * a negative start, is not written and reads as zeros.  heads > 0, head_dim 128.  No counterpart in the reference, whose
  * caches are bf16 (dyllm/engine/cache_manager.py:11-60).
@@ -457,8 +458,10 @@ int dyllm_attention_salient_rows_fp8_launches(int num_salient, int batch, int ma
 
 /* Exact attention of the listed query rows over the 8-bit keys and values of their sequence, read in place:
  *   out[i] = sum_j softmax_j(s_j) v_j,  s_j = scale * q[idx_salient_row[i]] . k_j,
- *   softcap > 0 (from 1e-6 to 2^125): s_j = softcap * tanh(s_j / softcap);  then slopes ([num_heads], nullable): s_j -= slopes[h] * |pos - j|,
- * pos the row's place in its sequence (the queries of a sequence are its last len_q rows).  key_ranges (int32 [total_q, 2],
+ *   softcap > 0 (from 1e-6 to 2^125): s_j = softcap * tanh(s_j / softcap);
+ *   then slopes ([num_heads], nullable): s_j -= slopes[h] * |pos - j|,
+ * scores and sums in fp32, weights in half precision (2^-11 of themselves, or 2^-28 of the row's largest), elements of a query
+ * below 2^-14.8 of its largest off by up to 2^-21.8 of that; pos the row's place in its sequence (the queries of a sequence are its last len_q rows).  key_ranges (int32 [total_q, 2],
  * nullable) gives every query row the keys [begin, end) that it sees, as places in its sequence, cut to [0, len_k): documents,
  * prefixes, windows.  A row that sees no key gives zeros.  q: [total_q, num_heads, 128] bf16, row pitch ldq (a multiple of
  * 8); out: [num_salient, num_heads, 128] bf16, of which the rows up to cu_salientlens[batch] (the live count, read on the
