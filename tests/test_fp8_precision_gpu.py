@@ -88,3 +88,17 @@ def test_a_cap_of_any_size_costs_its_scores_no_digits(cuda_device, lens, qlens, 
     """The bound of a score's error is that of the score: the cap takes no part (tanh by itself: 2^-18 of the score)."""
     got, want, mag, big, floor, _ = _attend(Batch(lens, qlens, seed=47), heads, hkv, counts, cap=cap, q_size=q_size, far=far)
     _check(got, want, mag, big, floor, 0.0)
+
+
+@pytest.mark.parametrize("lens,qlens,counts,heads,hkv", [SHAPES[1], SHAPES[3], SHAPES[6]])
+@pytest.mark.parametrize("mask", [None, "empty"])
+@pytest.mark.parametrize("far", [False, True])
+def test_a_query_without_numbers_is_alone_with_that(cuda_device, lens, qlens, counts, heads, hkv, mask, far):
+    """A head of a row with a NaN or an infinity gives NaN (zeros where it sees no key); rows and heads beside it are as ever."""
+    size = torch.ones(sum(qlens) * heads)
+    size[2::5], size[3::11] = float("inf"), float("nan")
+    got, want, mag, big, floor, cap = _attend(Batch(lens, qlens, seed=71), heads, hkv, counts, mask, q_size=size.view(-1, heads, 1), far=far)
+    assert not bool(torch.isnan(want).all())      # of three listed rows none may be such a one
+    fine = ~torch.isnan(want)
+    assert torch.equal(torch.isnan(got), ~fine)
+    _check(got.masked_fill(~fine, 0), want.masked_fill(~fine, 0), mag.nan_to_num(), big.nan_to_num(posinf=0.0), floor.nan_to_num(), cap)
